@@ -248,6 +248,119 @@ int kvhp_causal_gqa(const void* q, const void* k, const void* v, void* out,
                     int64_t seq_len, int64_t num_q_heads, int64_t num_kv_heads,
                     int64_t head_dim, void* stream);
 
+/* ---- Caches of bounded length.  No counterpart in the reference, whose cache
+ * keeps and attends every key (src/runtime/kv_cache.h:12-73).  Two ways to
+ * bound it: attend a sliding window and a few first tokens only (the pages
+ * between need not be kept), or cut the cache to a budget of slots, keeping
+ * those that received the most attention.
+ *
+ * Visible keys: the query at position p of its sequence attends key j when
+ * j <= p and (j < sinks or p - j < window); window 0 means no window (every
+ * j <= p).  Keys that no row of a call sees are never loaded, nor are the
+ * block-table entries of pages that hold none (such an entry may be -1 or name
+ * a page that was given away), and whatever a masked slot holds, NaN and
+ * infinities included, reaches no output.
+ *
+ * Sums: a cache cut by weight has two pools beside K and V, through the same
+ * block tables: weights, fp32 [Hkv][num_pages][16], the attention weight that
+ * each slot's key has received, summed over the query heads of its KV head;
+ * and ages, int32 [Hkv][num_pages][16] (may be NULL throughout), the position
+ * in the text of the token in a slot, which is the slot's own index until an
+ * eviction first moves tokens.  `newest` (device int32[batch], NULL: seq_lens[b] - 1)
+ * is the text position of each sequence's last key.  The last `new_keys` keys
+ * of a sequence are new to the sums: their weight starts from zero, whatever
+ * the slot held, and their age is set.  Block-table ids outside
+ * [0, num_pages) are clamped for reads of K and V as everywhere, and drop
+ * writes of sums.  A page belongs to one sequence: a page that several rows of
+ * a block table name (a shared prefix) must not be given sums or evicted.
+ *
+ * Lengths above max_seq_len (or the block table's reach) count as that, and
+ * sequences of length <= 0 have no keys.  Every call is asynchronous on
+ * `stream`, allocates nothing and may be captured; where a call takes a
+ * workspace, it must be 16-byte aligned and hold *_workspace_bytes bytes (0:
+ * NULL is fine), and calls that overlap need one each.  fp16 tensors, head_dim
+ * 1..256; the fast kernels take head_dim 64 and 128, 16-byte aligned tensors
+ * and rows, and one block table for K and V.  Sums of scores, softmax states
+ * and weights are fp32. */
+
+/* One new token per sequence, at position seq_lens[b] - 1: as
+ * kvhp_decode_attention over the visible keys.  Zeros for sequences without
+ * keys. */
+size_t kvhp_window_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int max_seq_len, int window, int sinks);
+int kvhp_window_decode(const void* q, const kvhp_kv_view* k_view, const kvhp_kv_view* v_view,
+                       const int32_t* seq_lens, void* out, int batch, int num_q_heads,
+                       int num_kv_heads, int head_dim, int max_seq_len, int window, int sinks,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows of a prompt, or of a chunk behind cached keys: row r of sequence b
+ * (q, out [batch][rows][Hq][D]) is at position q_start[b] + r (device int32,
+ * NULL: 0) and attends its visible keys among the views' first seq_lens[b]
+ * (device int32, NULL: max_seq_len), which hold the rows' own K/V too.  A
+ * prompt's token-major k, v [batch][S][Hkv][D] are strided views (stride_b =
+ * S Hkv D, stride_h = D, stride_s = Hkv D).  Rows at negative positions or at
+ * or past seq_lens[b] are padding: their out and lse stay as they were.
+ * lse (may be NULL): fp32 [batch][Hq][rows], the natural logarithm of the sum
+ * over a row's visible keys of exp(q.k / sqrt(D)). */
+size_t kvhp_window_prefill_workspace_bytes(int batch, int rows, int num_q_heads,
+                                           int num_kv_heads, int head_dim, int max_seq_len,
+                                           int window, int sinks);
+int kvhp_window_prefill(const void* q, const kvhp_kv_view* k_view, const kvhp_kv_view* v_view,
+                        const int32_t* q_start, const int32_t* seq_lens, void* out, float* lse,
+                        int batch, int rows, int num_q_heads, int num_kv_heads, int head_dim,
+                        int max_seq_len, int window, int sinks, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* kvhp_decode_attention that also adds each key's attention weight to its
+ * slot's sum (paged views only, else KVHP_ERR_UNSUPPORTED). */
+size_t kvhp_weighted_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
+                                            int head_dim, int max_seq_len);
+int kvhp_weighted_decode(const void* q, const kvhp_kv_view* k_view, const kvhp_kv_view* v_view,
+                         const int32_t* seq_lens, const int32_t* newest, void* out,
+                         float* weights, int32_t* ages, int batch, int num_q_heads,
+                         int num_kv_heads, int head_dim, int max_seq_len, int new_keys,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for rows of a prompt: adds to key j's slot the sum, over the rows
+ * of its sequence that see it and over the query heads of its KV head, of
+ * exp(q.k_j / sqrt(D) - lse), q and lse as kvhp_window_prefill takes and leaves
+ * them for these rows, window and sinks.  Passing only a prompt's last rows lets those say which
+ * keys matter.  Keys that no row sees add nothing (new keys among them start
+ * at zero).  Paged K view. */
+size_t kvhp_prompt_weights_workspace_bytes(int batch, int rows, int num_q_heads,
+                                           int num_kv_heads, int head_dim, int max_seq_len);
+int kvhp_prompt_weights(const void* q, const kvhp_kv_view* k_view, const float* lse,
+                        const int32_t* q_start, const int32_t* seq_lens, const int32_t* newest,
+                        float* weights, int32_t* ages, int batch, int rows, int num_q_heads,
+                        int num_kv_heads, int head_dim, int max_seq_len, int window, int sinks,
+                        int new_keys, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which slots stay when every sequence longer than `budget` is cut to it, for
+ * each KV head by itself, and the moves that bring them into the first
+ * `budget` slots.  Kept are, in this order: slots whose age is below `sinks`
+ * or above newest - recent; then the largest weights (a NaN counts as the
+ * smallest); among equals the lowest slot.  sinks + recent <= budget.  The
+ * evicted slots below `budget` and the kept ones at or past it, both in
+ * ascending order, are paired: moves [batch][Hkv][max_moves][2] int32 gets
+ * (from, to) slots, counts [batch][Hkv] int32 how many (entries past them are
+ * left as they were).  new_lens[b] = min(seq_lens[b], budget), which must not
+ * alias seq_lens.  max_moves must hold min(budget, max_seq_len - budget).
+ * seq_lens, newest, weights, ages and the pools are only read. */
+int kvhp_evict_plan(const float* weights, const int32_t* ages, const int32_t* block_tables,
+                    int max_pages, const int32_t* seq_lens, const int32_t* newest,
+                    int32_t* moves, int32_t* counts, int32_t* new_lens, int batch,
+                    int num_kv_heads, int num_pages, int max_seq_len, int budget, int sinks,
+                    int recent, int max_moves, void* stream);
+/* The moves, in place: K and V rows (pools [Hkv][num_pages][16][D]), weights
+ * and ages (each may be NULL) of slot `from` are copied to slot `to`; sources
+ * stay as they are, so applying a plan again changes nothing.  Moves whose
+ * slots lie outside the block table or whose page ids lie outside the pool are
+ * dropped.  Afterwards the pages past new_lens[b] are free. */
+int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int32_t* ages,
+                     const int32_t* block_tables, int max_pages, const int32_t* moves,
+                     const int32_t* counts, int batch, int num_kv_heads, int head_dim,
+                     int num_pages, int max_moves, void* stream);
+
 /* ---- Model operators around the KV-cache path (decoder-only model,
  * batch-1 decode).  fp16 tensors row-major; W [N][K] is the PyTorch linear
  * weight layout the reference uses (src/cuda/kernels.h:178-192). ---------- */

@@ -88,6 +88,26 @@ _SIGNATURES = {
     "kvhp_flash_prefill_paged": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp,
                                         _vp, _vp, _i32, _i32, _vp]),
     "kvhp_causal_gqa": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    # caches of bounded length
+    "kvhp_window_decode_workspace_bytes": (_sz, [_i32] * 7),
+    "kvhp_window_decode": (_i32, [_vp, ctypes.POINTER(KVView), ctypes.POINTER(KVView), _vp, _vp,
+                                  _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "kvhp_window_prefill_workspace_bytes": (_sz, [_i32] * 8),
+    "kvhp_window_prefill": (_i32, [_vp, ctypes.POINTER(KVView), ctypes.POINTER(KVView), _vp, _vp,
+                                   _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp,
+                                   _sz, _vp]),
+    "kvhp_weighted_decode_workspace_bytes": (_sz, [_i32] * 5),
+    "kvhp_weighted_decode": (_i32, [_vp, ctypes.POINTER(KVView), ctypes.POINTER(KVView), _vp, _vp,
+                                    _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz,
+                                    _vp]),
+    "kvhp_prompt_weights_workspace_bytes": (_sz, [_i32] * 6),
+    "kvhp_prompt_weights": (_i32, [_vp, ctypes.POINTER(KVView), _vp, _vp, _vp, _vp, _vp, _vp,
+                                   _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp,
+                                   _sz, _vp]),
+    "kvhp_evict_plan": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                               _i32, _i32, _i32, _i32, _i32, _vp]),
+    "kvhp_evict_apply": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
+                                _i32, _vp]),
     # model operators
     "kvhp_gemv": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
     "kvhp_gemv_residual": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _vp]),
@@ -395,6 +415,102 @@ def flash_prefill_paged(q, k, v, out, seq_len, num_q_heads, num_kv_heads, head_d
 def causal_gqa(q, k, v, out, seq_len, num_q_heads, num_kv_heads, head_dim, stream=None):
     _check(load().kvhp_causal_gqa(_ptr(q), _ptr(k), _ptr(v), _ptr(out), seq_len, num_q_heads,
                                   num_kv_heads, head_dim, _stream(stream)))
+
+
+# --------------------------------------------- caches of bounded length --
+def _bytes(ws) -> int:
+    return 0 if ws is None else ws.numel() * ws.element_size()
+
+
+def window_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len,
+                                  window, sinks=0) -> int:
+    return load().kvhp_window_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim,
+                                                     max_seq_len, window, sinks)
+
+
+def window_decode(q, k_view: KVView, v_view: KVView, seq_lens, out, num_q_heads, num_kv_heads,
+                  head_dim, max_seq_len, window, sinks=0, workspace=None, stream=None):
+    """decode_attention over each sequence's last `window` keys and its first
+    `sinks` ones (window 0: every key); workspace: a tensor of
+    window_decode_workspace_bytes bytes."""
+    _check(load().kvhp_window_decode(
+        _ptr(q), ctypes.byref(k_view), ctypes.byref(v_view), _ptr(seq_lens), _ptr(out),
+        seq_lens.shape[0], num_q_heads, num_kv_heads, head_dim, max_seq_len, window, sinks,
+        _ptr(workspace), _bytes(workspace), _stream(stream)))
+
+
+def window_prefill_workspace_bytes(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len,
+                                   window, sinks=0) -> int:
+    return load().kvhp_window_prefill_workspace_bytes(batch, rows, num_q_heads, num_kv_heads,
+                                                      head_dim, max_seq_len, window, sinks)
+
+
+def window_prefill(q, k_view: KVView, v_view: KVView, out, num_q_heads, num_kv_heads, head_dim,
+                   max_seq_len, window, sinks=0, q_start=None, seq_lens=None, lse=None,
+                   workspace=None, stream=None):
+    """Rows q [B][rows][Hq][D] at positions q_start[b] + r over the views' first
+    seq_lens[b] keys; out as q, lse fp32 [B][Hq][rows] (optional); padding rows
+    are left as they were."""
+    _check(load().kvhp_window_prefill(
+        _ptr(q), ctypes.byref(k_view), ctypes.byref(v_view), _ptr(q_start), _ptr(seq_lens),
+        _ptr(out), _ptr(lse), q.shape[0], q.shape[1], num_q_heads, num_kv_heads, head_dim,
+        max_seq_len, window, sinks, _ptr(workspace), _bytes(workspace), _stream(stream)))
+
+
+def weighted_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim,
+                                    max_seq_len) -> int:
+    return load().kvhp_weighted_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim,
+                                                       max_seq_len)
+
+
+def weighted_decode(q, k_view: KVView, v_view: KVView, seq_lens, out, weights, num_q_heads,
+                    num_kv_heads, head_dim, max_seq_len, new_keys=1, ages=None, newest=None,
+                    workspace=None, stream=None):
+    """decode_attention that adds every key's attention weight, summed over its
+    KV head's query heads, to its slot of weights (fp32 [Hkv][P][16]); the last
+    new_keys keys start from zero and get their age (int32 [Hkv][P][16])."""
+    _check(load().kvhp_weighted_decode(
+        _ptr(q), ctypes.byref(k_view), ctypes.byref(v_view), _ptr(seq_lens), _ptr(newest),
+        _ptr(out), _ptr(weights), _ptr(ages), seq_lens.shape[0], num_q_heads, num_kv_heads,
+        head_dim, max_seq_len, new_keys, _ptr(workspace), _bytes(workspace), _stream(stream)))
+
+
+def prompt_weights_workspace_bytes(batch, rows, num_q_heads, num_kv_heads, head_dim,
+                                   max_seq_len) -> int:
+    return load().kvhp_prompt_weights_workspace_bytes(batch, rows, num_q_heads, num_kv_heads,
+                                                      head_dim, max_seq_len)
+
+
+def prompt_weights(q, k_view: KVView, lse, weights, num_q_heads, num_kv_heads, head_dim,
+                   max_seq_len, new_keys, window=0, sinks=0, q_start=None, seq_lens=None,
+                   ages=None, newest=None, workspace=None, stream=None):
+    """Adds to weights the attention that the rows q [B][rows][Hq][D] give each
+    key, from the lse that window_prefill left for them."""
+    _check(load().kvhp_prompt_weights(
+        _ptr(q), ctypes.byref(k_view), _ptr(lse), _ptr(q_start), _ptr(seq_lens), _ptr(newest),
+        _ptr(weights), _ptr(ages), q.shape[0], q.shape[1], num_q_heads, num_kv_heads, head_dim,
+        max_seq_len, window, sinks, new_keys, _ptr(workspace), _bytes(workspace),
+        _stream(stream)))
+
+
+def evict_plan(weights, ages, block_tables, seq_lens, moves, counts, new_lens, max_seq_len,
+               budget, sinks=0, recent=0, newest=None, stream=None):
+    """The moves [B][Hkv][max_moves][2], counts [B][Hkv] and new_lens [B] that cut
+    each sequence to its budget of slots (weights, ages: [Hkv][P][16])."""
+    _check(load().kvhp_evict_plan(
+        _ptr(weights), _ptr(ages), _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens),
+        _ptr(newest), _ptr(moves), _ptr(counts), _ptr(new_lens), seq_lens.shape[0],
+        weights.shape[0], weights.shape[1], max_seq_len, budget, sinks, recent, moves.shape[2],
+        _stream(stream)))
+
+
+def evict_apply(pool_k, pool_v, weights, ages, block_tables, moves, counts, stream=None):
+    """Carries out evict_plan's moves on pools [Hkv][P][16][D] and on the sums."""
+    hkv, pages, _, d = pool_k.shape
+    _check(load().kvhp_evict_apply(
+        _ptr(pool_k), _ptr(pool_v), _ptr(weights), _ptr(ages), _ptr(block_tables),
+        block_tables.shape[1], _ptr(moves), _ptr(counts), counts.shape[0], hkv, d, pages,
+        moves.shape[2], _stream(stream)))
 
 
 # ------------------------------------------------------ model operators --
