@@ -39,7 +39,8 @@ struct BoundArgs {
     int32_t* ages;            // [Hkv][num_pages][16] or NULL
     const int32_t* newest;    // NULL: the length - 1
     int rows, Hq, Hkv, G, D;
-    int cap;                  // keys addressable per sequence
+    int cap;                  // keys addressable per sequence ...
+    int max_len;              // ... and the call's limit, which plans and workspaces go by
     int window, sinks;        // window 0: none
     int new_keys;
     int last_row;             // 1: decode, the one row is the last key's
@@ -97,5 +98,12 @@ inline bool bound_one_table(const kvhp_kv_view& k, const kvhp_kv_view& v) {
     return k.block_table == v.block_table &&
            (!k.block_table || (k.max_pages == v.max_pages && k.num_pages == v.num_pages));
 }
+
+// bounded_decode.hip: one token per sequence at D = 64 and 128, with the sums
+// (paged views) or with a window.
+size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int window, int sinks,
+                              bool sums);
+bool bound_decode_fits(const BoundArgs& a, int batch);
+int bound_decode(const BoundArgs& a, int batch, bool paged, bool sums, void* ws, hipStream_t s);
 
 }  // namespace kvhp

@@ -36,7 +36,7 @@ int bound_shapes(BoundArgs& a, const char* what, int batch, int hq, int hkv, int
     a.Hkv = hkv;
     a.G = hq / hkv;
     a.D = d;
-    a.cap = max_seq_len;
+    a.cap = a.max_len = max_seq_len;
     a.window = window;
     a.sinks = window > 0 ? sinks : 0;   // without a window every key is visible anyway
     a.scale_log2 = kLog2e / std::sqrt(static_cast<float>(d));
@@ -195,7 +195,8 @@ using namespace kvhp;
 extern "C" size_t kvhp_window_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
                                                      int head_dim, int max_seq_len, int window,
                                                      int sinks) {
-    return 0;
+    return bound_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len, window,
+                                  sinks, false);
 }
 
 extern "C" int kvhp_window_decode(const void* q, const kvhp_kv_view* k_view,
@@ -220,15 +221,22 @@ extern "C" int kvhp_window_decode(const void* q, const kvhp_kv_view* k_view,
                          kvhp_window_decode_workspace_bytes(batch, num_q_heads, num_kv_heads,
                                                             head_dim, max_seq_len, window, sinks));
     if (rc) return rc;
-    return launch_rows(a, batch, k_view->block_table != nullptr, what,
-                       static_cast<hipStream_t>(stream));
+    const bool paged = k_view->block_table != nullptr;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (aligned16(q) && aligned16(out) && bound_fast_view(*k_view) && bound_fast_view(*v_view) &&
+        bound_one_table(*k_view, *v_view) && bound_decode_fits(a, batch))
+        return bound_decode(a, batch, paged, false, workspace, s);
+    return launch_rows(a, batch, paged, what, s);
 }
 
 extern "C" size_t kvhp_weighted_decode_workspace_bytes(int batch, int num_q_heads,
                                                        int num_kv_heads, int head_dim,
                                                        int max_seq_len) {
     if (batch <= 0 || num_q_heads <= 0 || max_seq_len <= 0) return 0;
-    return sizeof(float) * (size_t)batch * num_q_heads;   // each head's log-sum-exp
+    // other shapes leave each head's log-sum-exp
+    return std::max(sizeof(float) * (size_t)batch * num_q_heads,
+                    bound_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim,
+                                           max_seq_len, 0, 0, true));
 }
 
 extern "C" int kvhp_weighted_decode(const void* q, const kvhp_kv_view* k_view,
@@ -258,8 +266,11 @@ extern "C" int kvhp_weighted_decode(const void* q, const kvhp_kv_view* k_view,
                          kvhp_weighted_decode_workspace_bytes(batch, num_q_heads, num_kv_heads,
                                                               head_dim, max_seq_len));
     if (rc) return rc;
-    a.lse = static_cast<float*>(workspace);
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (aligned16(q) && aligned16(out) && bound_fast_view(*k_view) && bound_fast_view(*v_view) &&
+        bound_one_table(*k_view, *v_view) && bound_decode_fits(a, batch))
+        return bound_decode(a, batch, true, true, workspace, s);
+    a.lse = static_cast<float*>(workspace);
     rc = launch_rows(a, batch, true, what, s);
     return rc ? rc : launch_weights(a, batch, what, s);
 }
