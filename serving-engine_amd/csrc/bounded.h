@@ -105,5 +105,10 @@ size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int wi
                               bool sums);
 bool bound_decode_fits(const BoundArgs& a, int batch);
 int bound_decode(const BoundArgs& a, int batch, bool paged, bool sums, void* ws, hipStream_t s);
+// window_prefill.hip: rows at D = 64 and 128.
+size_t window_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int max_len,
+                                int window, int sinks);
+bool window_prefill_fits(const BoundArgs& a, int batch);
+int window_prefill(const BoundArgs& a, int batch, bool paged, void* ws, hipStream_t s);
 
 }  // namespace kvhp

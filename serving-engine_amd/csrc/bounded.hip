@@ -196,7 +196,7 @@ extern "C" size_t kvhp_window_decode_workspace_bytes(int batch, int num_q_heads,
                                                      int head_dim, int max_seq_len, int window,
                                                      int sinks) {
     return bound_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len, window,
-                                  sinks, false);
+                                  window > 0 ? sinks : 0, false);
 }
 
 extern "C" int kvhp_window_decode(const void* q, const kvhp_kv_view* k_view,
@@ -278,7 +278,8 @@ extern "C" int kvhp_weighted_decode(const void* q, const kvhp_kv_view* k_view,
 extern "C" size_t kvhp_window_prefill_workspace_bytes(int batch, int rows, int num_q_heads,
                                                       int num_kv_heads, int head_dim,
                                                       int max_seq_len, int window, int sinks) {
-    return 0;
+    return window_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len,
+                                    window, window > 0 ? sinks : 0);
 }
 
 extern "C" int kvhp_window_prefill(const void* q, const kvhp_kv_view* k_view,
@@ -306,8 +307,12 @@ extern "C" int kvhp_window_prefill(const void* q, const kvhp_kv_view* k_view,
                                                              num_kv_heads, head_dim, max_seq_len,
                                                              window, sinks));
     if (rc) return rc;
-    return launch_rows(a, batch, k_view->block_table != nullptr, what,
-                       static_cast<hipStream_t>(stream));
+    const bool paged = k_view->block_table != nullptr;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (aligned16(q) && aligned16(out) && bound_fast_view(*k_view) && bound_fast_view(*v_view) &&
+        bound_one_table(*k_view, *v_view) && window_prefill_fits(a, batch))
+        return window_prefill(a, batch, paged, workspace, s);
+    return launch_rows(a, batch, paged, what, s);
 }
 
 extern "C" size_t kvhp_prompt_weights_workspace_bytes(int batch, int rows, int num_q_heads,
