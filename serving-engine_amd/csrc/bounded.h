@@ -110,5 +110,9 @@ size_t window_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int
                                 int window, int sinks);
 bool window_prefill_fits(const BoundArgs& a, int batch);
 int window_prefill(const BoundArgs& a, int batch, bool paged, void* ws, hipStream_t s);
+// prompt_weights.hip: the sums of rows at D = 64 and 128 (paged K).
+size_t prompt_weights_workspace(int batch, int rows, int hq, int hkv, int d, int max_len);
+bool prompt_weights_fits(const BoundArgs& a, int batch);
+int prompt_weights(const BoundArgs& a, int batch, void* ws, hipStream_t s);
 
 }  // namespace kvhp

@@ -115,6 +115,15 @@ __global__ void __launch_bounds__(kWave) bound_weights_kernel(const BoundArgs a)
     const int n = bound_len(a, b);
     if (j >= n) return;
     const int64_t first = bound_first(a, b, n);
+    // rows at positions j .. last that see key j
+    int64_t last = min(first + a.rows, (int64_t)n) - 1;
+    if (a.window > 0 && j >= a.sinks) last = min(last, (int64_t)j + a.window - 1);
+    // a key that none sees is not touched (its page may be another's by now), a new one
+    // starts at zero
+    if (max(max(first, (int64_t)0), (int64_t)j) > last) {
+        if (lane == 0 && (int64_t)j + a.new_keys >= n) bound_add(a, b, kvh, j, n, 0.f);
+        return;
+    }
     const f16* kr = a.k.data + kvh * a.k.stride_h + bound_row<true>(a.k, b, j) * a.k.stride_s;
     float kv[4];
 #pragma unroll
@@ -122,9 +131,6 @@ __global__ void __launch_bounds__(kWave) bound_weights_kernel(const BoundArgs a)
         const int d = lane + kWave * i;
         kv[i] = d < D ? static_cast<float>(kr[d * a.k.stride_d]) : 0.f;
     }
-    // rows at positions j .. last that see key j
-    int64_t last = min(first + a.rows, (int64_t)n) - 1;
-    if (a.window > 0 && j >= a.sinks) last = min(last, (int64_t)j + a.window - 1);
     float w = 0.f;
     for (int64_t p = max(first, (int64_t)j); p <= last; ++p) {
         const int64_t r = p - first;
@@ -318,7 +324,7 @@ extern "C" int kvhp_window_prefill(const void* q, const kvhp_kv_view* k_view,
 extern "C" size_t kvhp_prompt_weights_workspace_bytes(int batch, int rows, int num_q_heads,
                                                       int num_kv_heads, int head_dim,
                                                       int max_seq_len) {
-    return 0;
+    return prompt_weights_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
 }
 
 extern "C" int kvhp_prompt_weights(const void* q, const kvhp_kv_view* k_view, const float* lse,
@@ -350,5 +356,8 @@ extern "C" int kvhp_prompt_weights(const void* q, const kvhp_kv_view* k_view, co
                          kvhp_prompt_weights_workspace_bytes(batch, rows, num_q_heads,
                                                              num_kv_heads, head_dim, max_seq_len));
     if (rc) return rc;
-    return launch_weights(a, batch, what, static_cast<hipStream_t>(stream));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (aligned16(q) && bound_fast_view(*k_view) && prompt_weights_fits(a, batch))
+        return prompt_weights(a, batch, workspace, s);
+    return launch_weights(a, batch, what, s);
 }
