@@ -266,7 +266,7 @@ int kvhp_causal_gqa(const void* q, const void* k, const void* v, void* out,
  * each slot's key has received, summed over the query heads of its KV head;
  * and ages, int32 [Hkv][num_pages][16] (may be NULL throughout), the position
  * in the text of the token in a slot, which is the slot's own index until an
- * eviction first moves tokens.  `newest` (device int32[batch], NULL: seq_lens[b] - 1)
+ * eviction first moves tokens; both pools 16-byte aligned.  `newest` (device int32[batch], NULL: seq_lens[b] - 1)
  * is the text position of each sequence's last key.  The last `new_keys` keys
  * of a sequence are new to the sums: their weight starts from zero, whatever
  * the slot held, and their age is set.  Block-table ids outside
@@ -355,7 +355,8 @@ int kvhp_evict_plan(const float* weights, const int32_t* ages, const int32_t* bl
  * and ages (each may be NULL) of slot `from` are copied to slot `to`; sources
  * stay as they are, so applying a plan again changes nothing.  Moves whose
  * slots lie outside the block table or whose page ids lie outside the pool are
- * dropped.  Afterwards the pages past new_lens[b] are free. */
+ * dropped.  moves must be 8-byte aligned.  Afterwards the pages past
+ * new_lens[b] are free. */
 int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int32_t* ages,
                      const int32_t* block_tables, int max_pages, const int32_t* moves,
                      const int32_t* counts, int batch, int num_kv_heads, int head_dim,

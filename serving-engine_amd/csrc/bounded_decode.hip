@@ -42,12 +42,17 @@ struct DecodePlan {
     int balance;      // > 0: about this many splits per KV head over the batch
     int min_chunk, max_chunk;
     int groups;       // workgroups per KV head and split, of up to kHeads query heads
-    int scap;         // pitch of the scores
+    int scap;         // keys that the scores have room for, a multiple of 32
     float* ws_o;      // [B * Hq][nsplit][D]
     float* ws_ml;     // [B * Hq][nsplit][2], the maximum in log2 units
-    float* ws_s;      // [B * Hq][scap] raw scores
+    float* ws_s;      // [B][Hkv][scap / 32][G][32] raw scores
 };
 
+// Where the scores of the 32 keys from j (a multiple of 32) on lie: [head of the group][32].
+__device__ __forceinline__ int64_t score_at(const BoundArgs& a, const DecodePlan& p, int b,
+                                            int kvh, int j) {
+    return (((int64_t)b * a.Hkv + kvh) * p.scap + j) * a.G;
+}
 // Visible keys of sequence b.
 __device__ __forceinline__ int vis_len(const BoundArgs& a, int b) {
     const int n = bound_len(a, b);
@@ -68,7 +73,7 @@ __device__ __forceinline__ int chunk_of(const DecodePlan& p, int L, long long ke
     const int target = static_cast<int>(
         min(max((keys + p.balance - 1) / p.balance, (long long)p.min_chunk), (long long)p.max_chunk));
     const int n = min((L + target - 1) / target, p.nsplit);
-    return ((L + n - 1) / n + 15) / 16 * 16;   // at most max_chunk, a multiple of 16
+    return ((L + n - 1) / n + 31) / 32 * 32;   // at most max_chunk; whole steps
 }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
@@ -85,7 +90,8 @@ __device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
 }
 
 // W waves per workgroup take the steps of one split round robin and meet in LDS.
-template <int D, bool PAGED, bool SUMS, int W>
+// WIDE: rows may lie 2^32 bytes and more behind their head's first.
+template <int D, bool PAGED, bool SUMS, int W, bool WIDE = false>
 __global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
     constexpr int TOK = 32, NC = D / 32, ND = D / 16;
@@ -180,7 +186,8 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
         qb[c] = hvalid ? load_half8(a.q + (row0 + col) * D + 32 * c + 8 * g) : half8{};
 
     const int vrow = lane / LPR, vdim = 8 * (lane % LPR);
-    const uint64_t ssk = 2 * (uint64_t)a.k.stride_s, ssv = 2 * (uint64_t)a.v.stride_s;
+    using offset = std::conditional_t<WIDE, uint64_t, uint32_t>;
+    const offset ssk = 2 * (offset)a.k.stride_s, ssv = 2 * (offset)a.v.stride_s;
 
     // This lane's row of load j of the step at T0; past the split's last key: that one.
     auto rows = [&](int T0, uint32_t (&r)[NVL]) {
@@ -205,14 +212,14 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
 #pragma unroll
         for (int j = 0; j < NVL; ++j)
             kbuf[S][j] = load_half8_stream(
-                reinterpret_cast<const f16*>(kbase + r[j] * ssk) + vdim);
+                reinterpret_cast<const f16*>(kbase + ((offset)r[j] * ssk + 2u * vdim)));
     };
     auto load_v = [&](int T0) {
         uint32_t r[NVL];
         rows(T0, r);
 #pragma unroll
         for (int j = 0; j < NVL; ++j)
-            vbuf[j] = load_half8_stream(reinterpret_cast<const f16*>(vbase + r[j] * ssv) + vdim);
+            vbuf[j] = load_half8_stream(reinterpret_cast<const f16*>(vbase + ((offset)r[j] * ssv + 2u * vdim)));
     };
 
     float m_run = -1e30f, l_part = 0.f;
@@ -241,13 +248,12 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
             }
         }
         if constexpr (SUMS) {
-            // four keys of a head; the chunk ends at a multiple of 16 or with the
-            // sequence, behind which a pitch of scap leaves room
-            float* ss = p.ws_s + (row0 + col) * p.scap + T0 + 4 * g;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (hvalid && T0 + 16 * t + 4 * g < t_end)
-                    *reinterpret_cast<floatx4*>(ss + 16 * t) = C[t];
+            // the step's scores of a head, 128 bytes; the heads of a KV head side by side
+            float* ss = p.ws_s + score_at(a, p, b, kvh, T0) + 32 * (h0 + col) + 4 * g;
+            if (hvalid) {
+                *reinterpret_cast<floatx4*>(ss) = C[0];
+                *reinterpret_cast<floatx4*>(ss + 16) = C[1];
+            }
         }
         const bool tail = T0 + TOK > t_end;
         if (tail) {
@@ -484,43 +490,58 @@ bound_sums_kernel(const BoundArgs a, const DecodePlan p, int key_blocks) {
         if (nsb > 1) join_head<D>(a, p, row0 + at - key_blocks, nsb);
         return;
     }
+    // Four keys a thread.  Their scores, page id and sums are on their way before the
+    // heads' maxima and sums are folded (one memory round trip instead of three: 5.7 to
+    // 4.7 us at 2048 keys).
     const int j = at * kSumKeys + 4 * tid;
-    floatx4 w = {0.f, 0.f, 0.f, 0.f};
-    __shared__ float head[kHeads][2];   // -M in log2 units, 1 / sum
-    for (int g0 = 0; g0 < a.G; g0 += kHeads) {
-        const int gn = min(a.G - g0, kHeads);
-        for (int g = wave; g < gn; g += kJoinWaves) {
-            const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + (row0 + g0 + g) * p.nsplit;
-            float M = -3.0e38f, S = 0.f;
-            for (int i = lane; i < nsb; i += kWave) {
-                const float2 x = ml[i];
-                const float mn = fmaxf(M, x.x);
-                S = S * fast_exp2(M - mn) + x.y * fast_exp2(x.x - mn);
+    const int jc = min(j, n - 1) & ~3;
+    const float* sj = p.ws_s + score_at(a, p, b, kvh, jc & ~31) + (jc & 31);
+    const int64_t slot = bound_slot(a.k, b, kvh, jc);   // of four in one page
+    floatx4 old = {0.f, 0.f, 0.f, 0.f}, w = old;
+    if (slot >= 0) old = *reinterpret_cast<const floatx4*>(a.weights + slot);
+    constexpr int H = 8, HW = H / kJoinWaves;   // heads at a time, and per wave
+    __shared__ float head[H][2];                // -M in log2 units, 1 / sum
+    for (int g0 = 0; g0 < a.G; g0 += H) {
+        const int gn = min(a.G - g0, H);
+        floatx4 s[H];
+#pragma unroll
+        for (int g = 0; g < H; ++g)
+            s[g] = *reinterpret_cast<const floatx4*>(sj + 32 * (g0 + min(g, gn - 1)));
+        float2 x[HW];
+        const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + (row0 + g0) * p.nsplit;
+#pragma unroll
+        for (int i = 0; i < HW; ++i)
+            x[i] = ml[(int64_t)min(wave + i * kJoinWaves, gn - 1) * p.nsplit + min(lane, nsb - 1)];
+#pragma unroll
+        for (int i = 0; i < HW; ++i) {
+            const int g = wave + i * kJoinWaves;
+            if (g >= gn) continue;
+            float M = lane < nsb ? x[i].x : -3.0e38f, S = lane < nsb ? x[i].y : 0.f;
+            for (int t = lane + kWave; t < nsb; t += kWave) {
+                const float2 y = ml[(int64_t)g * p.nsplit + t];
+                const float mn = fmaxf(M, y.x);
+                S = S * fast_exp2(M - mn) + y.y * fast_exp2(y.x - mn);
                 M = mn;
             }
-            const float mx = wave_max(M);
-            S = wave_sum(S * fast_exp2(M - mx));
+            const float mx = wave_max_fast(M);
+            S = wave_sum_fast(S * fast_exp2(M - mx));
             if (lane == 0) {
                 head[g][0] = -mx;
                 head[g][1] = 1.f / S;
             }
         }
         __syncthreads();
-        if (j < n)
-            for (int g = 0; g < gn; ++g) {
-                const floatx4 s = *reinterpret_cast<const floatx4*>(
-                    p.ws_s + (row0 + g0 + g) * p.scap + j);
-                const float nm = head[g][0], inv = head[g][1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = fmaf(fast_exp2(fmaf(s[e], a.scale_log2, nm)), inv, w[e]);
-            }
+        for (int g = 0; g < H; ++g) {
+            if (g >= gn) break;
+            const float nm = head[g][0], inv = head[g][1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = fmaf(fast_exp2(fmaf(s[g][e], a.scale_log2, nm)), inv, w[e]);
+        }
         __syncthreads();
     }
-    if (j >= n) return;
-    const int64_t slot = bound_slot(a.k, b, kvh, j);   // of four in one page
-    if (slot < 0) return;
-    floatx4 old = *reinterpret_cast<const floatx4*>(a.weights + slot);
+    if (j >= n || slot < 0) return;
     const int64_t fresh = (int64_t)n - a.new_keys;     // keys from here on start anew
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -535,16 +556,19 @@ bound_sums_kernel(const BoundArgs a, const DecodePlan p, int key_blocks) {
 }
 
 // ------------------------------------------------------------------ plan --
-DecodePlan plan_of(int batch, int hkv, int G, int64_t maxv) {
+DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv) {
     DecodePlan p{};
     p.batch = batch;
     p.groups = (G + kHeads - 1) / kHeads;
     const int64_t units = (int64_t)batch * hkv * p.groups;
     const int64_t per = std::max<int64_t>(64, ((maxv + 63) / 64 + 63) / 64 * 64);
     int64_t s = std::min((maxv + per - 1) / per, units >= 6144 ? 1 : 6144 / units);
-    if (batch < 8 && maxv <= 512) s = 1;
-    int64_t chunk = ((maxv + s - 1) / s + 63) / 64 * 64;
-    chunk = std::min<int64_t>(chunk, kMaxChunk);
+    int64_t chunk = std::min<int64_t>(((maxv + s - 1) / s + 63) / 64 * 64, kMaxChunk);
+    // Up to 640 keys (192 at D = 128) a small batch takes one split: eight waves share its
+    // steps, and no second launch joins.  One sequence, 32/8 heads, us as one split / as
+    // splits of 64 keys: D = 64 300 keys 5.5 / 7.4, 700 7.2 / 7.4, 1024 8.6 / 7.5; D = 128
+    // 300 8.8 / 8.3.
+    if (batch < 8 && maxv <= (d == 64 ? 640 : 192)) chunk = (maxv + 31) / 32 * 32;
     p.chunk = static_cast<int>(chunk);
     p.nsplit = static_cast<int>((maxv + chunk - 1) / chunk);
     p.min_chunk = batch >= 16 ? 64 : 128;
@@ -565,7 +589,7 @@ size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int wi
                               bool sums) {
     if (batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || cap <= 0 || (d != 64 && d != 128))
         return 0;
-    const DecodePlan p = plan_of(batch, hkv, hq / hkv, most_visible(cap, window, sinks));
+    const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks));
     const size_t rows = (size_t)batch * hq;
     size_t n = p.nsplit > 1 || sums ? rows * p.nsplit * 2 : 0;
     if (p.nsplit > 1) n += rows * p.nsplit * d;
@@ -574,13 +598,15 @@ size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int wi
 }
 
 bool bound_decode_fits(const BoundArgs& a, int batch) {
-    const DecodePlan p = plan_of(batch, a.Hkv, a.G, most_visible(a.max_len, a.window, a.sinks));
+    const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, most_visible(a.max_len, a.window, a.sinks));
     return (a.D == 64 || a.D == 128) && p.nsplit <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
 }
 
 template <int D, bool PAGED, bool SUMS>
 static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s) {
     const int heads = a.Hkv * p.groups;
+    const int64_t reach = PAGED ? (int64_t)a.k.num_pages * kPage : a.cap;   // rows of a head
+    const bool wide = reach * std::max(a.k.stride_s, a.v.stride_s) >= (int64_t)1 << 31;
     dim3 grid(heads, p.nsplit, p.batch);
     if (p.batch >= 8) {
         p.balance = std::max(1, kWaveSlots / heads - p.batch / 2);
@@ -591,7 +617,14 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
         else
             p.balance = 0;
     }
-    if (p.balance == 0 && (D == 64 || p.nsplit == 1))
+    // one split: eight waves take its steps round robin; fixed splits at D = 64: four
+    // (at D = 128 four are no faster on one sequence and 26-52 % slower on four of 1024
+    // to 4000 keys)
+    if (wide)
+        hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 1, true>), grid, dim3(kWave), 0, s, a, p);
+    else if (p.balance == 0 && p.nsplit == 1)
+        hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 8>), grid, dim3(8 * kWave), 0, s, a, p);
+    else if (p.balance == 0 && D == 64)
         hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 4>), grid, dim3(4 * kWave), 0, s, a, p);
     else
         hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 1>), grid, dim3(kWave), 0, s, a, p);
@@ -610,7 +643,7 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
 // block table, 16-byte aligned.
 int bound_decode(const BoundArgs& a, int batch, bool paged, bool sums, void* ws, hipStream_t s) {
     const int64_t maxv = most_visible(a.max_len, a.window, a.sinks);
-    DecodePlan p = plan_of(batch, a.Hkv, a.G, maxv);
+    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, maxv);
     const size_t rows = (size_t)batch * a.Hq;
     p.scap = (a.max_len + 31) / 32 * 32;
     float* w = static_cast<float*>(ws);

@@ -162,6 +162,7 @@ def test_apply_arguments():
     for name in ("k", "v", "bt", "moves", "counts"):
         _refused(_apply(**{name: None}), kvhp.KVHP_ERR_INVALID, "null")
     _refused(_apply(hkv=0), kvhp.KVHP_ERR_INVALID, "positive")
+    _refused(_apply(moves=P + 4), kvhp.KVHP_ERR_INVALID, "aligned")
     _refused(_apply(d=300), kvhp.KVHP_ERR_UNSUPPORTED, "head_dim")
     _refused(_apply(batch=65536), kvhp.KVHP_ERR_UNSUPPORTED, "65535")
     assert _apply(most=0)[0] == kvhp.KVHP_OK and _apply(batch=0)[0] == kvhp.KVHP_OK
