@@ -256,10 +256,10 @@ int kvhp_causal_gqa(const void* q, const void* k, const void* v, void* out,
  *
  * Visible keys: the query at position p of its sequence attends key j when
  * j <= p and (j < sinks or p - j < window); window 0 means no window (every
- * j <= p).  Keys that no row of a call sees are never loaded, nor are the
- * block-table entries of pages that hold none (such an entry may be -1 or name
- * a page that was given away), and whatever a masked slot holds, NaN and
- * infinities included, reaches no output.
+ * j <= p).  A page that holds no key that some row of the call sees is not
+ * loaded, nor is its block-table entry (which may be -1 or name a page that was
+ * given away), and whatever a masked slot holds, NaN and infinities included,
+ * reaches no output.
  *
  * Sums: a cache cut by weight has two pools beside K and V, through the same
  * block tables: weights, fp32 [Hkv][num_pages][16], the attention weight that

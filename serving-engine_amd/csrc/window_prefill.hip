@@ -8,8 +8,10 @@
 // a chunk of a few rows still fills a wave.  With KG = 2 two wave groups take
 // the same pairs and half the keys of every tile, and join at the end.
 //
-// Keys: those that some row of the block sees, numbered through without the gap
-// between the first tokens and the earliest window: `nv` keys, 64 to a tile.
+// Keys: those that some row of the block sees, numbered through without the pages
+// between the first tokens' and the earliest window's: `nv` keys, 64 to a tile.  (The
+// gap is whole pages so that the rows of a load share a page, whose id is then
+// scalar; the rest of the two pages at its edges is masked.)
 // A block of a long prompt walks (window + sinks + its rows) / 64 tiles, all
 // blocks alike, where causal attention would walk up to S / 64.  Only tiles at the
 // window's two edges and those that hold first tokens need a mask.
@@ -20,7 +22,7 @@
 //   range, to which they are rounded for the product: 2^-11 each, over a sum of
 //   many); O^T += V^T P^T.
 // K and V rows go from memory to a ring of four LDS stages without registers
-// (global_load_lds, each lane its own row's address, page ids from LDS), two
+// (global_load_lds, a scalar base and the lane's fixed offset; page ids from LDS), two
 // tiles ahead; rows are stored with their 16-byte chunks XOR-swizzled so that
 // both operand reads touch all banks.  Waves 0-3 and 4-7, one of each per SIMD,
 // alternate a step of MFMAs and a step of exponentials.
@@ -43,6 +45,7 @@ namespace {
 
 constexpr int kBN = 64;               // keys per tile
 constexpr int kPages = 4088;          // page ids of a split held in LDS
+constexpr int kMaxStride = 1 << 24;   // halfs between rows: 15 rows stay below 2^31 bytes
 constexpr int kEdge = 6;              // tiles at either edge of the window in a block
 constexpr int kBadWords = 4 * kEdge;  // a bit per key of those
 constexpr int kCUs = 256;
@@ -60,12 +63,13 @@ __device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
 __device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
     return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-// Lane l's 16 bytes to lds_base + 16 l; only the ring's own waits order it.
-__device__ __forceinline__ void dma16(const char* src, f16* lds_base) {
+// 16 bytes from a scalar base and lane l's byte offset to lds_base + 16 l; only the
+// ring's own waits order it.
+__device__ __forceinline__ void dma16s(const char* base, uint32_t voff, f16* lds_base) {
     const uint32_t m0v = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((lds_void*)(lds_f16*)lds_base));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(m0v), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(m0v), "v"(voff), "s"(base) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -99,9 +103,10 @@ struct PrefillPlan {
 struct Block {
     int first;       // position of row 0
     int p_lo, p_hi;  // positions of the block's first and last live row; none: p_lo > p_hi
-    int sinks;       // keys in front of the gap
-    int shift;       // the gap
-    int nv;          // keys, numbered through
+    int sinks;       // first tokens that every row sees
+    int head;        // keys in front of the gap: up to the end of their page
+    int shift;       // the gap, whole pages; 0: none (head is 0 then)
+    int nv;          // keys, numbered through: v < head is key v, others key v + shift
 };
 __device__ __forceinline__ Block block_of(const BoundArgs& a, int b, int blk, int pairs) {
     Block k;
@@ -115,7 +120,9 @@ __device__ __forceinline__ Block block_of(const BoundArgs& a, int b, int blk, in
     k.p_hi = static_cast<int>(min(first + r1, (int64_t)n - 1));
     const int low = bound_low(k.p_lo, a.window);
     k.sinks = a.window > 0 ? min(a.sinks, k.p_hi + 1) : 0;
-    k.shift = max(low - k.sinks, 0);
+    k.head = (k.sinks + kPage - 1) & ~(kPage - 1);
+    k.shift = max((low & ~(kPage - 1)) - k.head, 0);
+    if (k.shift == 0) k.head = 0;
     k.nv = k.p_hi + 1 - k.shift;
     return k;
 }
@@ -158,17 +165,12 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         a.v.data + (PAGED ? 0 : b * a.v.stride_b) + kvh * a.v.stride_h);
     const uint64_t ssk = 2 * (uint64_t)a.k.stride_s, ssv = 2 * (uint64_t)a.v.stride_s;
 
-    // ---- page ids: those of this split's first tokens, then the others
-    int n_a = 0, p_a = 0, p_b = 0;
+    // ---- page ids of this split's keys, 16 to a page
     if constexpr (PAGED) {
         const int v0 = t_lo * kBN, v1 = min((t_lo + n_tiles) * kBN, k.nv);
-        const int sk = k.shift > 0 ? k.sinks : 0;
-        p_a = v0 >> 4;
-        n_a = v0 < sk ? ((min(v1, sk) - 1) >> 4) - p_a + 1 : 0;
-        p_b = (max(v0, sk) + k.shift) >> 4;
-        const int n_b = v1 > sk ? ((v1 - 1 + k.shift) >> 4) - p_b + 1 : 0;
-        for (int i = tid; i < n_a + n_b; i += NTH) {
-            const int pid = a.k.bt[(int64_t)b * a.k.max_pages + (i < n_a ? p_a + i : p_b + i - n_a)];
+        for (int i = tid; i < (v1 - v0 + kPage - 1) / kPage; i += NTH) {
+            const int v = v0 + i * kPage;
+            const int pid = a.k.bt[(int64_t)b * a.k.max_pages + ((v < k.head ? v : v + k.shift) >> 4)];
             ptab[i] = min(max(pid, 0), a.k.num_pages - 1);
         }
     }
@@ -185,37 +187,52 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
         qop[c] = live ? load_half8(a.q + at * D + 16 * c + 8 * h) : half8{};
-    // positions of the wave's first and last pair's rows, live or not (masks only)
+    // positions of the wave's first and last pair's rows, and whether all are live
     const int u_lo = k.first + static_cast<int>((((int64_t)blk * UPG + u) * 32) / a.G);
     const int u_hi = k.first + static_cast<int>((((int64_t)blk * UPG + u) * 32 + 31) / a.G);
+    const bool u_live = u_lo >= k.p_lo && u_hi <= k.p_hi;
 
-    // ---- DMA: this wave's rows (wave * IPW + i) * RPI + lane / CPR of a tile.  Tiles
-    //      past the last re-load it, so every wave issues the same loads.
-    int slot[IPW];   // the rows of the next issue
-    auto rows_of = [&](int tt) {
+    // ---- DMA: this wave's rows (wave * IPW + i) * RPI + lane / CPR of a tile, those of a
+    //      load in one page.  Tiles past the last re-load it, so every wave issues the
+    //      same loads; rows past the last key re-read it.
+    const uint32_t ssk32 = static_cast<uint32_t>(ssk), ssv32 = static_cast<uint32_t>(ssv);
+    uint32_t ko[IPW], vo[IPW];   // the lane's offsets inside the load's rows
 #pragma unroll
-        for (int i = 0; i < IPW; ++i) {
-            const int r = (wave * IPW + i) * RPI + lane / CPR;
-            const int v = min((t_lo + min(tt, last_tile)) * kBN + r, k.nv - 1);
-            const bool head = k.shift > 0 && v < k.sinks;
-            const int real = head ? v : v + k.shift;
-            if constexpr (PAGED)
-                slot[i] = ptab[(real >> 4) - (head ? p_a : p_b - n_a)] * kPage + (real & 15);
-            else
-                slot[i] = real;
-        }
+    for (int i = 0; i < IPW; ++i) {
+        const int r0 = (wave * IPW + i) * RPI, r = r0 + lane / CPR;
+        ko[i] = (r - r0) * ssk32 + 16 * ((lane % CPR) ^ kswz(r));
+        vo[i] = (r - r0) * ssv32 + 16 * ((lane % CPR) ^ vswz(r));
+    }
+    int pid_next[IPW];   // pages of the next issue, read one ahead
+    auto pages_of = [&](int tt) {
+        if constexpr (PAGED)
+#pragma unroll
+            for (int i = 0; i < IPW; ++i) {
+                const int v = min((t_lo + min(tt, last_tile)) * kBN + (wave * IPW + i) * RPI, k.nv - 1);
+                pid_next[i] = ptab[(v >> 4) - t_lo * (kBN / kPage)];
+            }
     };
     auto issue = [&](int tt) {
         f16* stg = ring + (tt % NSTAGE) * 2 * TB;
+        const int k0 = (t_lo + min(tt, last_tile)) * kBN;
 #pragma unroll
         for (int i = 0; i < IPW; ++i) {
-            const int blk_r = (wave * IPW + i) * RPI;
-            const int r = blk_r + lane / CPR;
-            const uint64_t s = static_cast<uint32_t>(slot[i]);
-            dma16(kb + s * ssk + 16 * ((lane % CPR) ^ kswz(r)), stg + blk_r * D);
-            dma16(vb + s * ssv + 16 * ((lane % CPR) ^ vswz(r)), stg + TB + blk_r * D);
+            const int r0 = (wave * IPW + i) * RPI;
+            const int v = min(k0 + r0, k.nv - 1);   // the load's first row
+            const int key = v < k.head ? v : v + k.shift;
+            int64_t row = key;
+            if constexpr (PAGED)
+                row = (int64_t)__builtin_amdgcn_readfirstlane(pid_next[i]) * kPage + (key & 15);
+            uint32_t x = ko[i], y = vo[i];
+            if (k0 + r0 + RPI > k.nv) {   // some of them lie past the last key
+                const int r = min(lane / CPR, k.nv - 1 - v);
+                x += (r - lane / CPR) * ssk32;
+                y += (r - lane / CPR) * ssv32;
+            }
+            dma16s(kb + row * (int64_t)ssk, x, stg + r0 * D);
+            dma16s(vb + row * (int64_t)ssv, y, stg + TB + r0 * D);
         }
-        rows_of(tt + 1);
+        pages_of(tt + 1);
     };
     int kro[NC], vro[NDB];
 #pragma unroll
@@ -239,7 +256,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
 
     wait_vmcnt<0>();   // q in registers before the ring: no other waits inside it
     __syncthreads();   // ptab, bad_keys
-    rows_of(0);
+    pages_of(0);
     issue(0);
     issue(1);
 
@@ -291,25 +308,26 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
     };
     auto sstep = [&](int j) {
         const int k0 = (t_lo + j) * kBN;
-        // every pair of the wave sees the whole tile: no first tokens in it that a gap
-        // follows, its last key at or before the first row, its first inside the last
-        // row's window
-        const bool whole = k0 >= k.sinks && k0 + kBN - 1 + k.shift <= u_lo &&
-                           u_hi - (k0 + k.shift) < window && u_lo >= k.p_lo && u_hi <= k.p_hi;
-        if (!whole) {
-            // element (kb2, i) is key k0 + 32 (kb2 + kgrp) + 4h + 8 (i / 4) + i % 4
-            const int v0 = k0 + 32 * kgrp + 4 * h;
+        // element (kb2, i) is key k0 + 32 (kb2 + kgrp) + 4h + 8 (i / 4) + i % 4
+        const int v0 = k0 + 32 * kgrp + 4 * h;
+        if (k0 + kBN - 1 + k.shift > u_lo || !u_live) {   // keys past some pair's row
             const int hi = live ? pos - k.shift - v0 : -1;
-            const int64_t low64 = (int64_t)pos - window - k.shift - v0;   // last key before the window
-            const int low = static_cast<int>(max(low64, (int64_t)-1));
-            const int head = k.sinks - v0;
 #pragma unroll
             for (int kb2 = 0; kb2 < NKB; ++kb2)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int e = 32 * kb2 + 8 * (i / 4) + (i % 4);
-                    if (e > hi || (e <= low && e >= head)) sc[kb2][i] = -INFINITY;
-                }
+                for (int i = 0; i < 16; ++i)
+                    sc[kb2][i] = 32 * kb2 + 8 * (i / 4) + (i % 4) > hi ? -INFINITY : sc[kb2][i];
+        }
+        if (u_hi - (k0 + k.shift) >= window && k0 + kBN > k.sinks) {   // keys that a window left
+            const int64_t left = (int64_t)pos - window - k.shift - v0;
+            const int head = k.sinks - v0;   // from it on and up to `left`
+            const uint32_t span = static_cast<uint32_t>(max(left - head + 1, (int64_t)0));
+#pragma unroll
+            for (int kb2 = 0; kb2 < NKB; ++kb2)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    sc[kb2][i] = static_cast<uint32_t>(32 * kb2 + 8 * (i / 4) + (i % 4) - head) < span
+                                     ? -INFINITY : sc[kb2][i];
         }
         float tmax = -INFINITY;
 #pragma unroll
@@ -459,11 +477,10 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
             const int e = i % (kEdge * kBN);
             const int v = (i < kEdge * kBN ? edge_lo : edge_hi) * kBN + e;
             if (v >= k.nv) continue;   // a repeated row
-            const bool head = k.shift > 0 && v < k.sinks;
-            const int key = head ? v : v + k.shift;
+            const int key = v < k.head ? v : v + k.shift;
             uint64_t s = key;
             if constexpr (PAGED)
-                s = (uint64_t)ptab[(key >> 4) - (head ? p_a : p_b - n_a)] * kPage + (key & 15);
+                s = (uint64_t)ptab[(v >> 4) - t_lo * (kBN / kPage)] * kPage + (v & 15);
             const f16* src = reinterpret_cast<const f16*>(vb + s * ssv) + 4 * h;
             const bool sees = live && key <= pos && (key < a.sinks || pos - key < window);
 #pragma unroll
@@ -582,11 +599,11 @@ PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window
     p.blocks = static_cast<int>((pairs + per - 1) / per);
     // the most keys that a block's rows see
     const int64_t block_rows = std::min<int64_t>((per + G - 1) / G + 1, rows);
-    const int64_t keys = window > 0 ? std::min<int64_t>(max_len, (int64_t)window + sinks + block_rows)
+    const int64_t keys = window > 0 ? std::min<int64_t>(max_len, (int64_t)window + sinks + block_rows + 2 * kPage)
                                     : max_len;
     const int64_t tiles = (keys + kBN - 1) / kBN;
     int64_t n = std::min<int64_t>(kCUs / wgs, tiles / 4);
-    n = std::max<int64_t>(n, (tiles * (kBN / kPage) + kPages - 13) / (kPages - 12));
+    n = std::max<int64_t>(n, (tiles * (kBN / kPage) + kPages - 5) / (kPages - 4));
     n = std::max<int64_t>(n, 1);
     p.tiles_per_split = static_cast<int>((tiles + n - 1) / n);
     p.nsplit = static_cast<int>((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
@@ -606,7 +623,9 @@ size_t window_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int
 
 bool window_prefill_fits(const BoundArgs& a, int batch) {
     const PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len, a.window, a.sinks);
-    return (a.D == 64 || a.D == 128) && p.nsplit <= 65535 && (int64_t)p.blocks * a.Hkv <= 1 << 22;
+    return (a.D == 64 || a.D == 128) && p.nsplit <= 65535 &&
+           (int64_t)p.blocks * a.Hkv <= 1 << 22 && a.k.stride_s < kMaxStride &&
+           a.v.stride_s < kMaxStride;
 }
 
 int window_prefill(const BoundArgs& a, int batch, bool paged, void* ws, hipStream_t s) {
