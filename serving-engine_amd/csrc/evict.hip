@@ -3,21 +3,27 @@
 //
 // Plan: slots rank by (protected by age, weight, lowest slot); the `budget`
 // first stay.  One workgroup of 1024 threads per (KV head, sequence).  Every
-// slot's rank is a 32-bit key whose order is that of the weights (protected:
-// all ones; NaN: zero); the budget-th largest key is found by a radix select
-// of 12 + 10 + 10 bits on histograms in LDS, ties going to the lowest slots.
-// Evicted slots below the budget ("holes") and kept ones at or past it
-// ("movers") are paired in ascending order, from two prefix sums: moving only
-// those costs min(evicted, kept past the budget) rows, where closing the gaps
-// in order would move nearly every kept row.  The order of the tokens changes,
-// which attention over all of them does not see; the ages say which is which.
+// slot has a 32-bit key in the order of the ranks; the budget-th largest is
+// found by a radix select of 12 + 10 + 10 bits on histograms in LDS, which
+// ends once all keys that share the digits so far are wanted, ties going to the
+// lowest slots.  12 bits come first because the weights of a cache span a few
+// binary orders: sign, exponent and three bits of mantissa spread a wave's 64
+// keys over many counters, while an 8-bit digit has nearly all of them in the
+// same two, and counts on one address go one by one.
 //
-// A thread owns consecutive slots, four to a load: up to 16 quads (65536
-// slots) are held in registers between the passes, longer caches are read
-// again.  12 bits come first because the weights of a cache span a few binary
-// orders: sign, exponent and three bits of mantissa spread a wave's 64 keys
-// over many histogram counters, while an 8-bit digit has nearly all of them
-// in the same two, and counts on one address go one by one.
+// Evicted slots below the budget ("holes") and kept ones at or past it
+// ("movers") are as many as each other and are paired in ascending order, from
+// one prefix sum over both: moving only those costs min(evicted, kept past the
+// budget) rows, where closing the gaps in order would move nearly every kept
+// row.  The order of the tokens changes, which attention over all of them does
+// not see; the ages say which is which.
+//
+// A thread owns consecutive slots, whose keys stay in registers between the
+// passes (up to 8192 slots), in LDS (32768), or are read again.  Bound by the
+// chain of some ten barriers and, in longer caches, by one CU's instructions
+// per slot: 7.8 us for one sequence of 2064 slots, 10.3 for 8192, 12.6 for 32 of
+// up to 8192, 21 for 16384, 33 for 32768 (their 8 bytes a slot are 2 us or less
+// at the card's rate).
 #include "kvhp_internal.h"
 
 #include <algorithm>
@@ -43,23 +49,36 @@ struct PlanArgs {
     int quads;                // quads of slots per thread
 };
 
-// Rank of a weight: order-preserving, 0 for NaN, below 0xFFFFFFFF; -0 counts as 0.
-__device__ __forceinline__ uint32_t rank_of(float w) {
-    if (w != w) return 0;
+// Keys: of a slot behind the sequence, of a NaN, of a weight of zero, of a protected slot.
+constexpr uint32_t kDead = 0, kNaN = 1, kZero = 0x80000000u, kGuard = 0xFFFFFFFFu;
+
+// Key of a weight, in the weights' order (-0 as 0), between kNaN and kGuard.
+__device__ __forceinline__ uint32_t key_of(float w) {
     const uint32_t u = __float_as_uint(w + 0.f);
-    return u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
+    const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+    return w != w ? kNaN : k;
+}
+
+// Inclusive prefix sum over the wave: shifts by 1, 2, 4, 8 lanes within rows of 16, then
+// the rows' last lanes broadcast to the rows behind (no LDS round trips).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+    x = dpp_add<0x111, 0xF>(x);
+    x = dpp_add<0x112, 0xF>(x);
+    x = dpp_add<0x114, 0xF>(x);
+    x = dpp_add<0x118, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);   // lane 15 of rows 0, 2 to rows 1, 3
+    return dpp_add<0x143, 0xC>(x);   // lane 31 to rows 2, 3
 }
 
 // Exclusive prefix sum over the workgroup's threads; `total` gets the sum.
 // red: kPlanWaves ints of LDS, free again after the caller's next barrier.
 __device__ __forceinline__ int block_scan(int x, int* red, int& total) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-    int inc = x;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int t = __shfl_up(inc, o);
-        if (lane >= o) inc += t;
-    }
+    const int inc = wave_scan(x);
     if (lane == kWave - 1) red[wave] = inc;
     __syncthreads();
     int before = 0;
@@ -74,12 +93,17 @@ __device__ __forceinline__ int block_scan(int x, int* red, int& total) {
     return before + inc - x;
 }
 
-// Q > 0: Q quads per thread in registers; 0: a.quads of them, read in each pass.
+// A thread's quads of keys between the passes: Q in registers (Q > 0), a.quads of them in
+// LDS (kInLds), or nowhere, read and made again in each pass (kAgain).
+constexpr int kInLds = 0, kAgain = -1;
+constexpr int kLdsQuads = 8;
+
 template <int Q>
 __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const PlanArgs a) {
     __shared__ uint32_t hist[kBins];
     __shared__ int red[kPlanWaves];
-    __shared__ int found[2];
+    __shared__ int found[3];
+    __shared__ int special[2];
     const int tid = threadIdx.x, kvh = blockIdx.x, b = blockIdx.y;
     const int n = min(max(a.seq_lens[b], 0), a.cap);
     if (tid == 0 && kvh == 0) a.new_lens[b] = min(n, a.budget);
@@ -96,9 +120,9 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const PlanArgs
 
     auto load = [&](int q, uint32_t (&k)[4]) {
         const int j = s0 + 4 * q;
-        if (j >= n) return;
-        const int pid = min(max(table[j >> 4], 0), a.num_pages - 1);
-        const int64_t at = ((int64_t)kvh * a.num_pages + pid) * kPage + (j & 15);
+        const int jc = min(j, n - 1) & ~3;   // behind the sequence: its last quad's, then dead
+        const int pid = min(max(table[jc >> 4], 0), a.num_pages - 1);
+        const int64_t at = ((int64_t)kvh * a.num_pages + pid) * kPage + (jc & 15);
         const floatx4 w = *reinterpret_cast<const floatx4*>(a.weights + at);
         int32_t age[4] = {j, j + 1, j + 2, j + 3};
         if (a.ages) {
@@ -107,63 +131,94 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const PlanArgs
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            k[e] = age[e] < a.sinks || age[e] > old ? 0xFFFFFFFFu : rank_of(w[e]);
+            k[e] = j + e >= n                              ? kDead
+                   : age[e] < a.sinks || age[e] > old ? kGuard
+                                                      : key_of(w[e]);
     };
     uint32_t held[Q > 0 ? Q : 1][4];
+    __shared__ u32x4 lds_keys[Q == kInLds ? kLdsQuads : 1][Q == kInLds ? kPlanThreads : 1];
     if constexpr (Q > 0) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) load(q, held[q]);
+    } else if constexpr (Q == kInLds) {
+        for (int q0 = 0; q0 < nq; q0 += 4) {   // read back by this thread only
+            uint32_t k[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load(min(q0 + i, nq - 1), k[i]);   // four under way
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                lds_keys[min(q0 + i, nq - 1)][tid] = u32x4{k[i][0], k[i][1], k[i][2], k[i][3]};
+        }
     }
-    // f(slot, key) for this thread's live slots in order
+    // f(slot, key) for this thread's slots in order
     auto each = [&](auto f) {
         if constexpr (Q > 0) {
 #pragma unroll
             for (int q = 0; q < Q; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (s0 + 4 * q + e < n) f(s0 + 4 * q + e, held[q][e]);
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t k = held[q][e];
+                    asm volatile("" : "+v"(k));   // (or every comparison's outcome is kept)
+                    f(s0 + 4 * q + e, k);
+                }
         } else {
             for (int q = 0; q < nq; ++q) {
                 uint32_t k[4];
-                load(q, k);
+                if constexpr (Q == kInLds) {
+                    const u32x4 x = lds_keys[q][tid];
+                    k[0] = x[0], k[1] = x[1], k[2] = x[2], k[3] = x[3];
+                } else {
+                    load(q, k);
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (s0 + 4 * q + e < n) f(s0 + 4 * q + e, k[e]);
+                for (int e = 0; e < 4; ++e) f(s0 + 4 * q + e, k[e]);
             }
         }
     };
+    // Two keys that many slots have, protected and never attended, are counted apart:
+    // counts on one address go one by one.
+    int guards = 0, zeros = 0;
+    each([&](int, uint32_t k) {
+        guards += k == kGuard;
+        zeros += k == kZero;
+    });
+    if (tid < 2) special[tid] = 0;
+    __syncthreads();
+    guards = wave_scan(guards);
+    zeros = wave_scan(zeros);
+    if ((tid & (kWave - 1)) == kWave - 1) {
+        atomicAdd(&special[0], guards);
+        atomicAdd(&special[1], zeros);
+    }
 
-    // ---- the budget-th largest key, digit by digit from the top
+    // ---- the budget-th largest key, digit by digit from the top, until those that share its
+    //      digits so far are all wanted (after two digits nearly always)
     uint32_t prefix = 0;       // its digits so far
     int want = a.budget;       // its rank among the keys with that prefix
     int shift = 32;
+    bool all = false;          // every key with that prefix is wanted
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
+    for (int pass = 0; pass < 3 && !all; ++pass) {
         const int bits = pass == 0 ? 12 : 10;
+        const int per = pass == 0 ? kBins / kPlanThreads : 1;   // counters per thread
+        const int from = shift;                                 // digits above it are `prefix`
         shift -= bits;
-        for (int i = tid; i < kBins; i += kPlanThreads) hist[i] = 0;
+        const uint32_t mask = (1u << bits) - 1;
+        for (int i = tid; i < per * kPlanThreads; i += kPlanThreads) hist[i] = 0;
         __syncthreads();
+        auto mine = [&](uint32_t k) { return pass == 0 || k >> from == prefix; };
+        if (tid < 2 && mine(tid ? kZero : kGuard))
+            atomicAdd(&hist[(tid ? kZero : kGuard) >> shift & mask], (uint32_t)special[tid]);
         each([&](int, uint32_t k) {
-            if (pass > 0 && (k >> (shift + bits)) != prefix) return;
-            const uint32_t digit = k >> shift & ((1u << bits) - 1);
-            // lanes that all count the same digit (protected slots, weights of
-            // zero) do it at once
-            const uint32_t lead = __builtin_amdgcn_readfirstlane(digit);
-            const uint64_t in = __builtin_amdgcn_read_exec();
-            if (__ballot(digit == lead) == in) {
-                if ((threadIdx.x & (kWave - 1)) == (unsigned)__builtin_ctzll(in))
-                    atomicAdd(&hist[lead], (uint32_t)__builtin_popcountll(in));
-            } else {
-                atomicAdd(&hist[digit], 1u);
-            }
+            if (k != kGuard && k != kZero && k != kDead && mine(k)) atomicAdd(&hist[k >> shift & mask], 1u);
         });
         __syncthreads();
-        // thread t holds the bins kBins - 1 - 4t .. - 3, largest first
-        uint32_t c[4];
-        int sum = 0;
+        // thread t holds `per` counters, the largest digits first
+        const int top = per * (kPlanThreads - tid) - 1;
+        int c[4], sum = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            c[i] = hist[kBins - 1 - 4 * tid - i];
+            c[i] = i < per ? hist[top - i] : 0;
             sum += c[i];
         }
         int total;
@@ -171,9 +226,10 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const PlanArgs
         if (above < want && above + sum >= want) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (above < want && above + (int)c[i] >= want) {
-                    found[0] = kBins - 1 - 4 * tid - i;
+                if (above < want && above + c[i] >= want) {
+                    found[0] = top - i;
                     found[1] = want - above;
+                    found[2] = c[i] == want - above;
                 }
                 above += c[i];
             }
@@ -181,29 +237,39 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const PlanArgs
         __syncthreads();
         prefix = prefix << bits | found[0];
         want = found[1];
+        all = found[2];
     }
-    // keys above `prefix` stay, and the first `want` that equal it
-
-    int ties = 0, total;
-    each([&](int, uint32_t k) { ties += k == prefix; });
-    int tie = block_scan(ties, red, total);
+    // Keys whose digits are above `prefix` stay, and the first `want` whose digits equal it.
+    int total, tie = 0;
+    if (!all) {
+        int ties = 0;
+        each([&](int, uint32_t k) { ties += k != kDead && (k >> shift) == prefix; });
+        tie = block_scan(ties, red, total);
+    }
     const int tie0 = tie;
-    int holes = 0, movers = 0;
-    auto kept = [&](uint32_t k) { return k > prefix || (k == prefix && tie++ < want); };
-    each([&](int j, uint32_t k) {
-        const bool stay = kept(k);
-        holes += j < a.budget && !stay;
-        movers += j >= a.budget && stay;
-    });
-    int hole = block_scan(holes, red, total);
-    int mover = block_scan(movers, red, total);
-    if (tid == 0) *count = total;
+    auto kept = [&](uint32_t k) {
+        const uint32_t d = k >> shift;
+        if (all) return k != kDead && d >= prefix;
+        const bool equal = k != kDead && d == prefix;
+        tie += equal;
+        return d > prefix || (equal && tie <= want);
+    };
+    // Holes below the budget and movers from it on are as many as each other: one prefix
+    // sum over both counts the holes, then the movers.
+    int here = 0;
+    each([&](int j, uint32_t k) { here += kept(k) == (j >= a.budget); });
+    int at = block_scan(here, red, total);
+    const int half = total / 2;
+    if (tid == 0) *count = half;
     tie = tie0;
     int32_t* const mv = a.moves + ((int64_t)b * a.Hkv + kvh) * a.max_moves * 2;
     each([&](int j, uint32_t k) {
-        const bool stay = kept(k);
-        if (j < a.budget && !stay) mv[2 * hole++ + 1] = j;
-        if (j >= a.budget && stay) mv[2 * mover++] = j;
+        if (kept(k) != (j >= a.budget)) return;
+        if (j < a.budget)
+            mv[2 * at + 1] = j;
+        else
+            mv[2 * (at - half)] = j;
+        ++at;
     });
 }
 
@@ -322,12 +388,12 @@ extern "C" int kvhp_evict_plan(const float* weights, const int32_t* ages,
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (a.quads <= 1)
         hipLaunchKernelGGL(evict_plan_kernel<1>, grid, blk, 0, s, a);
-    else if (a.quads <= 4)
-        hipLaunchKernelGGL(evict_plan_kernel<4>, grid, blk, 0, s, a);
-    else if (a.quads <= 16)
-        hipLaunchKernelGGL(evict_plan_kernel<16>, grid, blk, 0, s, a);
+    else if (a.quads <= 2)
+        hipLaunchKernelGGL(evict_plan_kernel<2>, grid, blk, 0, s, a);
+    else if (a.quads <= kLdsQuads)
+        hipLaunchKernelGGL(evict_plan_kernel<kInLds>, grid, blk, 0, s, a);
     else
-        hipLaunchKernelGGL(evict_plan_kernel<0>, grid, blk, 0, s, a);
+        hipLaunchKernelGGL(evict_plan_kernel<kAgain>, grid, blk, 0, s, a);
     return check_launch(what);
 }
 
