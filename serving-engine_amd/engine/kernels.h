@@ -163,6 +163,102 @@ inline void paged_gather_kv(const half* pool_k, const half* pool_v, const int32_
                                     out_k, out_v, stream));
 }
 
+// ---- Caches of bounded length (no reference counterpart; kvhp_c.h has the
+// semantics).  Attention over the last `window` keys and the first `sinks`
+// ones (window 0: every key), the sums of attention weight that cached keys
+// received, and the eviction that goes by them.  A workspace holds
+// *_workspace_bytes(...) bytes; every pointer is device memory.
+inline size_t window_decode_workspace_bytes(int batch_size, int num_q_heads, int num_kv_heads,
+                                            int head_dim, int max_seq_len, int window,
+                                            int sinks) {
+    return kvhp_window_decode_workspace_bytes(batch_size, num_q_heads, num_kv_heads, head_dim,
+                                              max_seq_len, window, sinks);
+}
+inline void window_decode(const half* q, const KVView& k_view, const KVView& v_view,
+                          const int* seq_lens, half* out, int batch_size, int num_q_heads,
+                          int num_kv_heads, int head_dim, int max_seq_len, int window, int sinks,
+                          void* workspace, size_t workspace_bytes, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_window_decode(q, k_view.c_view(), v_view.c_view(), seq_lens, out, batch_size,
+                                  num_q_heads, num_kv_heads, head_dim, max_seq_len, window, sinks,
+                                  workspace, workspace_bytes, stream));
+}
+
+// Rows q [B][rows][Hq][D] at positions q_start[b] + r; lse [B][Hq][rows] may be
+// nullptr, as may q_start (0) and seq_lens (max_seq_len).
+inline size_t window_prefill_workspace_bytes(int batch_size, int rows, int num_q_heads,
+                                             int num_kv_heads, int head_dim, int max_seq_len,
+                                             int window, int sinks) {
+    return kvhp_window_prefill_workspace_bytes(batch_size, rows, num_q_heads, num_kv_heads,
+                                               head_dim, max_seq_len, window, sinks);
+}
+inline void window_prefill(const half* q, const KVView& k_view, const KVView& v_view,
+                           const int* q_start, const int* seq_lens, half* out, float* lse,
+                           int batch_size, int rows, int num_q_heads, int num_kv_heads,
+                           int head_dim, int max_seq_len, int window, int sinks, void* workspace,
+                           size_t workspace_bytes, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_window_prefill(q, k_view.c_view(), v_view.c_view(), q_start, seq_lens, out,
+                                   lse, batch_size, rows, num_q_heads, num_kv_heads, head_dim,
+                                   max_seq_len, window, sinks, workspace, workspace_bytes,
+                                   stream));
+}
+
+// Decode attention that adds each key's weight to its slot (paged views);
+// ages and newest may be nullptr.
+inline size_t weighted_decode_workspace_bytes(int batch_size, int num_q_heads, int num_kv_heads,
+                                              int head_dim, int max_seq_len) {
+    return kvhp_weighted_decode_workspace_bytes(batch_size, num_q_heads, num_kv_heads, head_dim,
+                                                max_seq_len);
+}
+inline void weighted_decode(const half* q, const KVView& k_view, const KVView& v_view,
+                            const int* seq_lens, const int* newest, half* out, float* weights,
+                            int32_t* ages, int batch_size, int num_q_heads, int num_kv_heads,
+                            int head_dim, int max_seq_len, int new_keys, void* workspace,
+                            size_t workspace_bytes, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_weighted_decode(q, k_view.c_view(), v_view.c_view(), seq_lens, newest, out,
+                                    weights, ages, batch_size, num_q_heads, num_kv_heads,
+                                    head_dim, max_seq_len, new_keys, workspace, workspace_bytes,
+                                    stream));
+}
+
+// The weights that rows of a prompt gave each key, from window_prefill's lse.
+inline size_t prompt_weights_workspace_bytes(int batch_size, int rows, int num_q_heads,
+                                             int num_kv_heads, int head_dim, int max_seq_len) {
+    return kvhp_prompt_weights_workspace_bytes(batch_size, rows, num_q_heads, num_kv_heads,
+                                               head_dim, max_seq_len);
+}
+inline void prompt_weights(const half* q, const KVView& k_view, const float* lse,
+                           const int* q_start, const int* seq_lens, const int* newest,
+                           float* weights, int32_t* ages, int batch_size, int rows,
+                           int num_q_heads, int num_kv_heads, int head_dim, int max_seq_len,
+                           int window, int sinks, int new_keys, void* workspace,
+                           size_t workspace_bytes, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_prompt_weights(q, k_view.c_view(), lse, q_start, seq_lens, newest, weights,
+                                   ages, batch_size, rows, num_q_heads, num_kv_heads, head_dim,
+                                   max_seq_len, window, sinks, new_keys, workspace,
+                                   workspace_bytes, stream));
+}
+
+// The moves [B][Hkv][max_moves][2] that cut each sequence to `budget` slots,
+// and the same carried out in place (pools [Hkv][num_pages][16][D]); then
+// PagedKVCache::shrink gives the pages behind back.
+inline void evict_plan(const float* weights, const int32_t* ages, const int32_t* block_tables,
+                       int max_pages, const int* seq_lens, const int* newest, int32_t* moves,
+                       int32_t* counts, int32_t* new_lens, int batch_size, int num_kv_heads,
+                       int num_pages, int max_seq_len, int budget, int sinks, int recent,
+                       int max_moves, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_evict_plan(weights, ages, block_tables, max_pages, seq_lens, newest, moves,
+                               counts, new_lens, batch_size, num_kv_heads, num_pages, max_seq_len,
+                               budget, sinks, recent, max_moves, stream));
+}
+inline void evict_apply(half* pool_k, half* pool_v, float* weights, int32_t* ages,
+                        const int32_t* block_tables, int max_pages, const int32_t* moves,
+                        const int32_t* counts, int batch_size, int num_kv_heads, int head_dim,
+                        int num_pages, int max_moves, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_evict_apply(pool_k, pool_v, weights, ages, block_tables, max_pages, moves,
+                                counts, batch_size, num_kv_heads, head_dim, num_pages, max_moves,
+                                stream));
+}
+
 }  // namespace hip
 
 namespace cuda = hip;

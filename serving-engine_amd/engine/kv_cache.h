@@ -227,6 +227,28 @@ public:
         reserve(slot, len);
         lens_[slot] = len;
     }
+    // Cuts a sequence to its first `len` tokens and gives up the pages behind
+    // them (after an eviction moved the kept tokens into the first slots).
+    // None of its pages may be shared: an eviction writes into them.
+    void shrink(int slot, int len) {
+        check_slot(slot);
+        if (len < 0 || len > lens_[slot])
+            throw std::out_of_range("PagedKVCache::shrink: length outside 0..the present one");
+        const int keep = (len + kPage - 1) / kPage;
+        for (int i = 0; i < pages_used_[slot]; ++i)
+            if (refs_[tables_[(size_t)slot * max_pages_ + i]] > 1)
+                throw std::logic_error("PagedKVCache::shrink: a page is shared");
+        for (int i = keep; i < pages_used_[slot]; ++i) {
+            int32_t& e = tables_[(size_t)slot * max_pages_ + i];
+            refs_[e] = 0;
+            free_pages_.push_back(e);
+            e = -1;
+        }
+        pages_used_[slot] = std::min(pages_used_[slot], keep);
+        lens_[slot] = len;
+        cached_[slot] = 0;   // what the first slots hold is no shared prefix now
+        pos_[slot] = -1;
+    }
     // Prefix sharing: `dst` (an active slot holding no pages) takes the
     // full pages covering the first num_tokens positions of `src` (a partial
     // last page is never shared, so later writes stay private) and starts

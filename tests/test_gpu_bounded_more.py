@@ -1,0 +1,162 @@
+"""Bounded caches past 32-bit offsets, pages that were given away, and calls on
+two streams at once, against the definitions in 64 bits."""
+import numpy as np
+import pytest
+
+import kvhp
+from bounded_util import PAGE, Cache, check, decode_ref, plan_ref, workspace
+from gpu_util import from_gpu, note, sync, to_gpu
+from test_gpu_bounded import (_calls, _check_prefill, _check_sums, _prompt_ref, _prompt_weights,
+                              _q, _sums, _sums_ref, _weighted, _window_decode)
+
+pytestmark = pytest.mark.gpu
+
+
+def _far(c, far_pages):
+    """The cache's second half of pages at the end of a pool of far_pages pages per head
+    (never written in between); c.near_bt keeps the small pool's ids."""
+    import torch
+    c.upload()
+    n, half = c.pages, c.pages // 2
+    pools = []
+    for small in (c.pool_k, c.pool_v):
+        big = torch.empty((c.hkv, far_pages, PAGE, c.d), dtype=torch.float16, device="cuda")
+        big[:, :half].copy_(small[:, :half])
+        big[:, far_pages - (n - half):].copy_(small[:, half:])
+        pools.append(big)
+    c.near_bt = c.bt
+    c.bt = np.where(c.bt >= half, c.bt + far_pages - n, c.bt).astype(np.int32)
+    c.pages = far_pages
+    c.pool_k, c.pool_v = pools
+    c.bt_d = to_gpu(c.bt)
+    c.kv, c.vv = kvhp.paged_view(pools[0], c.bt_d), kvhp.paged_view(pools[1], c.bt_d)
+    return c
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (3, 1, 64)])
+def test_pools_past_32_bit_offsets(hq, hkv, d):
+    """Pages more than 2^32 bytes behind the start of their head's pool."""
+    rng = np.random.default_rng([hq, d])
+    c = _far(Cache(rng, [1500, 333], hkv, d), (1 << 32) // (2 * PAGE * d) + 200)
+    assert int(c.bt.max()) * PAGE * d * 2 >= 1 << 32
+    q = _q(rng, 2, hq, d)
+    for window, sinks in [(0, 0), (700, 4)]:
+        note(f"far pages: window_decode window={window}")
+        ref, tol, _, _ = decode_ref(q, c, window, sinks)
+        check(_window_decode(q, c, window, sinks), ref, tol)
+    qp = _q(rng, 2, 20, hq, d)
+    start = [1480, 313]
+    note("far pages: window_prefill")
+    _check_prefill(qp, c, start, 500, 3)
+    w, ages = _sums(rng, c)
+    note("far pages: weighted_decode")
+    out, gw, ga = _weighted(q, c, w, ages, 1, None)
+    ref, tol, sums, rel = decode_ref(q, c, 0, 0)
+    check(out, ref, tol)
+    rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 1, c.lens - 1)
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
+    note("far pages: prompt_weights")
+    lse, add, rel = _prompt_ref(qp, c, start, 500, 3)
+    gw, ga = _prompt_weights(qp, c, lse, w, ages, start, 500, 3, 20)
+    rw, tw, ra = _sums_ref(c, w, ages, add, rel, 20, c.lens - 1)
+    # keys that no row sees: not touched
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
+    note("far pages: eviction")
+    import torch
+    budget, moves = 256, torch.zeros(2, hkv, 256, 2, dtype=torch.int32, device="cuda")
+    counts = torch.zeros(2, hkv, dtype=torch.int32, device="cuda")
+    new = torch.zeros(2, dtype=torch.int32, device="cuda")
+    w_d, a_d = to_gpu(gw), to_gpu(ga)
+    kvhp.evict_plan(w_d, a_d, c.bt_d, c.lens_d, moves, counts, new, c.cap, budget, 4, 30)
+    kvhp.evict_apply(c.pool_k, c.pool_v, w_d, a_d, c.bt_d, moves, counts)
+    sync()
+    gm, gc = from_gpu(moves), from_gpu(counts)
+    crossed = 0
+    for b in range(2):
+        n = int(c.lens[b])
+        pg, sl = c.slots(b)
+        ids = torch.from_numpy(pg.astype(np.int64)).cuda()
+        ss = torch.from_numpy(sl.astype(np.int64)).cuda()
+        for h in range(hkv):
+            want = plan_ref(gw[h, pg, sl], ga[h, pg, sl], n, budget, 4, 30, n - 1)
+            assert [tuple(x) for x in gm[b, h, :gc[b, h]]] == want
+            order = np.arange(n)
+            for s, t in want:
+                order[t] = s
+                crossed += (pg[s] < 1000) != (pg[t] < 1000)
+            for pool, host in ((c.pool_k, c.k), (c.pool_v, c.v)):
+                # rows gathered page by page: each page is a view with a 64-bit offset
+                got = np.stack([from_gpu(pool[h, int(i)])[j] for i, j in zip(pg, sl)])
+                assert np.array_equal(got, host[b, h, order])
+    assert crossed > 10
+
+
+def test_prompt_weights_pages_given_away():
+    """Entries of pages that no row sees may be -1 or name a page that another sequence took:
+    nobody's sums there change but the owner's own."""
+    rng = np.random.default_rng(4)
+    c = Cache(rng, [640, 700], 2, 64).upload()
+    q = _q(rng, 2, 40, 8, 64)
+    window, sinks, start = 100, 20, [600, 660]
+    w, ages = _sums(rng, c)
+    lse, add, rel = _prompt_ref(q, c, start, window, sinks)
+    rw, tw, ra = _sums_ref(c, w, ages, add, rel, 40, c.lens - 1)
+    bt = c.bt.copy()
+    hidden = np.arange(2, (600 - 99) // PAGE)        # behind the sinks, before the window
+    bt[0, hidden[::2]] = -1
+    bt[0, hidden[1::2]] = bt[1, 40:40 + len(hidden[1::2])].max()   # one of sequence 1's in use
+    bt[1, 2] = bt[0, 39]
+    c.bt_d.copy_(to_gpu(bt))
+    note("prompt_weights over a table with pages given away")
+    gw, ga = _prompt_weights(q, c, lse, w, ages, start, window, sinks, 40)
+    # the keys of hidden pages: as they were
+    for b, pages in ((0, hidden), (1, [2])):
+        for i in pages:
+            rw[:, c.bt[b, i]], tw[:, c.bt[b, i]] = w[:, c.bt[b, i]], 0
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap, each with its own workspace and outputs."""
+    import torch
+    runs = [_calls(np.random.default_rng(s)) for s in (5, 6)]
+    wants = []
+    note("bounded attention on one stream, then on two at once")
+    for go, t, _ in runs:
+        go()
+        sync()
+        wants.append({k: x.clone() for k, x in t.items()})
+        for x in t.values():
+            x.zero_()
+    sync()
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(4):
+        for (go, t, _), st in zip(runs, streams):
+            with torch.cuda.stream(st):
+                t["w"].zero_()
+            go(st)
+    sync()
+    for (_, t, _), want in zip(runs, wants):
+        for k, x in t.items():
+            assert torch.equal(x, want[k]), k
+
+
+def test_padded_batches():
+    """Rows at negative positions, rows behind the last key, sequences without keys and with
+    one, all in one batch: padding keeps what its outputs held."""
+    rng = np.random.default_rng(9)
+    c = Cache(rng, [0, 1, 16, 90, 300], 2, 128).upload()
+    q = _q(rng, 5, 48, 4, 128)
+    start = [0, 0, -2 ** 31, 60, 2 ** 31 - 1]
+    note("window_prefill over a padded batch")
+    _check_prefill(q, c, start, 33, 2)
+    w, ages = _sums(rng, c)
+    lse, add, rel = _prompt_ref(q, c, start, 33, 2)
+    note("prompt_weights over a padded batch")
+    gw, ga = _prompt_weights(q, c, lse, w, ages, start, 33, 2, 5)
+    rw, tw, ra = _sums_ref(c, w, ages, add, rel, 5, c.lens - 1)
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
