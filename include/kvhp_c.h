@@ -256,23 +256,25 @@ int kvhp_causal_gqa(const void* q, const void* k, const void* v, void* out,
  *
  * Visible keys: the query at position p of its sequence attends key j when
  * j <= p and (j < sinks or p - j < window); window 0 means no window (every
- * j <= p).  A page that holds no key that some row of the call sees is not
- * loaded, nor is its block-table entry (which may be -1 or name a page that was
- * given away), and whatever a masked slot holds, NaN and infinities included,
- * reaches no output.
+ * j <= p).  The entry of a page that holds no key which some row of the call
+ * sees may be -1 or name a page that was given away (the attention calls load
+ * neither, and no call changes a slot there), and whatever a masked slot holds,
+ * NaN and infinities included, reaches no output.
  *
  * Sums: a cache cut by weight has two pools beside K and V, through the same
  * block tables: weights, fp32 [Hkv][num_pages][16], the attention weight that
  * each slot's key has received, summed over the query heads of its KV head;
  * and ages, int32 [Hkv][num_pages][16] (may be NULL throughout), the position
  * in the text of the token in a slot, which is the slot's own index until an
- * eviction first moves tokens; both pools 16-byte aligned.  `newest` (device int32[batch], NULL: seq_lens[b] - 1)
- * is the text position of each sequence's last key.  The last `new_keys` keys
- * of a sequence are new to the sums: their weight starts from zero, whatever
- * the slot held, and their age is set.  Block-table ids outside
- * [0, num_pages) are clamped for reads of K and V as everywhere, and drop
- * writes of sums.  A page belongs to one sequence: a page that several rows of
- * a block table name (a shared prefix) must not be given sums or evicted.
+ * eviction first moves tokens; both pools 16-byte aligned.  `newest` (device
+ * int32[batch], NULL: seq_lens[b] - 1) is the text position of each sequence's
+ * last key.  The last `new_keys` keys of a sequence are new to the sums,
+ * whether a row sees them or not: their weight starts from zero, whatever the
+ * slot held, and their age is set, so their pages must be the sequence's own.
+ * Block-table ids outside [0, num_pages) are clamped for reads of K and V as
+ * everywhere, and drop writes of sums.  A page belongs to one sequence: a page
+ * that several rows of a block table name (a shared prefix) must not be given
+ * sums or evicted.
  *
  * Lengths above max_seq_len (or the block table's reach) count as that, and
  * sequences of length <= 0 have no keys.  Every call is asynchronous on
@@ -324,9 +326,9 @@ int kvhp_weighted_decode(const void* q, const kvhp_kv_view* k_view, const kvhp_k
 /* The same for rows of a prompt: adds to key j's slot the sum, over the rows
  * of its sequence that see it and over the query heads of its KV head, of
  * exp(q.k_j / sqrt(D) - lse), q and lse as kvhp_window_prefill takes and leaves
- * them for these rows, window and sinks.  Passing only a prompt's last rows lets those say which
- * keys matter.  Keys that no row sees add nothing (new keys among them start
- * at zero).  Paged K view. */
+ * them for these rows, window and sinks.  Passing only a prompt's last rows
+ * lets those say which keys matter.  Keys that no row sees add nothing (new
+ * keys among them start at zero).  Paged K view. */
 size_t kvhp_prompt_weights_workspace_bytes(int batch, int rows, int num_q_heads,
                                            int num_kv_heads, int head_dim, int max_seq_len);
 int kvhp_prompt_weights(const void* q, const kvhp_kv_view* k_view, const float* lse,

@@ -18,13 +18,19 @@
 // with a window the chunks start anywhere in a page.  Up to 16 query heads of
 // a KV head go together; larger groups read the keys once per 16.
 //
-// Sums: the scores go to the workspace in fp32, [b][query head][key]; once the
-// maximum and the sum of every head are known from the chunks' partials, the
-// launch that joins the partials also turns the scores into weights, adds them
+// Sums: the scores go to the workspace in fp32, 32 keys of each head side by side;
+// once the maximum and the sum of every head are known from the chunks' partials,
+// the launch that joins the partials also turns the scores into weights, adds them
 // over the heads of a KV head and updates the slots.  (16 bytes a key and four
-// heads, written and read, beside 512 of K and V at D = 128.)
+// heads, written and read, beside 512 of K and V at D = 128.  Written past the
+// caches they cost 132 us instead of 125 below.)
 //
-// Bound by HBM: 4 D bytes per visible key and KV head.
+// Bound by HBM, 4 D bytes per visible key and KV head, where there is much of it.  32
+// sequences of up to 8192 keys, 32/8 heads of 128: windows of 4096 73.5 us, 412 MB at
+// 5.6 TB/s (shuffled pages alone read at 5.9-6.3); every key with its sums 125 us, of
+// which 114 are the first launch's, 579 MB at 5.1 TB/s, and 11 the second's.  One
+// sequence of 1024 visible keys at D = 64 takes 7.5 us and 2048 with sums 8.7: two
+// launches, and the latency of their loads.
 #include "bounded.h"
 
 #include <type_traits>
@@ -32,7 +38,7 @@
 namespace kvhp {
 namespace {
 
-constexpr int kMaxChunk = 960;    // keys per split: at most 64 pages, two of them cut
+constexpr int kMaxChunk = 960;    // keys per split: at most 64 pages, three of them cut
 constexpr int kHeads = 16;        // query heads per workgroup
 
 struct DecodePlan {
@@ -587,7 +593,8 @@ constexpr int kWaveSlots = 2048;
 
 size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int window, int sinks,
                               bool sums) {
-    if (batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || cap <= 0 || (d != 64 && d != 128))
+    if (batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || cap <= 0 || cap > 1 << 30 ||
+        (d != 64 && d != 128))
         return 0;
     const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks));
     const size_t rows = (size_t)batch * hq;

@@ -414,6 +414,8 @@ extern "C" int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int3
                  "%s: moves must be 8-byte aligned", what);
     KVHP_REQUIRE(batch <= 65535 && num_kv_heads <= 65535, KVHP_ERR_UNSUPPORTED,
                  "%s: more than 65535 sequences or KV heads", what);
+    KVHP_REQUIRE(max_moves <= 1 << 30, KVHP_ERR_UNSUPPORTED, "%s: max_moves=%d above 2^30", what,
+                 max_moves);
     MoveArgs a{static_cast<f16*>(pool_k), static_cast<f16*>(pool_v), weights, ages, block_tables,
                moves, counts, max_pages, num_pages, num_kv_heads, head_dim, max_moves};
     const bool vec = head_dim % 8 == 0 && aligned16(pool_k) && aligned16(pool_v);

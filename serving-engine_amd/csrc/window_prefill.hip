@@ -640,6 +640,8 @@ window_join_kernel(const BoundArgs a, const PrefillPlan p, int64_t threads) {
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
+// Ranges of keys until every CU has two workgroups, each of at least 4 tiles, and as many
+// as their page ids fit LDS in.
 PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window, int sinks) {
     PrefillPlan p{};
     const int64_t pairs = (int64_t)rows * G;

@@ -166,3 +166,11 @@ def test_apply_arguments():
     _refused(_apply(d=300), kvhp.KVHP_ERR_UNSUPPORTED, "head_dim")
     _refused(_apply(batch=65536), kvhp.KVHP_ERR_UNSUPPORTED, "65535")
     assert _apply(most=0)[0] == kvhp.KVHP_OK and _apply(batch=0)[0] == kvhp.KVHP_OK
+
+
+def test_sizes_that_no_call_has():
+    """Counts whose products leave 32 bits: refused, and their workspaces are nothing."""
+    lib = kvhp.load()
+    _refused(_apply(most=2 ** 31 - 1), kvhp.KVHP_ERR_UNSUPPORTED, "max_moves")
+    assert lib.kvhp_weighted_decode_workspace_bytes(2, 8, 2, 64, 2 ** 31 - 1) <= 2 * 8 * 4
+    assert lib.kvhp_window_decode_workspace_bytes(2, 8, 2, 64, 2 ** 31 - 1, 0, 0) == 0
