@@ -27,10 +27,12 @@
 //
 // Bound by HBM, 4 D bytes per visible key and KV head, where there is much of it.  32
 // sequences of up to 8192 keys, 32/8 heads of 128: windows of 4096 73.5 us, 412 MB at
-// 5.6 TB/s (shuffled pages alone read at 5.9-6.3); every key with its sums 125 us, of
+// 5.6 TB/s (shuffled pages alone read at 5.9-6.3); every key with its sums 122-125 us, of
 // which 114 are the first launch's, 579 MB at 5.1 TB/s, and 11 the second's.  One
-// sequence of 1024 visible keys at D = 64 takes 7.5 us and 2048 with sums 8.7: two
-// launches, and the latency of their loads.
+// sequence of 1028 visible keys at D = 64 takes 7.1 us, 500 5.1 in one launch, 2048 with
+// sums 8.7: launches, and the latency of their loads.  Where several waves share a split,
+// each joins the dims of one MFMA block for all of them (one wave joining everything cost
+// 0.7 us more at D = 64 and 2 at D = 128).
 #include "bounded.h"
 
 #include <type_traits>
@@ -337,57 +339,65 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
         }
     }
 
-    if constexpr (W > 1) {
-        // waves 1 .. leave (O, m, l) in their own K tile, 64 (D + 8) bytes of it
+    // Dims 16 (d0 + i) + 4g + e of head col: all of them, or wave d0's share of the waves' sum.
+    constexpr int NB = W > 1 ? 1 : ND;
+    floatx4 r[NB];
+    int d0 = 0;
+    if constexpr (W == 1) {
+#pragma unroll
+        for (int db = 0; db < ND; ++db) r[db] = o[db];
+    } else {
+        // every wave leaves (O, m, l) in its own K tile, 64 (D + 8) bytes of it
+        static_assert(W >= ND, "a wave for every 16 dims");
         float* xs = reinterpret_cast<float*>(k_lds);
-        if (wv > 0) {
 #pragma unroll
-            for (int db = 0; db < ND; ++db)
-                *reinterpret_cast<floatx4*>(&xs[(db * kWave + lane) * 4]) = o[db];
-            xs[ND * kWave * 4 + 2 * lane] = m_run;
-            xs[ND * kWave * 4 + 2 * lane + 1] = l_part;
-        }
+        for (int db = 0; db < ND; ++db)
+            *reinterpret_cast<floatx4*>(&xs[(db * kWave + lane) * 4]) = o[db];
+        *reinterpret_cast<float2*>(&xs[ND * kWave * 4 + 2 * lane]) = float2{m_run, l_part};
         __syncthreads();
-        if (wv > 0) return;
+        if (wv >= ND) return;
+        d0 = wv;
+        float2 ml[W];
+        floatx4 x[W];
 #pragma unroll
-        for (int w = 1; w < W; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float* xw = reinterpret_cast<const float*>(k_lds_all[w]);
-            const float mw = xw[ND * kWave * 4 + 2 * lane];
-            const float lw = xw[ND * kWave * 4 + 2 * lane + 1];
-            const float mn = fmaxf(m_run, mw);
-            const float a0 = fast_exp2((m_run - mn) * sc);
-            const float a1 = fast_exp2((mw - mn) * sc);
-            l_part = l_part * a0 + lw * a1;
+            ml[w] = *reinterpret_cast<const float2*>(&xw[ND * kWave * 4 + 2 * lane]);
+            x[w] = *reinterpret_cast<const floatx4*>(&xw[(d0 * kWave + lane) * 4]);
+            m_run = fmaxf(m_run, ml[w].x);
+        }
+        l_part = 0.f;
+        r[0] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int db = 0; db < ND; ++db)
-                o[db] = o[db] * a0 +
-                        *reinterpret_cast<const floatx4*>(&xw[(db * kWave + lane) * 4]) * a1;
-            m_run = mn;
+        for (int w = 0; w < W; ++w) {
+            const float al = fast_exp2((ml[w].x - m_run) * sc);
+            l_part = fmaf(ml[w].y, al, l_part);
+            r[0] += x[w] * al;
         }
     }
 
     const float l_tot = rows4_sum(l_part);
     if (!hvalid) return;
     const int64_t prow = (row0 + col) * p.nsplit + split;
-    if ((SUMS || nsb > 1) && g == 0) {
+    if ((SUMS || nsb > 1) && g == 0 && d0 == 0) {
         p.ws_ml[prow * 2] = m_run * sc;
         p.ws_ml[prow * 2 + 1] = l_tot;
     }
     if (nsb == 1) {
         const float inv = 1.f / l_tot;
-        f16* orow = a.out + (row0 + col) * D + 4 * g;
+        f16* orow = a.out + (row0 + col) * D + 16 * d0 + 4 * g;
 #pragma unroll
-        for (int db = 0; db < ND; ++db) {
+        for (int db = 0; db < NB; ++db) {
             half4 h;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = static_cast<f16>(o[db][e] * inv);
+            for (int e = 0; e < 4; ++e) h[e] = static_cast<f16>(r[db][e] * inv);
             *reinterpret_cast<half4*>(orow + 16 * db) = h;
         }
         return;
     }
-    float* po = p.ws_o + prow * D + 4 * g;
+    float* po = p.ws_o + prow * D + 16 * d0 + 4 * g;
 #pragma unroll
-    for (int db = 0; db < ND; ++db) *reinterpret_cast<floatx4*>(po + 16 * db) = o[db];
+    for (int db = 0; db < NB; ++db) *reinterpret_cast<floatx4*>(po + 16 * db) = r[db];
 }
 
 // ------------------------------------------------------------------ join --
@@ -562,7 +572,7 @@ bound_sums_kernel(const BoundArgs a, const DecodePlan p, int key_blocks) {
 }
 
 // ------------------------------------------------------------------ plan --
-DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv) {
+DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums) {
     DecodePlan p{};
     p.batch = batch;
     p.groups = (G + kHeads - 1) / kHeads;
@@ -570,11 +580,12 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv) {
     const int64_t per = std::max<int64_t>(64, ((maxv + 63) / 64 + 63) / 64 * 64);
     int64_t s = std::min((maxv + per - 1) / per, units >= 6144 ? 1 : 6144 / units);
     int64_t chunk = std::min<int64_t>(((maxv + s - 1) / s + 63) / 64 * 64, kMaxChunk);
-    // Up to 640 keys (192 at D = 128) a small batch takes one split: eight waves share its
+    // Up to kMaxChunk keys (576 at D = 128) a small batch takes one split: eight waves share its
     // steps, and no second launch joins.  One sequence, 32/8 heads, us as one split / as
-    // splits of 64 keys: D = 64 300 keys 5.5 / 7.4, 700 7.2 / 7.4, 1024 8.6 / 7.5; D = 128
-    // 300 8.8 / 8.3.
-    if (batch < 8 && maxv <= (d == 64 ? 640 : 192)) chunk = (maxv + 31) / 32 * 32;
+    // splits of 64 keys: D = 64 500 keys 5.2 / 7.0, 1028 6.8 / 7.1, 1500 8.1 / 7.0; D = 128
+    // 500 7.2 / 7.8, 700 8.6 / 8.0.  With sums there is a second launch anyway: 128 keys 8.2
+    // / 8.4 and 9.1 / 9.0, 350 9.1 / 8.4 and 10.7 / 9.1.
+    if (batch < 8 && maxv <= (sums ? 128 : d == 64 ? kMaxChunk : 576)) chunk = (maxv + 31) / 32 * 32;
     p.chunk = static_cast<int>(chunk);
     p.nsplit = static_cast<int>((maxv + chunk - 1) / chunk);
     p.min_chunk = batch >= 16 ? 64 : 128;
@@ -596,7 +607,7 @@ size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int wi
     if (batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || cap <= 0 || cap > 1 << 30 ||
         (d != 64 && d != 128))
         return 0;
-    const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks));
+    const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks), sums);
     const size_t rows = (size_t)batch * hq;
     size_t n = p.nsplit > 1 || sums ? rows * p.nsplit * 2 : 0;
     if (p.nsplit > 1) n += rows * p.nsplit * d;
@@ -605,7 +616,8 @@ size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int wi
 }
 
 bool bound_decode_fits(const BoundArgs& a, int batch) {
-    const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, most_visible(a.max_len, a.window, a.sinks));
+    const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, most_visible(a.max_len, a.window, a.sinks),
+                                 a.weights != nullptr);
     return (a.D == 64 || a.D == 128) && p.nsplit <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
 }
 
@@ -627,14 +639,17 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
     // one split: eight waves take its steps round robin; fixed splits at D = 64: four
     // (at D = 128 four are no faster on one sequence and 26-52 % slower on four of 1024
     // to 4000 keys)
+    auto go = [&](auto kernel, int waves) {
+        hipLaunchKernelGGL(kernel, grid, dim3(waves * kWave), 0, s, a, p);
+    };
     if (wide)
-        hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 1, true>), grid, dim3(kWave), 0, s, a, p);
+        go(bound_decode_kernel<D, PAGED, SUMS, 1, true>, 1);
     else if (p.balance == 0 && p.nsplit == 1)
-        hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 8>), grid, dim3(8 * kWave), 0, s, a, p);
-    else if (p.balance == 0 && D == 64)
-        hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 4>), grid, dim3(4 * kWave), 0, s, a, p);
+        go(bound_decode_kernel<D, PAGED, SUMS, 8>, 8);
+    else if (D == 64 && p.balance == 0)
+        go(bound_decode_kernel<D, PAGED, SUMS, D == 64 ? 4 : 1>, 4);
     else
-        hipLaunchKernelGGL((bound_decode_kernel<D, PAGED, SUMS, 1>), grid, dim3(kWave), 0, s, a, p);
+        go(bound_decode_kernel<D, PAGED, SUMS, 1>, 1);
     if (SUMS) {
         const int kb = (a.cap + kSumKeys - 1) / kSumKeys;
         hipLaunchKernelGGL((bound_sums_kernel<D>), dim3(kb + (p.nsplit > 1 ? a.G : 0), a.Hkv, p.batch),
@@ -650,7 +665,7 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
 // block table, 16-byte aligned.
 int bound_decode(const BoundArgs& a, int batch, bool paged, bool sums, void* ws, hipStream_t s) {
     const int64_t maxv = most_visible(a.max_len, a.window, a.sinks);
-    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, maxv);
+    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, maxv, sums);
     const size_t rows = (size_t)batch * a.Hq;
     p.scap = (a.max_len + 31) / 32 * 32;
     float* w = static_cast<float*>(ws);

@@ -419,7 +419,7 @@ def causal_gqa(q, k, v, out, seq_len, num_q_heads, num_kv_heads, head_dim, strea
 
 # --------------------------------------------- caches of bounded length --
 def _bytes(ws) -> int:
-    return 0 if ws is None else ws.numel() * ws.element_size()
+    return 0 if ws is None else ws.nbytes
 
 
 def window_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len,

@@ -160,3 +160,52 @@ def test_padded_batches():
     rw, tw, ra = _sums_ref(c, w, ages, add, rel, 5, c.lens - 1)
     _check_sums(gw, rw, tw)
     assert np.array_equal(ga, ra)
+
+
+@pytest.mark.parametrize("d,visible", [(64, 959), (64, 960), (64, 961), (128, 575), (128, 576),
+                                       (128, 577), (64, 31), (128, 33)])
+@pytest.mark.parametrize("sinks", [0, 1, 17])
+def test_window_decode_split_limits(d, visible, sinks):
+    """Visible keys on both sides of what one split takes, the window beginning and the first
+    tokens ending inside a page; three lengths, one that no gap divides."""
+    rng = np.random.default_rng([d, visible, sinks])
+    for paged in (True, False):
+        c = Cache(rng, [2011, visible, 1300], 2, d, paged=paged).upload()
+        q = _q(rng, 3, 14, d)
+        note(f"window_decode {visible} visible keys, {sinks} first, d={d} paged={paged}")
+        ref, tol, _, _ = decode_ref(q, c, visible - sinks, sinks)
+        check(_window_decode(q, c, visible - sinks, sinks), ref, tol)
+
+
+@pytest.mark.parametrize("n", [127, 128, 129, 160])
+@pytest.mark.parametrize("d", [64, 128])
+def test_weighted_decode_split_limits(n, d):
+    rng = np.random.default_rng([n, d])
+    c = Cache(rng, [n, 1, n - 1], 2, d).upload()
+    q = _q(rng, 3, 14, d)
+    w, ages = _sums(rng, c)
+    note(f"weighted_decode {n} keys, d={d}")
+    out, gw, ga = _weighted(q, c, w, ages, 1, None)
+    ref, tol, sums, rel = decode_ref(q, c, 0, 0)
+    check(out, ref, tol)
+    rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 1, c.lens - 1)
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
+
+
+@pytest.mark.parametrize("hq,hkv", [(71, 1), (33, 1), (12, 4), (2, 2)])
+@pytest.mark.parametrize("rows", [1, 3, 17, 33, 63, 64, 65, 130])
+def test_prompt_weights_tiles(hq, hkv, rows):
+    """Group sizes that no tile of heads divides, rows on both sides of a tile's."""
+    rng = np.random.default_rng([hq, rows])
+    c = Cache(rng, [rows + 77, max(1, rows - 5)], hkv, 64).upload()
+    q = _q(rng, 2, rows, hq, 64)
+    start = [77, -3]
+    w, ages = _sums(rng, c)
+    note(f"prompt_weights {hq}/{hkv}, {rows} rows")
+    for window, sinks in [(0, 0), (40, 3)]:
+        lse, add, rel = _prompt_ref(q, c, start, window, sinks)
+        gw, ga = _prompt_weights(q, c, lse, w, ages, start, window, sinks, rows)
+        rw, tw, ra = _sums_ref(c, w, ages, add, rel, rows, c.lens - 1)
+        _check_sums(gw, rw, tw)
+        assert np.array_equal(ga, ra)
