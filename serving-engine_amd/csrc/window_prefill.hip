@@ -586,48 +586,66 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
     store_pair<D>(a, p, x, b, h, all_tiles, o, m_run, halves_sum(l_part));
 }
 
-// Joins the partials of the blocks that were cut into ranges of keys, 8 dims of a
-// (row, head) a thread.
-__global__ void __launch_bounds__(256)
-window_join_kernel(const BoundArgs a, const PrefillPlan p, int64_t threads) {
-    const int64_t t = blockIdx.x * (int64_t)256 + threadIdx.x;
-    if (t >= threads) return;
-    const int cpr = a.D / 8, c = static_cast<int>(t % cpr);
-    const int64_t at = t / cpr;   // (sequence, row, head)
-    const int qh = static_cast<int>(at % a.Hq);
-    const int row = static_cast<int>(at / a.Hq % a.rows), b = static_cast<int>(at / a.Hq / a.rows);
-    const Block k = block_of(a, p, b, (row * a.G + qh % a.G) / kPairs, kPairs);
+// Joins the partials of the blocks that were cut into ranges of keys: R times D / 8 lanes
+// per (row, head), lane (r, c) taking dims 8c .. of every R-th range.
+template <int D, int R>
+__global__ void __launch_bounds__(256) window_join_kernel(const BoundArgs a, const PrefillPlan p) {
+    constexpr int LPR = D / 8;
+    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR % R;
+    const int b = blockIdx.y;
+    const uint32_t i = blockIdx.x * (256 / LPR / R) + threadIdx.x / (LPR * R);
+    const int row = static_cast<int>(i / a.Hq), qh = static_cast<int>(i % a.Hq);
+    if (row >= a.rows) return;
+    const Block k = block_of(a, p, b, (row * a.G + qh - row_of(p, qh) * a.G) / kPairs, kPairs);
     const int64_t pos = (int64_t)k.first + row;
     if (pos < k.p_lo || pos > k.p_hi) return;
     const int tiles = (k.nv + kBN - 1) / kBN;
     if (tiles <= p.tiles_per_split) return;
     const int n = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
-    const float* po = p.ws_o + at * p.nsplit * a.D + 8 * c;
+    const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
+    const float* po = p.ws_o + at * p.nsplit * D + 8 * c;
     const float2* pml = reinterpret_cast<const float2*>(p.ws_ml) + at * p.nsplit;
     float M = -3.0e38f, L = 0.f;
     floatx4 o0 = {0.f, 0.f, 0.f, 0.f}, o1 = o0;
-    constexpr int U = 4;
-    for (int j0 = 0; j0 < n; j0 += U) {
+    auto fold = [&](float m, float l, floatx4 x0, floatx4 x1) {
+        const float mn = fmaxf(M, m);
+        const float al = fast_exp2(M - mn), be = fast_exp2(m - mn);
+        o0 = o0 * al + x0 * be;
+        o1 = o1 * al + x1 * be;
+        L = fmaf(L, al, l * be);
+        M = mn;
+    };
+    auto some = [&](auto U_, int j0) {   // U ranges in flight
+        constexpr int U = decltype(U_)::value;
         float2 ml[U];
         floatx4 x[U][2];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int j = min(j0 + i, n - 1);
-            ml[i] = pml[j];
-            x[i][0] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * a.D);
-            x[i][1] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * a.D + 4);
+        for (int u = 0; u < U; ++u) {
+            const int j = min(j0 + R * u, n - 1);
+            ml[u] = pml[j];
+            x[u][0] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D);
+            x[u][1] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D + 4);
         }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (j0 + i >= n) continue;
-            const float mn = fmaxf(M, ml[i].x);
-            const float al = fast_exp2(M - mn), be = fast_exp2(ml[i].x - mn);
-            o0 = o0 * al + x[i][0] * be;
-            o1 = o1 * al + x[i][1] * be;
-            L = fmaf(L, al, ml[i].y * be);
-            M = mn;
+        for (int u = 0; u < U; ++u)
+            if (j0 + R * u < n) fold(ml[u].x, ml[u].y, x[u][0], x[u][1]);
+    };
+    if (n <= R)
+        some(std::integral_constant<int, 1>{}, r);
+    else
+        for (int j0 = r; j0 < n; j0 += 4 * R) some(std::integral_constant<int, 4>{}, j0);
+#pragma unroll
+    for (int s = LPR; s < LPR * R; s <<= 1) {
+        floatx4 x0, x1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x0[e] = __shfl_xor(o0[e], s);
+            x1[e] = __shfl_xor(o1[e], s);
         }
+        const float m = __shfl_xor(M, s), l = __shfl_xor(L, s);
+        fold(m, l, x0, x1);
     }
+    if (r > 0) return;
     const float inv = 1.f / L;
     half8 hv;
 #pragma unroll
@@ -635,13 +653,15 @@ window_join_kernel(const BoundArgs a, const PrefillPlan p, int64_t threads) {
         hv[e] = static_cast<f16>(o0[e] * inv);
         hv[4 + e] = static_cast<f16>(o1[e] * inv);
     }
-    store_half8(a.out + at * a.D + 8 * c, hv);
+    store_half8(a.out + at * D + 8 * c, hv);
     if (a.lse && c == 0)
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
-// Ranges of keys until every CU has two workgroups, each of at least 4 tiles, and as many
-// as their page ids fit LDS in.
+// Ranges of keys until every CU has two workgroups, each of at least 3 tiles, and as many
+// as their page ids fit LDS in.  (One sequence, us with at least 4 / 3 / 2 tiles: 16 rows of
+// 32/8 heads of 64, window 500, 13.1 / 11.0 / 10.9, 4000 13.8 / 11.9 / 11.8; of 128 15.1 /
+// 14.4 / 14.0; but 700 rows, window 200, 9.7 / 9.7 / 15.8: what the second launch costs.)
 PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window, int sinks) {
     PrefillPlan p{};
     const int64_t pairs = (int64_t)rows * G;
@@ -653,7 +673,7 @@ PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window
     const int64_t keys = window > 0 ? std::min<int64_t>(max_len, (int64_t)window + sinks + block_rows + 2 * kPage)
                                     : max_len;
     const int64_t tiles = (keys + kBN - 1) / kBN;
-    int64_t n = std::min<int64_t>(2 * kCUs / wgs, tiles / 4);
+    int64_t n = std::min<int64_t>(2 * kCUs / wgs, tiles / 3);
     n = std::max<int64_t>(n, (tiles * (kBN / kPage) + kPages - 5) / (kPages - 4));
     n = std::max<int64_t>(n, 1);
     p.tiles_per_split = static_cast<int>((tiles + n - 1) / n);
@@ -696,9 +716,19 @@ int window_prefill(const BoundArgs& a, int batch, bool paged, void* ws, hipStrea
     });
     const int rc = check_launch("window_prefill");
     if (rc || p.nsplit == 1) return rc;
-    const int64_t threads = (int64_t)rh * (a.D / 8);
-    hipLaunchKernelGGL(window_join_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)),
-                       dim3(256), 0, s, a, p, threads);
+    // A wave per (row, head) while they all run at once (16 rows of 32 heads over 16 ranges
+    // 13 us instead of 17), D / 8 lanes above (512 rows of 32 heads over 4: 48.8 instead of
+    // 52.4, rounds of waves that wait for their first loads).
+    const int64_t heads = (int64_t)batch * a.rows * a.Hq;   // rows Hq <= 2^29
+    auto join = [&](auto kernel, int lanes) {
+        const unsigned per = 256 / lanes;
+        hipLaunchKernelGGL(kernel, dim3((static_cast<unsigned>(a.rows) * a.Hq + per - 1) / per, batch),
+                           dim3(256), 0, s, a, p);
+    };
+    if (a.D == 64)
+        heads <= 32 * kCUs ? join(window_join_kernel<64, 8>, 64) : join(window_join_kernel<64, 1>, 8);
+    else
+        heads <= 32 * kCUs ? join(window_join_kernel<128, 4>, 64) : join(window_join_kernel<128, 1>, 16);
     return check_launch("window_prefill (join)");
 }
 

@@ -6,8 +6,9 @@ import pytest
 import kvhp
 from bounded_util import PAGE, Cache, check, decode_ref, plan_ref, workspace
 from gpu_util import from_gpu, note, sync, to_gpu
-from test_gpu_bounded import (_calls, _check_prefill, _check_sums, _prompt_ref, _prompt_weights,
-                              _q, _sums, _sums_ref, _weighted, _window_decode)
+from test_gpu_bounded import (_calls, _check_prefill, _check_sums, _prefill_ref, _prompt_ref,
+                              _prompt_weights, _q, _sums, _sums_ref, _weighted, _window_decode,
+                              _window_prefill)
 
 pytestmark = pytest.mark.gpu
 
@@ -209,3 +210,34 @@ def test_prompt_weights_tiles(hq, hkv, rows):
         rw, tw, ra = _sums_ref(c, w, ages, add, rel, rows, c.lens - 1)
         _check_sums(gw, rw, tw)
         assert np.array_equal(ga, ra)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("rows,n,window", [(16, 400, 0), (5, 1500, 0), (16, 4500, 0), (70, 3000, 1200),
+                                           (300, 700, 0)])
+def test_window_prefill_ranges(hq, hkv, d, rows, n, window):
+    """Few rows over many keys: 2 to dozens of ranges, some sequences with fewer than others
+    and none, rows enough for either way of joining them."""
+    rng = np.random.default_rng([hq, rows, n])
+    c = Cache(rng, [n, n // 3, 40], hkv, d).upload()
+    q = _q(rng, 3, rows, hq, d)
+    note(f"window_prefill {rows} rows over {n} keys, window {window}, {hq}/{hkv} x {d}")
+    _check_prefill(q, c, [n - rows, n // 3 - rows, 30], window, 5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_window_prefill_many_heads_over_ranges(d):
+    """More (row, head) pairs than waves run at once, over a few ranges."""
+    rng = np.random.default_rng([12, d])
+    c = Cache(rng, [900], 16, d).upload()
+    q = _q(rng, 1, 260, 32, d)
+    note(f"window_prefill 260 rows of 32/16 heads of {d} over 900 keys")
+    got, ls = _window_prefill(q, c, [640], 0, 0)
+    some = [0, 1, 31, 100, 258, 259]
+    ref, tol, lref, ltol = [], [], [], []
+    for r in some:
+        x = _prefill_ref(q[:, r:r + 1], c, [640 + r], 0, 0)
+        for acc, y in zip((ref, tol, lref, ltol), x):
+            acc.append(y)
+    check(got[:, some], np.concatenate(ref, 1), np.concatenate(tol, 1), "out")
+    check(ls[:, :, some], np.concatenate(lref, 2), np.concatenate(ltol, 2), "lse")
