@@ -17,12 +17,12 @@
 // cut into ranges of tiles whose sums a second launch adds in order, so the result does
 // not depend on timing.
 //
-// 4096 rows of 32/8 heads of 128 (69 GFLOP) take 93 us, 0.74 PFLOP/s, 32 rows of four
+// 4096 rows of 32/8 heads of 128 (69 GFLOP) take 88 us, 0.78 PFLOP/s, 32 rows of four
 // sequences of 3001 keys at 32/4 heads of 64 9.1.  Bound by the vector unit, per 32 x 32
 // scores 16 times (fma, exp, add) of 24 cycles, 47 us over the prompt if it never waited;
 // the 8 MFMAs of 32 cycles run beside it in other waves, four workgroups a CU.  The rest
 // is a causal prompt's last workgroups, the loads in front of a workgroup's first tile, and the
-// second launch (5).  One wave running the next pairs' MFMAs between the exponentials of
+// second launch (4).  One wave running the next pairs' MFMAs between the exponentials of
 // these was no faster (three workgroups a CU, 104 us); 64 keys a wave, half the LDS reads,
 // spill registers (136 to 300).
 #include "bounded.h"
@@ -83,18 +83,16 @@ __device__ __forceinline__ Rows rows_of(const BoundArgs& a, int b, int n) {
     r.p1 = static_cast<int>(max(min(r.first + a.rows, (int64_t)n) - 1, (int64_t)-1));
     return r;
 }
-// Tiles [lo, hi) of a range with rows that see a key of [j0, j1].
+// Tiles [lo, hi) with rows that see a key of [j0, j1].
 __device__ __forceinline__ void tiles_of(const BoundArgs& a, const SumPlan& p, const Rows& r,
-                                         int j0, int j1, int range, int& lo, int& hi) {
+                                         int j0, int j1, int& lo, int& hi) {
     const int q0 = max(r.p0, j0);
     int64_t q1 = r.p1;
     if (a.window > 0 && j0 >= a.sinks) q1 = min(q1, (int64_t)j1 + a.window - 1);
     lo = hi = 0;
     if (q1 < q0) return;
-    const int r0 = static_cast<int>(q0 - r.first), r1 = static_cast<int>(q1 - r.first);
-    lo = max((r0 >> p.lr) * p.nh, range * p.range);
-    hi = static_cast<int>(min((int64_t)((r1 >> p.lr) + 1) * p.nh, ((int64_t)range + 1) * p.range));
-    if (hi < lo) hi = lo;
+    lo = (static_cast<int>(q0 - r.first) >> p.lr) * p.nh;
+    hi = ((static_cast<int>(q1 - r.first) >> p.lr) + 1) * p.nh;
 }
 // Whether a live row sees key j.
 __device__ __forceinline__ bool key_seen(const BoundArgs& a, const Rows& r, int j) {
@@ -121,7 +119,9 @@ prompt_weights_kernel(const BoundArgs a, const SumPlan p) {
     if (j0 >= n) return;
     const Rows rr = rows_of(a, b, n);
     int f0, f1;
-    tiles_of(a, p, rr, j0, min(j0 + KB, n) - 1, range, f0, f1);
+    tiles_of(a, p, rr, j0, min(j0 + KB, n) - 1, f0, f1);
+    f0 = max(f0, range * p.range);
+    f1 = static_cast<int>(min((int64_t)f1, ((int64_t)range + 1) * p.range));
     const int n_tiles = f1 - f0;
     const int jw = j0 + 32 * wave;   // this wave's first key
     // the key whose sum this lane ends up with (lanes c32 < 16)
@@ -308,7 +308,8 @@ prompt_weights_kernel(const BoundArgs a, const SumPlan p) {
         bound_add(a, b, kvh, j, n, sum);
 }
 
-// Adds the ranges' sums in order and updates the slots.
+// Adds the ranges' sums in order and updates the slots.  (One load after the other the sums
+// of 56 ranges took 15 us, eight at a time 3.)
 __global__ void __launch_bounds__(256)
 prompt_weights_add_kernel(const BoundArgs a, const SumPlan p) {
     const int j = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, b = blockIdx.z;
@@ -318,19 +319,30 @@ prompt_weights_add_kernel(const BoundArgs a, const SumPlan p) {
     const int j0 = j / KB * KB, j1 = min(j0 + KB, n) - 1;
     const float* ws = p.ws + ((int64_t)b * a.Hkv + kvh) * p.keys_pitch + j;
     const int64_t step = (int64_t)gridDim.z * a.Hkv * p.keys_pitch;
+    int f0, f1;
+    tiles_of(a, p, rr, j0, j1, f0, f1);
     float sum = 0.f;
-    for (int r = 0; r < p.nrange; ++r) {
-        int lo, hi;
-        tiles_of(a, p, rr, j0, j1, r, lo, hi);
-        if (lo < hi) sum += ws[r * step];
+    if (f0 < f1) {
+        constexpr int U = 8;   // ranges in flight
+        const int last = (f1 - 1) / p.range;
+        for (int r = f0 / p.range; r <= last; r += U) {
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = ws[min(r + u, last) * step];
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum += r + u <= last ? x[u] : 0.f;
+        }
     }
     if (key_seen(a, rr, j) || (int64_t)j + a.new_keys >= n) bound_add(a, b, kvh, j, n, sum);
 }
 
 // Tiles of one head's 64 rows, or of all rows where they are fewer, of as many heads as fit.
-// Ranges of at least 4 tiles, for about 12 workgroups per CU, of which half see nothing in a
-// whole prompt (for 7 / 8 / 10 / 14 / 16: 101 / 105 / 97 / 97 / 101 us where 12 take 96:
-// whole rounds of four a CU).
+// Ranges of at least 6 tiles, for about 12 workgroups per CU, of which half see nothing in a
+// whole prompt (4096 rows of 32/8 heads of 128, for 7 / 8 / 10 / 12 / 14 / 16: 101 / 105 /
+// 97 / 96 / 97 / 101 us: whole rounds of four a CU); of at least 2 while all run at once (512
+// rows 10.6 us, 4 tiles 11.6, 8 15.4; but 1000 rows 18.2 / 16.8 / 17.6).  Up to 5 tiles
+// are not worth a second launch (64 rows of 4 heads 8.0 us whole, 10.4 in two; of 7 11.1 and
+// 9.6 in four).
 SumPlan plan_of(int batch, int rows, int hkv, int G, int max_len) {
     SumPlan p{};
     while (p.lr < 6 && (1 << p.lr) < rows) ++p.lr;
@@ -338,7 +350,9 @@ SumPlan plan_of(int batch, int rows, int hkv, int G, int max_len) {
     p.nh = (G + p.gc - 1) / p.gc;
     const int64_t tiles = (((int64_t)rows + (1 << p.lr) - 1) >> p.lr) * p.nh;
     const int64_t blocks = ((int64_t)max_len + KB - 1) / KB * hkv * batch;
-    const int64_t nr = std::min((3000 + blocks - 1) / blocks, (tiles + 3) / 4);
+    const int64_t most = (3000 + blocks - 1) / blocks, once = 1024 / blocks;
+    const int64_t nr = tiles <= 5 ? 1
+        : std::min(most, std::max((tiles + 5) / 6, std::min((tiles + 1) / 2, once)));
     p.range = static_cast<int>(std::min<int64_t>((tiles + nr - 1) / nr, INT32_MAX));
     p.nrange = static_cast<int>((tiles + p.range - 1) / p.range);
     p.keys_pitch = (max_len + 255) / 256 * 256;
