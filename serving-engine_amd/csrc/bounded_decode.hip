@@ -29,7 +29,7 @@
 // sequences of up to 8192 keys, 32/8 heads of 128: windows of 4096 73.5 us, 412 MB at
 // 5.6 TB/s (shuffled pages alone read at 5.9-6.3); every key with its sums 122-125 us, of
 // which 114 are the first launch's, 579 MB at 5.1 TB/s, and 11 the second's.  One
-// sequence of 1028 visible keys at D = 64 takes 7.1 us, 500 5.1 in one launch, 2048 with
+// sequence of 1028 visible keys at D = 64 takes 6.9 us and 500 5.1, in one launch, 2048 with
 // sums 8.7: launches, and the latency of their loads.  Where several waves share a split,
 // each joins the dims of one MFMA block for all of them (one wave joining everything cost
 // 0.7 us more at D = 64 and 2 at D = 128).
@@ -41,6 +41,7 @@ namespace kvhp {
 namespace {
 
 constexpr int kMaxChunk = 960;    // keys per split: at most 64 pages, three of them cut
+constexpr int kMaxOne = 1152;     // and where one split takes all, at D = 64
 constexpr int kHeads = 16;        // query heads per workgroup
 
 struct DecodePlan {
@@ -173,15 +174,21 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
     // Visible key v is position v + (v >= sinks ? shift : 0).
     const int shift = a.window > 0 ? bound_len(a, b) - L : 0;
     const int sinks = shift > 0 ? a.sinks : 0;
-    // Page ids of the chunk, one per lane: those of its first tokens, then the others.
-    int pidv = 0, n_a = 0, p_a = 0, p_b = 0;
+    // Page ids of the chunk, one per lane (two where one split takes all, up to 75 pages):
+    // those of its first tokens, then the others.
+    constexpr bool kTwo = W == 8 && D == 64 && !SUMS;
+    int pidv = 0, pid2 = 0, n_a = 0, p_a = 0, p_b = 0;
     if constexpr (PAGED) {
         p_a = t_begin >> 4;
         n_a = t_begin < sinks ? ((min(t_end, sinks) - 1) >> 4) - p_a + 1 : 0;
         p_b = (max(t_begin, sinks) + shift) >> 4;
         const int last = t_end > sinks ? (t_end - 1 + shift) >> 4 : (t_end - 1) >> 4;
-        const int pi = min(lane < n_a ? p_a + lane : p_b + lane - n_a, last);
-        pidv = min(max(a.k.bt[(int64_t)b * a.k.max_pages + pi], 0), a.k.num_pages - 1);
+        auto page = [&](int i) {
+            const int pi = min(i < n_a ? p_a + i : p_b + i - n_a, last);
+            return min(max(a.k.bt[(int64_t)b * a.k.max_pages + pi], 0), a.k.num_pages - 1);
+        };
+        pidv = page(lane);
+        if constexpr (kTwo) pid2 = page(lane + kWave);
     }
     const char* kbase = reinterpret_cast<const char*>(
         a.k.data + (PAGED ? 0 : b * a.k.stride_b) + kvh * a.k.stride_h);
@@ -206,7 +213,12 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
             const int real = first ? v : v + shift;
             if constexpr (PAGED) {
                 const int at = first ? (real >> 4) - p_a : (real >> 4) - p_b + n_a;
-                r[j] = (uint32_t)__builtin_amdgcn_ds_bpermute(at << 2, pidv) * kPage + (real & 15);
+                int pid = __builtin_amdgcn_ds_bpermute(at << 2, pidv);
+                if constexpr (kTwo) {
+                    const int other = __builtin_amdgcn_ds_bpermute(at << 2, pid2);
+                    pid = at < kWave ? pid : other;
+                }
+                r[j] = (uint32_t)pid * kPage + (real & 15);
             } else {
                 r[j] = real;
             }
@@ -580,12 +592,13 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums) {
     const int64_t per = std::max<int64_t>(64, ((maxv + 63) / 64 + 63) / 64 * 64);
     int64_t s = std::min((maxv + per - 1) / per, units >= 6144 ? 1 : 6144 / units);
     int64_t chunk = std::min<int64_t>(((maxv + s - 1) / s + 63) / 64 * 64, kMaxChunk);
-    // Up to kMaxChunk keys (576 at D = 128) a small batch takes one split: eight waves share its
+    // Up to kMaxOne keys (576 at D = 128) a small batch takes one split: eight waves share its
     // steps, and no second launch joins.  One sequence, 32/8 heads, us as one split / as
     // splits of 64 keys: D = 64 500 keys 5.2 / 7.0, 1028 6.8 / 7.1, 1500 8.1 / 7.0; D = 128
-    // 500 7.2 / 7.8, 700 8.6 / 8.0.  With sums there is a second launch anyway: 128 keys 8.2
-    // / 8.4 and 9.1 / 9.0, 350 9.1 / 8.4 and 10.7 / 9.1.
-    if (batch < 8 && maxv <= (sums ? 128 : d == 64 ? kMaxChunk : 576)) chunk = (maxv + 31) / 32 * 32;
+    // 500 7.2 / 7.8, 700 8.6 / 8.0 (replayed from a graph the splits win from 1000 and 550
+    // on, called among other work only from 1500 and 800).  With sums there is a second
+    // launch anyway: 128 keys 8.2 / 8.4 and 9.1 / 9.0, 350 9.1 / 8.4 and 10.7 / 9.1.
+    if (batch < 8 && maxv <= (sums ? 128 : d == 64 ? kMaxOne : 576)) chunk = (maxv + 31) / 32 * 32;
     p.chunk = static_cast<int>(chunk);
     p.nsplit = static_cast<int>((maxv + chunk - 1) / chunk);
     p.min_chunk = batch >= 16 ? 64 : 128;

@@ -23,13 +23,15 @@
 // lane's fixed offset; page ids from LDS), with their 16-byte chunks XOR-swizzled so that
 // both operand reads touch all banks.
 //
-// Bound, at 8192 rows, window 2048, 32/8 heads of 128 (258 us, 0.94 PFLOP/s): the MFMAs
-// alone take 172 us of it (1.45 PFLOP/s, the clock the card holds under them); without
-// the exponentials the kernel takes 228, without LDS operand reads 234, without loads
-// 225: LDS is busy 2/3 to 9/10 of the time, 64 KB read per wave pair and tile, and more
-// pairs a wave, which would halve that, need more registers than the 256 a lane of two
-// waves per SIMD has (64 pairs on one wave per SIMD, O and Q in accumulation registers:
-// 625 us, the compiler moves O between the register files at every branch).
+// At 8192 rows, window 2048, 32/8 heads of 128: 255-268 us by box, 0.90-0.95 PFLOP/s; four
+// chunks of 128 rows behind 4096 keys 47, of which the join 7.  Counters: matrix cores 55 %,
+// vector unit 50 %, LDS reads 28 % of the cycles, at the 1.6 GHz that the card holds under
+// this load (a large library product: 1.18 PFLOP/s).  The MFMAs alone take 172 us of 262;
+// without the exponentials the kernel takes 228, without LDS operand reads 234, without
+// loads 225.  More waves do not help (tiles of 32 keys, three workgroups a CU: 280); more
+// pairs a wave, half the LDS reads, need more registers than the 256 a lane of two waves
+// per SIMD has (64 pairs on one wave per SIMD, O and Q in accumulation registers: 625, the
+// compiler moves O between the register files at every branch).
 //
 // A masked key's weight is 0, but 0 times an infinite or NaN V is NaN: in the
 // tiles that some row sees only in part such elements are set to 0 in LDS, noted,

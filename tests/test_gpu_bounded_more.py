@@ -163,7 +163,8 @@ def test_padded_batches():
     assert np.array_equal(ga, ra)
 
 
-@pytest.mark.parametrize("d,visible", [(64, 959), (64, 960), (64, 961), (128, 575), (128, 576),
+@pytest.mark.parametrize("d,visible", [(64, 959), (64, 960), (64, 961), (64, 1029),
+                                       (64, 1151), (64, 1152), (64, 1153), (128, 575), (128, 576),
                                        (128, 577), (64, 31), (128, 33)])
 @pytest.mark.parametrize("sinks", [0, 1, 17])
 def test_window_decode_split_limits(d, visible, sinks):
