@@ -21,7 +21,8 @@
 // Sums: the scores go to the workspace in fp32, 32 keys of each head side by side;
 // once the maximum and the sum of every head are known from the chunks' partials,
 // the launch that joins the partials also turns the scores into weights, adds them
-// over the heads of a KV head and updates the slots.  (16 bytes a key and four
+// over the heads of a KV head and updates the slots; a workgroup that holds all heads and
+// keys of a KV head does so itself, without a second launch.  (16 bytes a key and four
 // heads, written and read, beside 512 of K and V at D = 128.  Written past the
 // caches they cost 132 us instead of 125 below.)
 //
@@ -51,6 +52,7 @@ struct DecodePlan {
     int balance;      // > 0: about this many splits per KV head over the batch
     int min_chunk, max_chunk;
     int groups;       // workgroups per KV head and split, of up to kHeads query heads
+    int fused;        // 1: one split and one workgroup per KV head, which adds its sums itself
     int scap;         // keys that the scores have room for, a multiple of 32
     float* ws_o;      // [B * Hq][nsplit][D]
     float* ws_ml;     // [B * Hq][nsplit][2], the maximum in log2 units
@@ -96,6 +98,34 @@ __device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
 }
 __device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
     return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Four keys of a KV head from j (a multiple of 4) on: their slot (-1: none) and sums.
+struct Quad {
+    int64_t slot;
+    floatx4 old;
+};
+__device__ __forceinline__ Quad quad_at(const BoundArgs& a, int b, int kvh, int j) {
+    Quad q{bound_slot(a.k, b, kvh, j), {0.f, 0.f, 0.f, 0.f}};   // four in one page
+    if (q.slot >= 0) q.old = *reinterpret_cast<const floatx4*>(a.weights + q.slot);
+    return q;
+}
+// Adds the weights w of keys j .. j + 3 to their sums, or starts them, with their ages.
+__device__ __forceinline__ void put_quad(const BoundArgs& a, const Quad& q, int b, int j, int n,
+                                         const floatx4& w) {
+    if (j >= n || q.slot < 0) return;
+    const int64_t fresh = (int64_t)n - a.new_keys;     // keys from here on start anew
+    floatx4 x = q.old;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < n) x[e] = j + e >= fresh ? w[e] : x[e] + w[e];
+    *reinterpret_cast<floatx4*>(a.weights + q.slot) = x;   // slots behind the sequence as they were
+    if (a.ages && j + 3 >= fresh) {
+        const int newest = a.newest ? a.newest[b] : n - 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < n && j + e >= fresh) a.ages[q.slot + e] = newest - (n - 1 - j - e);
+    }
 }
 
 // W waves per workgroup take the steps of one split round robin and meet in LDS.
@@ -351,6 +381,29 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
         }
     }
 
+    // One workgroup holds every head of its KV head and all keys: its thread t adds the sums of
+    // keys 4t .. 4t + 3, whose slots' loads start here.
+    constexpr bool kSums = SUMS && W == 8;
+    static_assert(!kSums || kMaxChunk <= 4 * W * kWave, "a quad of keys per thread");
+    __shared__ float head[kSums ? kHeads : 1][2];   // -M in log2 units, 1 / sum
+    const int j4 = 4 * threadIdx.x;
+    Quad quad{};
+    if constexpr (kSums)
+        if (p.fused) quad = quad_at(a, b, kvh, min(j4, L - 1) & ~3);
+    auto sums = [&]() {
+        __syncthreads();   // the heads, and every wave's scores
+        if (j4 >= L) return;
+        const float* sj = p.ws_s + score_at(a, p, b, kvh, j4 & ~31) + (j4 & 31);
+        floatx4 w = {0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < nh; ++h) {
+            const floatx4 x = *reinterpret_cast<const floatx4*>(sj + 32 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = fmaf(fast_exp2(fmaf(x[e], sc, head[h][0])), head[h][1], w[e]);
+        }
+        put_quad(a, quad, b, j4, L, w);
+    };
+
     // Dims 16 (d0 + i) + 4g + e of head col: all of them, or wave d0's share of the waves' sum.
     constexpr int NB = W > 1 ? 1 : ND;
     floatx4 r[NB];
@@ -367,7 +420,11 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
             *reinterpret_cast<floatx4*>(&xs[(db * kWave + lane) * 4]) = o[db];
         *reinterpret_cast<float2*>(&xs[ND * kWave * 4 + 2 * lane]) = float2{m_run, l_part};
         __syncthreads();
-        if (wv >= ND) return;
+        if (wv >= ND) {
+            if constexpr (kSums)
+                if (p.fused) sums();
+            return;
+        }
         d0 = wv;
         float2 ml[W];
         floatx4 x[W];
@@ -389,6 +446,15 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
     }
 
     const float l_tot = rows4_sum(l_part);
+    if constexpr (kSums) {
+        if (p.fused) {
+            if (hvalid && g == 0 && d0 == 0) {
+                head[col][0] = -m_run * sc;
+                head[col][1] = 1.f / l_tot;
+            }
+            sums();
+        }
+    }
     if (!hvalid) return;
     const int64_t prow = (row0 + col) * p.nsplit + split;
     if ((SUMS || nsb > 1) && g == 0 && d0 == 0) {
@@ -524,9 +590,8 @@ bound_sums_kernel(const BoundArgs a, const DecodePlan p, int key_blocks) {
     const int j = at * kSumKeys + 4 * tid;
     const int jc = min(j, n - 1) & ~3;
     const float* sj = p.ws_s + score_at(a, p, b, kvh, jc & ~31) + (jc & 31);
-    const int64_t slot = bound_slot(a.k, b, kvh, jc);   // of four in one page
-    floatx4 old = {0.f, 0.f, 0.f, 0.f}, w = old;
-    if (slot >= 0) old = *reinterpret_cast<const floatx4*>(a.weights + slot);
+    const Quad quad = quad_at(a, b, kvh, jc);
+    floatx4 w = {0.f, 0.f, 0.f, 0.f};
     constexpr int H = 8, HW = H / kJoinWaves;   // heads at a time, and per wave
     __shared__ float head[H][2];                // -M in log2 units, 1 / sum
     for (int g0 = 0; g0 < a.G; g0 += H) {
@@ -569,18 +634,7 @@ bound_sums_kernel(const BoundArgs a, const DecodePlan p, int key_blocks) {
         }
         __syncthreads();
     }
-    if (j >= n || slot < 0) return;
-    const int64_t fresh = (int64_t)n - a.new_keys;     // keys from here on start anew
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (j + e < n) old[e] = j + e >= fresh ? w[e] : old[e] + w[e];
-    *reinterpret_cast<floatx4*>(a.weights + slot) = old;   // slots behind the sequence as they were
-    if (a.ages && j + 3 >= fresh) {
-        const int newest = a.newest ? a.newest[b] : n - 1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (j + e < n && j + e >= fresh) a.ages[slot + e] = newest - (n - 1 - j - e);
-    }
+    put_quad(a, quad, b, j, n, w);
 }
 
 // ------------------------------------------------------------------ plan --
@@ -596,9 +650,12 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums) {
     // steps, and no second launch joins.  One sequence, 32/8 heads, us as one split / as
     // splits of 64 keys: D = 64 500 keys 5.2 / 7.0, 1028 6.8 / 7.1, 1500 8.1 / 7.0; D = 128
     // 500 7.2 / 7.8, 700 8.6 / 8.0 (replayed from a graph the splits win from 1000 and 550
-    // on, called among other work only from 1500 and 800).  With sums there is a second
-    // launch anyway: 128 keys 8.2 / 8.4 and 9.1 / 9.0, 350 9.1 / 8.4 and 10.7 / 9.1.
-    if (batch < 8 && maxv <= (sums ? 128 : d == 64 ? kMaxOne : 576)) chunk = (maxv + 31) / 32 * 32;
+    // on, called among other work only from 1500 and 800).  With sums, which the split's
+    // workgroup then adds itself: 128 keys 5.3 / 8.4, 700 7.8 / 8.6, 960 8.7 / 8.8; D = 128
+    // 350 7.9 / 9.2, 500 9.0 / 9.4.  (Of more than 16 heads a KV head a second launch adds the
+    // workgroups' sums: 128 keys 8.2 / 8.4, 350 9.1 / 8.4.)
+    const int one = !sums ? (d == 64 ? kMaxOne : 576) : p.groups > 1 ? 128 : d == 64 ? 704 : 448;
+    if (batch < 8 && maxv <= one) chunk = (maxv + 31) / 32 * 32;
     p.chunk = static_cast<int>(chunk);
     p.nsplit = static_cast<int>((maxv + chunk - 1) / chunk);
     p.min_chunk = batch >= 16 ? 64 : 128;
@@ -649,6 +706,7 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
         else
             p.balance = 0;
     }
+    p.fused = SUMS && !wide && p.balance == 0 && p.nsplit == 1 && p.groups == 1;
     // one split: eight waves take its steps round robin; fixed splits at D = 64: four
     // (at D = 128 four are no faster on one sequence and 26-52 % slower on four of 1024
     // to 4000 keys)
@@ -663,11 +721,11 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
         go(bound_decode_kernel<D, PAGED, SUMS, D == 64 ? 4 : 1>, 4);
     else
         go(bound_decode_kernel<D, PAGED, SUMS, 1>, 1);
-    if (SUMS) {
+    if (SUMS && !p.fused) {
         const int kb = (a.cap + kSumKeys - 1) / kSumKeys;
         hipLaunchKernelGGL((bound_sums_kernel<D>), dim3(kb + (p.nsplit > 1 ? a.G : 0), a.Hkv, p.batch),
                            dim3(kJoinWaves * kWave), 0, s, a, p, kb);
-    } else if (p.nsplit > 1) {
+    } else if (!SUMS && p.nsplit > 1) {
         hipLaunchKernelGGL((bound_join_kernel<D>), dim3(a.Hq, p.batch), dim3(kJoinWaves * kWave), 0,
                            s, a, p);
     }

@@ -179,14 +179,16 @@ def test_window_decode_split_limits(d, visible, sinks):
         check(_window_decode(q, c, visible - sinks, sinks), ref, tol)
 
 
-@pytest.mark.parametrize("n", [127, 128, 129, 160])
-@pytest.mark.parametrize("d", [64, 128])
-def test_weighted_decode_split_limits(n, d):
-    rng = np.random.default_rng([n, d])
-    c = Cache(rng, [n, 1, n - 1], 2, d).upload()
-    q = _q(rng, 3, 14, d)
+@pytest.mark.parametrize("n", [5, 127, 128, 129, 160, 447, 448, 449, 703, 704, 705])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (14, 2, 128), (16, 1, 64), (17, 1, 128)])
+def test_weighted_decode_split_limits(n, hq, hkv, d):
+    """Keys on both sides of what one workgroup a KV head takes, with its sums or without;
+    shorter sequences and none beside them."""
+    rng = np.random.default_rng([n, hq, d])
+    c = Cache(rng, [n, 1, 0, n - 1], hkv, d).upload()
+    q = _q(rng, 4, hq, d)
     w, ages = _sums(rng, c)
-    note(f"weighted_decode {n} keys, d={d}")
+    note(f"weighted_decode {n} keys, {hq}/{hkv} x {d}")
     out, gw, ga = _weighted(q, c, w, ages, 1, None)
     ref, tol, sums, rel = decode_ref(q, c, 0, 0)
     check(out, ref, tol)
