@@ -206,7 +206,7 @@ bound_decode_kernel(const BoundArgs a, const DecodePlan p) {
     const int sinks = shift > 0 ? a.sinks : 0;
     // Page ids of the chunk, one per lane (two where one split takes all, up to 75 pages):
     // those of its first tokens, then the others.
-    constexpr bool kTwo = W == 8 && D == 64 && !SUMS;
+    constexpr bool kTwo = (W == 8 || WIDE) && D == 64 && !SUMS;
     int pidv = 0, pid2 = 0, n_a = 0, p_a = 0, p_b = 0;
     if constexpr (PAGED) {
         p_a = t_begin >> 4;
@@ -646,16 +646,20 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums) {
     const int64_t per = std::max<int64_t>(64, ((maxv + 63) / 64 + 63) / 64 * 64);
     int64_t s = std::min((maxv + per - 1) / per, units >= 6144 ? 1 : 6144 / units);
     int64_t chunk = std::min<int64_t>(((maxv + s - 1) / s + 63) / 64 * 64, kMaxChunk);
-    // Up to kMaxOne keys (576 at D = 128) a small batch takes one split: eight waves share its
-    // steps, and no second launch joins.  One sequence, 32/8 heads, us as one split / as
-    // splits of 64 keys: D = 64 500 keys 5.2 / 7.0, 1028 6.8 / 7.1, 1500 8.1 / 7.0; D = 128
-    // 500 7.2 / 7.8, 700 8.6 / 8.0 (replayed from a graph the splits win from 1000 and 550
-    // on, called among other work only from 1500 and 800).  With sums, which the split's
-    // workgroup then adds itself: 128 keys 5.3 / 8.4, 700 7.8 / 8.6, 960 8.7 / 8.8; D = 128
-    // 350 7.9 / 9.2, 500 9.0 / 9.4.  (Of more than 16 heads a KV head a second launch adds the
-    // workgroups' sums: 128 keys 8.2 / 8.4, 350 9.1 / 8.4.)
-    const int one = !sums ? (d == 64 ? kMaxOne : 576) : p.groups > 1 ? 128 : d == 64 ? 704 : 448;
-    if (batch < 8 && maxv <= one) chunk = (maxv + 31) / 32 * 32;
+    // Up to `one` keys a sequence takes one split: eight waves share its steps, and no second
+    // launch joins.  One sequence, 32/8 heads, us as one split / as splits of 64 keys: D = 64
+    // 500 keys 5.2 / 7.0, 1028 6.8 / 7.1, 1500 8.1 / 7.0; D = 128 500 7.2 / 7.8, 700 8.6 / 8.0
+    // (replayed from a graph the splits win from 1000 and 550 on, called among other work only
+    // from 1500 and 800).  Batches, against splits of all lengths' size: 32 of up to 300 keys
+    // 5.0 / 10.8 and 6.4 / 12.1, of 1100 10.6 / 14.0 and 21.0 / 20.4; 256 of up to 560 40.6 /
+    // 48.7 and 64 / 78.  With sums, which the split's workgroup then adds itself: one of 128
+    // 5.3 / 8.4, 700 7.8 / 8.6, 960 8.7 / 8.8; D = 128 350 7.9 / 9.2, 500 9.0 / 9.4; 32 of up
+    // to 700 8.0 / 14.4 and 17.7 / 19.7.  (Of more than 16 heads a KV head a second launch
+    // adds the workgroups' sums: 128 keys 8.2 / 8.4, 350 9.1 / 8.4.)
+    const int one = d == 64 ? (!sums ? kMaxOne : p.groups > 1 ? 128 : batch < 8 ? 704 : kMaxChunk)
+                            : (!sums ? (batch < 8 ? 576 : kMaxChunk)
+                                     : p.groups > 1 ? 128 : batch < 8 ? 448 : 640);
+    if (maxv <= one) chunk = (maxv + 31) / 32 * 32;
     p.chunk = static_cast<int>(chunk);
     p.nsplit = static_cast<int>((maxv + chunk - 1) / chunk);
     p.min_chunk = batch >= 16 ? 64 : 128;
@@ -697,7 +701,7 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
     const int64_t reach = PAGED ? (int64_t)a.k.num_pages * kPage : a.cap;   // rows of a head
     const bool wide = reach * std::max(a.k.stride_s, a.v.stride_s) >= (int64_t)1 << 31;
     dim3 grid(heads, p.nsplit, p.batch);
-    if (p.batch >= 8) {
+    if (p.batch >= 8 && p.nsplit > 1) {
         p.balance = std::max(1, kWaveSlots / heads - p.batch / 2);
         const int64_t worst = (p.batch * maxv + p.max_chunk - 1) / p.max_chunk;
         const int64_t units = std::max<int64_t>(p.balance, worst) + p.batch;

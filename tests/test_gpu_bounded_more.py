@@ -41,7 +41,7 @@ def test_pools_past_32_bit_offsets(hq, hkv, d):
     c = _far(Cache(rng, [1500, 333], hkv, d), (1 << 32) // (2 * PAGE * d) + 200)
     assert int(c.bt.max()) * PAGE * d * 2 >= 1 << 32
     q = _q(rng, 2, hq, d)
-    for window, sinks in [(0, 0), (700, 4)]:
+    for window, sinks in [(0, 0), (700, 4), (1100, 20)]:
         note(f"far pages: window_decode window={window}")
         ref, tol, _, _ = decode_ref(q, c, window, sinks)
         check(_window_decode(q, c, window, sinks), ref, tol)
@@ -244,3 +244,22 @@ def test_window_prefill_many_heads_over_ranges(d):
             acc.append(y)
     check(got[:, some], np.concatenate(ref, 1), np.concatenate(tol, 1), "out")
     check(ls[:, :, some], np.concatenate(lref, 2), np.concatenate(ltol, 2), "lse")
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128), (17, 1, 64)])
+@pytest.mark.parametrize("n", [30, 639, 641, 959, 961, 1200])
+def test_batches_split_limits(n, hq, hkv, d):
+    """Batches of 9 ragged sequences on both sides of what one workgroup a KV head takes."""
+    rng = np.random.default_rng([n, hq, d])
+    c = Cache(rng, [n, 1, 0, n - 1, n // 2, 17, n, n // 3, 64][:9], hkv, d,
+              cap=n).upload()
+    q = _q(rng, 9, hq, d)
+    w, ages = _sums(rng, c)
+    note(f"batches: {n} keys, {hq}/{hkv} x {d}")
+    ref, tol, sums, rel = decode_ref(q, c, 0, 0)
+    check(_window_decode(q, c, 0, 0), ref, tol)
+    out, gw, ga = _weighted(q, c, w, ages, 1, None)
+    check(out, ref, tol)
+    rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 1, np.minimum(c.lens, c.cap) - 1)
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
