@@ -263,3 +263,24 @@ def test_batches_split_limits(n, hq, hkv, d):
     rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 1, np.minimum(c.lens, c.cap) - 1)
     _check_sums(gw, rw, tw)
     assert np.array_equal(ga, ra)
+
+
+@pytest.mark.parametrize("batch", [7, 15, 16, 17])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
+def test_batches_of_long_sequences(batch, hq, hkv, d):
+    """Fixed splits and the batch's own, with sequences of every length beside each other."""
+    rng = np.random.default_rng([batch, d])
+    lens = rng.integers(0, 2600, batch)
+    lens[:3] = [2600, 0, 1]
+    c = Cache(rng, lens, hkv, d).upload()
+    q = _q(rng, batch, hq, d)
+    w, ages = _sums(rng, c)
+    note(f"a batch of {batch}, {hq}/{hkv} x {d}")
+    ref, tol, _, _ = decode_ref(q, c, 1500, 4)
+    check(_window_decode(q, c, 1500, 4), ref, tol)
+    ref, tol, sums, rel = decode_ref(q, c, 0, 0)
+    out, gw, ga = _weighted(q, c, w, ages, 1, None)
+    check(out, ref, tol)
+    rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 1, c.lens - 1)
+    _check_sums(gw, rw, tw)
+    assert np.array_equal(ga, ra)
