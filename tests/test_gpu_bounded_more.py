@@ -284,3 +284,35 @@ def test_batches_of_long_sequences(batch, hq, hkv, d):
     rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 1, c.lens - 1)
     _check_sums(gw, rw, tw)
     assert np.array_equal(ga, ra)
+
+
+def test_graph_replays_of_short_sequences():
+    """One workgroup a KV head with its sums, captured once: each replay adds once more."""
+    import torch
+    rng = np.random.default_rng(21)
+    c = Cache(rng, [300, 17, 0, 101], 2, 64).upload()
+    q = to_gpu(_q(rng, 4, 8, 64))
+    out = torch.zeros_like(q)
+    w = torch.zeros(2, c.pages, PAGE, device="cuda")
+    ws = workspace(kvhp.weighted_decode_workspace_bytes(4, 8, 2, 64, 300))
+
+    def go():
+        kvhp.weighted_decode(q, c.kv, c.vv, c.lens_d, out, w, 8, 2, 64, 300, new_keys=0,
+                             workspace=ws)
+    note("weighted_decode of short sequences: eager")
+    go()
+    sync()
+    once, first = w.clone(), out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        go()
+    w.zero_()
+    want = torch.zeros_like(w)
+    for i in range(4):
+        note(f"replay {i}")
+        out.fill_(3)
+        sync()
+        g.replay()
+        sync()
+        want += once      # the same fp32 sums in the same order
+        assert torch.equal(w, want) and torch.equal(out, first)
