@@ -85,6 +85,14 @@ __device__ __forceinline__ void bound_add(const BoundArgs& a, int b, int kvh, in
 
 // ---------------------------------------------------------------- host ----
 int bound_check_view(const kvhp_kv_view* v, const char* what, const char* name);
+constexpr int kMaxBatch = 65535, kMaxKvHeads = 65535;   // grid dimensions
+constexpr int kMaxHeads = 1 << 25, kMaxLen = 1 << 30;
+// What bound_shapes takes: the size queries, which a caller asks first, plan for nothing else.
+inline bool bound_sizes(int batch, int hq, int hkv, int max_len, int window, int sinks) {
+    return batch > 0 && batch <= kMaxBatch && hkv > 0 && hkv <= kMaxKvHeads && hq > 0 &&
+           hq <= kMaxHeads && hq % hkv == 0 && max_len > 0 && max_len <= kMaxLen && window >= 0 &&
+           sinks >= 0;
+}
 // Shapes every call checks; fills the fields of `a` that they give.
 int bound_shapes(BoundArgs& a, const char* what, int batch, int hq, int hkv, int d,
                  int max_seq_len, int window, int sinks);

@@ -28,9 +28,10 @@ int bound_shapes(BoundArgs& a, const char* what, int batch, int hq, int hkv, int
                  d);
     KVHP_REQUIRE(window >= 0 && sinks >= 0, KVHP_ERR_INVALID,
                  "%s: window=%d and sinks=%d must not be negative", what, window, sinks);
-    KVHP_REQUIRE(batch <= 65535 && hkv <= 65535, KVHP_ERR_UNSUPPORTED,
+    KVHP_REQUIRE(batch <= kMaxBatch && hkv <= kMaxKvHeads, KVHP_ERR_UNSUPPORTED,
                  "%s: more than 65535 sequences or KV heads", what);
-    KVHP_REQUIRE(max_seq_len <= 1 << 30, KVHP_ERR_UNSUPPORTED, "%s: max_seq_len=%d above 2^30",
+    KVHP_REQUIRE(hq <= kMaxHeads, KVHP_ERR_UNSUPPORTED, "%s: num_q_heads=%d above 2^25", what, hq);
+    KVHP_REQUIRE(max_seq_len <= kMaxLen, KVHP_ERR_UNSUPPORTED, "%s: max_seq_len=%d above 2^30",
                  what, max_seq_len);
     a.Hq = hq;
     a.Hkv = hkv;
@@ -202,7 +203,7 @@ extern "C" size_t kvhp_window_decode_workspace_bytes(int batch, int num_q_heads,
                                                      int head_dim, int max_seq_len, int window,
                                                      int sinks) {
     return bound_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len, window,
-                                  window > 0 ? sinks : 0, false);
+                                  sinks, false);
 }
 
 extern "C" int kvhp_window_decode(const void* q, const kvhp_kv_view* k_view,
@@ -285,7 +286,7 @@ extern "C" size_t kvhp_window_prefill_workspace_bytes(int batch, int rows, int n
                                                       int num_kv_heads, int head_dim,
                                                       int max_seq_len, int window, int sinks) {
     return window_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len,
-                                    window, window > 0 ? sinks : 0);
+                                    window, sinks);
 }
 
 extern "C" int kvhp_window_prefill(const void* q, const kvhp_kv_view* k_view,

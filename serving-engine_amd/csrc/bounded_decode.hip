@@ -676,9 +676,7 @@ constexpr int kWaveSlots = 2048;
 
 size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int window, int sinks,
                               bool sums) {
-    if (batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || cap <= 0 || cap > 1 << 30 ||
-        (d != 64 && d != 128))
-        return 0;
+    if (!bound_sizes(batch, hq, hkv, cap, window, sinks) || (d != 64 && d != 128)) return 0;
     const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks), sums);
     const size_t rows = (size_t)batch * hq;
     size_t n = p.nsplit > 1 || sums ? rows * p.nsplit * 2 : 0;

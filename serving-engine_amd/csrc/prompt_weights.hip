@@ -35,6 +35,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 64;        // pairs per tile
 constexpr int KB = 32 * kWaves;  // keys per workgroup
+constexpr int kMaxRowHeads = 1 << 30;   // (row, query head) pairs of a KV head
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) f16 lds_f16;
@@ -362,17 +363,17 @@ SumPlan plan_of(int batch, int rows, int hkv, int G, int max_len) {
 }  // namespace
 
 size_t prompt_weights_workspace(int batch, int rows, int hq, int hkv, int d, int max_len) {
-    if (batch <= 0 || rows <= 0 || hkv <= 0 || hq < hkv || hq % hkv || max_len <= 0 ||
-        max_len > 1 << 30 || (d != 64 && d != 128))
+    if (rows <= 0 || !bound_sizes(batch, hq, hkv, max_len, 0, 0) ||
+        (int64_t)rows * (hq / hkv) > kMaxRowHeads || (d != 64 && d != 128))
         return 0;
     const SumPlan p = plan_of(batch, rows, hkv, hq / hkv, max_len);
     return p.nrange == 1 ? 0 : sizeof(float) * (size_t)p.nrange * batch * hkv * p.keys_pitch;
 }
 
 bool prompt_weights_fits(const BoundArgs& a, int batch) {
+    if ((int64_t)a.rows * a.G > kMaxRowHeads) return false;   // tiles in an int
     const SumPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len);
     return (a.D == 64 || a.D == 128) && p.nrange <= 65535 &&
-           (int64_t)a.rows * a.G <= 1 << 30 &&                // tiles in an int
            (int64_t)p.keys_pitch / KB * a.Hkv <= 1 << 22 &&
            (int64_t)kTile * a.Hq * 2 * a.D < (int64_t)1 << 32;   // a tile's offsets
 }

@@ -54,6 +54,7 @@ constexpr int kPages = 4000;          // page ids of a split held in LDS
 constexpr int kMaxStride = 1 << 24;   // halfs between rows: 15 rows stay below 2^31 bytes
 constexpr int kEdge = 6;              // tiles at either edge of the window in a block
 constexpr int kBadWords = 4 * kEdge;  // a bit per key of those
+constexpr int kMaxRowHeads = 1 << 29; // (row, query head) pairs of a sequence: a grid of 2^22
 constexpr int kCUs = 256;
 constexpr float kLazyLog2 = 8.f;
 
@@ -687,17 +688,18 @@ PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window
 
 size_t window_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int max_len,
                                 int window, int sinks) {
-    if (batch <= 0 || rows <= 0 || hkv <= 0 || hq < hkv || hq % hkv || max_len <= 0 || window < 0 ||
-        sinks < 0 || (d != 64 && d != 128))
+    if (rows <= 0 || !bound_sizes(batch, hq, hkv, max_len, window, sinks) ||
+        (int64_t)rows * hq > kMaxRowHeads || (d != 64 && d != 128))
         return 0;
     const PrefillPlan p = plan_of(batch, rows, hkv, hq / hkv, max_len, window, sinks);
     return p.nsplit == 1 ? 0 : sizeof(float) * (size_t)batch * rows * hq * p.nsplit * (d + 2);
 }
 
 bool window_prefill_fits(const BoundArgs& a, int batch) {
+    if ((int64_t)a.rows * a.Hq > kMaxRowHeads) return false;   // the plan counts them in an int
     const PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len, a.window, a.sinks);
     return (a.D == 64 || a.D == 128) && p.nsplit <= 65535 &&
-           (int64_t)p.blocks * a.Hkv <= 1 << 22 && a.k.stride_s < kMaxStride &&
+           (int64_t)p.blocks * a.Hkv <= kMaxRowHeads / kPairs && a.k.stride_s < kMaxStride &&
            (int64_t)a.rows * a.G * a.G < (int64_t)1 << 31 &&   // row_of, and pairs in an int
            a.v.stride_s < kMaxStride;
 }

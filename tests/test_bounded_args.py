@@ -174,3 +174,34 @@ def test_sizes_that_no_call_has():
     _refused(_apply(most=2 ** 31 - 1), kvhp.KVHP_ERR_UNSUPPORTED, "max_moves")
     assert lib.kvhp_weighted_decode_workspace_bytes(2, 8, 2, 64, 2 ** 31 - 1) <= 2 * 8 * 4
     assert lib.kvhp_window_decode_workspace_bytes(2, 8, 2, 64, 2 ** 31 - 1, 0, 0) == 0
+
+
+@pytest.mark.parametrize("window,sinks", [(1, -1), (5, -10), (-1, 0), (-5, 3), (0, -1), (-1, -1),
+                                          (-2 ** 31, -2 ** 31)])
+def test_size_queries_of_refused_windows(window, sinks):
+    """The size is asked before the call that refuses these: none is needed."""
+    lib = kvhp.load()
+    for d in (64, 128):
+        assert lib.kvhp_window_decode_workspace_bytes(1, 8, 2, d, 1000, window, sinks) == 0
+        assert lib.kvhp_window_prefill_workspace_bytes(1, 10, 8, 2, d, 1000, window, sinks) == 0
+
+
+@pytest.mark.parametrize("batch,rows,hq,hkv,cap", [
+    (1 << 30, 1 << 30, 1 << 30, 1, 1000), (1 << 20, 1 << 30, 1 << 30, 1 << 14, 1000),
+    (1 << 30, 64, 1 << 30, 1 << 30, 1 << 30), (65536, 10, 8, 2, 1000), (1, 10, 1 << 26, 1, 1000),
+    (1, 2 ** 31 - 1, 2 ** 31 - 1, 1, 2 ** 31 - 1), (1, 1 << 30, 1, 1, (1 << 30) + 1)])
+def test_size_queries_of_refused_counts(batch, rows, hq, hkv, cap):
+    """Counts whose products leave 64 bits, and others that no call takes."""
+    lib = kvhp.load()
+    assert lib.kvhp_window_decode_workspace_bytes(batch, hq, hkv, 64, cap, 5, 3) == 0
+    assert lib.kvhp_window_prefill_workspace_bytes(batch, rows, hq, hkv, 64, cap, 5, 3) == 0
+    assert lib.kvhp_prompt_weights_workspace_bytes(batch, rows, hq, hkv, 64, cap) == 0
+
+
+@pytest.mark.parametrize("call", ATTENTION)
+def test_more_heads_than_a_grid_has(call):
+    _refused(call(hq=1 << 26, hkv=1), kvhp.KVHP_ERR_UNSUPPORTED, "num_q_heads")
+
+
+def test_more_rows_than_a_grid_has():
+    _refused(_wp(rows=1 << 30), kvhp.KVHP_ERR_UNSUPPORTED, "rows")
