@@ -162,14 +162,17 @@ int launch_weights(const BoundArgs& a, int batch, const char* what, hipStream_t 
     return check_launch(what);
 }
 
-int views(BoundArgs& a, const kvhp_kv_view* kv, const kvhp_kv_view* vv, const char* what) {
-    int rc = bound_check_view(kv, what, "K");
+int k_view_of(BoundArgs& a, const kvhp_kv_view* kv, const char* what) {
+    const int rc = bound_check_view(kv, what, "K");
     if (rc) return rc;
     a.k = bound_view(*kv);
     if (kv->block_table) a.cap = static_cast<int>(std::min<int64_t>(a.cap, (int64_t)kv->max_pages * kPage));
-    if (!vv) return KVHP_OK;
-    rc = bound_check_view(vv, what, "V");
-    if (rc) return rc;
+    return KVHP_OK;
+}
+
+int views(BoundArgs& a, const kvhp_kv_view* kv, const kvhp_kv_view* vv, const char* what) {
+    int rc = k_view_of(a, kv, what);
+    if (rc || (rc = bound_check_view(vv, what, "V"))) return rc;
     KVHP_REQUIRE((kv->block_table == nullptr) == (vv->block_table == nullptr), KVHP_ERR_INVALID,
                  "%s: K and V views must both be paged or both strided", what);
     a.v = bound_view(*vv);
@@ -342,7 +345,7 @@ extern "C" int kvhp_prompt_weights(const void* q, const kvhp_kv_view* k_view, co
     BoundArgs a{};
     int rc = bound_shapes(a, what, batch, num_q_heads, num_kv_heads, head_dim, max_seq_len,
                           window, sinks);
-    if (rc || (rc = views(a, k_view, nullptr, what))) return rc;
+    if (rc || (rc = k_view_of(a, k_view, what))) return rc;
     a.q = static_cast<const f16*>(q);
     a.lse = const_cast<float*>(lse);
     a.q_start = q_start;

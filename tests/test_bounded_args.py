@@ -205,3 +205,17 @@ def test_more_heads_than_a_grid_has(call):
 
 def test_more_rows_than_a_grid_has():
     _refused(_wp(rows=1 << 30), kvhp.KVHP_ERR_UNSUPPORTED, "rows")
+
+
+def test_null_views():
+    lib, view = kvhp.load(), ctypes.byref(_view())
+    for k, v, name in ((None, view, "K view"), (view, None, "V view"), (None, None, "K view")):
+        _refused(_code(lib.kvhp_window_decode(P, k, v, P, P, 2, 8, 2, 64, 1000, 100, 4, P, 1 << 40,
+                                              None)), kvhp.KVHP_ERR_INVALID, name)
+        _refused(_code(lib.kvhp_window_prefill(P, k, v, P, P, P, P, 2, 10, 8, 2, 64, 1000, 100, 4,
+                                               P, 1 << 40, None)), kvhp.KVHP_ERR_INVALID, name)
+        _refused(_code(lib.kvhp_weighted_decode(P, k, v, P, None, P, P, P, 2, 8, 2, 64, 1000, 1, P,
+                                                1 << 40, None)), kvhp.KVHP_ERR_INVALID, name)
+    _refused(_code(lib.kvhp_prompt_weights(P, None, P, None, None, None, P, P, 2, 10, 8, 2, 64, 1000,
+                                           0, 0, 1, P, 1 << 40, None)), kvhp.KVHP_ERR_INVALID,
+             "K view")
