@@ -78,11 +78,9 @@ __device__ __forceinline__ void dma16s(const char* base, uint32_t voff, f16* lds
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(m0v), "v"(voff), "s"(base) : "memory", "m0");
 }
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
-}
+// This wave's loads have landed, and its reads of LDS have returned: the products that take
+// them need not have been issued before the barrier behind which a stage is loaded anew.
+__device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(0x7 << 4); }
 // A workgroup barrier that leaves the ring's loads in flight.
 __device__ __forceinline__ void ring_barrier() {
     asm volatile("" ::: "memory");
@@ -476,7 +474,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         pid_k = keys.page(g + 3);
     };
     auto begin = [&](int j) {
-        wait_vmcnt<0>();
+        wait_all();
         if (j >= 0) keys.clean(j, vring + (j & 1) * TB);
         ring_barrier();
         issue(j);
@@ -557,7 +555,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         }
     };
 
-    wait_vmcnt<0>();   // q in registers before the ring: no other waits inside it
+    wait_all();   // q in registers before the ring: no other waits inside it
     __syncthreads();   // ptab, bad
     pid_k = pid_v = keys.page(0);
     issue(-2);
@@ -584,7 +582,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         exps(s0[t], pa);
         pv(j, t, pa);
     }
-    wait_vmcnt<0>();   // the ring's trailing re-loads
+    wait_all();   // the ring's trailing re-loads
     keys.add_back(o, x.live, x.pos);
     store_pair<D>(a, p, x, b, h, all_tiles, o, m_run, halves_sum(l_part));
 }
