@@ -50,7 +50,8 @@ namespace {
 constexpr int kBN = 64;               // keys per tile
 constexpr int kWaves = 4;
 constexpr int kPairs = 32 * kWaves;   // (row, head) pairs per workgroup
-constexpr int kPages = 4000;          // page ids of a split held in LDS
+constexpr int kRing = 512;            // tiles whose page ids LDS holds, read in halves of it
+constexpr int kPages = kRing * (kBN / kPage);
 constexpr int kMaxStride = 1 << 24;   // halfs between rows: 15 rows stay below 2^31 bytes
 constexpr int kEdge = 6;              // tiles at either edge of the window in a block
 constexpr int kBadWords = 4 * kEdge;  // a bit per key of those
@@ -154,6 +155,7 @@ struct Keys {
     uint32_t* bad;
     int wave, lane, t_lo, last_tile, window;
     const char *kb, *vb;
+    const int32_t* table;
     uint32_t ssk, ssv;
     uint32_t ko[IPW], vo[IPW];   // the lane's offsets from the wave's first row of a tile
     int edge_hi, edge_lo, edge_end;
@@ -184,15 +186,27 @@ struct Keys {
         edge_lo = k.sinks / kBN;
         const int64_t left = (int64_t)k.p_hi - window - k.shift;
         edge_end = left < 0 ? -1 : static_cast<int>(left / kBN);
-        if constexpr (PAGED) {   // the split's page ids, 16 keys to a page
-            const int v0 = t_lo * kBN, v1 = min((t_lo + n_tiles) * kBN, k.nv);
-            for (int i = threadIdx.x; i < (v1 - v0 + kPage - 1) / kPage; i += kWaves * kWave) {
-                const int v = v0 + i * kPage;
-                const int pid = a.k.bt[(int64_t)b * a.k.max_pages + ((v < k.head ? v : v + k.shift) >> 4)];
-                ptab[i] = min(max(pid, 0), a.k.num_pages - 1);
-            }
+        if constexpr (PAGED) {
+            table = a.k.bt + (int64_t)b * a.k.max_pages;
+            pages_of(0, kRing);
         }
         if (threadIdx.x < kBadWords) bad[threadIdx.x] = 0;
+    }
+    __device__ __forceinline__ int key_of(int v) const { return v < k.head ? v : v + k.shift; }
+    __device__ __forceinline__ int page_of(int key) const {
+        return min(max(table[key >> 4], 0), a.k.num_pages - 1);
+    }
+    // Page ids of tiles [t0, t1) of the split's, 16 keys to a page, into their places in LDS.
+    __device__ __forceinline__ void pages_of(int t0, int t1) const {
+        const int v0 = t_lo * kBN, v1 = min((t_lo + min(t1, last_tile + 1)) * kBN, k.nv);
+        for (int i = t0 * (kBN / kPage) + threadIdx.x; v0 + i * kPage < v1; i += kWaves * kWave)
+            ptab[i & (kPages - 1)] = page_of(key_of(v0 + i * kPage));
+    }
+    // In front of iteration j: all waves have begun j - 1 and ask for pages from tile j + 2 on
+    // (issue), so the half ring before tile j is free for the tiles behind the next half.
+    __device__ __forceinline__ void more_pages(int j) const {
+        if constexpr (PAGED)
+            if (j % (kRing / 2) == 0 && j > 0) pages_of(j + kRing / 2, j + kRing);
     }
     // First row of this wave in a tile.  Tiles past the last re-load it, so every wave
     // issues the same loads.
@@ -201,13 +215,13 @@ struct Keys {
     }
     // The page of this wave's rows of a tile, read one issue ahead.
     __device__ __forceinline__ int page(int tt) const {
-        return PAGED ? ptab[(first_row(tt) >> 4) - t_lo * (kBN / kPage)] : 0;
+        return PAGED ? ptab[((first_row(tt) >> 4) - t_lo * (kBN / kPage)) & (kPages - 1)] : 0;
     }
     // One tile of a matrix to a stage; rows past the last key re-read it.
     __device__ __forceinline__ void issue(int tt, int pid, const char* base, uint32_t ss,
                                           const uint32_t (&off)[IPW], f16* stage) const {
         const int v = first_row(tt);
-        const int key = v < k.head ? v : v + k.shift;
+        const int key = key_of(v);
         const uint32_t row = PAGED ? __builtin_amdgcn_readfirstlane(pid) * kPage + (key & 15) : key;
         const char* src = base + (uint64_t)row * ss;
         f16* dst = stage + wave * IPW * RPI * D;
@@ -267,10 +281,9 @@ struct Keys {
             if (!(bad[i >> 5] >> (i & 31) & 1)) continue;
             const int v = (i < kEdge * kBN ? edge_lo : edge_hi) * kBN + i % (kEdge * kBN);
             if (v >= k.nv) continue;   // a repeated row
-            const int key = v < k.head ? v : v + k.shift;
+            const int key = key_of(v);
             int64_t s = key;
-            if constexpr (PAGED)
-                s = (int64_t)ptab[(v >> 4) - t_lo * (kBN / kPage)] * kPage + (v & 15);
+            if constexpr (PAGED) s = (int64_t)page_of(key) * kPage + (key & 15);
             const f16* src = reinterpret_cast<const f16*>(vb + s * (int64_t)ssv) + 4 * h;
             const bool sees = live && key <= pos && (key < a.sinks || pos - key < window);
 #pragma unroll
@@ -565,6 +578,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
     tmax = max_of(s0);
     int j = 0;
     for (; j + 2 < n; j += 2) {
+        keys.more_pages(j);
         iterate(j, s0, s1);
         iterate(j + 1, s1, s0);
     }
@@ -659,8 +673,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(const BoundArgs a, con
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
-// Ranges of keys until every CU has two workgroups, each of at least 3 tiles, and as many
-// as their page ids fit LDS in.  (One sequence, us with at least 4 / 3 / 2 tiles: 16 rows of
+// Ranges of keys until every CU has two workgroups, each of at least 3 tiles.  (One sequence, us with at least 4 / 3 / 2 tiles: 16 rows of
 // 32/8 heads of 64, window 500, 13.1 / 11.0 / 10.9, 4000 13.8 / 11.9 / 11.8; of 128 15.1 /
 // 14.4 / 14.0; but 700 rows, window 200, 9.7 / 9.7 / 15.8: what the second launch costs.)
 PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window, int sinks) {
@@ -675,7 +688,6 @@ PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len, int window
                                     : max_len;
     const int64_t tiles = (keys + kBN - 1) / kBN;
     int64_t n = std::min<int64_t>(2 * kCUs / wgs, tiles / 3);
-    n = std::max<int64_t>(n, (tiles * (kBN / kPage) + kPages - 5) / (kPages - 4));
     n = std::max<int64_t>(n, 1);
     p.tiles_per_split = static_cast<int>((tiles + n - 1) / n);
     p.nsplit = static_cast<int>((tiles + p.tiles_per_split - 1) / p.tiles_per_split);

@@ -219,3 +219,12 @@ def test_null_views():
     _refused(_code(lib.kvhp_prompt_weights(P, None, P, None, None, None, P, P, 2, 10, 8, 2, 64, 1000,
                                            0, 0, 1, P, 1 << 40, None)), kvhp.KVHP_ERR_INVALID,
              "K view")
+
+
+def test_long_prompts_need_no_workspace():
+    """A prompt of many rows fills the card by itself: its keys are not cut into ranges,
+    however many they are."""
+    lib = kvhp.load()
+    for rows in (60000, 65536, 131072, 200000, 1 << 20):
+        for d in (64, 128):
+            assert lib.kvhp_window_prefill_workspace_bytes(1, rows, 32, 8, d, rows, 0, 0) == 0

@@ -1,0 +1,92 @@
+"""Windowed prompts and chunks over caches and at sizes where a workgroup walks hundreds of
+tiles of keys, against the definition in 64 bits (tolerances: bounded_util)."""
+import math
+
+import numpy as np
+import pytest
+
+import kvhp
+from bounded_util import PAGE, U16, U32, check, workspace
+from gpu_util import from_gpu, note, sync, to_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(q, k, v, see):
+    """bounded_util.attend on the device: q [G, D], k, v [n, D] and see [n] on the GPU; the
+    output and its tolerance, lse and its own."""
+    import torch
+    q, k, v = q.double(), k[see].double(), v[see].double()
+    d, n = q.shape[1], k.shape[0]
+    s = (q @ k.T.contiguous()) / math.sqrt(d)
+    size = float(((q.abs() @ k.abs().T.contiguous()) / math.sqrt(d)).max())
+    ds = (d + 4) * U32 * size + 4 * U32 * float(s.abs().max())
+    m = s.amax(1, keepdim=True)
+    e = torch.exp(s - m)
+    l = e.sum(1, keepdim=True)
+    p = e / l
+    out = p @ v
+    small = n * 2.0 ** -25 * float(v.abs().max()) / l
+    tol = U16 * out.abs() + (2 * U16 + 2 * ds + 2 * n * U32) * (p @ v.abs()) + small + 2.0 ** -25
+    lse = (m + l.log())[:, 0]
+    return out, tol, lse, ds + (n + 8) * U32 + 4 * U32 * lse.abs()
+
+
+def _see(p, n, window, sinks):
+    import torch
+    j = torch.arange(n, device="cuda")
+    see = j <= p
+    if window > 0:
+        see &= (j < sinks) | (p - j < window)
+    return see
+
+
+def _shared(seed, B, hkv, d, n):
+    """Pools of n keys in shuffled pages that every one of B sequences reads (a shared prefix),
+    and the same keys in order, [Hkv][n][D]."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = (n + PAGE - 1) // PAGE
+    k, v = (torch.empty((hkv, pages, PAGE, d), dtype=torch.float16, device="cuda").normal_(
+        generator=g) for _ in range(2))
+    order = np.random.default_rng(seed).permutation(pages).astype(np.int32)
+    bt = to_gpu(np.broadcast_to(order, (B, pages)))
+    at = to_gpu(order).long()
+    return k, v, bt, [x[:, at].reshape(hkv, -1, d)[:, :n] for x in (k, v)]
+
+
+@pytest.mark.parametrize("d,window,sinks", [(64, 0, 0), (64, 70001, 21), (128, 0, 0),
+                                            (128, 40000, 500)])
+def test_one_range_of_hundreds_of_tiles(d, window, sinks):
+    """So many sequences that none is cut into ranges, over up to 140000 keys in shuffled
+    pages: lengths on both sides of 256, 512, 768 and 1024 tiles of 64 keys, and a key that
+    only the last row sees."""
+    import torch
+    B, hkv, R, n = 66, 4, 2, 140000
+    k, v, bt, (kk, vv) = _shared(d, B, hkv, d, n)
+    edges = [t * 64 + e for t in (256, 257, 258, 511, 512, 513, 768, 1024, 1280) for e in (-1, 0, 1, 2)]
+    lens = np.array((edges + [n, 2, 3, 64, 65, 1000] + list(range(90000, 140000, 2500)))[:B], np.int32)
+    lens = np.concatenate([lens, np.random.default_rng(d).integers(2, n, B - len(lens))]).astype(np.int32)
+    g = torch.Generator(device="cuda").manual_seed(d + 1)
+    q = torch.empty((B, R, hkv, d), dtype=torch.float16, device="cuda").normal_(generator=g)
+    out, lse = torch.zeros_like(q), torch.zeros((B, hkv, R), device="cuda")
+    assert kvhp.window_prefill_workspace_bytes(B, R, hkv, hkv, d, n, window, sinks) == 0
+    vv = vv.clone()
+    last = int(bt[0, (n - 1) // PAGE])
+    v[:, last, (n - 1) % PAGE] = math.inf
+    note(f"window_prefill: ranges of up to 2188 tiles, D = {d}, window {window}, {sinks} first")
+    kvhp.window_prefill(q, kvhp.paged_view(k, bt), kvhp.paged_view(v, bt), out, hkv, hkv, d, n,
+                        window, sinks, q_start=to_gpu(lens - R), seq_lens=to_gpu(lens), lse=lse)
+    sync()
+    for b in range(B):
+        for r in range(R):
+            p = int(lens[b]) - R + r
+            see = _see(p, p + 1, window, sinks)
+            for h in range(hkv):
+                o, tol, ls, ltol = _attend(q[b, r, h:h + 1], kk[h, :p + 1], vv[h, :p + 1], see)
+                what = f"sequence {b} of {lens[b]}, row {r}, head {h}"
+                if p == n - 1:
+                    assert bool((out[b, r, h] == math.inf).all()), what
+                else:
+                    check(from_gpu(out[b, r, h]), from_gpu(o[0]), from_gpu(tol[0]), what)
+                check(from_gpu(lse[b, h, r:r + 1]), from_gpu(ls), from_gpu(ltol), what)
