@@ -43,8 +43,9 @@ namespace {
 
 constexpr int kMaxChunk = 960;    // keys per split: at most 64 pages, three of them cut
 constexpr int kMinChunk = 64;     // (of a batch's own splits)
-constexpr int kMaxOne = 1152;     // and where one split takes all, at D = 64
+constexpr int kMaxOne = 1152;     // and where one split takes all, at D = 64 (75 pages)
 constexpr int kHeads = 16;        // query heads per workgroup
+constexpr int kBalanced = 16;     // sequences from which the splits are the whole batch's
 
 struct DecodePlan {
     int chunk;        // keys per split (fixed mode), a multiple of 32
@@ -638,7 +639,38 @@ bound_sums_kernel(const BoundArgs a, const DecodePlan p, int key_blocks) {
 }
 
 // ------------------------------------------------------------------ plan --
-DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums) {
+// Up to so many keys a sequence takes one split: eight waves share its steps, and no second
+// launch joins.  `units` is the workgroups of that launch.  us as one split / as splits, at as
+// many keys in every sequence, replayed from a graph (called among other work the second launch
+// costs up to 0.8 more, so the limits there lie higher):
+//   D = 64             1 to 16 units 768 keys 6.5 / 6.6, 896 6.8 / 6.5, 1088 7.7 / 6.7; 24 to 40
+//                      896 6.9 / 7.3, 1088 7.8 / 7.6; 48 and more 1088 7.8 / 9.1, of 256 11.8 / 18.4
+//   D = 128            to 16 512 7.5 / 7.6, 576 7.8 / 7.6, 900 11.0 / 7.7; 32 576 8.0 / 8.1, 640
+//                      8.2 / 8.2; 64 640 9.0 / 8.9, 768 10.0 / 9.4; 96 768 11.2 / 11.7, 900 13.8 /
+//                      12.9; 112 900 14.5 / 14.6
+//   with sums, which the workgroup then adds itself
+//     D = 64           to 16 704 7.3 / 7.3, 896 7.6 / 7.3; 32 896 7.8 / 7.9, 960 8.4 / 8.0; 48 960
+//                      8.6 / 8.9
+//     D = 128          to 16 384 7.6 / 8.3, 448 8.6 / 8.4; 40 512 9.0 / 9.0; 64 576 9.8 / 9.9, 640
+//                      10.6 / 10.0; 96 640 11.3 / 11.9, 900 15.6 / 14.3
+// Batches of 16 and more, whose splits go by a list of lengths: 16 units of 64 1088 7.7 / 9.8; of
+// 128 768 9.6 / 10.7, 900 11.4 / 10.8; 64 900 13.0 / 13.8, 256 21.8 / 28.3.  Strided views have
+// no page ids to wait for: D = 64, 8 units 800 5.7 / 6.3, 1152 6.6 / 6.3, but called among other
+// work 7.0 / 7.4, which is worth more; 32 1152 7.0 / 7.2.  Of more than 16 heads a KV head a
+// second launch adds the workgroups' sums either way (among other work 128 8.2 / 8.4, 350 9.1 / 8.4).
+int one_split_keys(int batch, int64_t units, int d, int groups, bool sums, bool paged) {
+    if (sums && groups > 1) return 128;
+    if (d == 64) {
+        if (!paged || batch >= kBalanced || units >= 48) return sums ? kMaxChunk : kMaxOne;
+        return units >= 24 ? 896 : sums ? 768 : 832;
+    }
+    if (batch >= kBalanced) return units < 64 ? 832 : kMaxChunk;
+    const int64_t keys = sums ? std::max<int64_t>(416, 352 + 4 * units)
+                              : std::max<int64_t>(units < 24 ? 544 : 608, 256 + 6 * units);
+    return static_cast<int>(std::min<int64_t>(kMaxChunk, keys));
+}
+
+DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums, bool paged) {
     DecodePlan p{};
     p.batch = batch;
     p.groups = (G + kHeads - 1) / kHeads;
@@ -646,19 +678,7 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t maxv, bool sums) {
     const int64_t per = std::max<int64_t>(64, ((maxv + 63) / 64 + 63) / 64 * 64);
     int64_t s = std::min((maxv + per - 1) / per, units >= 6144 ? 1 : 6144 / units);
     int64_t chunk = std::min<int64_t>(((maxv + s - 1) / s + 63) / 64 * 64, kMaxChunk);
-    // Up to `one` keys a sequence takes one split: eight waves share its steps, and no second
-    // launch joins.  One sequence, 32/8 heads, us as one split / as splits of 64 keys: D = 64
-    // 500 keys 5.2 / 7.0, 1028 6.8 / 7.1, 1500 8.1 / 7.0; D = 128 500 7.2 / 7.8, 700 8.6 / 8.0
-    // (replayed from a graph the splits win from 1000 and 550 on, called among other work only
-    // from 1500 and 800).  Batches, against splits of all lengths' size: 32 of up to 300 keys
-    // 5.0 / 10.8 and 6.4 / 12.1, of 1100 10.6 / 14.0 and 21.0 / 20.4; 256 of up to 560 40.6 /
-    // 48.7 and 64 / 78.  With sums, which the split's workgroup then adds itself: one of 128
-    // 5.3 / 8.4, 700 7.8 / 8.6, 960 8.7 / 8.8; D = 128 350 7.9 / 9.2, 500 9.0 / 9.4; 32 of up
-    // to 700 8.0 / 14.4 and 17.7 / 19.7.  (Of more than 16 heads a KV head a second launch
-    // adds the workgroups' sums: 128 keys 8.2 / 8.4, 350 9.1 / 8.4.)
-    const int one = d == 64 ? (!sums ? kMaxOne : p.groups > 1 ? 128 : batch < 8 ? 704 : kMaxChunk)
-                            : (!sums ? (batch < 8 ? 576 : kMaxChunk)
-                                     : p.groups > 1 ? 128 : batch < 8 ? 448 : 640);
+    const int one = one_split_keys(batch, units, d, p.groups, sums, paged);
     if (maxv <= one) chunk = (maxv + 31) / 32 * 32;
     p.chunk = static_cast<int>(chunk);
     p.nsplit = static_cast<int>((maxv + chunk - 1) / chunk);
@@ -677,7 +697,8 @@ constexpr int kWaveSlots = 2048;
 size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int window, int sinks,
                               bool sums) {
     if (!bound_sizes(batch, hq, hkv, cap, window, sinks) || (d != 64 && d != 128)) return 0;
-    const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks), sums);
+    // paged views: the lower limits of one split, so never less than strided ones need
+    const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, most_visible(cap, window, sinks), sums, true);
     const size_t rows = (size_t)batch * hq;
     size_t n = p.nsplit > 1 || sums ? rows * p.nsplit * 2 : 0;
     if (p.nsplit > 1) n += rows * p.nsplit * d;
@@ -687,7 +708,7 @@ size_t bound_decode_workspace(int batch, int hq, int hkv, int d, int cap, int wi
 
 bool bound_decode_fits(const BoundArgs& a, int batch) {
     const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, most_visible(a.max_len, a.window, a.sinks),
-                                 a.weights != nullptr);
+                                 a.weights != nullptr, a.k.bt != nullptr);
     return (a.D == 64 || a.D == 128) && p.nsplit <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
 }
 
@@ -700,7 +721,7 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
     // Batches of 16 and more cut each sequence by what the whole batch has (8 of up to 1200
     // keys, 32/8 heads of 128, 11.8 us so and 8.8 in fixed splits, 8000 34 and 29; 24 of up to
     // 8000 keys of 64 42.3 and 45.6).
-    if (p.batch >= 16 && p.nsplit > 1) {
+    if (p.batch >= kBalanced && p.nsplit > 1) {
         p.balance = std::max(1, kWaveSlots / heads - p.batch / 2);
         const int64_t worst = (p.batch * maxv + kMaxChunk - 1) / kMaxChunk;
         const int64_t units = std::max<int64_t>(p.balance, worst) + p.batch;
@@ -739,7 +760,7 @@ static int launch(const BoundArgs& a, DecodePlan p, int64_t maxv, hipStream_t s)
 // block table, 16-byte aligned.
 int bound_decode(const BoundArgs& a, int batch, bool paged, bool sums, void* ws, hipStream_t s) {
     const int64_t maxv = most_visible(a.max_len, a.window, a.sinks);
-    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, maxv, sums);
+    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, maxv, sums, paged);
     const size_t rows = (size_t)batch * a.Hq;
     p.scap = (a.max_len + 31) / 32 * 32;
     float* w = static_cast<float*>(ws);

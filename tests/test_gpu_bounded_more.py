@@ -316,3 +316,42 @@ def test_graph_replays_of_short_sequences():
         sync()
         want += once      # the same fp32 sums in the same order
         assert torch.equal(w, want) and torch.equal(out, first)
+
+
+@pytest.mark.parametrize("batch,hkv,d,limit", [(3, 2, 64, 832), (3, 8, 64, 896), (6, 8, 64, 1152),
+                                               (17, 1, 64, 1152), (2, 2, 128, 544),
+                                               (4, 8, 128, 608), (8, 8, 128, 640),
+                                               (15, 8, 128, 960), (17, 2, 128, 832),
+                                               (16, 8, 128, 960)])
+def test_one_split_limits_by_units(batch, hkv, d, limit):
+    """Visible keys on both sides of what one split takes, by how many workgroups it makes."""
+    rng = np.random.default_rng([batch, hkv, d])
+    q = _q(rng, batch, 2 * hkv, d)
+    for visible in (limit - 1, limit, limit + 1):
+        lens = [visible + 333, visible, 0, visible - 1, visible // 2, 31][:batch]
+        lens += list(rng.integers(1, visible + 300, batch - len(lens)))
+        for paged in (True, False):
+            c = Cache(rng, lens, hkv, d, paged).upload()
+            note(f"window_decode: {batch} x {hkv} KV heads of {d}, {visible} visible, paged={paged}")
+            ref, tol, _, _ = decode_ref(q, c, visible - 19, 19)
+            check(_window_decode(q, c, visible - 19, 19), ref, tol)
+
+
+@pytest.mark.parametrize("batch,hkv,d,limit", [(3, 2, 64, 768), (3, 8, 64, 896), (6, 8, 64, 960),
+                                               (17, 1, 64, 960), (4, 2, 128, 416),
+                                               (4, 8, 128, 480), (8, 8, 128, 608),
+                                               (17, 2, 128, 832), (16, 8, 128, 960)])
+def test_one_split_sums_limits_by_units(batch, hkv, d, limit):
+    rng = np.random.default_rng([batch, hkv, d, 1])
+    q = _q(rng, batch, 2 * hkv, d)
+    for n in (limit - 1, limit, limit + 1):
+        lens = [n, n - 1, 0, n // 2, 31, 1][:batch] + list(rng.integers(1, n + 1, max(batch - 6, 0)))
+        c = Cache(rng, lens, hkv, d).upload()
+        w, ages = _sums(rng, c)
+        note(f"weighted_decode: {batch} x {hkv} KV heads of {d}, {n} keys")
+        out, gw, ga = _weighted(q, c, w, ages, 2, None)
+        ref, tol, sums, rel = decode_ref(q, c, 0, 0)
+        check(out, ref, tol)
+        rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 2, c.lens - 1)
+        _check_sums(gw, rw, tw)
+        assert np.array_equal(ga, ra)
