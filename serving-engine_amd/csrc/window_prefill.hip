@@ -16,9 +16,10 @@
 // first tokens need a mask.
 //
 // Per tile, on v_mfma_f32_32x32x16_f16 with one lane per pair: S^T = K Q^T; an fp32 online
-// softmax in the log2 domain whose reference maximum moves when a row passes it by 2^8
-// (weights up to 2^8 stay far inside fp16's range, to which they are rounded for the
-// product: 2^-11 each, over a sum of many); O^T += V^T P^T.  K and V rows go from memory to
+// softmax in the log2 domain whose reference lies 2^7 to 2^15 below a row's largest weight
+// (it moves when a row passes it by 2^15).  Weights are rounded to fp16 for the product: 2^-11
+// each down to 2^-14 of the reference, an absolute 2^-25 of it below, so that 10^5 keys of
+// little weight beside a first token of much still count; O^T += V^T P^T.  K and V rows go from memory to
 // two LDS stages per matrix without registers (global_load_lds, a scalar base and the
 // lane's fixed offset; page ids from LDS), with their 16-byte chunks XOR-swizzled so that
 // both operand reads touch all banks.
@@ -57,7 +58,8 @@ constexpr int kEdge = 6;              // tiles at either edge of the window in a
 constexpr int kBadWords = 4 * kEdge;  // a bit per key of those
 constexpr int kMaxRowHeads = 1 << 29; // (row, query head) pairs of a sequence: a grid of 2^22
 constexpr int kCUs = 256;
-constexpr float kLazyLog2 = 8.f;
+constexpr float kRefLog2 = 7.f;       // a row's reference below its maximum where it is set,
+constexpr float kLazyLog2 = 15.f;     // and where it moves: weights up to 2^15 in fp16
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
@@ -102,7 +104,7 @@ struct PrefillPlan {
     int blocks;            // of pairs, per sequence and KV head
     int tiles_per_split, nsplit;
     float* ws_o;           // [batch * rows * Hq][nsplit][D]
-    float* ws_ml;          // [batch * rows * Hq][nsplit][2], the maximum in log2 units
+    float* ws_ml;          // [batch * rows * Hq][nsplit][2], the reference in log2 units
 };
 
 // Row of a pair: pair / G, exact for pair * G below 2^32.
@@ -475,7 +477,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
     float m_run = -1e30f, l_part = 0.f;
-    const float lazy_thr = kLazyLog2 / a.scale_log2;
+    const float lazy_thr = kLazyLog2 / a.scale_log2, ref = kRefLog2 / a.scale_log2;
 
     // Group g: K of tile g + 2 and V of tile g + 1, issued by iteration g into the stages
     // that iteration g - 1 was the last to read, and waited for by iteration g + 1.
@@ -520,13 +522,13 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
                     cat_half8(lds_read_tr16(q), lds_read_tr16(q + 8 * D)), pop[t], o[db], 0, 0, 0);
             }
     };
-    // Masks tile j's scores; moves the reference maximum where a row passes it by 2^8.
+    // Masks tile j's scores; moves the reference where a row passes it by 2^15.
     float tmax;
     auto refer = [&](int j, floatx16 (&s)[2]) {
         if (mask(k, x, keys.window, t_lo + j, (t_lo + j) * kBN + 4 * h, s)) tmax = max_of(s);
         tmax = halves_max(tmax);
         if (__builtin_amdgcn_read_exec() & __ballot(tmax > m_run + lazy_thr)) {
-            const float mn = fmaxf(m_run, tmax);
+            const float mn = fmaxf(m_run, tmax - ref);
             const float alpha = fast_exp2((m_run - mn) * a.scale_log2);
             l_part *= alpha;
 #pragma unroll

@@ -90,3 +90,40 @@ def test_one_range_of_hundreds_of_tiles(d, window, sinks):
                 else:
                     check(from_gpu(out[b, r, h]), from_gpu(o[0]), from_gpu(tol[0]), what)
                 check(from_gpu(lse[b, h, r:r + 1]), from_gpu(ls), from_gpu(ltol), what)
+
+
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (64, 100000)])
+def test_many_small_weights_beside_a_large_one(d, window):
+    """One key with most of the weight and 131071 with 2^-25 of it each, 2^-8 together: their
+    rounding to fp16 is an absolute 2^-25 of a reference at least 2^7 below the largest weight."""
+    import torch
+    B, hkv, R, n = 65, 4, 2, 131072
+    k, v, bt, (kk, vv) = _shared(d, B, hkv, d, n)
+    sinks = 1
+    k[..., 0], v[:] = 12 - 17.35, 1.0      # 17.35 = 25.03 log 2, times the query's sqrt(D) below
+    k[..., 1:] = 0
+    k[:, int(bt[0, 0]), 0, 0] = 12
+    v[:, int(bt[0, 0]), 0] = 0
+    q = torch.zeros((B, R, hkv, d), dtype=torch.float16, device="cuda")
+    q[..., 0] = math.sqrt(d)
+    lens = np.linspace(n // 2, n, B).astype(np.int32)
+    out = torch.zeros_like(q)
+    assert kvhp.window_prefill_workspace_bytes(B, R, hkv, hkv, d, n, window, sinks) == 0
+    note(f"window_prefill: many small weights, D = {d}, window {window}")
+    kvhp.window_prefill(q, kvhp.paged_view(k, bt), kvhp.paged_view(v, bt), out, hkv, hkv, d, n,
+                        window, sinks, q_start=to_gpu(lens - R), seq_lens=to_gpu(lens))
+    sync()
+    # the scores as the fp16 keys and query give them
+    x = np.float64(np.float16(math.sqrt(d))) / math.sqrt(d)
+    e = math.exp(x * (np.float64(np.float16(12 - 17.35)) - 12))
+    got = from_gpu(out).astype(np.float64)
+    for b in range(B):
+        for r in range(R):
+            p = int(lens[b]) - R + r
+            seen = p if window == 0 else min(p, window)
+            l = 1 + seen * e
+            want = seen * e / l
+            # relative: the output's and each weight's rounding, the scores' and the sums' in fp32
+            ds = (d + 8) * U32 * 18
+            tol = (3 * U16 + 2 * ds + 2 * seen * U32) * want + seen * 2.0 ** -32 / l + 2.0 ** -25
+            check(got[b, r], np.full((hkv, d), want), np.full((hkv, d), tol), f"{lens[b]} keys, row {r}")
