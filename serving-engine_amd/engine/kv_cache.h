@@ -227,17 +227,25 @@ public:
         reserve(slot, len);
         lens_[slot] = len;
     }
-    // Cuts a sequence to its first `len` tokens and gives up the pages behind
-    // them (after an eviction moved the kept tokens into the first slots).
-    // None of its pages may be shared: an eviction writes into them.
-    void shrink(int slot, int len) {
+    // Throws where another sequence holds one of the slot's pages.  To be called
+    // before anything that writes into them is enqueued: sums of weight, and an
+    // eviction's moves (evict_apply goes by block_tables(), shared pages included).
+    void require_private(int slot) const {
         check_slot(slot);
+        for (int i = 0; i < pages_used_[slot]; ++i)
+            if (refs_[tables_[(size_t)slot * max_pages_ + i]] > 1)
+                throw std::logic_error("PagedKVCache: slot " + std::to_string(slot) +
+                                       " shares a page");
+    }
+    // Cuts a sequence to its first `len` tokens and gives up the pages behind
+    // them, after an eviction moved the kept tokens into the first slots (so none
+    // of its pages may be shared; by now that is too late to find out, see
+    // require_private).
+    void shrink(int slot, int len) {
+        require_private(slot);
         if (len < 0 || len > lens_[slot])
             throw std::out_of_range("PagedKVCache::shrink: length outside 0..the present one");
         const int keep = (len + kPage - 1) / kPage;
-        for (int i = 0; i < pages_used_[slot]; ++i)
-            if (refs_[tables_[(size_t)slot * max_pages_ + i]] > 1)
-                throw std::logic_error("PagedKVCache::shrink: a page is shared");
         for (int i = keep; i < pages_used_[slot]; ++i) {
             int32_t& e = tables_[(size_t)slot * max_pages_ + i];
             refs_[e] = 0;

@@ -278,6 +278,7 @@ void case_served() {
     };
     for (int i = 0; i < steps; ++i) step(true, 0, 0, "weighted step");
     check_sums("steps");
+    for (int b = 0; b < kB; ++b) cache.require_private(b);
 
     // the eviction, by the sums as the device holds them
     const int n = S + steps, used = cache.pages_used(0);
@@ -346,6 +347,24 @@ void case_served() {
     step(true, 0, 0, "another step");
 }
 
+// What an eviction must not write into is refused before one is enqueued.
+void case_private() {
+    PagedKVCache cache(1, 1, 8, 8, 3, 4);
+    const int a = cache.add_sequence(), b = cache.add_sequence();
+    cache.require_private(a);   // nothing held
+    cache.set_seq_len(a, 40);
+    cache.require_private(a);
+    cache.share_prefix(b, a, 16);
+    EXPECT(refusal([&] { cache.require_private(a); }).find("slot 0 shares") != std::string::npos,
+           "a page lent");
+    EXPECT(refusal([&] { cache.require_private(b); }).find("slot 1 shares") != std::string::npos,
+           "a page borrowed");
+    EXPECT(!refusal([&] { cache.require_private(3); }).empty(), "no such slot");
+    EXPECT(!refusal([&] { cache.require_private(-1); }).empty(), "no such slot");
+    cache.release(b);
+    cache.require_private(a);
+}
+
 void case_shrink() {
     PagedKVCache cache(1, 1, 8, 8, 2, 4);
     const int a = cache.add_sequence(), b = cache.add_sequence();
@@ -388,6 +407,7 @@ int main(int argc, char** argv) {
         bool gpu;
         void (*fn)();
     } cases[] = {{"refusals", false, case_refusals},
+                 {"private", true, case_private},
                  {"shrink", true, case_shrink},
                  {"served", true, case_served}};
     for (const auto& c : cases) {
