@@ -209,11 +209,7 @@ public:
     // Returns the slot's pages to the free list.
     void release(int slot) {
         check_slot(slot);
-        for (int i = 0; i < pages_used_[slot]; ++i) {
-            int32_t& e = tables_[(size_t)slot * max_pages_ + i];
-            if (--refs_[e] == 0) free_pages_.push_back(e);
-            e = -1;
-        }
+        for (int i = 0; i < pages_used_[slot]; ++i) give_up(slot, i);
         pages_used_[slot] = 0;
         cached_[slot] = 0;
         lens_[slot] = 0;
@@ -224,14 +220,39 @@ public:
         check_slot(slot);
         if (len < 0)
             throw std::invalid_argument("PagedKVCache::set_seq_len: negative length");
+        if (len < lens_[slot] && has_holes(slot))
+            throw std::logic_error("PagedKVCache::set_seq_len: a shorter text's window begins in "
+                                   "pages that were given up");
         reserve(slot, len);
         lens_[slot] = len;
     }
-    // Throws where another sequence holds one of the slot's pages.  To be called
-    // before anything that writes into them is enqueued: sums of weight, and an
-    // eviction's moves (evict_apply goes by block_tables(), shared pages included).
+    // Gives up the pages of which no row at the sequence's last position or later
+    // sees a key, attending its last `window` keys and the text's first `sinks`
+    // (kvhp_c.h, caches of bounded length): their table entries become -1.  From
+    // then on the sequence is for the window operators with this window or a
+    // shorter one and no more first tokens, and its length only grows.  Returns
+    // how many pages it gave up.
+    int drop_hidden(int slot, int window, int sinks) {
+        check_slot(slot);
+        if (window <= 0 || sinks < 0)
+            throw std::invalid_argument("PagedKVCache::drop_hidden: window must be positive and "
+                                        "sinks not negative");
+        const int first = sinks / kPage + (sinks % kPage != 0);
+        const int end = std::max(lens_[slot] - window, 0) / kPage;
+        int n = 0;
+        for (int i = first; i < end; ++i) n += give_up(slot, i);
+        if (first < end) cached_[slot] = std::min(cached_[slot], first * kPage);
+        return n;
+    }
+    // Throws where another sequence holds one of the slot's pages, or some were
+    // given up.  To be called before anything that writes into them is enqueued:
+    // sums of weight, and an eviction's moves (evict_apply goes by block_tables(),
+    // shared pages included).
     void require_private(int slot) const {
         check_slot(slot);
+        if (has_holes(slot))
+            throw std::logic_error("PagedKVCache: slot " + std::to_string(slot) +
+                                   " has given up pages");
         for (int i = 0; i < pages_used_[slot]; ++i)
             if (refs_[tables_[(size_t)slot * max_pages_ + i]] > 1)
                 throw std::logic_error("PagedKVCache: slot " + std::to_string(slot) +
@@ -246,12 +267,7 @@ public:
         if (len < 0 || len > lens_[slot])
             throw std::out_of_range("PagedKVCache::shrink: length outside 0..the present one");
         const int keep = (len + kPage - 1) / kPage;
-        for (int i = keep; i < pages_used_[slot]; ++i) {
-            int32_t& e = tables_[(size_t)slot * max_pages_ + i];
-            refs_[e] = 0;
-            free_pages_.push_back(e);
-            e = -1;
-        }
+        for (int i = keep; i < pages_used_[slot]; ++i) give_up(slot, i);
         pages_used_[slot] = std::min(pages_used_[slot], keep);
         lens_[slot] = len;
         cached_[slot] = 0;   // what the first slots hold is no shared prefix now
@@ -271,6 +287,9 @@ public:
         if (num_tokens < 0 || num_tokens > lens_[src])
             throw std::out_of_range("PagedKVCache::share_prefix: prefix longer than the source");
         const int n = num_tokens / kPage;
+        for (int i = 0; i < n; ++i)
+            if (tables_[(size_t)src * max_pages_ + i] < 0)
+                throw std::logic_error("PagedKVCache::share_prefix: the source has given up pages of it");
         for (int i = 0; i < n; ++i) {
             const int32_t page = tables_[(size_t)src * max_pages_ + i];
             tables_[(size_t)dst * max_pages_ + i] = page;
@@ -407,6 +426,18 @@ private:
     hip::KVView view(int layer, int is_v) const {
         return hip::paged_view(get_layer_ptr(layer, is_v), num_pages_, head_dim_, block_tables(),
                                max_pages_);
+    }
+    // Takes page i out of the slot's table; 0 where it had been given up before.
+    int give_up(int slot, int i) {
+        int32_t& e = tables_[(size_t)slot * max_pages_ + i];
+        if (e < 0) return 0;
+        if (--refs_[e] == 0) free_pages_.push_back(e);
+        e = -1;
+        return 1;
+    }
+    bool has_holes(int slot) const {
+        const int32_t* t = host_block_table(slot);
+        return std::find(t, t + pages_used_[slot], -1) != t + pages_used_[slot];
     }
     void check_slot(int slot) const {
         if (slot < 0 || slot >= max_batch_)

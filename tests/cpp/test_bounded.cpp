@@ -1,7 +1,8 @@
 // test_bounded.cpp -- the C++ API of the caches of bounded length
-// (serving-engine_amd/engine/kernels.h, PagedKVCache::shrink): a prompt with
-// its weights, decode steps that add theirs, an eviction and steps over what
-// it left, through one PagedKVCache, against definitions in double.
+// (serving-engine_amd/engine/kernels.h, PagedKVCache::shrink, require_private and
+// drop_hidden): a prompt with its weights, decode steps that add theirs, an
+// eviction and steps over what it left, and windowed steps that give hidden
+// pages away, through one PagedKVCache, against definitions in double.
 //
 //   test_bounded --cpu   refusals
 //   test_bounded --gpu   every case
@@ -365,6 +366,111 @@ void case_private() {
     cache.require_private(a);
 }
 
+void case_drop_hidden() {
+    PagedKVCache cache(1, 1, 8, 12, 3, 8);
+    const int a = cache.add_sequence(), b = cache.add_sequence();
+    EXPECT(cache.drop_hidden(a, 5, 0) == 0, "nothing held");
+    cache.set_seq_len(a, 100);   // pages 0 .. 6
+    EXPECT(!refusal([&] { cache.drop_hidden(a, 0, 4); }).empty(), "no window");
+    EXPECT(!refusal([&] { cache.drop_hidden(a, 10, -1); }).empty(), "negative first tokens");
+    EXPECT(!refusal([&] { cache.drop_hidden(3, 10, 4); }).empty(), "no such slot");
+    EXPECT(cache.drop_hidden(a, INT32_MAX, 0) == 0 && cache.drop_hidden(a, 10, INT32_MAX) == 0 &&
+               cache.drop_hidden(a, 85, 0) == 0 && cache.drop_hidden(a, 20, 80) == 0,
+           "no page is hidden");
+    cache.share_prefix(b, a, 48);
+    // position 99 sees keys 60 .. 99 and 0 .. 16: page 2 is hidden
+    EXPECT(cache.drop_hidden(a, 40, 17) == 1 && cache.host_block_table(a)[2] == -1 &&
+               cache.host_block_table(a)[1] >= 0 && cache.host_block_table(a)[3] >= 0,
+           "page 2 alone");
+    EXPECT(cache.page_refs(cache.host_block_table(b)[2]) == 1 && cache.free_page_count() == 5,
+           "the other sequence's page");
+    EXPECT(cache.drop_hidden(a, 40, 17) == 0 && cache.drop_hidden(a, 36, 17) == 1 &&
+               cache.free_page_count() == 6, "page 3 too, keys 48 .. 63");
+    EXPECT(!refusal([&] { cache.require_private(a); }).empty() &&
+               !refusal([&] { cache.shrink(a, 20); }).empty(), "an eviction needs every page");
+    EXPECT(!refusal([&] { cache.set_seq_len(a, 99); }).empty(), "shorter");
+    const int c = cache.add_sequence();
+    EXPECT(!refusal([&] { cache.share_prefix(c, a, 48); }).empty() && cache.pages_used(c) == 0 &&
+               cache.free_page_count() == 6, "a prefix with pages missing");
+    EXPECT(cache.share_prefix(c, a, 32) == 32, "one without");
+    cache.release(c);
+    EXPECT(cache.cached_tokens(b) == 48 && cache.drop_hidden(b, 1, 1) == 1 &&
+               cache.cached_tokens(b) == 16, "cached tokens end in front of the first page given up");
+    cache.set_seq_len(a, 112);
+    cache.sync();
+    cache.release(b);
+    cache.begin_decode_step(2);
+    EXPECT(cache.seq_len(a) == 113 && cache.pages_used(a) == 8, "the sequence goes on");
+    cache.release(a);
+    EXPECT(cache.free_page_count() == 12, "every page came back once");
+}
+
+// Windowed steps over a cache that keeps the window's pages and the first tokens' only; what
+// was given up goes to another sequence, which fills it with NaN.
+void case_windowed() {
+    std::mt19937 rng(5);
+    const int S = 90, steps = 60, window = 37, sinks = 4;
+    // two sequences of at most 1 + 4 pages, one of which grows before the other is cut
+    PagedKVCache cache(1, kHkv, kD, 14, kB + 1, 12);
+    EXPECT(cache.add_sequence() == 0 && cache.add_sequence() == 1, "slots");
+    Head head[kB][kHkv];
+    const int cap = cache.max_pages_per_seq() * PagedKVCache::kPage;
+    auto extend = [&](const std::vector<half>& k, const std::vector<half>& v) {
+        for (int b = 0; b < kB; ++b)
+            for (int h = 0; h < kHkv; ++h) {
+                const size_t at = ((size_t)b * kHkv + h) * kD;
+                std::vector<double> kr(kD), vr(kD);
+                for (int i = 0; i < kD; ++i) {
+                    kr[i] = half_to_float(k[at + i]);
+                    vr[i] = half_to_float(v[at + i]);
+                }
+                head[b][h].k.push_back(kr);
+                head[b][h].v.push_back(vr);
+            }
+    };
+    DeviceBuffer<char> ws(std::max<size_t>(
+        hip::window_decode_workspace_bytes(kB, kHq, kHkv, kD, cap, window, sinks), 16));
+    double want[kD], spread[kD];
+    for (int t = 0; t < S + steps; ++t) {
+        auto q = random_half(rng, (size_t)kB * kHq * kD);
+        auto k = random_half(rng, (size_t)kB * kHkv * kD);
+        auto v = random_half(rng, k.size());
+        cache.begin_decode_step(kB);
+        if (t % 5 == 4)
+            for (int b = 0; b < kB; ++b) cache.drop_hidden(b, window, sinks);
+        cache.sync();
+        auto dq = upload(q), dk = upload(k), dv = upload(v);
+        cache.append(0, dk.data(), dv.data(), kB, 1);
+        extend(k, v);
+        DeviceBuffer<half> out(q.size());
+        hip::window_decode(dq.data(), cache.k_view(0), cache.v_view(0), cache.seq_lens(), out.data(),
+                           kB, kHq, kHkv, kD, cap, window, sinks, ws.data(), ws.size());
+        HIP_CHECK(hipDeviceSynchronize());
+        if (t < S) continue;
+        const auto got = download(out);
+        for (int b = 0; b < kB; ++b)
+            for (int h = 0; h < kHq; ++h) {
+                row(&q[((size_t)b * kHq + h) * kD], head[b][h / kG], t, window, sinks, false, want, spread);
+                check_row(&got[((size_t)b * kHq + h) * kD], want, spread, window + sinks, "windowed step");
+            }
+        if (t % 20 == 0) {   // the pages given up, as their next owner leaves them
+            const int c = cache.add_sequence(), n = cache.free_page_count() * PagedKVCache::kPage;
+            cache.reserve(c, n);
+            std::vector<half> nan((size_t)n * kHkv * kD, float_to_half(NAN));
+            auto dn = upload(nan);
+            DeviceBuffer<int32_t> table = upload(std::vector<int32_t>(
+                cache.host_block_table(c), cache.host_block_table(c) + cache.pages_used(c)));
+            auto zero = upload(std::vector<int32_t>(1, 0));
+            hip::paged_append_kv(dn.data(), dn.data(), cache.get_layer_ptr(0, 0),
+                                 cache.get_layer_ptr(0, 1), table.data(), cache.pages_used(c),
+                                 zero.data(), 1, n, kHkv, kD, cache.num_pages());
+            HIP_CHECK(hipDeviceSynchronize());
+            cache.release(c);
+        }
+    }
+    EXPECT(cache.free_page_count() >= 14 - kB * 5, "pages held: %d", 14 - cache.free_page_count());
+}
+
 void case_shrink() {
     PagedKVCache cache(1, 1, 8, 8, 2, 4);
     const int a = cache.add_sequence(), b = cache.add_sequence();
@@ -408,6 +514,8 @@ int main(int argc, char** argv) {
         void (*fn)();
     } cases[] = {{"refusals", false, case_refusals},
                  {"private", true, case_private},
+                 {"drop_hidden", true, case_drop_hidden},
+                 {"windowed", true, case_windowed},
                  {"shrink", true, case_shrink},
                  {"served", true, case_served}};
     for (const auto& c : cases) {
