@@ -276,13 +276,23 @@ int kvhp_causal_gqa(const void* q, const void* k, const void* v, void* out,
  * that several rows of a block table name (a shared prefix) must not be given
  * sums or evicted.
  *
+ * Positions: after an eviction a sequence's next token stands at newest + 1 of
+ * the text but goes into slot new_lens[b].  Keys keep the rotation of their
+ * place in the text, so a cut cache takes its tokens from
+ * kvhp_split_qkv_rope_rows at text positions and kvhp_paged_append_kv at slots;
+ * the fused kvhp_rmsnorm_qkv_rope_append* calls rotate and write at one and the
+ * same position and are for caches that were never cut (windowed ones among
+ * them, whose slots are the text's positions).
+ *
  * Lengths above max_seq_len (or the block table's reach) count as that, and
  * sequences of length <= 0 have no keys.  Every call is asynchronous on
  * `stream`, allocates nothing and may be captured; where a call takes a
  * workspace, it must be 16-byte aligned and hold *_workspace_bytes bytes (0:
  * NULL is fine), and calls that overlap need one each.  fp16 tensors, head_dim
  * 1..256; the fast kernels take head_dim 64 and 128, 16-byte aligned tensors
- * and rows, and one block table for K and V.  Sums of scores, softmax states
+ * and rows, and one block table for K and V.  How the work is cut goes by
+ * max_seq_len, the window and the sinks, not by the lengths on the device: pass
+ * the longest length of the step, not the cache's capacity.  Sums of scores, softmax states
  * and weights are fp32. */
 
 /* One new token per sequence, at position seq_lens[b] - 1: as

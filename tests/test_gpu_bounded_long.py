@@ -50,7 +50,7 @@ def _shared(seed, B, hkv, d, n):
     k, v = (torch.empty((hkv, pages, PAGE, d), dtype=torch.float16, device="cuda").normal_(
         generator=g) for _ in range(2))
     order = np.random.default_rng(seed).permutation(pages).astype(np.int32)
-    bt = to_gpu(np.broadcast_to(order, (B, pages)))
+    bt = to_gpu(np.tile(order, (B, 1)))
     at = to_gpu(order).long()
     return k, v, bt, [x[:, at].reshape(hkv, -1, d)[:, :n] for x in (k, v)]
 
@@ -127,3 +127,51 @@ def test_many_small_weights_beside_a_large_one(d, window):
             ds = (d + 8) * U32 * 18
             tol = (3 * U16 + 2 * ds + 2 * seen * U32) * want + seen * 2.0 ** -32 / l + 2.0 ** -25
             check(got[b, r], np.full((hkv, d), want), np.full((hkv, d), tol), f"{lens[b]} keys, row {r}")
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(700, 20), (0, 0), (1500, 0)])
+@pytest.mark.parametrize("paged", [False, True])
+def test_long_prompts(hq, hkv, d, window, sinks, paged):
+    """Prompts whose blocks of rows have their window wholly inside the text, and causal ones
+    with their log-sum-exp: every row of every head."""
+    import torch
+    S, G = 2611, hq // hkv
+    g = torch.Generator(device="cuda").manual_seed(S + d)
+    if paged:
+        k, v, bt, (kk, vv) = _shared(d, 1, hkv, d, S)
+        views = [kvhp.paged_view(x, bt) for x in (k, v)]
+    else:
+        k, v = (torch.empty((1, S, hkv, d), dtype=torch.float16, device="cuda").normal_(generator=g)
+                for _ in range(2))
+        views = [kvhp.strided_view(x, x.stride(0), x.stride(2), x.stride(1)) for x in (k, v)]
+        kk, vv = (x[0].transpose(0, 1) for x in (k, v))
+    q = torch.empty((1, S, hq, d), dtype=torch.float16, device="cuda").normal_(generator=g)
+    out, lse = torch.zeros_like(q), torch.zeros((1, hq, S), device="cuda")
+    ws = workspace(kvhp.window_prefill_workspace_bytes(1, S, hq, hkv, d, S, window, sinks))
+    note(f"window_prefill: a prompt of {S}, {hq}/{hkv} x {d}, window {window}, paged={paged}")
+    kvhp.window_prefill(q, *views, out, hq, hkv, d, S, window, sinks, lse=lse, workspace=ws)
+    sync()
+    j = torch.arange(S, device="cuda")
+    see = j[None] <= j[:, None]
+    if window > 0:
+        see &= (j[None] < sinks) | (j[:, None] - j[None] < window)
+    for h in range(hq):
+        kd, vd = kk[h // G].double(), vv[h // G].double()
+        qd = q[0, :, h].double()
+        s = (qd @ kd.T.contiguous()) / math.sqrt(d)
+        s.masked_fill_(~see, -math.inf)
+        size = ((qd.abs() @ kd.abs().T.contiguous()) / math.sqrt(d)).masked_fill_(~see, 0).amax(1)
+        m = s.amax(1)
+        ds = (d + 4) * U32 * size + 4 * U32 * s.masked_fill(~see, 0).abs().amax(1)
+        e = torch.exp(s - m[:, None])
+        l, n = e.sum(1), see.sum(1)
+        p = e / l[:, None]
+        want = p @ vd
+        small = n * 2.0 ** -25 * vd.abs().max() / l
+        tol = (U16 * want.abs() + (2 * U16 + 2 * ds + 2 * n * U32)[:, None] * (p @ vd.abs()) +
+               small[:, None] + 2.0 ** -25)
+        check(from_gpu(out[0, :, h]), from_gpu(want), from_gpu(tol), f"head {h}")
+        want = m + l.log()
+        check(from_gpu(lse[0, h]), from_gpu(want),
+              from_gpu(ds + (n + 8) * U32 + 4 * U32 * want.abs()), f"lse of head {h}")

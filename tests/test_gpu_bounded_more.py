@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kvhp
-from bounded_util import PAGE, Cache, check, decode_ref, plan_ref, workspace
+from bounded_util import PAGE, Cache, attend, check, decode_ref, plan_ref, workspace
 from gpu_util import from_gpu, note, sync, to_gpu
 from test_gpu_bounded import (_calls, _check_prefill, _check_sums, _prefill_ref, _prompt_ref,
                               _prompt_weights, _q, _sums, _sums_ref, _weighted, _window_decode,
@@ -355,3 +355,106 @@ def test_one_split_sums_limits_by_units(batch, hkv, d, limit):
         rw, tw, ra = _sums_ref(c, w, ages, sums, rel, 2, c.lens - 1)
         _check_sums(gw, rw, tw)
         assert np.array_equal(ga, ra)
+
+
+def test_steps_over_a_cut_cache_with_rope():
+    """Tokens behind an eviction: rotated at their place in the text, appended at their slot,
+    attended with what was kept, and cut again."""
+    import torch
+    rng = np.random.default_rng(31)
+    B, hq, hkv, d, n, budget, theta = 3, 8, 2, 64, 150, 96, 10000.0
+    c = Cache(rng, [n, n - 30, 40], hkv, d).upload()
+    text = c.lens.copy()                       # tokens of the text so far
+    pages = c.pages + 6
+    pools = [torch.zeros(hkv, pages, PAGE, d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for big, small in zip(pools, (c.pool_k, c.pool_v)):
+        big[:, :c.pages] = small
+    bt = np.concatenate([c.bt, np.full((B, 1), -1, np.int32)], 1)
+    bt[2, 3] = c.pages                         # one more page for the short one
+    bt_d = to_gpu(bt)
+    kv, vv = kvhp.paged_view(pools[0], bt_d), kvhp.paged_view(pools[1], bt_d)
+    w = to_gpu(rng.random((hkv, pages, PAGE)).astype(np.float32))
+    ages = torch.zeros(hkv, pages, PAGE, dtype=torch.int32, device="cuda")
+    for b in range(B):
+        pg, sl = c.slots(b)
+        ages[:, to_gpu(pg).long(), to_gpu(sl).long()] = torch.arange(
+            int(c.lens[b]), dtype=torch.int32, device="cuda")
+    lens, newest = to_gpu(c.lens), to_gpu(text - 1)
+    moves = torch.zeros(B, hkv, 96, 2, dtype=torch.int32, device="cuda")
+    counts = torch.zeros(B, hkv, dtype=torch.int32, device="cuda")
+    new = torch.zeros(B, dtype=torch.int32, device="cuda")
+    cap = 10 * PAGE
+    ws = workspace(kvhp.weighted_decode_workspace_bytes(B, hq, hkv, d, cap))
+    for cut in range(2):
+        note(f"cut {cut}: eviction")
+        kvhp.evict_plan(w, ages, bt_d, lens, moves, counts, new, cap, budget, 4, 20, newest=newest)
+        kvhp.evict_apply(pools[0], pools[1], w, ages, bt_d, moves, counts)
+        lens.copy_(new)
+        for step in range(5):
+            qkv = to_gpu(_q(rng, B, (hq + 2 * hkv) * d))
+            q, k, v = (torch.zeros(B, h, d, dtype=torch.float16, device="cuda") for h in (hq, hkv, hkv))
+            newest += 1
+            text += 1
+            note(f"cut {cut}: step {step}")
+            kvhp.split_qkv_rope_rows(qkv, B, hq, hkv, d, newest, theta, q, k, v)
+            kvhp.paged_append_kv(k, v, pools[0], pools[1], bt_d, lens, B, 1, hkv, d)
+            lens += 1
+            out = torch.zeros_like(q)
+            kvhp.weighted_decode(q, kv, vv, lens, out, w, hq, hkv, d, cap, new_keys=1, ages=ages,
+                                 newest=newest, workspace=ws)
+            sync()
+            slots = from_gpu(lens) - 1
+            assert (slots[:2] == budget + step + 0).all() and (from_gpu(newest) == text - 1).all()
+            hk, hv, ha = from_gpu(pools[0]), from_gpu(pools[1]), from_gpu(ages)
+            for b in range(B):
+                # one row at its place in the text, as a prompt's rows are rotated
+                one = [torch.zeros(1, h, d, dtype=torch.float16, device="cuda") for h in (hq, hkv, hkv)]
+                kvhp.split_qkv_rope(qkv[b:b + 1], 1, hq, hkv, d, int(text[b]) - 1, theta, *one)
+                sync()
+                m = int(slots[b])
+                pg, sl = bt[b, m // PAGE], m % PAGE
+                assert torch.equal(one[0][0], q[b])
+                assert np.array_equal(hk[:, pg, sl], from_gpu(one[1][0]))
+                assert np.array_equal(hv[:, pg, sl], from_gpu(one[2][0]))
+                assert (ha[:, pg, sl] == text[b] - 1).all()
+                j = np.arange(m + 1)
+                hq_ = from_gpu(q[b]).reshape(hkv, -1, d)
+                for h in range(hkv):
+                    o, tol, _, _, _ = attend(hq_[h], hk[h, bt[b, j // PAGE], j % PAGE],
+                                             hv[h, bt[b, j // PAGE], j % PAGE], j >= 0)
+                    check(from_gpu(out[b]).reshape(hkv, -1, d)[h], o, tol, f"sequence {b}, head {h}")
+                    a = ha[h, bt[b, j // PAGE], j % PAGE]
+                    assert len(set(a)) == m + 1 and a.max() == text[b] - 1   # each token once
+
+
+@pytest.mark.parametrize("d", [64, 128, 96])
+def test_prompt_weights_hidden_keys_reach_nothing(d):
+    """NaN and infinite K in slots that the window hides from every row, from some, and above
+    the diagonal: the sums of keys that the rows see are as without them, and a key's own sum
+    is not finite only where a row sees it."""
+    rng = np.random.default_rng([d, 77])
+    n, rows, window, sinks = 300, 70, 50, 5
+    c = Cache(rng, [n, 130], 2, d)
+    q = _q(rng, 2, rows, 8, d)
+    start = [n - rows, 130 - rows]
+    w, ages = _sums(rng, c)
+    lse, add, rel = _prompt_ref(q, c, start, window, sinks)
+    rw, tw, ra = _sums_ref(c, w, ages, add, rel, 20, c.lens - 1)
+    # hidden from every row; seen by the first rows only; by the last only; a first token
+    for key in (100, 200, n - 2, 3):
+        for bad in (np.nan, np.inf):
+            k = c.k.copy()
+            c.k[0, :, key] = bad
+            c.upload()
+            note(f"prompt_weights: K of key {key} is {bad}, d={d}")
+            gw, ga = _prompt_weights(q, c, lse, w, ages, start, window, sinks, 20)
+            c.k = k
+            pg, sl = c.bt[0, key // PAGE], key % PAGE
+            hit = gw[:, pg, sl].copy()
+            gw[:, pg, sl], want = rw[:, pg, sl], rw.copy()
+            _check_sums(gw, want, tw)
+            assert np.array_equal(ga, ra)
+            if key == 100:
+                assert np.array_equal(hit, w[:, pg, sl])      # no row sees it: not touched
+            else:
+                assert not np.isfinite(hit).any()
