@@ -123,11 +123,13 @@ __device__ __forceinline__ void dma16s(const f16* sbase, uint32_t voff, f16* lds
                  :: "s"(m0v), "v"(voff), "s"(sbase) : "memory", "m0");
 }
 
-// s_waitcnt vmcnt(N) (expcnt / lgkmcnt left free).
+// s_waitcnt vmcnt(N) lgkmcnt(0): all but N loads have landed, and this wave's reads
+// of LDS have returned, so that behind the next barrier a stage may be written anew
+// although the products that take the operands are ordered behind it.
 template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
+__device__ __forceinline__ void wait_ring() {
     static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4));
 }
 
 // Orders this wave's LDS accesses across the barrier without the vmcnt(0)
@@ -392,7 +394,7 @@ prefill_mfma_kernel(const PrefillArgs a) {
             pid_next = ptab[page_of(0) - t_lo * 4];
         }
 
-        wait_vmcnt<0>();  // q in registers before the ring: no compiler waits inside it
+        wait_ring<0>();  // q in registers before the ring: no compiler waits inside it
         ring_barrier();   // everyone is done with the previous pass's stages
         issue(ring, 0);
         issue(ring + 2 * TB, 1);
@@ -554,7 +556,7 @@ prefill_mfma_kernel(const PrefillArgs a) {
             __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): written before the barrier
         };
         auto phase_start = [&](int j) {   // barrier into phase 2j, then tile j+2
-            wait_vmcnt<LPT>();
+            wait_ring<LPT>();
             if (CACHED && j >= cut0 && j < n_tiles) clean(j);
             ring_barrier();
             const int tt = j + 2;
@@ -589,7 +591,7 @@ prefill_mfma_kernel(const PrefillArgs a) {
             ring_barrier();
             pv(n_tiles - 1);
         }
-        wait_vmcnt<0>();  // drain the ring's trailing re-loads
+        wait_ring<0>();  // drain the ring's trailing re-loads
 
         // ---- pages: this query block's own K/V rows, once per KV head.  Rows
         //      of the pass's last tile come from its ring stage (still intact:
@@ -724,7 +726,7 @@ prefill_mfma_kernel(const PrefillArgs a) {
             }
         }
 
-        wait_vmcnt<0>();   // page and output stores complete before the next ring starts
+        wait_ring<0>();   // page and output stores complete before the next ring starts
     }
 }
 
