@@ -1,5 +1,6 @@
-// bounded.h -- shared by the kernels of caches of bounded length (bounded.hip,
-// window_prefill.hip, evict.hip): views, visibility, argument checks.
+// bounded.h -- shared by the attention kernels of caches of bounded length (bounded.hip,
+// bounded_decode.hip, window_prefill.hip, prompt_weights.hip): views, visibility,
+// argument checks.
 #pragma once
 
 #include "kvhp_internal.h"

@@ -88,19 +88,6 @@ __device__ __forceinline__ int chunk_of(const DecodePlan& p, int L, long long ke
     return ((L + n - 1) / n + 31) / 32 * 32;   // at most kMaxChunk; whole steps
 }
 
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) short4v lds_short4v;
-typedef __attribute__((address_space(3))) f16 lds_f16;
-
-// Transposing 8-byte LDS read: a 16-lane block that addresses four rows' 4-element
-// groups gets one column of the 4 x 16 tile per lane.
-__device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(lds_f16*)p);
-}
-__device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
-    return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
 // Four keys of a KV head from j (a multiple of 4) on: their slot (-1: none) and sums.
 struct Quad {
     int64_t slot;

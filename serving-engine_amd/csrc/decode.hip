@@ -139,23 +139,6 @@ __device__ __forceinline__ int chunk_of(const DecodeArgs& a, int L, long long ke
     return ((L + n - 1) / n + kPage - 1) / kPage * kPage;
 }
 
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) short4v lds_short4v;
-typedef __attribute__((address_space(3))) f16 lds_f16;
-
-// ds_read_b64_tr_b16: within each 16-lane block, lane i receives element
-// (i % 4) of the 8-byte groups addressed by lanes 4k + i/4, k = 0..3.
-// So if lane j addresses the 4 consecutive elements [col0 + 4(j%4), +4) of
-// row R(j/4), lane i gets column col0 + i of rows R(0..3): a 4 x 16 tile
-// transposed into the MFMA operand layout.
-__device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(lds_f16*)p);
-}
-
-__device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
-    return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
 // One workgroup of W waves per (split, kv_head, sequence); wave w takes the
 // split's 32-token steps w, w+W, ... and the waves' states meet in LDS at
 // the end (W = 1: the wave's state is the split's).  Both contractions

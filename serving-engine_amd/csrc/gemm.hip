@@ -36,10 +36,6 @@ namespace kvhp {
 
 namespace {
 
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) f16 lds_f16;
-typedef __attribute__((address_space(3))) void lds_void;
-
 enum GemmEpi : int { kGemmResidual = 0, kGemmSwiglu = 1, kGemmQKV = 2, kGemmF32 = 3 };
 
 struct GemmArgs {

@@ -230,6 +230,16 @@ __device__ __forceinline__ float rows4_sum(float x) {
 __device__ __forceinline__ float wave_sum_fast(float x) { return rows4_sum(row16_sum(x)); }
 __device__ __forceinline__ float wave_max_fast(float x) { return rows4_max(row16_max(x)); }
 
+// Sum / max across the two 32-lane halves of a wave (v_permlane32_swap).
+__device__ __forceinline__ float halves_max(float x) {
+    auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+
 __device__ __forceinline__ half8 load_half8(const f16* p) {
     return *reinterpret_cast<const half8*>(p);
 }
@@ -245,6 +255,53 @@ __device__ __forceinline__ void store_half8(f16* p, half8 v) {
 
 __device__ __forceinline__ float fast_exp2(float x) {
     return __builtin_amdgcn_exp2f(x);
+}
+
+// ---- LDS operands and rings of stages ----
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+typedef __attribute__((address_space(3))) f16 lds_f16;
+typedef __attribute__((address_space(3))) void lds_void;
+
+// ds_read_b64_tr_b16: within each 16-lane block, lane i receives element
+// (i % 4) of the 8-byte groups addressed by lanes 4k + i/4, k = 0..3.
+// So if lane j addresses the 4 consecutive elements [col0 + 4(j%4), +4) of
+// row R(j/4), lane i gets column col0 + i of rows R(0..3): a 4 x 16 tile
+// transposed into the MFMA operand layout.
+__device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(lds_f16*)p);
+}
+__device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
+    return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(lds_f16*)p));
+}
+// global_load_lds_dwordx4: 16 bytes per lane from a wave-uniform base and the
+// lane's byte offset, lane l's to lds_base + 16 l (M0 holds the wave-uniform LDS
+// base).  Issued as inline asm so that only the explicit vmcnt waits of a ring
+// order it against the LDS reads: the compiler's own tracking cannot tell ring
+// stages apart and would otherwise drain every in-flight stage before each read.
+__device__ __forceinline__ void dma16s(const void* base, uint32_t voff, const void* lds_base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(lds_at(lds_base)), "v"(voff), "s"(base) : "memory", "m0");
+}
+// s_waitcnt vmcnt(N) lgkmcnt(0): all but N loads have landed, and this wave's reads
+// of LDS have returned, so that behind the next barrier a stage may be written anew
+// although the products that take the operands are ordered behind it.
+template <int N>
+__device__ __forceinline__ void wait_ring() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4));
+}
+// Orders this wave's LDS accesses across the barrier without the vmcnt(0)
+// drain a __syncthreads() fence implies (which would empty the ring).
+__device__ __forceinline__ void ring_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 }  // namespace kvhp

@@ -88,71 +88,13 @@ struct PrefillArgs {
     float* ws_ml;           // [S * Hq][nsplit][2]  (max in log2 units, sum)
 };
 
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) short4v lds_short4v;
-typedef __attribute__((address_space(3))) f16 lds_f16;
-typedef __attribute__((address_space(3))) void lds_void;
-
-// ds_read_b64_tr_b16: within each 16-lane block, lane i receives element
-// (i % 4) of the 8-byte groups addressed by lanes 4k + i/4, k = 0..3.
-__device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(lds_f16*)p);
-}
-
-__device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
-    return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// global_load_lds_dwordx4: lane l's 16 bytes land at lds_base + 16*l (M0
-// holds the wave-uniform LDS base).  Issued as inline asm so that only the
-// explicit vmcnt waits of the ring order it against the LDS reads: the
-// compiler's own tracking cannot tell ring stages apart and would otherwise
-// drain every in-flight stage before each read.
+// dma16s with each lane's own address.
 __device__ __forceinline__ void dma16(const f16* src, f16* lds_base) {
-    const uint32_t m0v = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((lds_void*)(lds_f16*)lds_base));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(m0v), "v"(src) : "memory", "m0");
+                 :: "s"(lds_at(lds_base)), "v"(src) : "memory", "m0");
 }
-
-// Same with a wave-uniform base in SGPRs and a 32-bit per-lane byte offset.
-__device__ __forceinline__ void dma16s(const f16* sbase, uint32_t voff, f16* lds_base) {
-    const uint32_t m0v = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((lds_void*)(lds_f16*)lds_base));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(m0v), "v"(voff), "s"(sbase) : "memory", "m0");
-}
-
-// s_waitcnt vmcnt(N) lgkmcnt(0): all but N loads have landed, and this wave's reads
-// of LDS have returned, so that behind the next barrier a stage may be written anew
-// although the products that take the operands are ordered behind it.
-template <int N>
-__device__ __forceinline__ void wait_ring() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4));
-}
-
-// Orders this wave's LDS accesses across the barrier without the vmcnt(0)
-// drain a __syncthreads() fence implies (which would empty the DMA ring).
-__device__ __forceinline__ void ring_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLazyLog2 = 8.f;  // P stays below 2^8 between rescales
-
-// Sum / max across the two 32-lane halves of a wave (v_permlane32_swap).
-__device__ __forceinline__ float halves_max(float x) {
-    auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-    auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-}
 
 // A workgroup of 8 waves serves one KV head and a query block of 32*RB rows
 // for all G query heads of that KV head: G*RB units of (head, 32 rows).  With

@@ -37,10 +37,6 @@ constexpr int kTile = 64;        // pairs per tile
 constexpr int KB = 32 * kWaves;  // keys per workgroup
 constexpr int kMaxRowHeads = 1 << 30;   // (row, query head) pairs of a KV head
 
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) f16 lds_f16;
-typedef __attribute__((address_space(3))) void lds_void;
-
 // A tile is 2^lr rows of `gc` heads, 64 pairs, row fastest; tile f is row tile f / nh and
 // heads (f % nh) * gc on.
 struct SumPlan {
@@ -51,25 +47,10 @@ struct SumPlan {
     float* ws;        // [nrange][batch][Hkv][keys_pitch], nrange > 1
 };
 
-// 16 (4) bytes from a scalar base and lane l's byte offset to lds_base + 16 l (4 l); only
-// the ring's own waits order it.
-__device__ __forceinline__ uint32_t lds_at(const void* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(lds_f16*)p));
-}
-__device__ __forceinline__ void dma16s(const char* base, uint32_t voff, f16* lds_base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(lds_at(lds_base)), "v"(voff), "s"(base) : "memory", "m0");
-}
+// dma16s with 4 bytes a lane.
 __device__ __forceinline__ void dma4s(const char* base, uint32_t voff, float* lds_base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                  :: "s"(lds_at(lds_base)), "v"(voff), "s"(base) : "memory", "m0");
-}
-// This wave's loads have landed, and its reads of LDS have returned.
-__device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(0x7 << 4); }
-__device__ __forceinline__ void ring_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
 }
 
 // The live rows' positions [p0, p1] of a sequence (p0 > p1: none).
@@ -216,7 +197,7 @@ prompt_weights_kernel(const BoundArgs a, const SumPlan p) {
 
     // Tile t has landed everywhere, and every wave is past tile t - 1.
     auto begin = [&](int t) {
-        wait_all();
+        wait_ring<0>();
         ring_barrier();
         issue(t + 1);
     };
@@ -291,7 +272,7 @@ prompt_weights_kernel(const BoundArgs a, const SumPlan p) {
         begin(t + 1);
     }
     for (; t < n_tiles; ++t) begin(t + 1);
-    wait_all();   // the ring's trailing re-loads
+    wait_ring<0>();   // the ring's trailing re-loads
 
     // ---- over the 32 lanes of a half; lane c32 < 16 keeps element c32
     float sum = 0.f;

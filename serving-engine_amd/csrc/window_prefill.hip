@@ -61,43 +61,6 @@ constexpr int kCUs = 256;
 constexpr float kRefLog2 = 7.f;       // a row's reference below its maximum where it is set,
 constexpr float kLazyLog2 = 15.f;     // and where it moves: weights up to 2^15 in fp16
 
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) short4v lds_short4v;
-typedef __attribute__((address_space(3))) f16 lds_f16;
-typedef __attribute__((address_space(3))) void lds_void;
-
-__device__ __forceinline__ short4v lds_read_tr16(const f16* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(lds_f16*)p);
-}
-__device__ __forceinline__ half8 cat_half8(short4v lo, short4v hi) {
-    return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-// 16 bytes from a scalar base and lane l's byte offset to lds_base + 16 l; only the
-// ring's own waits order it.
-__device__ __forceinline__ void dma16s(const char* base, uint32_t voff, f16* lds_base) {
-    const uint32_t m0v = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((lds_void*)(lds_f16*)lds_base));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(m0v), "v"(voff), "s"(base) : "memory", "m0");
-}
-// This wave's loads have landed, and its reads of LDS have returned: the products that take
-// them need not have been issued before the barrier behind which a stage is loaded anew.
-__device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(0x7 << 4); }
-// A workgroup barrier that leaves the ring's loads in flight.
-__device__ __forceinline__ void ring_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ float halves_max(float x) {
-    auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-    auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-}
 
 struct PrefillPlan {
     uint32_t inv_g;        // ceil(2^32 / G), 0 for G = 1
@@ -489,7 +452,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         pid_k = keys.page(g + 3);
     };
     auto begin = [&](int j) {
-        wait_all();
+        wait_ring<0>();
         if (j >= 0) keys.clean(j, vring + (j & 1) * TB);
         ring_barrier();
         issue(j);
@@ -570,7 +533,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         }
     };
 
-    wait_all();   // q in registers before the ring: no other waits inside it
+    wait_ring<0>();   // q in registers before the ring: no other waits inside it
     __syncthreads();   // ptab, bad
     pid_k = pid_v = keys.page(0);
     issue(-2);
@@ -598,7 +561,7 @@ window_prefill_kernel(const BoundArgs a, const PrefillPlan p) {
         exps(s0[t], pa);
         pv(j, t, pa);
     }
-    wait_all();   // the ring's trailing re-loads
+    wait_ring<0>();   // the ring's trailing re-loads
     keys.add_back(o, x.live, x.pos);
     store_pair<D>(a, p, x, b, h, all_tiles, o, m_run, halves_sum(l_part));
 }
