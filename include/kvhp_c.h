@@ -290,7 +290,8 @@ int kvhp_causal_gqa(const void* q, const void* k, const void* v, void* out,
  * workspace, it must be 16-byte aligned and hold *_workspace_bytes bytes (0:
  * NULL is fine), and calls that overlap need one each.  fp16 tensors, head_dim
  * 1..256; the fast kernels take head_dim 64 and 128, 16-byte aligned tensors
- * and rows, and one block table for K and V.  How the work is cut goes by
+ * and rows, and one block table for K and V; other shapes run on kernels for any,
+ * which are tens of times slower in long caches.  How the work is cut goes by
  * max_seq_len, the window and the sinks, not by the lengths on the device: pass
  * the longest length of the step, not the cache's capacity.  Sums of scores, softmax states
  * and weights are fp32. */

@@ -4,7 +4,13 @@
 //
 // Any head_dim <= 256, any strides, any group: one wave per (query head, row),
 // one pass over its visible keys with an online softmax, fp32 throughout; and
-// one wave per (key, KV head) for the weights that rows gave a key.
+// one wave per (key, KV head) for the weights that rows gave a key.  These are for
+// rare shapes and no more: one key per trip behind a six-step sum over the wave, K
+// and V read again for every query head, no split over the keys.  At D = 96, 32/8
+// heads, windows of 4096 in 32 sequences take 5.9 ms where memory would need 65 us,
+// a 2048-row prompt with window 512 2.9 ms, its sums 7.7 ms (D = 256 13, 4.5 and 14
+// ms): 2 to 8 times the elementary torch operations.  What bounds them is latency,
+// a wave's loads one after the other.
 #include "bounded.h"
 
 namespace kvhp {

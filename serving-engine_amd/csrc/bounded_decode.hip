@@ -10,9 +10,9 @@
 // a lane owns one query head through the online softmax,
 //   S^T = K Q^T      A = K rows through LDS, B = Q^T in registers
 //   O^T += V^T P^T   A = V^T by transposing LDS reads, B = P^T from S^T's
-//                    accumulators, rounded to fp16 (half a step of 2^-11 on
-//                    weights that are summed over many keys; the softmax's sum
-//                    takes them unrounded)
+//                    accumulators, rounded to fp16 (2^-11 of each down to 2^-14 of
+//                    the split's largest, an absolute 2^-25 of it below, less than
+//                    2^-14 over a split; the softmax's sum takes them unrounded)
 // K is fetched two steps ahead and V one, as whole rows.  A key's row is found
 // through the chunk's page ids, one per lane, by an exchange between lanes:
 // with a window the chunks start anywhere in a page.  Up to 16 query heads of

@@ -20,10 +20,11 @@
 //
 // A thread owns consecutive slots, whose keys stay in registers between the
 // passes (up to 8192 slots), in LDS (32768), or are read again.  Bound by the
-// chain of some ten barriers and, in longer caches, by one CU's instructions
-// per slot: 7.8 us for one sequence of 2064 slots, 10.3 for 8192, 12.6 for 32 of
-// up to 8192, 21 for 16384, 33 for 32768 (their 8 bytes a slot are 2 us or less
-// at the card's rate).
+// chain of 13 barriers (5 a digit, two digits nearly always) and, in longer
+// caches, by one CU's instructions per slot: 8.6 us for one sequence of 2064 slots
+// cut to 2048, 7.3 for 4096 to half, 10.3 for 8192, 12.5 for 32 of up to 8192, 21
+// for 16384, 33 for 32768, 131 for 65536 read again (their 8 bytes a slot are 4 us
+// or less at the card's rate).
 #include "kvhp_internal.h"
 
 #include <algorithm>

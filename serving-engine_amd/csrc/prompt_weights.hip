@@ -20,9 +20,10 @@
 // 4096 rows of 32/8 heads of 128 (69 GFLOP) take 88 us, 0.78 PFLOP/s, 32 rows of four
 // sequences of 3001 keys at 32/4 heads of 64 9.1.  Bound by the vector unit, per 32 x 32
 // scores 16 times (fma, exp, add) of 24 cycles, 47 us over the prompt if it never waited;
-// the 8 MFMAs of 32 cycles run beside it in other waves, four workgroups a CU.  The rest
-// is a causal prompt's last workgroups, the loads in front of a workgroup's first tile, and the
-// second launch (4).  One wave running the next pairs' MFMAs between the exponentials of
+// the 8 MFMAs of 32 cycles run beside it in other waves, four workgroups a CU.  The second
+// launch takes 4; waves wait for a quarter of their cycles (counters: vector unit 65 % busy,
+// matrix cores 45 %, LDS 24 %), at what is not known: it is not whole rounds of workgroups, see
+// the ranges below.  One wave running the next pairs' MFMAs between the exponentials of
 // these was no faster (three workgroups a CU, 104 us); 64 keys a wave, half the LDS reads,
 // spill registers (136 to 300).
 #include "bounded.h"
@@ -320,8 +321,8 @@ prompt_weights_add_kernel(const BoundArgs a, const SumPlan p) {
 
 // Tiles of one head's 64 rows, or of all rows where they are fewer, of as many heads as fit.
 // Ranges of at least 6 tiles, for about 12 workgroups per CU, of which half see nothing in a
-// whole prompt (4096 rows of 32/8 heads of 128, for 7 / 8 / 10 / 12 / 14 / 16: 101 / 105 /
-// 97 / 96 / 97 / 101 us: whole rounds of four a CU); of at least 2 while all run at once (512
+// whole prompt (4096 rows of 32/8 heads of 128, for 7 / 8 / 10 / 12 / 14 / 16 / 20: 91.4 / 94.5 /
+// 88.0 / 86.2 / 87.8 / 89.7 / 87.2 us; 2048 34.4 / 33.8 / 32.7 / 32.7 / 32.9 / 32.6 / 32.7); of at least 2 while all run at once (512
 // rows 10.6 us, 4 tiles 11.6, 8 15.4; but 1000 rows 18.2 / 16.8 / 17.6).  Up to 5 tiles
 // are not worth a second launch (64 rows of 4 heads 8.0 us whole, 10.4 in two; of 7 11.1 and
 // 9.6 in four).

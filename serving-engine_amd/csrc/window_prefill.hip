@@ -19,13 +19,16 @@
 // softmax in the log2 domain whose reference lies 2^7 to 2^15 below a row's largest weight
 // (it moves when a row passes it by 2^15).  Weights are rounded to fp16 for the product: 2^-11
 // each down to 2^-14 of the reference, an absolute 2^-25 of it below, so that 10^5 keys of
-// little weight beside a first token of much still count; O^T += V^T P^T.  K and V rows go from memory to
-// two LDS stages per matrix without registers (global_load_lds, a scalar base and the
-// lane's fixed offset; page ids from LDS), with their 16-byte chunks XOR-swizzled so that
-// both operand reads touch all banks.
+// little weight beside a first token of much still count; O^T += V^T P^T.  K and V rows go
+// from memory to two LDS stages per matrix without registers (global_load_lds, a scalar base
+// and the lane's fixed offset; page ids from LDS), with their 16-byte chunks XOR-swizzled so
+// that both operand reads touch all banks.
 //
-// At 8192 rows, window 2048, 32/8 heads of 128: 255-268 us by box, 0.90-0.95 PFLOP/s; four
-// chunks of 128 rows behind 4096 keys 47, of which the join 7.  Counters: matrix cores 55 %,
+// At 8192 rows, window 2048, 32/8 heads of 128: 255-273 us by box, 0.89-0.95 PFLOP/s; a chunk
+// of 128 rows of each of four sequences of 1062 to 8192 keys, window 4096, 47-49, of which the
+// join 7 (the ranges go by the window, so 96 of their 512 workgroups have no keys and the
+// others up to 17 tiles).  Without a window, with lse, 512 / 2048 / 8192 rows take 18.3 / 48.7 /
+// 512 us where the causal prefill without lse takes 14.7 / 45.7 / 508.  Counters: matrix cores 55 %,
 // vector unit 50 %, LDS reads 28 % of the cycles, at the 1.6 GHz that the card holds under
 // this load (a large library product: 1.18 PFLOP/s).  The MFMAs alone take 172 us of 262;
 // without the exponentials the kernel takes 228, without LDS operand reads 234, without
