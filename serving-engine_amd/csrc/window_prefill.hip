@@ -64,7 +64,6 @@ constexpr int kCUs = 256;
 constexpr float kRefLog2 = 7.f;       // a row's reference below its maximum where it is set,
 constexpr float kLazyLog2 = 15.f;     // and where it moves: weights up to 2^15 in fp16
 
-
 struct PrefillPlan {
     uint32_t inv_g;        // ceil(2^32 / G), 0 for G = 1
     int blocks;            // of pairs, per sequence and KV head
