@@ -12,10 +12,11 @@ Each case names a `path` and its sizes:
 
 Four bits: a row x of D values (a token's K or V of one KV head) has codes n of 0 to
 15 and two numbers in fp16, s and r, and stands for s (n + r).  s is (max x - min x) /
-15; r is min x / s, rounded so that n + r is exact in fp16 (to steps of 2^-6 where it
-lies in -15 .. 15); n is x / s - r, rounded.  A row of equal values c has s = c, r = 1
-and codes 0.  A page of a KV head holds 16 rows: K codes [16][D/2] (the even dim in the
-low half of a byte), V codes, K's (s, r) [16][2], V's.
+15, or max |x| / 1984 where that is more, rounded up; r is min x / s, rounded so that
+n + r is exact in fp16 (to steps of 2^-6 where it lies in -15 .. 15); n is x / s - r,
+rounded.  A row of equal values c has s = c, r = 1 and codes 0.  A page of a KV head
+holds 16 rows: K codes [16][D/2] (the even dim in the low half of a byte), V codes, K's
+(s, r) [16][2], V's.
 
 Sizes are those of the repository's configurations (32/8 heads of 128, 32/4 and 14/2
 heads of 64; contexts of up to 8K for batches, 16K for one sequence).
@@ -192,14 +193,16 @@ def _codes(x):
     """fp16 rows [..., D] as packed codes [..., D/2] and their (s, r) [..., 2]."""
     x = x.float()
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
-    s = ((hi - lo) / 15).half().float()
-    flat = s == 0
-    s = torch.where(flat, lo, s)
+    flat = lo == hi
+    t = torch.maximum((hi - lo) / 15, torch.maximum(lo.abs(), hi.abs()) / 1984)
+    s = t.half()
+    s = torch.where(s.float() < t, (s.view(torch.int16) + 1).view(torch.float16), s).float()
+    s = torch.where(flat, torch.ones_like(lo), s)
     r = lo / s
     step = torch.ldexp(torch.ones_like(r), torch.frexp(r.abs() + 16).exponent - 11)
-    r = torch.where(flat, 1.0, torch.round(r / step) * step)
-    n = torch.round((x - s * r) / s).clamp(0, 15)
-    n = torch.where(flat, 0.0, n).to(torch.uint8)
+    r = torch.round(r / step) * step
+    n = torch.where(flat, 0.0, torch.round((x - s * r) / s).clamp(0, 15)).to(torch.uint8)
+    s, r = torch.where(flat, lo, s), torch.where(flat, 1.0, r)
     return n[..., 0::2] | (n[..., 1::2] << 4), torch.cat([s, r], -1).half()
 
 
@@ -407,7 +410,10 @@ def _stood(x):
     """What fp16 rows stand for in 4 bits, in 64."""
     x = x.double()
     lo, hi = x.min(-1, keepdim=True).values, x.max(-1, keepdim=True).values
-    s = ((hi - lo) / 15).half().double()
+    t = torch.maximum((hi - lo) / 15, torch.maximum(lo.abs(), hi.abs()) / 1984).float()
+    s = t.half().float()
+    up = (t.half().view(torch.int16) + 1).view(torch.float16).float()
+    s = torch.where(s < t, up, s).double()
     step = 2.0 ** (torch.floor(torch.log2((lo / s).abs() + 16)) - 10)
     r = step * torch.round(lo / s / step)
     return s * (torch.round(x / s - r).clamp(0, 15) + r)
