@@ -375,6 +375,92 @@ int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int32_t* ages,
                      const int32_t* counts, int batch, int num_kv_heads, int head_dim,
                      int num_pages, int max_moves, void* stream);
 
+/* ---- Appends that rotate on the way, and caches held in 4 bits.  No counterpart
+ * in the reference, which rotates and appends in calls of their own
+ * (src/cuda/kernels.h:57-70, src/runtime/kv_cache.h:80-91) and holds fp16.
+ *
+ * Rows: q [batch][rows][Hq][D], k and v [batch][rows][Hkv][D], consecutive tokens
+ * q_stride, k_stride and v_stride halfs apart (at least Hq D and Hkv D; the heads of a
+ * token in a row), so that the three may be parts of one fused projection [batch][rows]
+ * [(Hq + 2 Hkv) D].  Row r of sequence b stands at position positions[b] + r of the
+ * text (device int32, NULL: 0), to which q and k are rotated as kvhp_apply_rope does,
+ * and goes to slot slots[b] + r of its sequence (device int32, NULL: the position; they
+ * differ in a cache that was cut).  The rotation's angle is held in 64 bits: where
+ * kvhp_apply_rope and the fused projections lose up to 2^-11 of a turn's radian at
+ * position 8192, this keeps fp16's accuracy.  rope_theta 0: no rotation (k is rotated
+ * already, or never is).  q_out [batch][rows][Hq][D] may be q itself if q_stride is
+ * Hq D; q and q_out both NULL: K and V only.
+ * Rows at negative slots or at or past seq_lens[b] (device int32, NULL: no limit) are
+ * padding: neither read nor written, q_out included.  K and V of a slot past the block
+ * table, or whose page id lies outside [0, num_pages), are dropped (write tables hold -1
+ * for shared pages); its q is rotated all the same.  batch rows (Hq + 2 Hkv) is at most
+ * 2^31 - 1, head_dim even and at most 256. */
+int kvhp_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
+                     int64_t k_stride, int64_t v_stride, const int32_t* positions,
+                     const int32_t* slots, const int32_t* seq_lens, float rope_theta, void* q_out,
+                     void* pool_k, void* pool_v, const int32_t* block_tables, int max_pages,
+                     int num_pages, int batch, int rows, int num_q_heads, int num_kv_heads,
+                     int head_dim, void* stream);
+
+/* A cache in 4 bits: one pool [Hkv][num_pages][kvhp_q4_page_bytes(D)] of bytes for K and
+ * V, 16-byte aligned, through block tables as everywhere; head_dim a multiple of 8 up to
+ * 256.  A row x (a token's K or V of one KV head) has a code n of 0..15 per value and two
+ * fp16 numbers s and r, and stands for s (n + r):
+ *   s = max((max x - min x) / 15, max |x| / 1984), rounded up;
+ *   r = min x / s, to the nearest multiple of 2^(floor(log2(|min x / s| + 16)) - 10), so
+ *       that n + r is an exact fp16 number;
+ *   n = x / s - r, to the nearest, in 0..15.
+ * A row of equal values c: s = c, r = 1, n = 0.  A row with a value that is not finite
+ * stands for NaN throughout.  A page of a KV head is 16 (D + 8) bytes: K codes [16][D/2]
+ * (the even dim in the low half of a byte), V codes, K's (s, r) [16], V's.  At D = 128
+ * that is 4.25 bits a value, at 64 4.5 (and at 8 8).  kvhp_q4_page_bytes is 0 for other
+ * head_dims. */
+size_t kvhp_q4_page_bytes(int head_dim);
+/* kvhp_rope_append into 4-bit pages: what fp16 pages would hold, in 4 bits. */
+int kvhp_q4_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
+                        int64_t k_stride, int64_t v_stride, const int32_t* positions,
+                        const int32_t* slots, const int32_t* seq_lens, float rope_theta,
+                        void* q_out, void* pool, const int32_t* block_tables, int max_pages,
+                        int num_pages, int batch, int rows, int num_q_heads, int num_kv_heads,
+                        int head_dim, void* stream);
+/* Rows read back, each value rounded to fp16: out_k, out_v [batch][Hkv][max_len][D] (either
+ * may be NULL; 16-byte aligned) <- positions start[b] + t (device int32, NULL: 0), t <
+ * max_len; zeros at negative positions and from seq_lens[b] (device int32) on.  Page ids
+ * are clamped into the pool. */
+int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int max_pages, int num_pages,
+                   const int32_t* start, const int32_t* seq_lens, void* out_k, void* out_v,
+                   int batch, int num_kv_heads, int head_dim, int max_len, void* stream);
+/* kvhp_decode_attention over a 4-bit cache: one new token per sequence, q, out
+ * [batch][Hq][D], over the keys 0..seq_lens[b] - 1; zeros for sequences without keys.
+ * Lengths above max_seq_len (or the block table's reach) count as that, page ids are
+ * clamped, and whatever slots past the lengths hold reaches no output.  Scores, softmax
+ * states and sums are fp32; a weight is rounded to fp16 once, with its row's share of s.
+ * Asynchronous, allocates nothing, may be captured.  The workspace must be 16-byte aligned
+ * and hold *_workspace_bytes bytes (0: NULL is fine); calls that overlap need one each.
+ * How the work is cut goes by max_seq_len: pass the longest length of the step.  The fast
+ * kernels take head_dim 64 and 128 with q and out 16-byte aligned; other shapes run on a
+ * kernel for any, which is tens of times slower in long caches. */
+size_t kvhp_q4_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                      int max_seq_len);
+int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables, int max_pages,
+                   int num_pages, const int32_t* seq_lens, void* out, int batch, int num_q_heads,
+                   int num_kv_heads, int head_dim, int max_seq_len, void* workspace,
+                   size_t workspace_bytes, void* stream);
+/* Rows of a prompt, or of a chunk behind cached keys, over a 4-bit cache that holds the
+ * rows' own K and V too: row r of sequence b (q, out [batch][rows][Hq][D]) is at position
+ * q_start[b] + r (device int32, NULL: 0) and attends the keys up to itself.  Rows at
+ * negative positions or at or past seq_lens[b] (device int32, NULL: max_seq_len) are
+ * padding: their out and lse stay as they were.  lse (may be NULL): fp32
+ * [batch][Hq][rows], the natural logarithm of the sum over a row's keys of
+ * exp(q.k / sqrt(D)).  Otherwise as kvhp_q4_decode. */
+size_t kvhp_q4_prefill_workspace_bytes(int batch, int rows, int num_q_heads, int num_kv_heads,
+                                       int head_dim, int max_seq_len);
+int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* block_tables, int max_pages,
+                    int num_pages, const int32_t* q_start, const int32_t* seq_lens, void* out,
+                    float* lse, int batch, int rows, int num_q_heads, int num_kv_heads,
+                    int head_dim, int max_seq_len, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 /* ---- Model operators around the KV-cache path (decoder-only model,
  * batch-1 decode).  fp16 tensors row-major; W [N][K] is the PyTorch linear
  * weight layout the reference uses (src/cuda/kernels.h:178-192). ---------- */

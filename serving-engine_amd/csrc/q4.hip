@@ -1,0 +1,231 @@
+// q4.hip -- attention over a paged cache held in 4 bits, and its rows read back: entry
+// points, and the attention kernel that takes any shape.
+//
+// Any head_dim that is a multiple of 8, any group: one wave per (query head, row), one pass
+// over its visible keys with an online softmax, fp32 throughout.  For rare shapes and no
+// more: one key per trip behind a six-step sum over the wave.
+#include "q4.h"
+
+#include <algorithm>
+
+namespace kvhp {
+namespace {
+
+// One wave per (row, query head) of a sequence.
+__global__ void __launch_bounds__(kWave) q4_rows_kernel(const Q4Args a) {
+    const int lane = threadIdx.x;
+    const int row = blockIdx.x / a.Hq, qh = blockIdx.x % a.Hq, b = blockIdx.y;
+    const int kvh = qh / a.G, D = a.D;
+    const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
+    const int n = q4_len(a, b);
+    const int64_t p = q4_first(a, b, n) + row;
+    if (p < 0 || p >= n) {
+        if (a.last_row)   // no keys
+            for (int d = lane; d < D; d += kWave) a.out[at * D + d] = f16(0);
+        return;
+    }
+    float qv[4], acc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + kWave * i;
+        qv[i] = d < D ? static_cast<float>(a.q[at * D + d]) : 0.f;
+        acc[i] = 0.f;
+    }
+    const int32_t* bt = a.bt + (int64_t)b * a.max_pages;
+    const int sh = 4 * (lane & 1);   // dims lane + 64 i: the same half of a byte
+    float m = -1e30f, l = 0.f;
+    for (int j = 0; j <= static_cast<int>(p); ++j) {
+        const uint8_t* pg = q4_page(a.pool, a.num_pages, D, kvh, bt[j >> 4]);
+        const int o = j & 15;
+        const Q4Row kp = q4_row(*reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, 0, o)));
+        const Q4Row vp = q4_row(*reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, 1, o)));
+        float dot = 0.f, v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = lane + kWave * i;
+            v[i] = 0.f;
+            if (d < D) {
+                const int kn = pg[q4_codes_at(D, 0, o) + d / 2] >> sh & 15;
+                const int vn = pg[q4_codes_at(D, 1, o) + d / 2] >> sh & 15;
+                dot = fmaf(qv[i], static_cast<float>(kn) + kp.r, dot);
+                v[i] = vp.s * (static_cast<float>(vn) + vp.r);
+            }
+        }
+        const float s = wave_sum(dot) * kp.s * a.scale_log2;
+        const float mn = fmaxf(m, s);
+        const float al = fast_exp2(m - mn), w = fast_exp2(s - mn);
+        l = l * al + w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * al);
+        m = mn;
+    }
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + kWave * i;
+        if (d < D) a.out[at * D + d] = static_cast<f16>(acc[i] * inv);
+    }
+    if (a.lse && lane == 0)
+        a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Rows read back: one thread per 8 dims of a position, K and V.
+__global__ void __launch_bounds__(256)
+q4_gather_kernel(const uint8_t* pool, const int32_t* bt, int max_pages, int num_pages,
+                 const int32_t* start, const int32_t* seq_lens, f16* out_k, f16* out_v,
+                 int64_t items, int Hkv, int D, int max_len) {
+    const int cpr = D / 8;
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < items;
+         i += (int64_t)gridDim.x * 256) {
+        const int c = static_cast<int>(i % cpr);
+        const int64_t row = i / cpr;                 // (b Hkv + h) max_len + t
+        const int t = static_cast<int>(row % max_len);
+        const int64_t bh = row / max_len;
+        const int b = static_cast<int>(bh / Hkv), h = static_cast<int>(bh % Hkv);
+        const int64_t pos = (start ? start[b] : 0) + (int64_t)t;
+        const int n = static_cast<int>(min((int64_t)max(seq_lens[b], 0), (int64_t)max_pages * kPage));
+        const bool in = pos >= 0 && pos < n;
+        const uint8_t* pg = nullptr;
+        if (in) pg = q4_page(pool, num_pages, D, h, bt[(int64_t)b * max_pages + (pos >> 4)]);
+        const int o = static_cast<int>(pos & 15);
+#pragma unroll
+        for (int is_v = 0; is_v < 2; ++is_v) {
+            f16* out = is_v ? out_v : out_k;
+            if (!out) continue;
+            half8 y = {};
+            if (in) {
+                const Q4Row p = q4_row(*reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, is_v, o)));
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(pg + q4_codes_at(D, is_v, o) + 4 * c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    y[e] = static_cast<f16>(p.s * (static_cast<float>(x >> 4 * e & 15) + p.r));
+            }
+            store_half8(out + i * 8, y);
+        }
+    }
+}
+
+// Shapes, pool and tables that every attention call checks; fills what they give.
+int q4_shapes(Q4Args& a, const char* what, const void* pool, const int32_t* bt, int max_pages,
+              int num_pages, int batch, int hq, int hkv, int d, int max_seq_len) {
+    KVHP_REQUIRE(pool && bt, KVHP_ERR_INVALID, "%s: null pool or block tables", what);
+    KVHP_REQUIRE(aligned16(pool), KVHP_ERR_INVALID, "%s: pool not 16-byte aligned", what);
+    KVHP_REQUIRE(max_pages > 0 && num_pages > 0, KVHP_ERR_INVALID,
+                 "%s: max_pages=%d and num_pages=%d must be positive", what, max_pages, num_pages);
+    KVHP_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, KVHP_ERR_INVALID,
+                 "%s: num_q_heads=%d must be a positive multiple of num_kv_heads=%d", what, hq,
+                 hkv);
+    KVHP_REQUIRE(d > 0 && d <= 256 && d % 8 == 0, KVHP_ERR_UNSUPPORTED,
+                 "%s: head_dim=%d is no multiple of 8 up to 256", what, d);
+    KVHP_REQUIRE(batch <= kMaxBatch && hkv <= kMaxKvHeads, KVHP_ERR_UNSUPPORTED,
+                 "%s: more than 65535 sequences or KV heads", what);
+    KVHP_REQUIRE(hq <= kMaxHeads, KVHP_ERR_UNSUPPORTED, "%s: num_q_heads=%d above 2^25", what, hq);
+    KVHP_REQUIRE(max_seq_len <= kMaxLen, KVHP_ERR_UNSUPPORTED, "%s: max_seq_len=%d above 2^30",
+                 what, max_seq_len);
+    a.pool = static_cast<const uint8_t*>(pool);
+    a.bt = bt;
+    a.max_pages = max_pages;
+    a.num_pages = num_pages;
+    a.Hq = hq;
+    a.Hkv = hkv;
+    a.G = hq / hkv;
+    a.D = d;
+    a.max_len = max_seq_len;
+    a.cap = static_cast<int>(std::min<int64_t>(max_seq_len, (int64_t)max_pages * kPage));
+    a.scale_log2 = kLog2e / std::sqrt(static_cast<float>(d));
+    return KVHP_OK;
+}
+
+int launch_rows(const Q4Args& a, int batch, const char* what, hipStream_t s) {
+    KVHP_REQUIRE((int64_t)a.rows * a.Hq <= 1 << 25, KVHP_ERR_UNSUPPORTED,   // 2^31 threads
+                 "%s: %d rows of %d heads", what, a.rows, a.Hq);
+    hipLaunchKernelGGL(q4_rows_kernel, dim3(static_cast<unsigned>(a.rows) * a.Hq, batch),
+                       dim3(kWave), 0, s, a);
+    return check_launch(what);
+}
+
+}  // namespace
+}  // namespace kvhp
+
+using namespace kvhp;
+
+extern "C" size_t kvhp_q4_page_bytes(int head_dim) {
+    return head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0 ? q4_page_bytes(head_dim) : 0;
+}
+
+extern "C" int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int max_pages,
+                              int num_pages, const int32_t* start, const int32_t* seq_lens,
+                              void* out_k, void* out_v, int batch, int num_kv_heads, int head_dim,
+                              int max_len, void* stream) {
+    clear_error();
+    if (batch <= 0 || max_len <= 0) return KVHP_OK;
+    const char* what = "q4_gather";
+    KVHP_REQUIRE(seq_lens && (out_k || out_v), KVHP_ERR_INVALID, "%s: null pointer", what);
+    Q4Args a{};
+    int rc = q4_shapes(a, what, pool, block_tables, max_pages, num_pages, batch, num_kv_heads,
+                       num_kv_heads, head_dim, max_len);
+    if (rc) return rc;
+    KVHP_REQUIRE(aligned16(out_k) && aligned16(out_v), KVHP_ERR_INVALID,
+                 "%s: outputs not 16-byte aligned", what);
+    const int64_t items = (int64_t)batch * num_kv_heads * max_len * (head_dim / 8);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((items + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL(q4_gather_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       a.pool, block_tables, max_pages, num_pages, start, seq_lens,
+                       static_cast<f16*>(out_k), static_cast<f16*>(out_v), items, num_kv_heads,
+                       head_dim, max_len);
+    return check_launch(what);
+}
+
+extern "C" size_t kvhp_q4_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
+                                                 int head_dim, int max_seq_len) {
+    return 0;
+}
+
+extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables,
+                              int max_pages, int num_pages, const int32_t* seq_lens, void* out,
+                              int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                              int max_seq_len, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    clear_error();
+    if (batch <= 0 || max_seq_len <= 0) return KVHP_OK;
+    const char* what = "q4_decode";
+    KVHP_REQUIRE(q && out && seq_lens, KVHP_ERR_INVALID, "%s: null pointer", what);
+    Q4Args a{};
+    int rc = q4_shapes(a, what, pool, block_tables, max_pages, num_pages, batch, num_q_heads,
+                       num_kv_heads, head_dim, max_seq_len);
+    if (rc) return rc;
+    a.q = static_cast<const f16*>(q);
+    a.out = static_cast<f16*>(out);
+    a.seq_lens = seq_lens;
+    a.rows = 1;
+    a.last_row = 1;
+    return launch_rows(a, batch, what, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t kvhp_q4_prefill_workspace_bytes(int batch, int rows, int num_q_heads,
+                                                  int num_kv_heads, int head_dim,
+                                                  int max_seq_len) {
+    return 0;
+}
+
+extern "C" int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* block_tables,
+                               int max_pages, int num_pages, const int32_t* q_start,
+                               const int32_t* seq_lens, void* out, float* lse, int batch, int rows,
+                               int num_q_heads, int num_kv_heads, int head_dim, int max_seq_len,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    if (batch <= 0 || rows <= 0 || max_seq_len <= 0) return KVHP_OK;
+    const char* what = "q4_prefill";
+    KVHP_REQUIRE(q && out, KVHP_ERR_INVALID, "%s: null pointer", what);
+    Q4Args a{};
+    int rc = q4_shapes(a, what, pool, block_tables, max_pages, num_pages, batch, num_q_heads,
+                       num_kv_heads, head_dim, max_seq_len);
+    if (rc) return rc;
+    a.q = static_cast<const f16*>(q);
+    a.out = static_cast<f16*>(out);
+    a.lse = lse;
+    a.q_start = q_start;
+    a.seq_lens = seq_lens;
+    a.rows = rows;
+    return launch_rows(a, batch, what, static_cast<hipStream_t>(stream));
+}

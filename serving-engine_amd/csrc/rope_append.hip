@@ -1,0 +1,250 @@
+// rope_append.hip -- rows of q, k and v as the projections leave them: q and k rotated to
+// their place in the text, K and V written into the cache's pages, fp16 or 4 bits.
+//
+// The rotation's angle is counted in turns in 64 bits, p theta^(-2i/D) / 2 pi, and its sine
+// and cosine are rounded to fp32 once, so that far positions lose nothing: in fp32 the angle
+// itself is off by up to 2^-11 at position 2^13 and 2^-10 at 2^14, more than fp16 rounds.
+// One wave per (token, head), a lane per pair of dims.
+#include "q4.h"
+
+#include <algorithm>
+
+namespace kvhp {
+namespace {
+
+struct AppendArgs {
+    const f16 *q, *k, *v;
+    int64_t sq, sk, sv;       // between tokens
+    const int32_t* positions; // NULL: 0
+    const int32_t* slots;     // NULL: the positions
+    const int32_t* seq_lens;  // NULL: no limit
+    f16* q_out;
+    f16 *pool_k, *pool_v;     // fp16 pages, or
+    uint8_t* pool;            // 4-bit pages
+    const int32_t* bt;
+    int max_pages, num_pages;
+    int batch, rows, Hq, Hkv, D;   // Hq 0: no q
+    double log2_theta;        // theta > 0
+    int rotate;
+};
+
+// cos and sin of position p times theta^(-2i/D), each rounded once to fp32.  The turns are
+// reduced to an eighth in 64 bits; there the Taylor series to x^13 and x^14 leave 2^-46.
+__device__ __forceinline__ float2 rotation(int64_t p, int i, int D, double log2_theta) {
+    const double freq = exp2(-log2_theta * (2 * i) / D);
+    double t = static_cast<double>(p) * (freq * 0.15915494309189533577);   // 1 / 2 pi
+    t -= rint(t);
+    const double k = rint(4 * t);
+    const double x = (t - 0.25 * k) * 6.283185307179586477;
+    const double y = x * x;
+    double s = 1.0 / 6227020800, c = -1.0 / 87178291200;
+    s = fma(s, y, -1.0 / 39916800);
+    c = fma(c, y, 1.0 / 479001600);
+    s = fma(s, y, 1.0 / 362880);
+    c = fma(c, y, -1.0 / 3628800);
+    s = fma(s, y, -1.0 / 5040);
+    c = fma(c, y, 1.0 / 40320);
+    s = fma(s, y, 1.0 / 120);
+    c = fma(c, y, -1.0 / 720);
+    s = fma(s, y, -1.0 / 6);
+    c = fma(c, y, 1.0 / 24);
+    s = fma(s * y, x, x);
+    c = fma(c, y, -0.5);
+    c = fma(c, y, 1.0);
+    const int quarter = static_cast<int>(k) & 3;   // k in -2 .. 2
+    const float fs = static_cast<float>(quarter & 1 ? c : s);
+    const float fc = static_cast<float>(quarter & 1 ? s : c);
+    return float2{quarter == 1 || quarter == 2 ? -fc : fc, quarter >= 2 ? -fs : fs};
+}
+
+// The rotation's two products and their sum are rounded to fp32 one after the other (no fused
+// multiply-add, whose choice would be the compiler's, kernel by kernel), the result once to fp16.
+__device__ __forceinline__ void rotate(float a, float b, float2 cs, f16& x, f16& y) {
+#pragma clang fp contract(off)
+    const float ac = a * cs.x, bs = b * cs.y, bc = b * cs.x, as = a * cs.y;
+    const float u = ac - bs, v = bc + as;
+    x = static_cast<f16>(u);
+    y = static_cast<f16>(v);
+}
+
+// One wave per (token, head).
+template <bool Q4>
+__global__ void __launch_bounds__(kWave) append_row_kernel(const AppendArgs a) {
+    const int lane = threadIdx.x, D = a.D, half = D / 2;
+    const int H = a.Hq + 2 * a.Hkv;
+    const int64_t token = blockIdx.x / H;
+    const int h = blockIdx.x % H;
+    const int b = static_cast<int>(token / a.rows), row = static_cast<int>(token % a.rows);
+    const int64_t pos = (a.positions ? a.positions[b] : 0) + (int64_t)row;
+    const int64_t slot = a.slots ? a.slots[b] + (int64_t)row : pos;
+    if (slot < 0 || (a.seq_lens && slot >= a.seq_lens[b])) return;
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+    const int kvh = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
+    int pid = -1;
+    if (!is_q) {
+        if (slot >= (int64_t)a.max_pages * kPage) return;
+        pid = a.bt[(int64_t)b * a.max_pages + (slot >> 4)];
+        if (pid < 0 || pid >= a.num_pages) return;
+    }
+    const f16* src = is_q ? a.q + token * a.sq + (int64_t)h * D
+                          : (is_v ? a.v + token * a.sv : a.k + token * a.sk) + (int64_t)kvh * D;
+    f16 x[2][2] = {};   // pairs lane, lane + 64: dims i, i + half
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int i = lane + kWave * u;
+        if (i >= half) continue;
+        x[u][0] = src[i];
+        x[u][1] = src[i + half];
+        if (a.rotate && !is_v)
+            rotate(static_cast<float>(x[u][0]), static_cast<float>(x[u][1]),
+                   rotation(pos, i, D, a.log2_theta), x[u][0], x[u][1]);
+    }
+    const int o = static_cast<int>(slot & 15);
+    if (is_q || !Q4) {
+        f16* dst = is_q ? a.q_out + (token * a.Hq + h) * D
+                        : (is_v ? a.pool_v : a.pool_k) +
+                              (((int64_t)kvh * a.num_pages + pid) * kPage + o) * D;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = lane + kWave * u;
+            if (i >= half) continue;
+            dst[i] = x[u][0];
+            dst[i + half] = x[u][1];
+        }
+        return;
+    }
+    float lo = INFINITY, hi = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (lane + kWave * u < half)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float f = static_cast<float>(x[u][e]);
+                lo = fminf(lo, f);
+                hi = fmaxf(hi, f);
+                bad |= !(fabsf(f) < INFINITY);
+            }
+    lo = -wave_max(-lo);
+    hi = wave_max(hi);
+    bad = __ballot(bad) != 0;
+    Q4Quant z = q4_quant(bad ? 0.f : lo, bad ? 0.f : hi);
+    if (bad) z.bits = kQ4NanRow;
+    uint8_t* pg = a.pool + ((int64_t)kvh * a.num_pages + pid) * q4_page_bytes(D);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int i = lane + kWave * u;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t n = bad || z.flat ? 0 : q4_code(z, static_cast<float>(x[u][e]));
+            const uint32_t next = __shfl_down(n, 1);   // half is even: the pair's other dim
+            if (i < half && !(i & 1))
+                pg[q4_codes_at(D, is_v, o) + (i + e * half) / 2] = static_cast<uint8_t>(n | next << 4);
+        }
+    }
+    if (lane == 0) *reinterpret_cast<uint32_t*>(pg + q4_params_at(D, is_v, o)) = z.bits;
+}
+
+int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq, int hkv, int d,
+           float theta, hipStream_t s) {
+    KVHP_REQUIRE(a.k && a.v && a.bt && (q4 ? a.pool != nullptr : a.pool_k && a.pool_v) &&
+                     (a.q == nullptr) == (a.q_out == nullptr),
+                 KVHP_ERR_INVALID, "%s: null pointer", what);
+    KVHP_REQUIRE(a.max_pages > 0 && a.num_pages > 0, KVHP_ERR_INVALID,
+                 "%s: max_pages=%d and num_pages=%d must be positive", what, a.max_pages,
+                 a.num_pages);
+    KVHP_REQUIRE(hkv > 0 && (hq > 0 || !a.q), KVHP_ERR_INVALID,
+                 "%s: num_q_heads=%d and num_kv_heads=%d must be positive", what, hq, hkv);
+    KVHP_REQUIRE(theta >= 0.f && theta < INFINITY, KVHP_ERR_INVALID,
+                 "%s: rope_theta=%g must be 0 (no rotation) or positive", what, (double)theta);
+    if (q4)
+        KVHP_REQUIRE(d > 0 && d <= 256 && d % 8 == 0, KVHP_ERR_UNSUPPORTED,
+                     "%s: head_dim=%d is no multiple of 8 up to 256", what, d);
+    else
+        KVHP_REQUIRE(d > 0 && d <= 256 && d % 2 == 0, KVHP_ERR_UNSUPPORTED,
+                     "%s: head_dim=%d is no even number up to 256", what, d);
+    KVHP_REQUIRE(!q4 || aligned16(a.pool), KVHP_ERR_INVALID, "%s: pool not 16-byte aligned", what);
+    a.Hq = a.q ? hq : 0;
+    a.Hkv = hkv;
+    a.D = d;
+    a.batch = batch;
+    a.rows = rows;
+    KVHP_REQUIRE(hkv <= kMaxKvHeads && a.Hq <= kMaxHeads, KVHP_ERR_UNSUPPORTED,
+                 "%s: %d query heads, %d KV heads", what, a.Hq, hkv);
+    KVHP_REQUIRE((!a.q || a.sq >= (int64_t)hq * d) && a.sk >= (int64_t)hkv * d &&
+                     a.sv >= (int64_t)hkv * d,
+                 KVHP_ERR_INVALID, "%s: a token's rows overlap the next one's", what);
+    a.rotate = theta > 0.f;
+    a.log2_theta = a.rotate ? std::log2(static_cast<double>(theta)) : 0.0;
+    const int64_t waves = (int64_t)batch * rows * (a.Hq + 2 * hkv);
+    KVHP_REQUIRE((int64_t)batch * rows <= 1 << 25 && waves <= 1 << 25, KVHP_ERR_UNSUPPORTED,
+                 "%s: %d x %d rows of %d heads", what, batch, rows, a.Hq + 2 * hkv);
+    const dim3 grid(static_cast<unsigned>(waves));
+    if (q4)
+        hipLaunchKernelGGL(append_row_kernel<true>, grid, dim3(kWave), 0, s, a);
+    else
+        hipLaunchKernelGGL(append_row_kernel<false>, grid, dim3(kWave), 0, s, a);
+    return check_launch(what);
+}
+
+}  // namespace
+}  // namespace kvhp
+
+using namespace kvhp;
+
+extern "C" int kvhp_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
+                                int64_t k_stride, int64_t v_stride, const int32_t* positions,
+                                const int32_t* slots, const int32_t* seq_lens, float rope_theta,
+                                void* q_out, void* pool_k, void* pool_v,
+                                const int32_t* block_tables, int max_pages, int num_pages,
+                                int batch, int rows, int num_q_heads, int num_kv_heads,
+                                int head_dim, void* stream) {
+    clear_error();
+    if (batch <= 0 || rows <= 0) return KVHP_OK;
+    AppendArgs a{};
+    a.q = static_cast<const f16*>(q);
+    a.k = static_cast<const f16*>(k);
+    a.v = static_cast<const f16*>(v);
+    a.sq = q_stride;
+    a.sk = k_stride;
+    a.sv = v_stride;
+    a.positions = positions;
+    a.slots = slots;
+    a.seq_lens = seq_lens;
+    a.q_out = static_cast<f16*>(q_out);
+    a.pool_k = static_cast<f16*>(pool_k);
+    a.pool_v = static_cast<f16*>(pool_v);
+    a.bt = block_tables;
+    a.max_pages = max_pages;
+    a.num_pages = num_pages;
+    return append(a, "rope_append", false, batch, rows, num_q_heads, num_kv_heads, head_dim,
+                  rope_theta, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int kvhp_q4_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
+                                   int64_t k_stride, int64_t v_stride, const int32_t* positions,
+                                   const int32_t* slots, const int32_t* seq_lens,
+                                   float rope_theta, void* q_out, void* pool,
+                                   const int32_t* block_tables, int max_pages, int num_pages,
+                                   int batch, int rows, int num_q_heads, int num_kv_heads,
+                                   int head_dim, void* stream) {
+    clear_error();
+    if (batch <= 0 || rows <= 0) return KVHP_OK;
+    AppendArgs a{};
+    a.q = static_cast<const f16*>(q);
+    a.k = static_cast<const f16*>(k);
+    a.v = static_cast<const f16*>(v);
+    a.sq = q_stride;
+    a.sk = k_stride;
+    a.sv = v_stride;
+    a.positions = positions;
+    a.slots = slots;
+    a.seq_lens = seq_lens;
+    a.q_out = static_cast<f16*>(q_out);
+    a.pool = static_cast<uint8_t*>(pool);
+    a.bt = block_tables;
+    a.max_pages = max_pages;
+    a.num_pages = num_pages;
+    return append(a, "q4_rope_append", true, batch, rows, num_q_heads, num_kv_heads, head_dim,
+                  rope_theta, static_cast<hipStream_t>(stream));
+}

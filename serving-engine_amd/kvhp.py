@@ -108,6 +108,20 @@ _SIGNATURES = {
                                _i32, _i32, _i32, _i32, _i32, _vp]),
     "kvhp_evict_apply": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
                                 _i32, _vp]),
+    # appends that rotate, caches in 4 bits
+    "kvhp_rope_append": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _f32, _vp, _vp,
+                                _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "kvhp_q4_page_bytes": (_sz, [_i32]),
+    "kvhp_q4_rope_append": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _f32, _vp, _vp,
+                                   _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "kvhp_q4_gather": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
+                              _vp]),
+    "kvhp_q4_decode_workspace_bytes": (_sz, [_i32] * 5),
+    "kvhp_q4_decode": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+                              _vp, _sz, _vp]),
+    "kvhp_q4_prefill_workspace_bytes": (_sz, [_i32] * 6),
+    "kvhp_q4_prefill": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                               _i32, _i32, _i32, _vp, _sz, _vp]),
     # model operators
     "kvhp_gemv": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
     "kvhp_gemv_residual": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _vp]),
@@ -511,6 +525,101 @@ def evict_apply(pool_k, pool_v, weights, ages, block_tables, moves, counts, stre
         _ptr(pool_k), _ptr(pool_v), _ptr(weights), _ptr(ages), _ptr(block_tables),
         block_tables.shape[1], _ptr(moves), _ptr(counts), counts.shape[0], hkv, d, pages,
         moves.shape[2], _stream(stream)))
+
+
+# ------------------------- appends that rotate, caches held in 4 bits --
+def _token_rows(t, what):
+    """(batch, rows, stride) of q, k or v [B][rows][H][D]: consecutive tokens stride
+    halfs apart, the heads of a token in a row."""
+    B, R, H, D = t.shape
+    sb, sr, sh, sd = t.stride()
+    step = sr if R > 1 else sb if B > 1 else H * D   # a dimension of one has no stride
+    if (D > 1 and sd != 1) or (H > 1 and sh != D) or (R > 1 and B > 1 and sb != R * sr):
+        raise KVHPError(KVHP_ERR_INVALID,
+                        f"{what}: tokens of rows [H][D] at one stride wanted, got strides "
+                        f"{tuple(t.stride())} of shape {tuple(t.shape)}")
+    return B, R, step
+
+
+def _append_rows(q, k, v, q_out, what):
+    B, R, sk = _token_rows(k, what)
+    sv = _token_rows(v, what)[2]
+    sq = 0 if q is None else _token_rows(q, what)[2]
+    if any(t is not None and tuple(t.shape[:2]) != (B, R) for t in (q, v, q_out)):
+        raise KVHPError(KVHP_ERR_INVALID, f"{what}: q, k, v and q_out of different rows")
+    if q_out is not None and not q_out.is_contiguous():
+        raise KVHPError(KVHP_ERR_INVALID, f"{what}: q_out must be contiguous")
+    return B, R, sq, sk, sv
+
+
+def rope_append(q, k, v, positions, q_out, pool_k, pool_v, block_tables, num_q_heads,
+                num_kv_heads, head_dim, theta, slots=None, seq_lens=None, stream=None):
+    """Rotates rows q [B][rows][Hq][D] (to q_out) and k [B][rows][Hkv][D] to text
+    positions positions[b] + r and writes K and V to slots slots[b] + r of the pools
+    [Hkv][P][16][D].  q, k, v may be parts of one fused projection; theta 0: no rotation."""
+    B, R, sq, sk, sv = _append_rows(q, k, v, q_out, "rope_append")
+    _check(load().kvhp_rope_append(
+        _ptr(q), _ptr(k), _ptr(v), sq, sk, sv, _ptr(positions), _ptr(slots), _ptr(seq_lens),
+        theta, _ptr(q_out), _ptr(pool_k), _ptr(pool_v), _ptr(block_tables),
+        block_tables.shape[1], pool_k.shape[1], B, R, num_q_heads, num_kv_heads, head_dim,
+        _stream(stream)))
+
+
+def q4_page_bytes(head_dim) -> int:
+    """Bytes of a 4-bit page (16 tokens' K and V of one KV head)."""
+    return load().kvhp_q4_page_bytes(head_dim)
+
+
+def q4_rope_append(q, k, v, positions, q_out, pool, block_tables, num_q_heads, num_kv_heads,
+                   head_dim, theta, slots=None, seq_lens=None, stream=None):
+    """rope_append into a 4-bit pool, uint8 [Hkv][P][q4_page_bytes(D)]."""
+    B, R, sq, sk, sv = _append_rows(q, k, v, q_out, "q4_rope_append")
+    _check(load().kvhp_q4_rope_append(
+        _ptr(q), _ptr(k), _ptr(v), sq, sk, sv, _ptr(positions), _ptr(slots), _ptr(seq_lens),
+        theta, _ptr(q_out), _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1],
+        B, R, num_q_heads, num_kv_heads, head_dim, _stream(stream)))
+
+
+def q4_gather(pool, block_tables, seq_lens, out_k, out_v, start=None, stream=None):
+    """Positions start[b] + t of a 4-bit pool as fp16 [B][Hkv][max_len][D] (either output
+    may be None), zeros from seq_lens[b] on."""
+    B, hkv, n, d = (out_k if out_k is not None else out_v).shape
+    _check(load().kvhp_q4_gather(
+        _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1], _ptr(start),
+        _ptr(seq_lens), _ptr(out_k), _ptr(out_v), B, hkv, d, n, _stream(stream)))
+
+
+def q4_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len) -> int:
+    return load().kvhp_q4_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim,
+                                                 max_seq_len)
+
+
+def q4_decode(q, pool, block_tables, seq_lens, out, num_q_heads, num_kv_heads, head_dim,
+              max_seq_len, workspace=None, stream=None):
+    """decode_attention over a 4-bit pool; workspace: a tensor of
+    q4_decode_workspace_bytes bytes."""
+    _check(load().kvhp_q4_decode(
+        _ptr(q), _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1],
+        _ptr(seq_lens), _ptr(out), seq_lens.shape[0], num_q_heads, num_kv_heads, head_dim,
+        max_seq_len, _ptr(workspace), _bytes(workspace), _stream(stream)))
+
+
+def q4_prefill_workspace_bytes(batch, rows, num_q_heads, num_kv_heads, head_dim,
+                               max_seq_len) -> int:
+    return load().kvhp_q4_prefill_workspace_bytes(batch, rows, num_q_heads, num_kv_heads,
+                                                  head_dim, max_seq_len)
+
+
+def q4_prefill(q, pool, block_tables, out, num_q_heads, num_kv_heads, head_dim, max_seq_len,
+               q_start=None, seq_lens=None, lse=None, workspace=None, stream=None):
+    """Rows q [B][rows][Hq][D] at positions q_start[b] + r, each over the keys of the 4-bit
+    pool up to itself; out as q, lse fp32 [B][Hq][rows] (optional); padding rows are left
+    as they were."""
+    _check(load().kvhp_q4_prefill(
+        _ptr(q), _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1],
+        _ptr(q_start), _ptr(seq_lens), _ptr(out), _ptr(lse), q.shape[0], q.shape[1], num_q_heads,
+        num_kv_heads, head_dim, max_seq_len, _ptr(workspace), _bytes(workspace),
+        _stream(stream)))
 
 
 # ------------------------------------------------------ model operators --
