@@ -110,4 +110,9 @@ __device__ __forceinline__ const uint8_t* q4_page(const uint8_t* pool, int num_p
     return pool + ((int64_t)kvh * num_pages + min(max(pid, 0), num_pages - 1)) * q4_page_bytes(d);
 }
 
+// q4_decode.hip: one token per sequence at D = 64 and 128.
+size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len);
+bool q4_decode_fits(const Q4Args& a, int batch);
+int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s);
+
 }  // namespace kvhp

@@ -136,6 +136,14 @@ int q4_shapes(Q4Args& a, const char* what, const void* pool, const int32_t* bt, 
     return KVHP_OK;
 }
 
+int workspace_check(const char* what, const void* ws, size_t bytes, size_t need) {
+    if (need == 0) return KVHP_OK;
+    KVHP_REQUIRE(ws && bytes >= need, KVHP_ERR_WORKSPACE,
+                 "%s: workspace of %zu bytes, %zu needed", what, ws ? bytes : 0, need);
+    KVHP_REQUIRE(aligned16(ws), KVHP_ERR_INVALID, "%s: workspace not 16-byte aligned", what);
+    return KVHP_OK;
+}
+
 int launch_rows(const Q4Args& a, int batch, const char* what, hipStream_t s) {
     KVHP_REQUIRE((int64_t)a.rows * a.Hq <= 1 << 25, KVHP_ERR_UNSUPPORTED,   // 2^31 threads
                  "%s: %d rows of %d heads", what, a.rows, a.Hq);
@@ -178,7 +186,7 @@ extern "C" int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int
 
 extern "C" size_t kvhp_q4_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
                                                  int head_dim, int max_seq_len) {
-    return 0;
+    return q4_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len);
 }
 
 extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables,
@@ -199,6 +207,11 @@ extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* bl
     a.seq_lens = seq_lens;
     a.rows = 1;
     a.last_row = 1;
+    rc = workspace_check(what, workspace, workspace_bytes,
+                         q4_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len));
+    if (rc) return rc;
+    if (q4_decode_fits(a, batch))
+        return q4_decode(a, batch, workspace, static_cast<hipStream_t>(stream));
     return launch_rows(a, batch, what, static_cast<hipStream_t>(stream));
 }
 
