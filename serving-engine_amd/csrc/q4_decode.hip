@@ -18,27 +18,82 @@
 #include "q4.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace kvhp {
 namespace {
 
 constexpr int kTok = 64;          // keys per tile: one page per 16 lanes
-constexpr int kMaxChunk = 1024;   // keys per split: 64 page ids, one per lane
+constexpr int kMaxTiles = 16;     // per wave and split: 64 page ids, one per lane
 constexpr int kHeads = 16;        // query heads per workgroup
 constexpr float kBias = 10.f;
 
 struct DecodePlan {
     int chunk;        // keys per split, a multiple of kTok
-    int nsplit;
+    int nsplit;       // split slots in the workspace
+    int batch;
+    int balance;      // > 0: about this many splits per KV head over the batch
     int groups;       // workgroups per KV head and split, of up to kHeads query heads
     float* ws_o;      // [B * Hq][nsplit][D]
     float* ws_ml;     // [B * Hq][nsplit][2], the maximum in log2 units
 };
 
-// global_load_lds_dwordx4 from an address per lane.
-__device__ __forceinline__ void dma16(const void* src, const void* lds_base) {
+__device__ __forceinline__ int tiles_of(int L) { return (L + kTok - 1) / kTok; }
+// Tiles of the whole batch (at most 2^30: the splits are as long as they may be far below).
+__device__ __forceinline__ uint32_t batch_tiles(const Q4Args& a, int batch, int lane) {
+    uint32_t t = 0;
+    for (int i = lane; i < batch; i += kWave) t = min(t + tiles_of(q4_len(a, i)), 1u << 24);
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) t += __shfl_xor(t, o);
+    return t;
+}
+// Keys per split of a sequence of L keys; split and join agree on it.
+__device__ __forceinline__ int chunk_of(const DecodePlan& p, int L, uint32_t tiles) {
+    if (p.balance <= 0 || L <= 0) return p.chunk;
+    const uint32_t target = min((tiles + p.balance - 1) / p.balance, (uint32_t)kMaxTiles);
+    const uint32_t t = tiles_of(L), n = min((t + target - 1) / target, (uint32_t)p.nsplit);
+    return static_cast<int>((t + n - 1) / n * kTok);   // at most kMaxTiles tiles: nsplit of them hold the longest
+}
+// The i-th split of the batch, counted in sequence order (sequences without keys keep one,
+// which writes their zeros).
+__device__ __forceinline__ bool share_of(const Q4Args& a, const DecodePlan& p, int i, int lane, int& b,
+                                         int& split, int& L, int& chunk) {
+    const uint32_t tiles = batch_tiles(a, p.batch, lane);
+    int base = 0;
+    for (int g0 = 0; g0 < p.batch; g0 += kWave) {
+        const bool in = g0 + lane < p.batch;
+        const int li = in ? q4_len(a, g0 + lane) : 0;
+        const int ci = chunk_of(p, li, tiles);
+        const int ni = in ? (li > 0 ? (li + ci - 1) / ci : 1) : 0;
+        int inc = ni;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int t = __shfl_up(inc, o);
+            if (lane >= o) inc += t;
+        }
+        const int tot = __shfl(inc, kWave - 1);
+        if (i < base + tot) {
+            const int owner = __builtin_ctzll(__ballot(base + inc > i));
+            b = __builtin_amdgcn_readfirstlane(g0 + owner);
+            split = __builtin_amdgcn_readfirstlane(i - base - (__shfl(inc, owner) - __shfl(ni, owner)));
+            L = __builtin_amdgcn_readfirstlane(__shfl(li, owner));
+            chunk = __builtin_amdgcn_readfirstlane(__shfl(ci, owner));
+            return true;
+        }
+        base += tot;
+    }
+    return false;
+}
+
+// global_load_lds_dwordx4 to LDS offset `to`, from a wave-uniform base and the lane's offset,
+// or from an address per lane.
+__device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(to), "v"(voff), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma16(const void* src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(lds_at(lds_base)), "v"(src) : "memory", "m0");
+                 :: "s"(to), "v"(src) : "memory", "m0");
 }
 
 // A stage of a wave.  Operand reads touch a page's rows in all four pages at once, so the
@@ -55,35 +110,48 @@ struct Stage {
     __device__ __forceinline__ static int vswz(int t) { return D == 128 ? t >> 2 : t >> 3; }
 };
 
-// Eight codes as n + r times a power of two: E (16 + n) + F in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ half2v code_pair(uint32_t x) {
-    return __builtin_bit_cast(half2v, (x & 0x03c003c0u) | 0x4c004c00u);
-}
+// Eight codes of K as 2^-9 (n + r), in the order 0 4 1 5 2 6 3 7: four bits at the bottom of a
+// half are the denormal n 2^-24 (at bits 4..7 n 2^-20), a multiply-add away from it, exact;
+// f = 2^-9 r.
+__device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
 __device__ __forceinline__ half8 cat4(half2v a, half2v b, half2v c, half2v d) {
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 __device__ __forceinline__ half8 k_operand(uint32_t x, half2v f) {
-    return cat4(code_pair(x << 6) + f, code_pair(x << 2) + f, code_pair(x >> 2) + f, code_pair(x >> 6) + f);
+    const half2v lo = {f16(32768), f16(32768)}, hi = {f16(2048), f16(2048)};
+    const uint32_t y = x >> 8;
+    return cat4(__builtin_elementwise_fma(as_half2(x & 0x000f000fu), lo, f),
+                __builtin_elementwise_fma(as_half2(x & 0x00f000f0u), hi, f),
+                __builtin_elementwise_fma(as_half2(y & 0x000f000fu), lo, f),
+                __builtin_elementwise_fma(as_half2(y & 0x00f000f0u), hi, f));
 }
-__device__ __forceinline__ half8 v_operand(uint32_t x, const half2v (&e)[4], const half2v (&f)[4]) {
-    return cat4(__builtin_elementwise_fma(code_pair(x << 6), e[0], f[0]),
-                __builtin_elementwise_fma(code_pair(x << 2), e[1], f[1]),
-                __builtin_elementwise_fma(code_pair(x >> 2), e[2], f[2]),
-                __builtin_elementwise_fma(code_pair(x >> 6), e[3], f[3]));
-}
-// Scales of two rows as m E: E a power of two of at least 2^-14, m of 4 to 8 above that.
-struct Scales {
-    half2v e, f, m;
+// Eight codes of V, of eight rows, as (n + r) E: four bits in mantissa bits 6..9 below the
+// exponent of 16 are 16 + n; times E and + (r - 16) E, exact again.  (The denormals' way would
+// want E 2^24, past fp16.)
+struct CodeBits {
+    uint32_t mask = 0x03c003c0u, sixteen = 0x4c004c00u;
+    // in registers: as literals they would keep v_and_or_b32 from taking both
+    __device__ __forceinline__ CodeBits() { asm("" : "+s"(mask), "+v"(sixteen)); }
 };
-__device__ __forceinline__ Scales scales(uint32_t a, uint32_t b) {
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    const uint32_t s = __builtin_amdgcn_perm(b, a, 0x05040100u), r = __builtin_amdgcn_perm(b, a, 0x07060302u);
-    u16x2 e = __builtin_bit_cast(u16x2, s & 0x7c007c00u);
-    e = __builtin_elementwise_max(__builtin_elementwise_sub_sat(e, u16x2{0x0800, 0x0800}), u16x2{0x0400, 0x0400});
-    Scales x;
-    x.e = __builtin_bit_cast(half2v, e);
-    x.m = __builtin_bit_cast(half2v, s) * __builtin_bit_cast(half2v, u16x2{0x7800, 0x7800} - e);   // by 1 / E
-    x.f = (__builtin_bit_cast(half2v, r) + half2v{f16(-16), f16(-16)}) * x.e;
+__device__ __forceinline__ half8 v_operand(uint32_t x, const u32x4& e, const u32x4& f, const CodeBits& c) {
+    auto pair = [&](uint32_t y, int i) {
+        return __builtin_elementwise_fma(as_half2((y & c.mask) | c.sixteen), as_half2(e[i]), as_half2(f[i]));
+    };
+    return cat4(pair(x << 6, 0), pair(x << 2, 1), pair(x >> 2, 2), pair(x >> 6, 3));
+}
+// A row's scale as m E: E a power of two of at least 2^-14, m of 4 to 8 (less where s is below
+// 2^-12), and f = (r - 16) E.
+struct Scale {
+    f16 e, f;
+    float m;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t sr) {
+    const int e = max((int)(sr & 0x7c00u) - 0x0800, 0x0400);
+    const half2v h = as_half2(sr);
+    Scale x;
+    x.e = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
+    x.m = static_cast<float>(h[0]) * static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
+    x.f = (h[1] - f16(16)) * x.e;
     return x;
 }
 typedef int v2i __attribute__((ext_vector_type(2)));
@@ -94,19 +162,34 @@ __device__ __forceinline__ v2i lds_read_tr4(const uint8_t* p) {
     return __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(__attribute__((address_space(3))) uint8_t*)p);
 }
 
+// What the lanes of a tile's keys leave for the others: lane group g reads page g's.
+struct __attribute__((aligned(16))) Prepared {
+    float2 sm[kTok];      // K's s and V's m
+    f16 e[kTok], f[kTok]; // V's E and (r - 16) E, in the order of the codes' pairs
+};
+
+// W waves per workgroup take the tiles of one split round robin and meet in LDS.
 template <int D, int W>
 __global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     using St = Stage<D>;
     constexpr int NS = D / 32, ND = D / 16, PB = q4_page_bytes(D), RB = St::RB;
     __shared__ __attribute__((aligned(16))) uint8_t ring[W][2][St::BYTES];
+    __shared__ Prepared prep_all[W];
 
     const int lane = threadIdx.x & (kWave - 1);
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wv = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     const int g = lane >> 4, col = lane & 15;
     const int kvh = blockIdx.x / p.groups, h0 = blockIdx.x % p.groups * kHeads;
-    const int split = blockIdx.y, b = blockIdx.z;
-    const int L = q4_len(a, b);
+    int b, split, L, chunk;
+    if (W == 1 && p.balance > 0) {
+        if (!share_of(a, p, blockIdx.y, lane, b, split, L, chunk)) return;
+    } else {
+        split = blockIdx.y;
+        b = blockIdx.z;
+        L = q4_len(a, b);
+        chunk = p.chunk;
+    }
     const int nh = min(a.G - h0, kHeads);
     const int64_t row0 = (int64_t)b * a.Hq + (int64_t)kvh * a.G + h0;
     if (L <= 0) {
@@ -115,16 +198,18 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
                 store_half8(a.out + row0 * D + 8 * i, half8{});
         return;
     }
-    const int nsb = (L + p.chunk - 1) / p.chunk;
+    const int nsb = (L + chunk - 1) / chunk;
     if (split >= nsb) return;
-    const int t_begin = split * p.chunk, t_end = min(L, t_begin + p.chunk);
+    const int t_begin = split * chunk, t_end = min(L, t_begin + chunk);
     const int n_iter = (t_end - t_begin + kTok - 1) / kTok;
+    const int n_w = n_iter > wv ? (n_iter - wv + W - 1) / W : 0;   // this wave's tiles
     const bool hvalid = col < nh;
 
+    // Page ids of this wave's tiles, four to a tile; past the split's last key: its page.
     const uint8_t* head = a.pool + (int64_t)kvh * a.num_pages * PB;
-    const int last = (t_end - 1 - t_begin) >> 4;   // page of the split's last key
-    const int pidv = min(max(a.bt[(int64_t)b * a.max_pages + (t_begin >> 4) + min(lane, last)], 0),
-                         a.num_pages - 1);
+    const int last = (t_end - 1) >> 4;
+    const int pi = min((t_begin >> 4) + 4 * (wv + W * (lane >> 2)) + (lane & 3), last);
+    const int pidv = min(max(a.bt[(int64_t)b * a.max_pages + pi], 0), a.num_pages - 1);
     half8 qb[NS];   // lane (g, col): head col, dims (D/4) g + 8 s .., in the codes' order
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -141,16 +226,16 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         const int t = (lane & 31) >> 1;
         ko = lane < 32 ? 16 * lane : 512 + 32 * t + 16 * ((lane & 1) ^ St::vswz(t));
     }
-    auto issue = [&](int it, uint8_t* st) {
-        const int pg = 4 * it;
+    const uint32_t ring0 = lds_at(ring[wv][0]);
+    auto issue = [&](int j) {   // this wave's j-th tile
+        const uint32_t st = ring0 + (j & 1) * St::BYTES;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int pid = __builtin_amdgcn_readlane(pidv, min(pg + i, last));
-            const uint8_t* src = head + (int64_t)pid * PB;
-            dma16s(src, ko, st + St::kpage(i));
-            if constexpr (D == 128) dma16s(src, vo, st + St::vpage(i));
+            const uint8_t* src = head + (int64_t)__builtin_amdgcn_readlane(pidv, 4 * j + i) * PB;
+            dma16(src, ko, st + St::kpage(i));
+            if constexpr (D == 128) dma16(src, vo, st + St::vpage(i));
         }
-        const int pid = __shfl(pidv, min(pg + (lane >> 3 & 3), last));
+        const int pid = __shfl(pidv, 4 * j + (lane >> 3 & 3));
         if (lane < 32) dma16(head + (int64_t)pid * PB + kPage * D + 16 * (lane & 7), st + St::PAR);
     };
 
@@ -158,10 +243,24 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     floatx4 o[ND];   // lane (g, col): dims 16 db + 4 g + e of head col
 #pragma unroll
     for (int db = 0; db < ND; ++db) o[db] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const float sc = a.scale_log2;
+    const float sc = a.scale_log2 * 512.f;   // K's operands are 2^-9 (n + r)
+    Prepared& prep = prep_all[wv];
+    const int at = 16 * g + 8 * (col >> 3) + 2 * (col & 3) + (col >> 2 & 1);
 
-    auto step = [&](int it, const uint8_t* st) {
+    const CodeBits bits;
+    // LAST: only a wave's last tile may reach past the split's last key
+    auto step = [&](auto LAST_, int it, const uint8_t* st) {
+        constexpr bool LAST = decltype(LAST_)::value;
         const int T0 = t_begin + kTok * it;
+        {   // this lane's key, for all
+            const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 4 * col);
+            uint32_t vp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 64 + 4 * col);
+            if (LAST && T0 + lane >= t_end) vp = 0;   // nothing of a row behind the last key
+            const Scale z = scale_of(vp);
+            prep.sm[lane] = float2{q4_row(kp).s, z.m};
+            prep.e[at] = z.e;
+            prep.f[at] = z.f;
+        }
         // scores: tile i's row m is page m / 4, key 4 i + m % 4
         const uint8_t* kr = st + St::kpage(0) + (col >> 2) * 1024 +
                             (D == 128 ? (col >> 2) * 16 : (col >> 2 & 1) * 16 + (col >> 3) * 128) +
@@ -170,7 +269,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         floatx4 C[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f16 r = __builtin_bit_cast(half2v, *reinterpret_cast<const uint32_t*>(kpar + 16 * i))[1] - f16(16);
+            const f16 r = as_half2(*reinterpret_cast<const uint32_t*>(kpar + 16 * i))[1] * f16(1.f / 512);
             const half2v f = {r, r};
             uint32_t x[NS];
             if constexpr (D == 128) {
@@ -187,25 +286,20 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             for (int s = 0; s < NS; ++s)
                 C[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_operand(x[s], f), qb[s], C[i], 0, 0, 0);
         }
-        // page g's (s, r) of K and V
-        const uint8_t* par = st + St::PAR + g * 128;
-        u32x4 vp[4];
+        const floatx4* sm = reinterpret_cast<const floatx4*>(&prep.sm[16 * g]);
+        float m[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const u32x4 kp = *reinterpret_cast<const u32x4*>(par + 16 * i);
-            vp[i] = *reinterpret_cast<const u32x4*>(par + 64 + 16 * i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) C[i][e] *= q4_row(kp[e]).s;
+        for (int t = 0; t < 16; t += 2) {
+            const floatx4 z = sm[t / 2];
+            C[t / 4][t % 4] *= z[0];
+            C[t / 4][t % 4 + 1] *= z[2];
+            m[t] = z[1];
+            m[t + 1] = z[3];
         }
-        if (T0 + kTok > t_end) {   // behind the last key: no weight, and nothing of the row
+        if constexpr (LAST) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (T0 + 16 * g + 4 * i + e >= t_end) {
-                        C[i][e] = -INFINITY;
-                        vp[i][e] = 0;
-                    }
+            for (int t = 0; t < 16; ++t)
+                if (T0 + 16 * g + t >= t_end) C[t / 4][t % 4] = -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -217,19 +311,15 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         m_run = mn;
         const float nm = hvalid ? kBias - mn * sc : -INFINITY;
         float ps = 0.f;
-        half2v e[2][4], f[2][4];
         half8 pt[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {   // keys 8 u + j and 8 u + j + 4
-                const Scales z = scales(vp[2 * u][j], vp[2 * u + 1][j]);
-                e[u][j] = z.e;
-                f[u][j] = z.f;
                 const float x = fast_exp2(fmaf(C[2 * u][j], sc, nm));
                 const float y = fast_exp2(fmaf(C[2 * u + 1][j], sc, nm));
-                pt[u][2 * j] = static_cast<f16>(x * static_cast<float>(z.m[0]));
-                pt[u][2 * j + 1] = static_cast<f16>(y * static_cast<float>(z.m[1]));
+                pt[u][2 * j] = static_cast<f16>(x * m[8 * u + j]);
+                pt[u][2 * j + 1] = static_cast<f16>(y * m[8 * u + j + 4]);
                 ps += x + y;
             }
         l_part = fmaf(l_part, alpha, ps);
@@ -239,55 +329,78 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[db][i] *= alpha;
         }
+        u32x4 e[2], f[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            e[u] = *reinterpret_cast<const u32x4*>(&prep.e[16 * g + 8 * u]);
+            f[u] = *reinterpret_cast<const u32x4*>(&prep.f[16 * g + 8 * u]);
+        }
         const uint8_t* vr = st + St::vpage(0) + (D == 128 ? g * 1024 : g * 1024 + (g & 1) * 16 + (g >> 1) * 128) +
                             col * RB;
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
             const v2i x = lds_read_tr4(vr + 16 * (db / 2 ^ St::vswz(col)) + 8 * (db & 1));
-            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[0], e[0], f[0]), pt[0], o[db], 0, 0, 0);
-            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[1], e[1], f[1]), pt[1], o[db], 0, 0, 0);
+            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[0], e[0], f[0], bits), pt[0], o[db], 0, 0, 0);
+            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[1], e[1], f[1], bits), pt[1], o[db], 0, 0, 0);
         }
     };
 
-    const int n_w = n_iter > wv ? (n_iter - wv + W - 1) / W : 0;   // this wave's tiles
     if (n_w > 0) {
         asm volatile("" ::: "memory");
         wait_ring<0>();
-        issue(wv, ring[wv][0]);
-        for (int j = 0; j < n_w; ++j) {
+        issue(0);
+        int j = 0;
+        for (; j + 1 < n_w; ++j) {
             __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): the other stage's reads have returned
-            if (j + 1 < n_w) {
-                issue(wv + W * (j + 1), ring[wv][(j + 1) & 1]);
-                wait_ring<St::LOADS>();
-            } else {
-                wait_ring<0>();
-            }
+            issue(j + 1);
+            wait_ring<St::LOADS>();
             asm volatile("" ::: "memory");
-            step(wv + W * j, ring[wv][j & 1]);
+            step(std::false_type{}, wv + W * j, ring[wv][j & 1]);
             asm volatile("" ::: "memory");
         }
+        wait_ring<0>();
+        asm volatile("" ::: "memory");
+        step(std::true_type{}, wv + W * j, ring[wv][j & 1]);
+        asm volatile("" ::: "memory");
     }
 
-    // The waves leave (O, m, l) in their rings; each joins every W-th 16 dims.
-    static_assert((ND * kWave * 4 + 2 * kWave) * 4 <= 2 * St::BYTES, "a wave's state in its ring");
-    float* xs = reinterpret_cast<float*>(ring[wv][0]);
+    // Dims 16 db + 4 g + e of head col: all of them, or every W-th 16 of the waves' sum.
+    constexpr int NB = (ND + W - 1) / W;
+    floatx4 r[NB];
+    float m = m_run, l = l_part;
+    if constexpr (W == 1) {
 #pragma unroll
-    for (int db = 0; db < ND; ++db)
-        *reinterpret_cast<floatx4*>(&xs[(db * kWave + lane) * 4]) = o[db];
-    *reinterpret_cast<float2*>(&xs[ND * kWave * 4 + 2 * lane]) = float2{m_run, l_part};
-    __syncthreads();
-    if (wv >= ND) return;
-    float2 ml[W];
-    float m = -1e30f, l = 0.f;
+        for (int db = 0; db < ND; ++db) r[db] = o[db];
+    } else {
+        // the waves leave (O, m, l) in their rings
+        static_assert((ND * kWave * 4 + 2 * kWave) * 4 <= 2 * St::BYTES, "a wave's state in its ring");
+        float* xs = reinterpret_cast<float*>(ring[wv][0]);
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        ml[w] = *reinterpret_cast<const float2*>(&reinterpret_cast<const float*>(ring[w][0])[ND * kWave * 4 + 2 * lane]);
-        m = fmaxf(m, ml[w].x);
-    }
+        for (int db = 0; db < ND; ++db)
+            *reinterpret_cast<floatx4*>(&xs[(db * kWave + lane) * 4]) = o[db];
+        *reinterpret_cast<float2*>(&xs[ND * kWave * 4 + 2 * lane]) = float2{m_run, l_part};
+        __syncthreads();
+        if (wv >= ND) return;
+        float2 ml[W];
+        l = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        ml[w].x = fast_exp2((ml[w].x - m) * sc);
-        l = fmaf(ml[w].y, ml[w].x, l);
+        for (int w = 0; w < W; ++w) {
+            ml[w] = *reinterpret_cast<const float2*>(
+                &reinterpret_cast<const float*>(ring[w][0])[ND * kWave * 4 + 2 * lane]);
+            m = fmaxf(m, ml[w].x);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) r[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float al = fast_exp2((ml[w].x - m) * sc);
+            l = fmaf(ml[w].y, al, l);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                if (W * i + wv < ND)
+                    r[i] += al * *reinterpret_cast<const floatx4*>(
+                        &reinterpret_cast<const float*>(ring[w][0])[((W * i + wv) * kWave + lane) * 4]);
+        }
     }
     l = rows4_sum(l);
     if (!hvalid) return;
@@ -298,20 +411,16 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     }
     const float inv = 1.f / l;
 #pragma unroll
-    for (int d0 = 0; d0 < ND; d0 += W) {
-        const int db = d0 + wv;
+    for (int i = 0; i < NB; ++i) {
+        const int db = W * i + wv;
         if (db >= ND) break;
-        floatx4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-            r += *reinterpret_cast<const floatx4*>(&reinterpret_cast<const float*>(ring[w][0])[(db * kWave + lane) * 4]) * ml[w].x;
         if (nsb == 1) {
             half4 h;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = static_cast<f16>(r[i] * inv);
+            for (int e = 0; e < 4; ++e) h[e] = static_cast<f16>(r[i][e] * inv);
             *reinterpret_cast<half4*>(a.out + (row0 + col) * D + 16 * db + 4 * g) = h;
         } else {
-            *reinterpret_cast<floatx4*>(p.ws_o + prow * D + 16 * db + 4 * g) = r;
+            *reinterpret_cast<floatx4*>(p.ws_o + prow * D + 16 * db + 4 * g) = r[i];
         }
     }
 }
@@ -319,21 +428,41 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
 template <int D>
 __global__ void __launch_bounds__(kJoinWaves * kWave)
 q4_join_kernel(const Q4Args a, const DecodePlan p) {
-    const int b = blockIdx.y, L = q4_len(a, b);
-    const int nsb = (L + p.chunk - 1) / p.chunk;
+    const int b = blockIdx.y, lane = threadIdx.x & (kWave - 1);
+    const int L = q4_len(a, b);
+    if (L <= 0) return;
+    const int chunk = chunk_of(p, L, p.balance > 0 ? batch_tiles(a, p.batch, lane) : 0);
+    const int nsb = (L + chunk - 1) / chunk;
     if (nsb > 1) join_head<D>(a.out, p.ws_o, p.ws_ml, p.nsplit, (int64_t)b * a.Hq + blockIdx.x, nsb);
 }
 
+constexpr int kBalanced = 16;      // sequences from which the splits are the whole batch's
+constexpr int kWaveSlots = 2048;   // one wave per split, two per SIMD of 256 CUs
+constexpr int kWaves = 4;          // per workgroup in fixed splits
+
 DecodePlan plan_of(int batch, int hkv, int G, int64_t max_len) {
     DecodePlan p{};
+    p.batch = batch;
     p.groups = (G + kHeads - 1) / kHeads;
-    const int64_t units = (int64_t)batch * hkv * p.groups;
-    int64_t s = std::max<int64_t>(1, 1024 / units);          // splits wanted
-    int64_t chunk = (max_len + s - 1) / s;
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 255) / 256 * 256, 256), kMaxChunk);
-    p.chunk = static_cast<int>(chunk);
-    p.nsplit = static_cast<int>((max_len + chunk - 1) / chunk);
+    const int64_t heads = (int64_t)hkv * p.groups, tiles = (max_len + kTok - 1) / kTok;
+    if (batch >= kBalanced) {
+        p.balance = static_cast<int>(std::max<int64_t>(1, kWaveSlots / heads - batch / 2));
+        // splits of a sequence: of the target, which is the least where it alone has keys
+        const int64_t target = std::min<int64_t>((tiles + p.balance - 1) / p.balance, kMaxTiles);
+        p.nsplit = static_cast<int>((tiles + target - 1) / target);
+        return p;
+    }
+    const int64_t want = std::max<int64_t>(1, 512 / (heads * batch));   // workgroups per head
+    const int64_t per = std::min<int64_t>(std::max<int64_t>((tiles + want - 1) / want, kWaves), kWaves * kMaxTiles);
+    p.chunk = static_cast<int>(per * kTok);
+    p.nsplit = static_cast<int>((tiles + per - 1) / per);
     return p;
+}
+// Workgroups of the first launch along its second axis.
+int64_t units_of(const DecodePlan& p, int64_t max_len) {
+    if (p.balance == 0) return p.nsplit;
+    const int64_t worst = (p.batch * ((max_len + kTok - 1) / kTok) + kMaxTiles - 1) / kMaxTiles;
+    return std::max<int64_t>(p.balance, worst) + p.batch;
 }
 
 }  // namespace
@@ -346,8 +475,8 @@ size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len) {
 
 bool q4_decode_fits(const Q4Args& a, int batch) {
     const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.max_len);
-    return (a.D == 64 || a.D == 128) && aligned16(a.q) && aligned16(a.out) && p.nsplit <= 65535 &&
-           (int64_t)a.Hkv * p.groups <= INT32_MAX;
+    return (a.D == 64 || a.D == 128) && aligned16(a.q) && aligned16(a.out) &&
+           units_of(p, a.max_len) <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
 }
 
 // The workspace holds q4_decode_workspace bytes.
@@ -355,16 +484,21 @@ int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s) {
     DecodePlan p = plan_of(batch, a.Hkv, a.G, a.max_len);
     p.ws_o = static_cast<float*>(ws);
     p.ws_ml = p.ws_o + (size_t)batch * a.Hq * p.nsplit * a.D;
-    const dim3 grid(a.Hkv * p.groups, p.nsplit, batch);
-    auto go = [&](auto kernel, auto join) {
-        hipLaunchKernelGGL(kernel, grid, dim3(4 * kWave), 0, s, a, p);
-        if (p.nsplit > 1)
-            hipLaunchKernelGGL(join, dim3(a.Hq, batch), dim3(kJoinWaves * kWave), 0, s, a, p);
+    const dim3 grid(a.Hkv * p.groups, static_cast<unsigned>(units_of(p, a.max_len)), p.balance ? 1 : batch);
+    auto go = [&](auto kernel, int waves) {
+        hipLaunchKernelGGL(kernel, grid, dim3(waves * kWave), 0, s, a, p);
     };
     if (a.D == 64)
-        go(q4_decode_kernel<64, 4>, q4_join_kernel<64>);
+        p.balance ? go(q4_decode_kernel<64, 1>, 1) : go(q4_decode_kernel<64, kWaves>, kWaves);
     else
-        go(q4_decode_kernel<128, 4>, q4_join_kernel<128>);
+        p.balance ? go(q4_decode_kernel<128, 1>, 1) : go(q4_decode_kernel<128, kWaves>, kWaves);
+    if (p.nsplit > 1) {
+        const dim3 rows(a.Hq, batch), threads(kJoinWaves * kWave);
+        if (a.D == 64)
+            hipLaunchKernelGGL(q4_join_kernel<64>, rows, threads, 0, s, a, p);
+        else
+            hipLaunchKernelGGL(q4_join_kernel<128>, rows, threads, 0, s, a, p);
+    }
     return check_launch("q4_decode");
 }
 
