@@ -3,8 +3,8 @@
 //
 // Split-K decode: a workgroup takes a range of a sequence's keys for one KV head and up to 16
 // of its query heads, its waves the range's tiles of 64 keys, four whole pages, round robin.
-// A tile's pages go to the wave's own LDS stages as they are (global_load_lds), the next
-// tile's on their way while this one is worked on; codes become operands in registers:
+// A tile's pages go to the wave's own LDS stage as they are (global_load_lds), the next tile's
+// K as soon as this one's is read and V after it; codes become operands in registers:
 //   S^T = K Q^T       v_mfma_f32_16x16x32_f16, A = n + r of K, rows of the tile so dealt out
 //                     that lane group g receives the scores of page g's 16 keys
 //   O^T += V^T W^T    A = V's codes by ds_read_b64_tr_b4: a lane gets all 16 keys' codes of a
@@ -96,17 +96,20 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t to) {
                  :: "s"(to), "v"(src) : "memory", "m0");
 }
 
-// A stage of a wave.  Operand reads touch a page's rows in all four pages at once, so the
-// pages lie apart by what keeps them on distinct banks.
+// A wave's tile in LDS.  Operand reads touch a page's rows in all four pages at once, so K's
+// pages lie apart by what keeps them on distinct banks (D = 64, where a load brings two: by
+// the chunks' order in every other page, and by pairs).
 template <int D>
 struct Stage {
     static constexpr int RB = D / 2;             // bytes of a row's codes
-    static constexpr int kpage(int p) { return D == 128 ? p * 1040 : p * 1024 + (p & 1) * 16 + (p >> 1) * 128; }
-    static constexpr int vpage(int p) { return D == 128 ? 4 * 1040 + p * 1024 : kpage(p) + 512; }
-    static constexpr int PAR = D == 128 ? 4 * 1040 + 4096 : kpage(3) + 1024;   // (s, r): [page][K, V][16]
+    static constexpr int PAGE = kPage * RB;
+    static constexpr int PPL = 1024 / PAGE;      // pages per load
+    static constexpr int kpage(int p) { return D == 128 ? p * 1040 : p * 512 + (p >> 1) * 128; }
+    static constexpr int VOFF = kpage(3) + PAGE;
+    static constexpr int PAR = VOFF + 4 * PAGE;  // (s, r): [page][K, V][16]
     static constexpr int BYTES = PAR + 512;
-    static constexpr int LOADS = D == 128 ? 9 : 5;
-    // V's 16-byte chunk c of row t lies at c ^ vswz(t): a transposing read's 16 rows on 16 banks
+    static constexpr int LOADS = 4 / PPL;        // of K's codes, or of V's
+    // 16-byte chunk c of V's row t lies at c ^ vswz(t): a transposing read's 16 rows on 16 banks
     __device__ __forceinline__ static int vswz(int t) { return D == 128 ? t >> 2 : t >> 3; }
 };
 
@@ -170,11 +173,11 @@ struct __attribute__((aligned(16))) Prepared {
 
 // W waves per workgroup take the tiles of one split round robin and meet in LDS.
 template <int D, int W>
-__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 4)))
 q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     using St = Stage<D>;
     constexpr int NS = D / 32, ND = D / 16, PB = q4_page_bytes(D), RB = St::RB;
-    __shared__ __attribute__((aligned(16))) uint8_t ring[W][2][St::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[W][St::BYTES];
     __shared__ Prepared prep_all[W];
 
     const int lane = threadIdx.x & (kWave - 1);
@@ -217,26 +220,31 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         qb[s] = __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
     }
 
-    // The lane's place in a page of codes: D = 128 1 KB of K and 1 KB of V; D = 64 both in one
-    uint32_t ko, vo = 0;
-    if constexpr (D == 128) {
-        ko = 16 * lane;
-        vo = 1024 + 64 * (lane >> 2) + 16 * ((lane & 3) ^ St::vswz(lane >> 2));
-    } else {
-        const int t = (lane & 31) >> 1;
-        ko = lane < 32 ? 16 * lane : 512 + 32 * t + 16 * ((lane & 1) ^ St::vswz(t));
-    }
-    const uint32_t ring0 = lds_at(ring[wv][0]);
-    auto issue = [&](int j) {   // this wave's j-th tile
-        const uint32_t st = ring0 + (j & 1) * St::BYTES;
+    // The lane's place in a page's codes of K and of V
+    const int lt = lane / (RB / 16) % kPage, lc = lane % (RB / 16);
+    const uint32_t ko = RB * lt + 16 * (D == 128 ? lc : lc ^ (lane >> 5));
+    const uint32_t vo = St::PAGE + RB * lt + 16 * (lc ^ St::vswz(lt));
+    uint8_t* const st = stage[wv];
+    const uint32_t st0 = lds_at(st);
+    auto issue = [&](int j, uint32_t off, uint32_t to, auto kpage) {   // one matrix of this wave's j-th tile
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint8_t* src = head + (int64_t)__builtin_amdgcn_readlane(pidv, 4 * j + i) * PB;
-            dma16(src, ko, st + St::kpage(i));
-            if constexpr (D == 128) dma16(src, vo, st + St::vpage(i));
+        for (int i = 0; i < St::LOADS; ++i) {
+            if constexpr (D == 128) {
+                const int pid = __builtin_amdgcn_readlane(pidv, 4 * j + i);
+                dma16(head + (int64_t)pid * PB, off, to + kpage(i));
+            } else {
+                const int pid = __shfl(pidv, 4 * j + 2 * i + (lane >> 5));
+                dma16(head + (int64_t)pid * PB + off, to + kpage(2 * i));
+            }
         }
+    };
+    auto issue_k = [&](int j) {   // and both matrices' (s, r)
+        issue(j, ko, st0, [](int i) { return St::kpage(i); });
         const int pid = __shfl(pidv, 4 * j + (lane >> 3 & 3));
-        if (lane < 32) dma16(head + (int64_t)pid * PB + kPage * D + 16 * (lane & 7), st + St::PAR);
+        if (lane < 32) dma16(head + (int64_t)pid * PB + kPage * D + 16 * (lane & 7), st0 + St::PAR);
+    };
+    auto issue_v = [&](int j) {
+        issue(j, vo, st0 + St::VOFF, [](int i) { return i * St::PAGE; });
     };
 
     float m_run = -1e30f, l_part = 0.f;
@@ -249,9 +257,11 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
 
     const CodeBits bits;
     // LAST: only a wave's last tile may reach past the split's last key
-    auto step = [&](auto LAST_, int it, const uint8_t* st) {
+    auto step = [&](auto LAST_, int j) {
         constexpr bool LAST = decltype(LAST_)::value;
-        const int T0 = t_begin + kTok * it;
+        const int T0 = t_begin + kTok * (wv + W * j);
+        wait_ring<St::LOADS>();   // K and the numbers have landed, V may be on its way
+        asm volatile("" ::: "memory");
         {   // this lane's key, for all
             const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 4 * col);
             uint32_t vp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 64 + 4 * col);
@@ -262,9 +272,8 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             prep.f[at] = z.f;
         }
         // scores: tile i's row m is page m / 4, key 4 i + m % 4
-        const uint8_t* kr = st + St::kpage(0) + (col >> 2) * 1024 +
-                            (D == 128 ? (col >> 2) * 16 : (col >> 2 & 1) * 16 + (col >> 3) * 128) +
-                            (col & 3) * RB + g * (RB / 4);
+        const uint8_t* kr = st + (col >> 2) * St::PAGE + (D == 128 ? (col >> 2) * 16 : (col >> 3) * 128) +
+                            (col & 3) * RB + (D == 128 ? 16 * g : 8 * g ^ (col & 4) * 4);
         const uint8_t* kpar = st + St::PAR + (col >> 2) * 128 + (col & 3) * 4;
         floatx4 C[4];
 #pragma unroll
@@ -285,6 +294,11 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
 #pragma unroll
             for (int s = 0; s < NS; ++s)
                 C[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_operand(x[s], f), qb[s], C[i], 0, 0, 0);
+        }
+        if constexpr (!LAST) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): all of it has been read
+            issue_k(j + 1);
         }
         const floatx4* sm = reinterpret_cast<const floatx4*>(&prep.sm[16 * g]);
         float m[16];
@@ -335,32 +349,32 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             e[u] = *reinterpret_cast<const u32x4*>(&prep.e[16 * g + 8 * u]);
             f[u] = *reinterpret_cast<const u32x4*>(&prep.f[16 * g + 8 * u]);
         }
-        const uint8_t* vr = st + St::vpage(0) + (D == 128 ? g * 1024 : g * 1024 + (g & 1) * 16 + (g >> 1) * 128) +
-                            col * RB;
+        if constexpr (LAST)
+            wait_ring<0>();
+        else
+            wait_ring<St::LOADS + 1>();
+        asm volatile("" ::: "memory");
+        const uint8_t* vr = st + St::VOFF + g * St::PAGE + col * RB;
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
             const v2i x = lds_read_tr4(vr + 16 * (db / 2 ^ St::vswz(col)) + 8 * (db & 1));
             o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[0], e[0], f[0], bits), pt[0], o[db], 0, 0, 0);
             o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[1], e[1], f[1], bits), pt[1], o[db], 0, 0, 0);
         }
+        if constexpr (!LAST) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+            issue_v(j + 1);
+        }
     };
 
     if (n_w > 0) {
         asm volatile("" ::: "memory");
         wait_ring<0>();
-        issue(0);
-        int j = 0;
-        for (; j + 1 < n_w; ++j) {
-            __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): the other stage's reads have returned
-            issue(j + 1);
-            wait_ring<St::LOADS>();
-            asm volatile("" ::: "memory");
-            step(std::false_type{}, wv + W * j, ring[wv][j & 1]);
-            asm volatile("" ::: "memory");
-        }
-        wait_ring<0>();
-        asm volatile("" ::: "memory");
-        step(std::true_type{}, wv + W * j, ring[wv][j & 1]);
+        issue_k(0);
+        issue_v(0);
+        for (int j = 0; j + 1 < n_w; ++j) step(std::false_type{}, j);
+        step(std::true_type{}, n_w - 1);
         asm volatile("" ::: "memory");
     }
 
@@ -372,9 +386,9 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
 #pragma unroll
         for (int db = 0; db < ND; ++db) r[db] = o[db];
     } else {
-        // the waves leave (O, m, l) in their rings
-        static_assert((ND * kWave * 4 + 2 * kWave) * 4 <= 2 * St::BYTES, "a wave's state in its ring");
-        float* xs = reinterpret_cast<float*>(ring[wv][0]);
+        // the waves leave (O, m, l) in their stages
+        static_assert((ND * kWave * 4 + 2 * kWave) * 4 <= St::BYTES, "a wave's state in its stage");
+        float* xs = reinterpret_cast<float*>(stage[wv]);
 #pragma unroll
         for (int db = 0; db < ND; ++db)
             *reinterpret_cast<floatx4*>(&xs[(db * kWave + lane) * 4]) = o[db];
@@ -386,7 +400,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             ml[w] = *reinterpret_cast<const float2*>(
-                &reinterpret_cast<const float*>(ring[w][0])[ND * kWave * 4 + 2 * lane]);
+                &reinterpret_cast<const float*>(stage[w])[ND * kWave * 4 + 2 * lane]);
             m = fmaxf(m, ml[w].x);
         }
 #pragma unroll
@@ -399,7 +413,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             for (int i = 0; i < NB; ++i)
                 if (W * i + wv < ND)
                     r[i] += al * *reinterpret_cast<const floatx4*>(
-                        &reinterpret_cast<const float*>(ring[w][0])[((W * i + wv) * kWave + lane) * 4]);
+                        &reinterpret_cast<const float*>(stage[w])[((W * i + wv) * kWave + lane) * 4]);
         }
     }
     l = rows4_sum(l);
@@ -437,7 +451,7 @@ q4_join_kernel(const Q4Args a, const DecodePlan p) {
 }
 
 constexpr int kBalanced = 16;      // sequences from which the splits are the whole batch's
-constexpr int kWaveSlots = 2048;   // one wave per split, two per SIMD of 256 CUs
+constexpr int kWaveSlots = 3072;   // one wave per split, three per SIMD of 256 CUs
 constexpr int kWaves = 4;          // per workgroup in fixed splits
 
 DecodePlan plan_of(int batch, int hkv, int G, int64_t max_len) {
