@@ -9,12 +9,17 @@
 //                     that lane group g receives the scores of page g's 16 keys
 //   O^T += V^T W^T    A = V's codes by ds_read_b64_tr_b4: a lane gets all 16 keys' codes of a
 //                     page for one dim, which are the 16 keys whose weights its group holds
-// so no score or weight crosses a lane.  A code becomes fp16 by its place: with its four bits
-// in mantissa bits 6..9 below the exponent of 16 it is 16 + n, and + (r - 16) gives n + r
-// without rounding (q4.h).  K's scale s multiplies the fp32 score.  V's is split into a power
-// of two E, which goes with the codes, (16 + n) E + (r - 16) E, exact again, and s / E, of 4
-// to 8 for all but the smallest, which multiplies the weight before its one rounding to fp16.
-// Weights are biased by 2^10, so that 2^-11 of each holds down to 2^-24 of the largest.
+// A code becomes an operand as the denormal it is: four bits at the bottom of a half are n 2^-24
+// (n 2^-20 at bits 4..7), which a packed multiply-add takes to (n + r) 2^-9, or to (n + r) E
+// for V, without rounding (q4.h): a shift, four ands and four multiply-adds for eight codes.
+// K's scale s multiplies the fp32 score.  V's is split into a power of two E of 2^-14 to 2^-9,
+// which goes with the codes, and s / E, of 4 to 4096, which multiplies the weight before its
+// one rounding to fp16.  (Scales past 8, rows with values past 60 or so, lower a wave's weights
+// by a common power of two.)  A weight's 2^-11 holds down to 2^-16 of the largest; below it is
+// an absolute 2^-25 of at most a quarter of that.
+// With up to 4 query heads (8), three (one) of four lanes of a 16-column product are idle: the
+// scores of the four row tiles are dealt out to them, so that a lane has 4 (8) exponentials a
+// tile instead of 16.
 #include "q4.h"
 
 #include <algorithm>
@@ -26,7 +31,8 @@ namespace {
 constexpr int kTok = 64;          // keys per tile: one page per 16 lanes
 constexpr int kMaxTiles = 16;     // per wave and split: 64 page ids, one per lane
 constexpr int kHeads = 16;        // query heads per workgroup
-constexpr float kBias = 10.f;
+constexpr float kLazyLog2 = 3.f;  // a row's reference moves when a score passes it by this
+constexpr float kMostM = 4096.f;  // s / E: weights up to 2^15 in fp16
 
 struct DecodePlan {
     int chunk;        // keys per split, a multiple of kTok
@@ -128,34 +134,41 @@ __device__ __forceinline__ half8 k_operand(uint32_t x, half2v f) {
                 __builtin_elementwise_fma(as_half2(y & 0x000f000fu), lo, f),
                 __builtin_elementwise_fma(as_half2(y & 0x00f000f0u), hi, f));
 }
-// Eight codes of V, of eight rows, as (n + r) E: four bits in mantissa bits 6..9 below the
-// exponent of 16 are 16 + n; times E and + (r - 16) E, exact again.  (The denormals' way would
-// want E 2^24, past fp16.)
-struct CodeBits {
-    uint32_t mask = 0x03c003c0u, sixteen = 0x4c004c00u;
-    // in registers: as literals they would keep v_and_or_b32 from taking both
-    __device__ __forceinline__ CodeBits() { asm("" : "+s"(mask), "+v"(sixteen)); }
-};
-__device__ __forceinline__ half8 v_operand(uint32_t x, const u32x4& e, const u32x4& f, const CodeBits& c) {
+// Eight codes of V, of eight rows, as (n + r) E: e = E 2^24, or E 2^20 for those that lie in
+// bits 4..7, f = E r.
+__device__ __forceinline__ half8 v_operand(uint32_t x, const u32x4& e, const u32x4& f) {
     auto pair = [&](uint32_t y, int i) {
-        return __builtin_elementwise_fma(as_half2((y & c.mask) | c.sixteen), as_half2(e[i]), as_half2(f[i]));
+        return __builtin_elementwise_fma(as_half2(y), as_half2(e[i]), as_half2(f[i]));
     };
-    return cat4(pair(x << 6, 0), pair(x << 2, 1), pair(x >> 2, 2), pair(x >> 6, 3));
+    const uint32_t y = x >> 8;
+    return cat4(pair(x & 0x000f000fu, 0), pair(x & 0x00f000f0u, 1), pair(y & 0x000f000fu, 2),
+                pair(y & 0x00f000f0u, 3));
 }
-// A row's scale as m E: E a power of two of at least 2^-14, m of 4 to 8 (less where s is below
-// 2^-12), and f = (r - 16) E.
+// The scale of row t as m E, E a power of two.
 struct Scale {
-    f16 e, f;
+    uint16_t e;
+    f16 f;
     float m;
 };
-__device__ __forceinline__ Scale scale_of(uint32_t sr) {
-    const int e = max((int)(sr & 0x7c00u) - 0x0800, 0x0400);
+__device__ __forceinline__ Scale scale_of(uint32_t sr, int t) {
+    const int e = min(max((int)(sr & 0x7c00u) - 0x0800, 0x0400), 0x1800);   // 2^-14 .. 2^-9
     const half2v h = as_half2(sr);
     Scale x;
-    x.e = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
+    x.e = static_cast<uint16_t>(e + (t & 1 ? 0x5000 : 0x6000));
+    x.f = h[1] * __builtin_bit_cast(f16, static_cast<uint16_t>(e));
     x.m = static_cast<float>(h[0]) * static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
-    x.f = (h[1] - f16(16)) * x.e;
     return x;
+}
+// Moves within 16 lanes: lane n gets lane n - S (or n + S: ROW_SHL) of x, in the quads of MASK;
+// others keep `old`.
+template <int CTRL, int MASK>
+__device__ __forceinline__ uint32_t row_move(uint32_t old, uint32_t x) {
+    return __builtin_amdgcn_update_dpp(old, x, CTRL, 0xf, MASK, false);
+}
+constexpr int kShl = 0x100, kShr = 0x110, kRor = 0x120;   // + the distance
+template <int CTRL, int MASK>
+__device__ __forceinline__ float row_move(float old, float x) {
+    return __uint_as_float(row_move<CTRL, MASK>(__float_as_uint(old), __float_as_uint(x)));
 }
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) v2i lds_v2i;
@@ -165,14 +178,17 @@ __device__ __forceinline__ v2i lds_read_tr4(const uint8_t* p) {
     return __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(__attribute__((address_space(3))) uint8_t*)p);
 }
 
-// What the lanes of a tile's keys leave for the others: lane group g reads page g's.
+// What the lanes of a tile's keys leave for the others: lane group g reads page g's, 16 keys in
+// the order 0 4 1 5 2 6 3 7, 8 12 .. of the codes' pairs.
 struct __attribute__((aligned(16))) Prepared {
-    float2 sm[kTok];      // K's s and V's m
-    f16 e[kTok], f[kTok]; // V's E and (r - 16) E, in the order of the codes' pairs
+    float2 sm[kTok];        // K's s and V's m
+    uint16_t e[kTok];       // V's E 2^24 or E 2^20 ...
+    f16 f[kTok];            // ... and E r
 };
 
 // W waves per workgroup take the tiles of one split round robin and meet in LDS.
-template <int D, int W>
+// PK: parts that a tile's scores are dealt out to, 16 / PK query heads or fewer.
+template <int D, int W, int PK>
 __global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 4)))
 q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     using St = Stage<D>;
@@ -206,7 +222,8 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     const int t_begin = split * chunk, t_end = min(L, t_begin + chunk);
     const int n_iter = (t_end - t_begin + kTok - 1) / kTok;
     const int n_w = n_iter > wv ? (n_iter - wv + W - 1) / W : 0;   // this wave's tiles
-    const bool hvalid = col < nh;
+    const int hcol = col % (kHeads / PK), part = col / (kHeads / PK);   // of the scores dealt out
+    const bool hvalid = hcol < nh;
 
     // Page ids of this wave's tiles, four to a tile; past the split's last key: its page.
     const uint8_t* head = a.pool + (int64_t)kvh * a.num_pages * PB;
@@ -216,13 +233,14 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     half8 qb[NS];   // lane (g, col): head col, dims (D/4) g + 8 s .., in the codes' order
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const half8 x = hvalid ? load_half8(a.q + (row0 + col) * D + RB / 2 * g + 8 * s) : half8{};
+        const half8 x = col < nh ? load_half8(a.q + (row0 + col) * D + RB / 2 * g + 8 * s) : half8{};
         qb[s] = __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
     }
 
     // The lane's place in a page's codes of K and of V
     const int lt = lane / (RB / 16) % kPage, lc = lane % (RB / 16);
-    const uint32_t ko = RB * lt + 16 * (D == 128 ? lc : lc ^ (lane >> 5));
+    const int kt = (lt & 9) | (lt & 2) << 1 | (lt & 4) >> 1;   // K's rows in the order of the tiles' reads
+    const uint32_t ko = RB * kt + 16 * (D == 128 ? lc : lc ^ (lane >> 5));
     const uint32_t vo = St::PAGE + RB * lt + 16 * (lc ^ St::vswz(lt));
     uint8_t* const st = stage[wv];
     const uint32_t st0 = lds_at(st);
@@ -247,15 +265,22 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         issue(j, vo, st0 + St::VOFF, [](int i) { return i * St::PAGE; });
     };
 
-    float m_run = -1e30f, l_part = 0.f;
+    float m_run = -1e30f, l_part = 0.f, down = 1.f;
     floatx4 o[ND];   // lane (g, col): dims 16 db + 4 g + e of head col
 #pragma unroll
     for (int db = 0; db < ND; ++db) o[db] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto scale_o = [&](float x) {
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[db][i] *= x;
+    };
     const float sc = a.scale_log2 * 512.f;   // K's operands are 2^-9 (n + r)
+    const float lazy = kLazyLog2 / sc;
     Prepared& prep = prep_all[wv];
-    const int at = 16 * g + 8 * (col >> 3) + 2 * (col & 3) + (col >> 2 & 1);
+    const int at = 16 * g + 8 * (col >> 3) + 2 * (col & 3) + (col >> 2 & 1);   // of key `col` of page g
+    constexpr int X = 16 / PK;   // scores of a lane
 
-    const CodeBits bits;
     // LAST: only a wave's last tile may reach past the split's last key
     auto step = [&](auto LAST_, int j) {
         constexpr bool LAST = decltype(LAST_)::value;
@@ -266,19 +291,27 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 4 * col);
             uint32_t vp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 64 + 4 * col);
             if (LAST && T0 + lane >= t_end) vp = 0;   // nothing of a row behind the last key
-            const Scale z = scale_of(vp);
-            prep.sm[lane] = float2{q4_row(kp).s, z.m};
+            Scale z = scale_of(vp, col);
+            const float size = fabsf(z.m);
+            if (__ballot(size * down > kMostM)) {
+                const float most = wave_max_fast(size < INFINITY ? size : 0.f) * (1.f / kMostM);
+                const float to = __uint_as_float(0x7f000000u - ((__float_as_uint(most) + 0x007fffffu) & 0x7f800000u));
+                scale_o(to / down);
+                down = to;
+            }
+            prep.sm[at] = float2{q4_row(kp).s, z.m * down};
             prep.e[at] = z.e;
             prep.f[at] = z.f;
         }
-        // scores: tile i's row m is page m / 4, key 4 i + m % 4
+        // scores: row 4 p + e of tile i is page p's key 0 2 8 10 (i) + 0 4 1 5 (e)
         const uint8_t* kr = st + (col >> 2) * St::PAGE + (D == 128 ? (col >> 2) * 16 : (col >> 3) * 128) +
-                            (col & 3) * RB + (D == 128 ? 16 * g : 8 * g ^ (col & 4) * 4);
-        const uint8_t* kpar = st + St::PAR + (col >> 2) * 128 + (col & 3) * 4;
+                            (2 * (col & 1) + (col >> 1 & 1)) * RB + (D == 128 ? 16 * g : 8 * g ^ (col & 4) * 4);
+        const uint8_t* kpar = st + St::PAR + (col >> 2) * 128 + ((col >> 1 & 1) + 4 * (col & 1)) * 4;
         floatx4 C[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f16 r = as_half2(*reinterpret_cast<const uint32_t*>(kpar + 16 * i))[1] * f16(1.f / 512);
+            const uint32_t sr = *reinterpret_cast<const uint32_t*>(kpar + 4 * (8 * (i >> 1) + 2 * (i & 1)));
+            const f16 r = as_half2(sr)[1] * f16(1.f / 512);
             const half2v f = {r, r};
             uint32_t x[NS];
             if constexpr (D == 128) {
@@ -300,49 +333,69 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): all of it has been read
             issue_k(j + 1);
         }
-        const floatx4* sm = reinterpret_cast<const floatx4*>(&prep.sm[16 * g]);
-        float m[16];
+        // this lane's scores, of keys X part .. in the prepared order, of head hcol
+        float x[X], m[X];
 #pragma unroll
-        for (int t = 0; t < 16; t += 2) {
+        for (int t = 0; t < X; ++t) {
+            x[t] = C[t / 4][t % 4];
+            if constexpr (PK == 2) x[t] = row_move<kShr + 8, 0xc>(x[t], C[2 + t / 4][t % 4]);
+            if constexpr (PK == 4) {
+                x[t] = row_move<kShr + 4, 0x2>(x[t], C[1][t]);
+                x[t] = row_move<kShr + 8, 0x4>(x[t], C[2][t]);
+                x[t] = row_move<kShr + 12, 0x8>(x[t], C[3][t]);
+            }
+        }
+        const floatx4* sm = reinterpret_cast<const floatx4*>(&prep.sm[16 * g + X * part]);
+#pragma unroll
+        for (int t = 0; t < X; t += 2) {
             const floatx4 z = sm[t / 2];
-            C[t / 4][t % 4] *= z[0];
-            C[t / 4][t % 4 + 1] *= z[2];
+            x[t] *= z[0];
+            x[t + 1] *= z[2];
             m[t] = z[1];
             m[t + 1] = z[3];
         }
         if constexpr (LAST) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t)
-                if (T0 + 16 * g + t >= t_end) C[t / 4][t % 4] = -INFINITY;
+            for (int t = 0; t < X; ++t) {
+                const int pos = X * part + t;
+                const int key = (pos & 8) + (pos >> 1 & 3) + 4 * (pos & 1);
+                if (T0 + 16 * g + key >= t_end) x[t] = -INFINITY;
+            }
         }
-        float mx = -INFINITY;
+        float mx = x[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            mx = fmaxf(mx, fmaxf(fmaxf(C[i][0], C[i][1]), fmaxf(C[i][2], C[i][3])));
+        for (int t = 1; t < X; ++t) mx = fmaxf(mx, x[t]);
+        if constexpr (PK == 4) mx = fmaxf(mx, row_move<kRor + 4, 0xf>(mx, mx));
+        if constexpr (PK >= 2) mx = fmaxf(mx, row_move<kRor + 8, 0xf>(mx, mx));
         mx = rows4_max(mx);
-        const float mn = fmaxf(m_run, mx);
-        const float alpha = fast_exp2((m_run - mn) * sc);
-        m_run = mn;
-        const float nm = hvalid ? kBias - mn * sc : -INFINITY;
-        float ps = 0.f;
-        half8 pt[2];
+        if (__builtin_amdgcn_read_exec() & __ballot(mx > m_run + lazy)) {
+            const float mn = fmaxf(m_run, mx);
+            const float alpha = fast_exp2((m_run - mn) * sc);
+            m_run = mn;
+            l_part *= alpha;
+            scale_o(alpha);
+        }
+        const float nm = hvalid ? -m_run * sc : -INFINITY;
+        uint32_t w[X / 2];
+#pragma unroll
+        for (int t = 0; t < X; t += 2) {
+            const float y = fast_exp2(fmaf(x[t], sc, nm)), z = fast_exp2(fmaf(x[t + 1], sc, nm));
+            l_part += y + z;
+            w[t / 2] = __builtin_bit_cast(uint32_t, half2v{static_cast<f16>(y * m[t]), static_cast<f16>(z * m[t + 1])});
+        }
+        u32x4 pt[2];   // the weights of page g's keys, of head col
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {   // keys 8 u + j and 8 u + j + 4
-                const float x = fast_exp2(fmaf(C[2 * u][j], sc, nm));
-                const float y = fast_exp2(fmaf(C[2 * u + 1][j], sc, nm));
-                pt[u][2 * j] = static_cast<f16>(x * m[8 * u + j]);
-                pt[u][2 * j + 1] = static_cast<f16>(y * m[8 * u + j + 4]);
-                ps += x + y;
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (PK == 1) pt[u][i] = w[4 * u + i];
+                if constexpr (PK == 2) pt[u][i] = u == 0 ? w[i] : row_move<kShl + 8, 0xf>(w[i], w[i]);
+                if constexpr (PK == 4) {
+                    const uint32_t v = w[i % 2];
+                    pt[u][i] = u == 0 ? (i < 2 ? v : row_move<kShl + 4, 0xf>(v, v))
+                                      : (i < 2 ? row_move<kShl + 8, 0xf>(v, v) : row_move<kShl + 12, 0xf>(v, v));
+                }
             }
-        l_part = fmaf(l_part, alpha, ps);
-        if (__builtin_amdgcn_read_exec() & __ballot(alpha != 1.f)) {
-#pragma unroll
-            for (int db = 0; db < ND; ++db)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[db][i] *= alpha;
-        }
         u32x4 e[2], f[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -357,9 +410,11 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         const uint8_t* vr = st + St::VOFF + g * St::PAGE + col * RB;
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
-            const v2i x = lds_read_tr4(vr + 16 * (db / 2 ^ St::vswz(col)) + 8 * (db & 1));
-            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[0], e[0], f[0], bits), pt[0], o[db], 0, 0, 0);
-            o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(x[1], e[1], f[1], bits), pt[1], o[db], 0, 0, 0);
+            const v2i y = lds_read_tr4(vr + 16 * (db / 2 ^ St::vswz(col)) + 8 * (db & 1));
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(y[u], e[u], f[u]),
+                                                               __builtin_bit_cast(half8, pt[u]), o[db], 0, 0, 0);
         }
         if constexpr (!LAST) {
             asm volatile("" ::: "memory");
@@ -377,6 +432,9 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         step(std::true_type{}, n_w - 1);
         asm volatile("" ::: "memory");
     }
+    if (down != 1.f) scale_o(1.f / down);
+    if constexpr (PK == 4) l_part += row_move<kRor + 4, 0xf>(l_part, l_part);
+    if constexpr (PK >= 2) l_part += row_move<kRor + 8, 0xf>(l_part, l_part);
 
     // Dims 16 db + 4 g + e of head col: all of them, or every W-th 16 of the waves' sum.
     constexpr int NB = (ND + W - 1) / W;
@@ -417,7 +475,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         }
     }
     l = rows4_sum(l);
-    if (!hvalid) return;
+    if (col >= nh) return;
     const int64_t prow = (row0 + col) * p.nsplit + split;
     if (nsb > 1 && g == 0 && wv == 0) {
         p.ws_ml[prow * 2] = m * sc;
@@ -499,13 +557,22 @@ int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s) {
     p.ws_o = static_cast<float*>(ws);
     p.ws_ml = p.ws_o + (size_t)batch * a.Hq * p.nsplit * a.D;
     const dim3 grid(a.Hkv * p.groups, static_cast<unsigned>(units_of(p, a.max_len)), p.balance ? 1 : batch);
-    auto go = [&](auto kernel, int waves) {
-        hipLaunchKernelGGL(kernel, grid, dim3(waves * kWave), 0, s, a, p);
+    auto go = [&](auto d, auto pk) {
+        constexpr int D = decltype(d)::value, PK = decltype(pk)::value;
+        if (p.balance)
+            hipLaunchKernelGGL((q4_decode_kernel<D, 1, PK>), grid, dim3(kWave), 0, s, a, p);
+        else
+            hipLaunchKernelGGL((q4_decode_kernel<D, kWaves, PK>), grid, dim3(kWaves * kWave), 0, s, a, p);
     };
-    if (a.D == 64)
-        p.balance ? go(q4_decode_kernel<64, 1>, 1) : go(q4_decode_kernel<64, kWaves>, kWaves);
-    else
-        p.balance ? go(q4_decode_kernel<128, 1>, 1) : go(q4_decode_kernel<128, kWaves>, kWaves);
+    auto parts = [&](auto d) {
+        if (a.G <= 4)
+            go(d, std::integral_constant<int, 4>{});
+        else if (a.G <= 8)
+            go(d, std::integral_constant<int, 2>{});
+        else
+            go(d, std::integral_constant<int, 1>{});
+    };
+    a.D == 64 ? parts(std::integral_constant<int, 64>{}) : parts(std::integral_constant<int, 128>{});
     if (p.nsplit > 1) {
         const dim3 rows(a.Hq, batch), threads(kJoinWaves * kWave);
         if (a.D == 64)
