@@ -84,82 +84,6 @@ __device__ __forceinline__ void bound_add(const BoundArgs& a, int b, int kvh, in
     if (fresh && a.ages) a.ages[at] = (a.newest ? a.newest[b] : n - 1) - (n - 1 - j);
 }
 
-// ---- join of decode splits (bounded_decode.hip, q4_decode.hip) ----
-constexpr int kJoinWaves = 4;
-
-// Joins the nsb partials of one query head of one sequence (ws_o [rows][nsplit][D], ws_ml
-// [rows][nsplit][2], the maximum in log2 units and the sum), kJoinWaves waves: lane (r, c)
-// owns dims 8c .. of every (4R)-th split, U of them in flight.
-template <int D>
-__device__ __forceinline__ void join_head(f16* out, const float* ws_o, const float* ws_ml,
-                                          int nsplit, int64_t row, int nsb) {
-    constexpr int LPR = D / 8, R = kWave / LPR, STRIDE = kJoinWaves * R, U = 4;
-    __shared__ __attribute__((aligned(16))) float red[kJoinWaves - 1][LPR][12];
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane % LPR, r = lane / LPR;
-    const float* po = ws_o + row * nsplit * D + 8 * c;
-    const float* pml = ws_ml + row * nsplit * 2;
-    float M = -3.0e38f, S = 0.f;
-    floatx4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
-    auto fold = [&](float m, float s, floatx4 y0, floatx4 y1) {
-        const float mn = fmaxf(M, m);
-        const float al = fast_exp2(M - mn), be = fast_exp2(m - mn);
-        x0 = x0 * al + y0 * be;
-        x1 = x1 * al + y1 * be;
-        S = S * al + s * be;
-        M = mn;
-    };
-    for (int j0 = wave * R + r; j0 < nsb; j0 += STRIDE * U) {
-        float2 ml[U];
-        floatx4 y[U][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = min(j0 + STRIDE * u, nsb - 1);
-            ml[u] = *reinterpret_cast<const float2*>(pml + 2 * j);
-            y[u][0] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D);
-            y[u][1] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D + 4);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (j0 + STRIDE * u < nsb) fold(ml[u].x, ml[u].y, y[u][0], y[u][1]);
-    }
-#pragma unroll
-    for (int o = LPR; o < kWave; o <<= 1) {
-        floatx4 y0, y1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            y0[e] = __shfl_xor(x0[e], o);
-            y1[e] = __shfl_xor(x1[e], o);
-        }
-        const float m = __shfl_xor(M, o), s = __shfl_xor(S, o);
-        fold(m, s, y0, y1);
-    }
-    if (wave > 0 && r == 0) {
-        float* q = red[wave - 1][c];
-        *reinterpret_cast<floatx4*>(q) = x0;
-        *reinterpret_cast<floatx4*>(q + 4) = x1;
-        q[8] = M;
-        q[9] = S;
-    }
-    __syncthreads();
-    if (wave != 0 || r != 0) return;
-#pragma unroll
-    for (int w = 0; w < kJoinWaves - 1; ++w) {
-        const float* q = red[w][c];
-        fold(q[8], q[9], *reinterpret_cast<const floatx4*>(q),
-             *reinterpret_cast<const floatx4*>(q + 4));
-    }
-    const float inv = 1.f / S;
-    half8 h;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        h[e] = static_cast<f16>(x0[e] * inv);
-        h[4 + e] = static_cast<f16>(x1[e] * inv);
-    }
-    store_half8(out + row * D + 8 * c, h);
-}
-
 // ---------------------------------------------------------------- host ----
 int bound_check_view(const kvhp_kv_view* v, const char* what, const char* name);
 constexpr int kMaxBatch = 65535, kMaxKvHeads = 65535;   // grid dimensions

@@ -42,48 +42,50 @@ struct DecodePlan {
     int groups;       // workgroups per KV head and split, of up to kHeads query heads
     float* ws_o;      // [B * Hq][nsplit][D]
     float* ws_ml;     // [B * Hq][nsplit][2], the maximum in log2 units
+    int32_t* ws_n;    // [B] splits
 };
 
 __device__ __forceinline__ int tiles_of(int L) { return (L + kTok - 1) / kTok; }
-// Tiles of the whole batch (at most 2^30: the splits are as long as they may be far below).
-__device__ __forceinline__ uint32_t batch_tiles(const Q4Args& a, int batch, int lane) {
-    uint32_t t = 0;
-    for (int i = lane; i < batch; i += kWave) t = min(t + tiles_of(q4_len(a, i)), 1u << 24);
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) t += __shfl_xor(t, o);
-    return t;
+// Sums over lanes 0 .. this one, by row shifts and row broadcasts.
+__device__ __forceinline__ uint32_t prefix_sum(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);
+    return x;
 }
-// Keys per split of a sequence of L keys; split and join agree on it.
-__device__ __forceinline__ int chunk_of(const DecodePlan& p, int L, uint32_t tiles) {
-    if (p.balance <= 0 || L <= 0) return p.chunk;
-    const uint32_t target = min((tiles + p.balance - 1) / p.balance, (uint32_t)kMaxTiles);
-    const uint32_t t = tiles_of(L), n = min((t + target - 1) / target, (uint32_t)p.nsplit);
-    return static_cast<int>((t + n - 1) / n * kTok);   // at most kMaxTiles tiles: nsplit of them hold the longest
+// Tiles of a sequence's splits where the batch has `tiles`.
+__device__ __forceinline__ uint32_t share_tiles(const DecodePlan& p, uint32_t t, uint32_t target) {
+    const uint32_t n = min((t + target - 1) / target, (uint32_t)p.nsplit);
+    return t > 0 ? (t + n - 1) / n : 1;   // at most kMaxTiles: nsplit of them hold the longest
 }
 // The i-th split of the batch, counted in sequence order (sequences without keys keep one,
 // which writes their zeros).
-__device__ __forceinline__ bool share_of(const Q4Args& a, const DecodePlan& p, int i, int lane, int& b,
+__device__ __forceinline__ bool share_of(const Q4Args& a, const DecodePlan& p, uint32_t i, int lane, int& b,
                                          int& split, int& L, int& chunk) {
-    const uint32_t tiles = batch_tiles(a, p.batch, lane);
-    int base = 0;
+    uint32_t tiles = 0;
+    int li = lane < p.batch ? q4_len(a, lane) : 0;
+    for (int g0 = 0; g0 < p.batch; g0 += kWave) {
+        // at most 2^24 a sequence and 65535 of them: what 32 bits lose is only a balance
+        const int l = g0 == 0 ? li : g0 + lane < p.batch ? q4_len(a, g0 + lane) : 0;
+        tiles = min(tiles + (uint32_t)__builtin_amdgcn_readlane(prefix_sum(tiles_of(l)), kWave - 1), 1u << 30);
+    }
+    const uint32_t target = min((tiles + p.balance - 1) / p.balance, (uint32_t)kMaxTiles);
+    uint32_t base = 0;
     for (int g0 = 0; g0 < p.batch; g0 += kWave) {
         const bool in = g0 + lane < p.batch;
-        const int li = in ? q4_len(a, g0 + lane) : 0;
-        const int ci = chunk_of(p, li, tiles);
-        const int ni = in ? (li > 0 ? (li + ci - 1) / ci : 1) : 0;
-        int inc = ni;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int t = __shfl_up(inc, o);
-            if (lane >= o) inc += t;
-        }
-        const int tot = __shfl(inc, kWave - 1);
+        if (g0 > 0) li = in ? q4_len(a, g0 + lane) : 0;
+        const uint32_t t = tiles_of(li), ti = share_tiles(p, t, max(target, 1u));
+        const uint32_t ni = in ? max((t + ti - 1) / ti, 1u) : 0;
+        const uint32_t inc = prefix_sum(ni), tot = __builtin_amdgcn_readlane(inc, kWave - 1);
         if (i < base + tot) {
             const int owner = __builtin_ctzll(__ballot(base + inc > i));
-            b = __builtin_amdgcn_readfirstlane(g0 + owner);
-            split = __builtin_amdgcn_readfirstlane(i - base - (__shfl(inc, owner) - __shfl(ni, owner)));
-            L = __builtin_amdgcn_readfirstlane(__shfl(li, owner));
-            chunk = __builtin_amdgcn_readfirstlane(__shfl(ci, owner));
+            b = g0 + owner;
+            split = i - base - (__builtin_amdgcn_readlane(inc, owner) - __builtin_amdgcn_readlane(ni, owner));
+            L = __builtin_amdgcn_readlane(li, owner);
+            chunk = __builtin_amdgcn_readlane(ti, owner) * kTok;
             return true;
         }
         base += tot;
@@ -211,13 +213,14 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     }
     const int nh = min(a.G - h0, kHeads);
     const int64_t row0 = (int64_t)b * a.Hq + (int64_t)kvh * a.G + h0;
+    const int nsb = L > 0 ? (L + chunk - 1) / chunk : 0;
+    if (p.nsplit > 1 && split == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.ws_n[b] = nsb;
     if (L <= 0) {
         if (split == 0)
             for (int i = threadIdx.x; i < nh * (D / 8); i += W * kWave)
                 store_half8(a.out + row0 * D + 8 * i, half8{});
         return;
     }
-    const int nsb = (L + chunk - 1) / chunk;
     if (split >= nsb) return;
     const int t_begin = split * chunk, t_end = min(L, t_begin + chunk);
     const int n_iter = (t_end - t_begin + kTok - 1) / kTok;
@@ -497,19 +500,74 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kJoinWaves * kWave)
-q4_join_kernel(const Q4Args a, const DecodePlan p) {
-    const int b = blockIdx.y, lane = threadIdx.x & (kWave - 1);
-    const int L = q4_len(a, b);
-    if (L <= 0) return;
-    const int chunk = chunk_of(p, L, p.balance > 0 ? batch_tiles(a, p.batch, lane) : 0);
-    const int nsb = (L + chunk - 1) / chunk;
-    if (nsb > 1) join_head<D>(a.out, p.ws_o, p.ws_ml, p.nsplit, (int64_t)b * a.Hq + blockIdx.x, nsb);
+// Joins the splits of a row (a query head of a sequence), a wave per row: lane (r, c) takes
+// dims 8c .. of every (64 / (D/8))-th split, U of them at once.  The first are on their way
+// before it is known how many there are (the workspace holds nsplit).
+constexpr int kJoinRows = 4;   // waves per workgroup
+template <int D, int U>
+__global__ void __launch_bounds__(kJoinRows * kWave) q4_join_kernel(const Q4Args a, const DecodePlan p) {
+    constexpr int LPR = D / 8, R = kWave / LPR;
+    const int lane = threadIdx.x & (kWave - 1), c = lane % LPR, r = lane / LPR;
+    const int head = blockIdx.x * kJoinRows + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.y;
+    if (head >= a.Hq) return;
+    const int64_t row = (int64_t)b * a.Hq + head;
+    const float* po = p.ws_o + row * p.nsplit * D + 8 * c;
+    const float2* pml = reinterpret_cast<const float2*>(p.ws_ml) + row * p.nsplit;
+    float M = -3.0e38f, S = 0.f;
+    floatx4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+    auto fold = [&](float m, float s, floatx4 y0, floatx4 y1) {
+        const float mn = fmaxf(M, m);
+        const float al = fast_exp2(M - mn), be = fast_exp2(m - mn);
+        x0 = x0 * al + y0 * be;
+        x1 = x1 * al + y1 * be;
+        S = S * al + s * be;
+        M = mn;
+    };
+    float2 ml[U];
+    floatx4 y[U][2];
+    auto load = [&](int j0, int n) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = min(j0 + R * u + r, n - 1);
+            ml[u] = pml[j];
+            y[u][0] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D);
+            y[u][1] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D + 4);
+        }
+    };
+    load(0, p.nsplit);
+    const int nsb = p.ws_n[b];
+    if (nsb <= 1) return;   // no keys, or written by its one split
+    for (int j0 = 0;;) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j0 + R * u + r < nsb) fold(ml[u].x, ml[u].y, y[u][0], y[u][1]);
+        if ((j0 += R * U) >= nsb) break;
+        load(j0, nsb);
+    }
+#pragma unroll
+    for (int o = LPR; o < kWave; o <<= 1) {
+        floatx4 y0, y1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            y0[e] = __shfl_xor(x0[e], o);
+            y1[e] = __shfl_xor(x1[e], o);
+        }
+        const float m = __shfl_xor(M, o), s = __shfl_xor(S, o);
+        fold(m, s, y0, y1);
+    }
+    if (r > 0) return;
+    const float inv = 1.f / S;
+    half8 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        h[e] = static_cast<f16>(x0[e] * inv);
+        h[4 + e] = static_cast<f16>(x1[e] * inv);
+    }
+    store_half8(a.out + row * D + 8 * c, h);
 }
 
 constexpr int kBalanced = 16;      // sequences from which the splits are the whole batch's
-constexpr int kWaveSlots = 3072;   // one wave per split, three per SIMD of 256 CUs
+constexpr int kWaveSlots = 2048;   // one wave per split, two per SIMD of 256 CUs
 constexpr int kWaves = 4;          // per workgroup in fixed splits
 
 DecodePlan plan_of(int batch, int hkv, int G, int64_t max_len) {
@@ -542,7 +600,7 @@ int64_t units_of(const DecodePlan& p, int64_t max_len) {
 size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len) {
     if (!bound_sizes(batch, hq, hkv, max_len, 0, 0) || (d != 64 && d != 128)) return 0;
     const DecodePlan p = plan_of(batch, hkv, hq / hkv, max_len);
-    return p.nsplit == 1 ? 0 : sizeof(float) * (size_t)batch * hq * p.nsplit * (d + 2);
+    return p.nsplit == 1 ? 0 : sizeof(float) * ((size_t)batch * hq * p.nsplit * (d + 2) + batch);
 }
 
 bool q4_decode_fits(const Q4Args& a, int batch) {
@@ -556,6 +614,7 @@ int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s) {
     DecodePlan p = plan_of(batch, a.Hkv, a.G, a.max_len);
     p.ws_o = static_cast<float*>(ws);
     p.ws_ml = p.ws_o + (size_t)batch * a.Hq * p.nsplit * a.D;
+    p.ws_n = reinterpret_cast<int32_t*>(p.ws_ml + (size_t)batch * a.Hq * p.nsplit * 2);
     const dim3 grid(a.Hkv * p.groups, static_cast<unsigned>(units_of(p, a.max_len)), p.balance ? 1 : batch);
     auto go = [&](auto d, auto pk) {
         constexpr int D = decltype(d)::value, PK = decltype(pk)::value;
@@ -574,11 +633,16 @@ int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s) {
     };
     a.D == 64 ? parts(std::integral_constant<int, 64>{}) : parts(std::integral_constant<int, 128>{});
     if (p.nsplit > 1) {
-        const dim3 rows(a.Hq, batch), threads(kJoinWaves * kWave);
-        if (a.D == 64)
-            hipLaunchKernelGGL(q4_join_kernel<64>, rows, threads, 0, s, a, p);
-        else
-            hipLaunchKernelGGL(q4_join_kernel<128>, rows, threads, 0, s, a, p);
+        const dim3 rows((a.Hq + kJoinRows - 1) / kJoinRows, batch), threads(kJoinRows * kWave);
+        auto join = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            const int u = (p.nsplit * (D / 8) + kWave - 1) / kWave;   // splits of a lane
+            if (u == 1)
+                hipLaunchKernelGGL((q4_join_kernel<D, 1>), rows, threads, 0, s, a, p);
+            else
+                hipLaunchKernelGGL((q4_join_kernel<D, 2>), rows, threads, 0, s, a, p);
+        };
+        a.D == 64 ? join(std::integral_constant<int, 64>{}) : join(std::integral_constant<int, 128>{});
     }
     return check_launch("q4_decode");
 }
