@@ -114,5 +114,9 @@ __device__ __forceinline__ const uint8_t* q4_page(const uint8_t* pool, int num_p
 size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len);
 bool q4_decode_fits(const Q4Args& a, int batch);
 int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s);
+// q4_prefill.hip: rows at D = 64 and 128.
+size_t q4_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int max_len);
+bool q4_prefill_fits(const Q4Args& a, int batch);
+int q4_prefill(const Q4Args& a, int batch, void* ws, hipStream_t s);
 
 }  // namespace kvhp

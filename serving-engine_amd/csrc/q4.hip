@@ -218,7 +218,7 @@ extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* bl
 extern "C" size_t kvhp_q4_prefill_workspace_bytes(int batch, int rows, int num_q_heads,
                                                   int num_kv_heads, int head_dim,
                                                   int max_seq_len) {
-    return 0;
+    return q4_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
 }
 
 extern "C" int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* block_tables,
@@ -240,5 +240,11 @@ extern "C" int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* b
     a.q_start = q_start;
     a.seq_lens = seq_lens;
     a.rows = rows;
+    rc = workspace_check(what, workspace, workspace_bytes,
+                         q4_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim,
+                                              max_seq_len));
+    if (rc) return rc;
+    if (q4_prefill_fits(a, batch))
+        return q4_prefill(a, batch, workspace, static_cast<hipStream_t>(stream));
     return launch_rows(a, batch, what, static_cast<hipStream_t>(stream));
 }

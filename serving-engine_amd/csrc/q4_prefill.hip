@@ -1,0 +1,508 @@
+// q4_prefill.hip -- rows of prompts and chunks over a paged cache held in 4 bits (gfx950,
+// head_dim 64 and 128).
+//
+// A workgroup of W waves takes one KV head of one sequence and 32 W of its (row, query head)
+// pairs, query head fastest, 32 pairs a wave, and walks the keys up to its last row in tiles of
+// 64.  Each tile's codes are turned into operands once for all its waves: a wave loads the
+// codes of its share of the tile's pages into registers, one tile ahead, and writes them to LDS
+// as fp16 while the matrix cores are at the tile before.  The operands are exact (q4.h): a code
+// with its four bits in mantissa bits 6..9 below the exponent of 16 is 16 + n, and times E
+// plus (r - 16) E it is (n + r) E; E = 1 for K, for V the power of two that leaves s / E = m
+// between 4 and 8 (less for scales below 2^-12).  K's s multiplies the scores inside the
+// exponent's multiply-add, V's m a weight before its one rounding to fp16.
+//
+// Per tile, on v_mfma_f32_32x32x16_f16 with one lane per pair: S^T = K Q^T of the next tile
+// beside the exponentials of this one; then O^T += V^T W^T beside the next codes' conversion.
+// Weights are taken against a reference that moves when one of a row passes it by 2^12 (to
+// 2^4), seen from the weights themselves, so that no maximum of the scores is needed: 2^-11 of
+// each holds down to 2^-16 of the reference, below it is an absolute 2^-27 of it.
+//
+// A row that holds NaN has operands of 0 and a scale of NaN, so it reaches the rows that see
+// it and, their weights' place being 0, no others.
+//
+// Few rows over a long cache are cut into ranges of keys (blockIdx.z) whose partials a second
+// launch joins.
+#include "q4.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace kvhp {
+namespace {
+
+constexpr int kBN = 64;               // keys per tile
+constexpr int kMaxRowHeads = 1 << 29; // (row, query head) pairs of a sequence: a grid of 2^22
+constexpr int kCUs = 256;
+constexpr float kRefLog2 = 4.f;       // weights where a row's reference is set,
+constexpr float kMostWeight = 4096.f; // and where it moves
+
+struct PrefillPlan {
+    uint32_t inv_g;        // ceil(2^32 / G), 0 for G = 1
+    int blocks;            // of pairs, per sequence and KV head
+    int tiles_per_split, nsplit;
+    float* ws_o;           // [batch * rows * Hq][nsplit][D]
+    float* ws_ml;          // [batch * rows * Hq][nsplit][2], the reference in log2 units
+};
+
+// Row of a pair: pair / G, exact for pair * G below 2^32.
+__device__ __forceinline__ int row_of(const PrefillPlan& p, uint32_t pair) {
+    return static_cast<int>(p.inv_g ? __umulhi(pair, p.inv_g) : pair);
+}
+// The rows of a block that lie in their sequence.
+struct Block {
+    int first;       // position of row 0
+    int p_lo, p_hi;  // positions of the block's first and last live row; none: p_lo > p_hi
+    __device__ __forceinline__ int tiles() const { return p_hi / kBN + 1; }
+};
+__device__ __forceinline__ Block block_of(const Q4Args& a, const PrefillPlan& p, int b, int blk, int pairs) {
+    Block k;
+    const int n = q4_len(a, b);
+    // a start outside +-2^30 leaves no row among at most 2^30 keys
+    const int64_t first = min(max(q4_first(a, b, n), -(int64_t)(1 << 30)), (int64_t)(1 << 30));
+    const int r0 = row_of(p, blk * pairs), r1 = min(row_of(p, (blk + 1) * pairs - 1), a.rows - 1);
+    k.first = static_cast<int>(first);
+    k.p_lo = static_cast<int>(max(first + r0, (int64_t)0));
+    k.p_hi = static_cast<int>(min(first + r1, (int64_t)n - 1));
+    return k;
+}
+
+// The 16-byte chunks of LDS rows lie at c ^ swizzle(row): the 16 rows of an operand read of K,
+// the four rows x four chunks of a transposing read of V, and the conversion's writes each on
+// distinct banks (V's two by two at D = 128).  V's is the same for rows 8 apart.
+template <int D>
+__device__ __forceinline__ int kswz(int r) { return D == 128 ? r & 15 : r >> 1 & 7; }
+template <int D>
+__device__ __forceinline__ int vswz(int r) {
+    return (D == 128 ? 4 * (r & 3) : (r & 3) << 1) | (r >> 2 & 1);
+}
+
+__device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
+struct CodeBits {
+    uint32_t mask = 0x03c003c0u, sixteen = 0x4c004c00u;
+    // in registers: as literals they would keep v_and_or_b32 from taking both
+    __device__ __forceinline__ CodeBits() { asm("" : "+s"(mask), "+v"(sixteen)); }
+};
+// Eight codes as (n + r) E, in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ half8 operand(uint32_t x, half2v e, half2v f, const CodeBits& c) {
+    auto pair = [&](uint32_t y) {
+        return __builtin_elementwise_fma(as_half2((y & c.mask) | c.sixteen), e, f);
+    };
+    const half2v p0 = pair(x << 6), p1 = pair(x << 2), p2 = pair(x >> 2), p3 = pair(x >> 6);
+    return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+
+// A tile's (s log2(e) / sqrt(D), m) in the order a lane of half h takes them: [h][32 keys].
+template <int D>
+struct __attribute__((aligned(16))) Tiles {
+    f16 k[2][kBN * D], v[2][kBN * D];
+    float s[2][kBN], m[2][kBN];
+};
+
+template <int D, int W>
+__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
+q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
+    constexpr int NC = D / 16, NDB = D / 32, RB = D / 2, PB = q4_page_bytes(D), PAIRS = 32 * W;
+    // 16-byte chunks of codes: a thread has one of K and one of V, or half a wave has K's
+    constexpr int BOTH = D / (16 * W) == 2;
+    static_assert(BOTH || D == 16 * W, "one or two chunks a thread");
+    __shared__ Tiles<D> lds;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int h = lane >> 5, c32 = lane & 31;
+    const int kvh = blockIdx.x % a.Hkv;
+    const int blk = p.blocks - 1 - static_cast<int>(blockIdx.x / a.Hkv);   // longest first
+    const int b = blockIdx.y;
+    const Block k = block_of(a, p, b, blk, PAIRS);
+    if (k.p_lo > k.p_hi) return;
+    const int t_lo = static_cast<int>(blockIdx.z) * p.tiles_per_split;
+    const int all_tiles = k.tiles();
+    const int n = min(all_tiles - t_lo, p.tiles_per_split);
+    if (n <= 0) return;
+
+    // This lane's pair.
+    const int pair0 = blk * PAIRS + 32 * wave, pair = pair0 + c32;
+    const int row = row_of(p, pair), qh = kvh * a.G + pair - row * a.G, pos = k.first + row;
+    const bool live = row < a.rows && pos >= k.p_lo && pos <= k.p_hi;
+    const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
+    // tiles (of the block's) from `past` on hold keys that some pair of the wave does not see
+    const int lo = k.first + row_of(p, pair0), hi = k.first + row_of(p, pair0 + 31);
+    const int past = lo < k.p_lo || hi > k.p_hi || lo < kBN - 1 ? 0 : (lo - (kBN - 1)) / kBN + 1;
+    half8 qop[NC];   // in the codes' order
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const half8 x = live ? load_half8(a.q + at * D + 16 * c + 8 * h) : half8{};
+        qop[c] = __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
+    }
+
+    // ---- codes to operands: this thread's row of a tile, and its 32 dims of it
+    constexpr int CPR = RB / 16;                       // chunks of codes in a row
+    constexpr int TPW = kBN / W;                       // rows of a wave, in one page
+    const int item = BOTH ? lane : lane & 31;
+    const int crow = TPW * wave + item / CPR, cc = item % CPR;
+    const bool is_v = !BOTH && h == 1;                 // what the first chunk is
+    const int32_t* bt = a.bt + (int64_t)b * a.max_pages;
+    const uint8_t* head = a.pool + (int64_t)kvh * a.num_pages * PB;
+    const int last_page = k.p_hi >> 4;
+    auto page_of = [&](int t) {   // of this wave's rows of a tile: ids are clamped into the pool
+        const int pi = min((t_lo + min(t, n - 1)) * (kBN / kPage) + TPW * wave / kPage, last_page);
+        return min(max(bt[pi], 0), a.num_pages - 1);
+    };
+    struct Raw {
+        u32x4 x;       // codes
+        uint32_t sr;   // their row's numbers
+    };
+    auto load_raw = [&](int pid, bool v) {
+        const uint8_t* pg = head + (int64_t)pid * PB;
+        const int r = crow & 15;
+        Raw w;
+        w.x = *reinterpret_cast<const u32x4*>(pg + (v ? kPage * RB : 0) + r * RB + 16 * cc);
+        w.sr = *reinterpret_cast<const uint32_t*>(pg + kPage * D + (v ? 4 * kPage : 0) + 4 * r);
+        return w;
+    };
+    const CodeBits bits;
+    auto convert = [&](int t, const Raw& w, bool v, f16* tile) {
+        uint32_t sr = w.sr;
+        if ((t_lo + t) * kBN + crow > k.p_hi) sr = 0;              // behind the last key
+        if ((sr & 0x7c00u) == 0x7c00u) sr = 0;                     // NaN: the scale tells
+        const int e = v ? max((int)(sr & 0x7c00u) - 0x0800, 0x0400) : 0x3c00;
+        const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
+        const f16 fh = (as_half2(sr)[1] - f16(16)) * eh;
+        const half2v e2 = {eh, eh}, f2 = {fh, fh};
+        const int swz = v ? vswz<D>(crow) : kswz<D>(crow);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            store_half8(tile + crow * D + 8 * ((4 * cc + i) ^ swz), operand(w.x[i], e2, f2, bits));
+    };
+    // A row's s and m, by one of its threads: key 32 n + 8 q + 4 h + e to [h][16 n + 4 q + e].
+    const int sat = 32 * (crow >> 2 & 1) + 16 * (crow >> 5) + 4 * (crow >> 3 & 3) + (crow & 3);
+    auto put_scale = [&](int t, uint32_t sr, bool v) {
+        if (cc != 0) return;
+        if (v) {
+            if ((t_lo + t) * kBN + crow > k.p_hi) sr = 0;
+            const int e = max((int)(sr & 0x7c00u) - 0x0800, 0x0400);
+            lds.m[t & 1][sat] = static_cast<float>(as_half2(sr)[0]) *
+                                static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
+        } else {
+            lds.s[t & 1][sat] = static_cast<float>(as_half2(sr)[0]) * a.scale_log2;
+        }
+    };
+
+    // ---- operand reads
+    int kro[NC], vro[NDB];
+    {
+        const int j16 = lane & 15, blk2 = lane >> 4 & 1;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kro[c] = c32 * D + 8 * ((2 * c + h) ^ kswz<D>(c32));
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+            const int r = 4 * h + j16 / 4;
+            vro[db] = r * D + 8 * ((4 * db + 2 * blk2 + ((j16 & 3) >> 1)) ^ vswz<D>(r)) + 4 * (j16 & 1);
+        }
+    }
+    floatx16 o[NDB];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+    float m_run = -1e30f, l_part = 0.f;
+
+    auto qk = [&](int j, floatx16 (&s)[2]) {
+        const f16* Kt = lds.k[j & 1];
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[n2][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int n2 = 0; n2 < 2; ++n2)
+                s[n2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    *reinterpret_cast<const half8*>(&Kt[kro[c] + 32 * n2 * D]), qop[c], s[n2], 0, 0, 0);
+    };
+    // Weights of tile j as the operands of O^T's product; element (n, i) is key 32 n + 8 (i / 4)
+    // + 4 h + i % 4.  Returns the largest and adds up the sum before the rounding.
+    auto weights = [&](int j, const floatx16 (&s)[2], half8 (&w)[4], float& sum) {
+        float most = 0.f, ps[2] = {0.f, 0.f};
+        const bool masked = t_lo + j >= past;
+        const int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const floatx4 ks = *reinterpret_cast<const floatx4*>(&lds.s[j & 1][32 * h + 16 * n2 + 4 * q4]);
+                const floatx4 vm = *reinterpret_cast<const floatx4*>(&lds.m[j & 1][32 * h + 16 * n2 + 4 * q4]);
+                float x[4], y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = fast_exp2(fmaf(s[n2][4 * q4 + e], ks[e], -m_run));
+                    y[e] = x[e] * vm[e];
+                }
+                if (masked) {
+                    asm volatile("");   // a branch: no selects in every tile
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (32 * n2 + 8 * q4 + e > seen) x[e] = y[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[2 * n2 + q4 / 2][4 * (q4 & 1) + e] = static_cast<f16>(y[e]);
+                    most = fmaxf(most, x[e]);
+                    ps[e & 1] += x[e];
+                }
+            }
+        sum = ps[0] + ps[1];
+        return most;
+    };
+    // Moves the reference of rows with a weight past 2^12 to 2^4 below their largest score.
+    auto refer = [&](int j, const floatx16 (&s)[2]) {
+        float t = -INFINITY;
+        const int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = s[n2][i] * lds.s[j & 1][32 * h + 16 * n2 + i];
+                if (32 * n2 + 8 * (i / 4) + i % 4 <= seen) t = fmaxf(t, x);
+            }
+        t = halves_max(t);
+        const float mn = fmaxf(m_run, t - kRefLog2);
+        const float alpha = fast_exp2(m_run - mn);
+        l_part *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db] *= alpha;
+        m_run = mn;
+    };
+    auto pv = [&](int j, const half8 (&w)[4]) {
+        const f16* Vt = lds.v[j & 1];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) {
+                const f16* q = &Vt[vro[db] + 16 * t * D];
+                o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    cat_half8(lds_read_tr16(q), lds_read_tr16(q + 8 * D)), w[t], o[db], 0, 0, 0);
+            }
+    };
+
+    // ---- the pipeline: iteration j works on tile j, converts the codes of tile j + 1 and asks
+    // for those of j + 2
+    Raw rk, rv;
+    uint32_t rs;      // K's numbers of the tile whose V is in rv
+    int pid;          // page to ask for next
+    auto ask_k = [&](int pid) { rk = load_raw(pid, false); };
+    auto ask_v = [&](int pid) {
+        rv = load_raw(pid, true);
+        rs = *reinterpret_cast<const uint32_t*>(head + (int64_t)pid * PB + kPage * D + 4 * (crow & 15));
+    };
+    // without BOTH, half a wave's lanes have K's chunk in rk and the other half V's in rv
+    auto put_k = [&](int t) {
+        if (BOTH || !is_v) convert(t, rk, false, lds.k[t & 1]);
+    };
+    auto put_v = [&](int t) {
+        if (BOTH || is_v) {
+            convert(t, rv, true, lds.v[t & 1]);
+            put_scale(t, rv.sr, true);
+            put_scale(t, rs, false);
+        }
+    };
+    {
+        const int p0 = page_of(0), p1 = page_of(1);
+        pid = page_of(2);
+        ask_k(p0);
+        ask_v(p0);
+        put_k(0);
+        put_v(0);
+        ask_k(p1);
+        ask_v(p1);
+    }
+    auto iterate = [&](auto LAST_, int j) {
+        constexpr bool LAST = decltype(LAST_)::value;
+        __syncthreads();
+        floatx16 s[2];
+        half8 w[4];
+        float sum;
+        qk(j, s);
+        float most = weights(j, s, w, sum);
+        if (__builtin_amdgcn_read_exec() & __ballot(most > kMostWeight)) {
+            refer(j, s);
+            weights(j, s, w, sum);
+        }
+        l_part += sum;
+        pv(j, w);
+        if constexpr (!LAST) {
+            put_k(j + 1);
+            put_v(j + 1);
+            ask_k(pid);
+            ask_v(pid);
+            pid = page_of(j + 3);
+        }
+    };
+    for (int j = 0; j + 1 < n; ++j) iterate(std::false_type{}, j);
+    iterate(std::true_type{}, n - 1);
+    if (!live) return;
+
+    // Dims of a lane: 32 db + 8 q + (0 4 1 5 for h = 0, 2 6 3 7 for h = 1).
+    const float l = halves_sum(l_part);
+    const int d0 = 2 * h;
+    if (all_tiles > p.tiles_per_split) {   // joined by q4_prefill_join_kernel
+        const int64_t prow = at * p.nsplit + blockIdx.z;
+        float* po = p.ws_o + prow * D + d0;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                *reinterpret_cast<float2*>(po + 32 * db + 8 * q4) = float2{o[db][4 * q4], o[db][4 * q4 + 2]};
+                *reinterpret_cast<float2*>(po + 32 * db + 8 * q4 + 4) = float2{o[db][4 * q4 + 1], o[db][4 * q4 + 3]};
+            }
+        if (h == 0) {
+            p.ws_ml[prow * 2] = m_run;
+            p.ws_ml[prow * 2 + 1] = l;
+        }
+        return;
+    }
+    const float inv = 1.f / l;
+    f16* orow = a.out + at * D + d0;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const half2v x = {static_cast<f16>(o[db][4 * q4] * inv), static_cast<f16>(o[db][4 * q4 + 2] * inv)};
+            const half2v y = {static_cast<f16>(o[db][4 * q4 + 1] * inv), static_cast<f16>(o[db][4 * q4 + 3] * inv)};
+            *reinterpret_cast<half2v*>(orow + 32 * db + 8 * q4) = x;
+            *reinterpret_cast<half2v*>(orow + 32 * db + 8 * q4 + 4) = y;
+        }
+    if (a.lse && h == 0)
+        a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m_run + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Joins the partials of the blocks that were cut into ranges of keys: R times D / 8 lanes per
+// (row, head), lane (r, c) taking dims 8c .. of every R-th range.
+template <int D, int R>
+__global__ void __launch_bounds__(256) q4_prefill_join_kernel(const Q4Args a, const PrefillPlan p, int pairs) {
+    constexpr int LPR = D / 8;
+    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR % R;
+    const int b = blockIdx.y;
+    const uint32_t i = blockIdx.x * (256 / LPR / R) + threadIdx.x / (LPR * R);
+    const int row = static_cast<int>(i / a.Hq), qh = static_cast<int>(i % a.Hq);
+    if (row >= a.rows) return;
+    const Block k = block_of(a, p, b, (row * a.G + qh - row_of(p, qh) * a.G) / pairs, pairs);
+    const int64_t pos = (int64_t)k.first + row;
+    if (pos < k.p_lo || pos > k.p_hi) return;
+    const int tiles = k.tiles();
+    if (tiles <= p.tiles_per_split) return;
+    const int n = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+    const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
+    const float* po = p.ws_o + at * p.nsplit * D + 8 * c;
+    const float2* pml = reinterpret_cast<const float2*>(p.ws_ml) + at * p.nsplit;
+    float M = -3.0e38f, L = 0.f;
+    floatx4 o0 = {0.f, 0.f, 0.f, 0.f}, o1 = o0;
+    auto fold = [&](float m, float l, floatx4 x0, floatx4 x1) {
+        const float mn = fmaxf(M, m);
+        const float al = fast_exp2(M - mn), be = fast_exp2(m - mn);
+        o0 = o0 * al + x0 * be;
+        o1 = o1 * al + x1 * be;
+        L = fmaf(L, al, l * be);
+        M = mn;
+    };
+    constexpr int U = 4;   // ranges in flight
+    for (int j0 = r; j0 < n; j0 += U * R) {
+        float2 ml[U];
+        floatx4 x[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = min(j0 + R * u, n - 1);
+            ml[u] = pml[j];
+            x[u][0] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D);
+            x[u][1] = *reinterpret_cast<const floatx4*>(po + (int64_t)j * D + 4);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j0 + R * u < n) fold(ml[u].x, ml[u].y, x[u][0], x[u][1]);
+    }
+#pragma unroll
+    for (int s = LPR; s < LPR * R; s <<= 1) {
+        floatx4 x0, x1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x0[e] = __shfl_xor(o0[e], s);
+            x1[e] = __shfl_xor(o1[e], s);
+        }
+        const float m = __shfl_xor(M, s), l = __shfl_xor(L, s);
+        fold(m, l, x0, x1);
+    }
+    if (r > 0) return;
+    const float inv = 1.f / L;
+    half8 hv;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hv[e] = static_cast<f16>(o0[e] * inv);
+        hv[4 + e] = static_cast<f16>(o1[e] * inv);
+    }
+    store_half8(a.out + at * D + 8 * c, hv);
+    if (a.lse && c == 0)
+        a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
+}
+
+constexpr int kWaves = 4;
+constexpr int kPairs = 32 * kWaves;
+
+// Ranges of keys until every CU has two workgroups, each of at least 3 tiles.
+PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len) {
+    PrefillPlan p{};
+    const int64_t pairs = (int64_t)rows * G;
+    const int64_t wgs = (pairs + kPairs - 1) / kPairs * hkv * batch;
+    p.inv_g = G == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + G - 1) / G);
+    p.blocks = static_cast<int>((pairs + kPairs - 1) / kPairs);
+    const int64_t tiles = ((int64_t)max_len + kBN - 1) / kBN;
+    const int64_t n = std::max<int64_t>(std::min<int64_t>(2 * kCUs / wgs, tiles / 3), 1);
+    p.tiles_per_split = static_cast<int>((tiles + n - 1) / n);
+    p.nsplit = static_cast<int>((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+    return p;
+}
+
+}  // namespace
+
+size_t q4_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int max_len) {
+    if (rows <= 0 || !bound_sizes(batch, hq, hkv, max_len, 0, 0) ||
+        (int64_t)rows * hq > kMaxRowHeads || (d != 64 && d != 128))
+        return 0;
+    const PrefillPlan p = plan_of(batch, rows, hkv, hq / hkv, max_len);
+    return p.nsplit == 1 ? 0 : sizeof(float) * (size_t)batch * rows * hq * p.nsplit * (d + 2);
+}
+
+bool q4_prefill_fits(const Q4Args& a, int batch) {
+    if ((int64_t)a.rows * a.Hq > kMaxRowHeads) return false;   // the plan counts them in an int
+    const PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len);
+    return (a.D == 64 || a.D == 128) && aligned16(a.q) && aligned16(a.out) && p.nsplit <= 65535 &&
+           (int64_t)p.blocks * a.Hkv <= kMaxRowHeads / kPairs &&
+           (int64_t)a.rows * a.G * a.G < (int64_t)1 << 31;   // row_of, and pairs in an int
+}
+
+// The workspace holds q4_prefill_workspace bytes.
+int q4_prefill(const Q4Args& a, int batch, void* ws, hipStream_t s) {
+    PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len);
+    const size_t rh = (size_t)batch * a.rows * a.Hq;
+    p.ws_o = static_cast<float*>(ws);
+    p.ws_ml = p.ws_o + rh * p.nsplit * a.D;
+    const dim3 grid(p.blocks * a.Hkv, batch, p.nsplit), threads(kWaves * kWave);
+    if (a.D == 64)
+        hipLaunchKernelGGL((q4_prefill_kernel<64, kWaves>), grid, threads, 0, s, a, p);
+    else
+        hipLaunchKernelGGL((q4_prefill_kernel<128, kWaves>), grid, threads, 0, s, a, p);
+    const int rc = check_launch("q4_prefill");
+    if (rc || p.nsplit == 1) return rc;
+    // A wave per (row, head) while they all run at once, D / 8 lanes above.
+    const int64_t heads = (int64_t)batch * a.rows * a.Hq;   // rows Hq <= 2^29
+    auto join = [&](auto kernel, int lanes) {
+        const unsigned per = 256 / lanes;
+        hipLaunchKernelGGL(kernel, dim3((static_cast<unsigned>(a.rows) * a.Hq + per - 1) / per, batch),
+                           dim3(256), 0, s, a, p, kPairs);
+    };
+    if (a.D == 64)
+        heads <= 32 * kCUs ? join(q4_prefill_join_kernel<64, 8>, 64) : join(q4_prefill_join_kernel<64, 1>, 8);
+    else
+        heads <= 32 * kCUs ? join(q4_prefill_join_kernel<128, 4>, 64) : join(q4_prefill_join_kernel<128, 1>, 16);
+    return check_launch("q4_prefill (join)");
+}
+
+}  // namespace kvhp
