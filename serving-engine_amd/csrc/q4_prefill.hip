@@ -17,8 +17,8 @@
 // 2^4), seen from the weights themselves, so that no maximum of the scores is needed: 2^-11 of
 // each holds down to 2^-16 of the reference, below it is an absolute 2^-27 of it.
 //
-// A row that holds NaN has operands of 0 and a scale of NaN, so it reaches the rows that see
-// it and, their weights' place being 0, no others.
+// A key that holds NaN has operands of 0.  K's scale is NaN, which a row that does not see the
+// key drops with its weight; of V's the first is kept, and the rows at or past it are NaN.
 //
 // Few rows over a long cache are cut into ranges of keys (blockIdx.z) whose partials a second
 // launch joins.
@@ -91,12 +91,23 @@ __device__ __forceinline__ half8 operand(uint32_t x, half2v e, half2v f, const C
     return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-// A tile's (s log2(e) / sqrt(D), m) in the order a lane of half h takes them: [h][32 keys].
+// Operands of K and V in two stages each, as multiples of 8 KB in LDS (an operand's place in a
+// row is then an exclusive or with its address), and a tile's s log2(e) / sqrt(D) and m in the
+// order a lane of half h takes them: [h][32 keys].
 template <int D>
-struct __attribute__((aligned(16))) Tiles {
+struct __attribute__((aligned(8192))) Tiles {
     f16 k[2][kBN * D], v[2][kBN * D];
     float s[2][kBN], m[2][kBN];
+    int bad;   // first key whose V is NaN
 };
+
+template <typename T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) T*>(at);
+}
+__device__ __forceinline__ short4v lds_tr16(uint32_t at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_short4v*>(at));
+}
 
 template <int D, int W>
 __global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
@@ -163,7 +174,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     auto convert = [&](int t, const Raw& w, bool v, f16* tile) {
         uint32_t sr = w.sr;
         if ((t_lo + t) * kBN + crow > k.p_hi) sr = 0;              // behind the last key
-        if ((sr & 0x7c00u) == 0x7c00u) sr = 0;                     // NaN: the scale tells
+        if ((sr & 0x7c00u) == 0x7c00u) sr = 0;                     // NaN: told apart by put_scale
         const int e = v ? max((int)(sr & 0x7c00u) - 0x0800, 0x0400) : 0x3c00;
         const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
         const f16 fh = (as_half2(sr)[1] - f16(16)) * eh;
@@ -178,7 +189,12 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     auto put_scale = [&](int t, uint32_t sr, bool v) {
         if (cc != 0) return;
         if (v) {
-            if ((t_lo + t) * kBN + crow > k.p_hi) sr = 0;
+            const int key = (t_lo + t) * kBN + crow;
+            if (key > k.p_hi) sr = 0;
+            if ((sr & 0x7c00u) == 0x7c00u) {
+                sr = 0;
+                atomicMin(&lds.bad, key);
+            }
             const int e = max((int)(sr & 0x7c00u) - 0x0800, 0x0400);
             lds.m[t & 1][sat] = static_cast<float>(as_half2(sr)[0]) *
                                 static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
@@ -187,17 +203,14 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         }
     };
 
-    // ---- operand reads
-    int kro[NC], vro[NDB];
+    // ---- operand reads: K's chunk 2 c + h of row c32 (and 32), V's of 32-dim block db
+    constexpr uint32_t TB = 2 * kBN * D;   // bytes of a stage
+    const uint32_t lds0 = lds_at(&lds);
+    const uint32_t kat = lds0 + 2 * c32 * D + 16 * (h ^ kswz<D>(c32));
+    uint32_t vat;
     {
-        const int j16 = lane & 15, blk2 = lane >> 4 & 1;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) kro[c] = c32 * D + 8 * ((2 * c + h) ^ kswz<D>(c32));
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-            const int r = 4 * h + j16 / 4;
-            vro[db] = r * D + 8 * ((4 * db + 2 * blk2 + ((j16 & 3) >> 1)) ^ vswz<D>(r)) + 4 * (j16 & 1);
-        }
+        const int j16 = lane & 15, r = 4 * h + j16 / 4;
+        vat = lds0 + 2 * TB + 2 * r * D + 16 * ((2 * (lane >> 4 & 1) + ((j16 & 3) >> 1)) ^ vswz<D>(r)) + 8 * (j16 & 1);
     }
     floatx16 o[NDB];
 #pragma unroll
@@ -207,7 +220,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     float m_run = -1e30f, l_part = 0.f;
 
     auto qk = [&](int j, floatx16 (&s)[2]) {
-        const f16* Kt = lds.k[j & 1];
+        const uint32_t Kt = kat + (j & 1) * TB;
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2)
 #pragma unroll
@@ -217,46 +230,38 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
 #pragma unroll
             for (int n2 = 0; n2 < 2; ++n2)
                 s[n2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    *reinterpret_cast<const half8*>(&Kt[kro[c] + 32 * n2 * D]), qop[c], s[n2], 0, 0, 0);
+                    lds_read<half8>((Kt ^ 32 * c) + 64 * n2 * D), qop[c], s[n2], 0, 0, 0);
     };
     // Weights of tile j as the operands of O^T's product; element (n, i) is key 32 n + 8 (i / 4)
     // + 4 h + i % 4.  Returns the largest and adds up the sum before the rounding.
-    auto weights = [&](int j, const floatx16 (&s)[2], half8 (&w)[4], float& sum) {
+    auto weights = [&](auto MASKED_, int j, const floatx16 (&s)[2], half8 (&w)[4], float& sum) {
+        constexpr bool MASKED = decltype(MASKED_)::value;
         float most = 0.f, ps[2] = {0.f, 0.f};
-        const bool masked = t_lo + j >= past;
-        const int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+        int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+        asm volatile("" : "+v"(seen));   // compared where it is used: 32 kept masks would spill
+        const float* ks = &lds.s[j & 1][32 * h];
+        const float* vm = &lds.m[j & 1][32 * h];
 #pragma unroll
-        for (int n2 = 0; n2 < 2; ++n2)
+        for (int i = 0; i < 32; i += 4) {
+            const floatx4 k4 = *reinterpret_cast<const floatx4*>(ks + i);
+            const floatx4 m4 = *reinterpret_cast<const floatx4*>(vm + i);
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const floatx4 ks = *reinterpret_cast<const floatx4*>(&lds.s[j & 1][32 * h + 16 * n2 + 4 * q4]);
-                const floatx4 vm = *reinterpret_cast<const floatx4*>(&lds.m[j & 1][32 * h + 16 * n2 + 4 * q4]);
-                float x[4], y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] = fast_exp2(fmaf(s[n2][4 * q4 + e], ks[e], -m_run));
-                    y[e] = x[e] * vm[e];
-                }
-                if (masked) {
-                    asm volatile("");   // a branch: no selects in every tile
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (32 * n2 + 8 * q4 + e > seen) x[e] = y[e] = 0.f;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[2 * n2 + q4 / 2][4 * (q4 & 1) + e] = static_cast<f16>(y[e]);
-                    most = fmaxf(most, x[e]);
-                    ps[e & 1] += x[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                float x = fast_exp2(fmaf(s[i / 16][i % 16 + e], k4[e], -m_run));
+                if (MASKED && 2 * i + e > seen) x = 0.f;
+                w[i / 8][i % 8 + e] = static_cast<f16>(x * m4[e]);
+                most = fmaxf(most, x);
+                ps[e & 1] += x;
             }
+        }
         sum = ps[0] + ps[1];
         return most;
     };
     // Moves the reference of rows with a weight past 2^12 to 2^4 below their largest score.
     auto refer = [&](int j, const floatx16 (&s)[2]) {
         float t = -INFINITY;
-        const int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+        int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+        asm volatile("" : "+v"(seen));
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2)
 #pragma unroll
@@ -273,14 +278,14 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         m_run = mn;
     };
     auto pv = [&](int j, const half8 (&w)[4]) {
-        const f16* Vt = lds.v[j & 1];
+        const uint32_t Vt = vat + (j & 1) * TB;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int db = 0; db < NDB; ++db) {
-                const f16* q = &Vt[vro[db] + 16 * t * D];
+                const uint32_t q = (Vt ^ 64 * db) + 32 * t * D;
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    cat_half8(lds_read_tr16(q), lds_read_tr16(q + 8 * D)), w[t], o[db], 0, 0, 0);
+                    cat_half8(lds_tr16(q), lds_tr16(q + 16 * D)), w[t], o[db], 0, 0, 0);
             }
     };
 
@@ -305,6 +310,8 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
             put_scale(t, rs, false);
         }
     };
+    if (threadIdx.x == 0) lds.bad = INT32_MAX;
+    __syncthreads();
     {
         const int p0 = page_of(0), p1 = page_of(1);
         pid = page_of(2);
@@ -322,11 +329,14 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         half8 w[4];
         float sum;
         qk(j, s);
-        float most = weights(j, s, w, sum);
+        __builtin_amdgcn_sched_barrier(0);
+        const float most = t_lo + j >= past ? weights(std::true_type{}, j, s, w, sum)
+                                            : weights(std::false_type{}, j, s, w, sum);
         if (__builtin_amdgcn_read_exec() & __ballot(most > kMostWeight)) {
-            refer(j, s);
-            weights(j, s, w, sum);
+            refer(j, s);   // now none is past 2^4
+            weights(std::true_type{}, j, s, w, sum);
         }
+        __builtin_amdgcn_sched_barrier(0);
         l_part += sum;
         pv(j, w);
         if constexpr (!LAST) {
@@ -340,6 +350,12 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     for (int j = 0; j + 1 < n; ++j) iterate(std::false_type{}, j);
     iterate(std::true_type{}, n - 1);
     if (!live) return;
+    if (pos >= lds.bad) {   // no writes since the last barrier
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] = NAN;
+    }
 
     // Dims of a lane: 32 db + 8 q + (0 4 1 5 for h = 0, 2 6 3 7 for h = 1).
     const float l = halves_sum(l_part);
