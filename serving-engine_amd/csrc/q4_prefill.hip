@@ -91,16 +91,6 @@ __device__ __forceinline__ half8 operand(uint32_t x, half2v e, half2v f, const C
     return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-// Operands of K and V in two stages each, as multiples of 8 KB in LDS (an operand's place in a
-// row is then an exclusive or with its address), and a tile's s log2(e) / sqrt(D) and m in the
-// order a lane of half h takes them: [h][32 keys].
-template <int D>
-struct __attribute__((aligned(8192))) Tiles {
-    f16 k[2][kBN * D], v[2][kBN * D];
-    float s[2][kBN], m[2][kBN];
-    int bad;   // first key whose V is NaN
-};
-
 template <typename T>
 __device__ __forceinline__ T lds_read(uint32_t at) {
     return *reinterpret_cast<const __attribute__((address_space(3))) T*>(at);
@@ -109,21 +99,46 @@ __device__ __forceinline__ short4v lds_tr16(uint32_t at) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_short4v*>(at));
 }
 
-template <int D, int W>
-__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
+// global_load_lds_dwordx4 to LDS offset `to`, from a wave-uniform base and the lane's offset.
+__device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(to), "v"(voff), "s"(base) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_raw() {   // all but N loads have landed, and reads of LDS returned
+    wait_ring<N>();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void reads_done() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+}
+
+constexpr int kWaves = 4;             // each converts one page of a tile
+constexpr int kPairs = 32 * kWaves;   // (row, head) pairs per workgroup
+static_assert(kBN == kWaves * kPage, "a page per wave");
+
+template <int D>
+__global__ void __launch_bounds__(kWaves * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
-    constexpr int NC = D / 16, NDB = D / 32, RB = D / 2, PB = q4_page_bytes(D), PAIRS = 32 * W;
-    // 16-byte chunks of codes: a thread has one of K and one of V, or half a wave has K's
-    constexpr int BOTH = D / (16 * W) == 2;
-    static_assert(BOTH || D == 16 * W, "one or two chunks a thread");
-    __shared__ Tiles<D> lds;
+    constexpr int NC = D / 16, NDB = D / 32, RB = D / 2, PB = q4_page_bytes(D);
+    constexpr uint32_t TB = 2 * kBN * D;   // bytes of a stage of operands
+    constexpr int RAW = 2 * kPage * RB + 128;   // a page as it is in the pool, per wave
+    constexpr int RST = D == 128 ? 1 : 2;       // stages of those
+    // K's operands in two stages, then V's: multiples of 8 KB in LDS, so that an operand's place in
+    // its row is an exclusive or with its address
+    __shared__ __attribute__((aligned(8192))) f16 tiles[4 * kBN * D];
+    __shared__ __attribute__((aligned(16))) uint8_t raw[kWaves][RST][RAW];
+    // a tile's s log2(e) / sqrt(D) and m in the order a lane of half h takes them: [h][32 keys]
+    __shared__ __attribute__((aligned(16))) float scale_s[2][kBN], scale_m[2][kBN];
+    __shared__ int bad;                    // first key whose V is NaN
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int h = lane >> 5, c32 = lane & 31;
     const int kvh = blockIdx.x % a.Hkv;
     const int blk = p.blocks - 1 - static_cast<int>(blockIdx.x / a.Hkv);   // longest first
     const int b = blockIdx.y;
-    const Block k = block_of(a, p, b, blk, PAIRS);
+    const Block k = block_of(a, p, b, blk, kPairs);
     if (k.p_lo > k.p_hi) return;
     const int t_lo = static_cast<int>(blockIdx.z) * p.tiles_per_split;
     const int all_tiles = k.tiles();
@@ -131,13 +146,14 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     if (n <= 0) return;
 
     // This lane's pair.
-    const int pair0 = blk * PAIRS + 32 * wave, pair = pair0 + c32;
+    const int pair0 = blk * kPairs + 32 * wave, pair = pair0 + c32;
     const int row = row_of(p, pair), qh = kvh * a.G + pair - row * a.G, pos = k.first + row;
     const bool live = row < a.rows && pos >= k.p_lo && pos <= k.p_hi;
     const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
-    // tiles (of the block's) from `past` on hold keys that some pair of the wave does not see
+    // halves of tiles from `past` on (of the range's) hold keys that some pair of the wave does not see
     const int lo = k.first + row_of(p, pair0), hi = k.first + row_of(p, pair0 + 31);
-    const int past = lo < k.p_lo || hi > k.p_hi || lo < kBN - 1 ? 0 : (lo - (kBN - 1)) / kBN + 1;
+    const int past = (lo < k.p_lo || hi > k.p_hi || lo < 31 ? 0 : (lo - 31) / 32 + 1) - 2 * t_lo;
+    const int seen0 = live ? pos - t_lo * kBN - 4 * h : -1;
     half8 qop[NC];   // in the codes' order
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -145,67 +161,80 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         qop[c] = __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
     }
 
-    // ---- codes to operands: this thread's row of a tile, and its 32 dims of it
-    constexpr int CPR = RB / 16;                       // chunks of codes in a row
-    constexpr int TPW = kBN / W;                       // rows of a wave, in one page
-    const int item = BOTH ? lane : lane & 31;
-    const int crow = TPW * wave + item / CPR, cc = item % CPR;
-    const bool is_v = !BOTH && h == 1;                 // what the first chunk is
+    // ---- codes: a wave loads its page of each tile and converts it, a lane D / 4 dims of a row
+    const int crow = lane >> 2, cc = lane & 3;
+    const int key0 = t_lo * kBN + kPage * wave + crow;   // in the range's first tile
     const int32_t* bt = a.bt + (int64_t)b * a.max_pages;
     const uint8_t* head = a.pool + (int64_t)kvh * a.num_pages * PB;
     const int last_page = k.p_hi >> 4;
-    auto page_of = [&](int t) {   // of this wave's rows of a tile: ids are clamped into the pool
-        const int pi = min((t_lo + min(t, n - 1)) * (kBN / kPage) + TPW * wave / kPage, last_page);
-        return min(max(bt[pi], 0), a.num_pages - 1);
+    auto page_of = [&](int t) {   // ids are clamped into the pool
+        const int pi = min((t_lo + min(t, n - 1)) * kWaves + wave, last_page);
+        return __builtin_amdgcn_readfirstlane(min(max(bt[pi], 0), a.num_pages - 1));
     };
-    struct Raw {
-        u32x4 x;       // codes
-        uint32_t sr;   // their row's numbers
-    };
-    auto load_raw = [&](int pid, bool v) {
+    const uint8_t* const raw0 = raw[wave][0];
+    const uint32_t raw_at = __builtin_amdgcn_readfirstlane(lds_at(raw0));
+    // D = 128: K's codes and the numbers, then V's codes; D = 64: all at once, to a stage of its own
+    auto ask_k = [&](int t, int pid) {
         const uint8_t* pg = head + (int64_t)pid * PB;
-        const int r = crow & 15;
-        Raw w;
-        w.x = *reinterpret_cast<const u32x4*>(pg + (v ? kPage * RB : 0) + r * RB + 16 * cc);
-        w.sr = *reinterpret_cast<const uint32_t*>(pg + kPage * D + (v ? 4 * kPage : 0) + 4 * r);
-        return w;
+        const uint32_t to = raw_at + (RST == 2 ? (t & 1) * RAW : 0);
+        dma16(pg, 16 * lane, to);
+        if (lane < 8) dma16(pg, kPage * D + 16 * lane, to + 2 * kPage * RB);
+    };
+    auto ask_v = [&](int pid) {
+        if constexpr (D == 128) dma16(head + (int64_t)pid * PB, 1024 + 16 * lane, raw_at + 1024);
     };
     const CodeBits bits;
-    auto convert = [&](int t, const Raw& w, bool v, f16* tile) {
-        uint32_t sr = w.sr;
-        if ((t_lo + t) * kBN + crow > k.p_hi) sr = 0;              // behind the last key
-        if ((sr & 0x7c00u) == 0x7c00u) sr = 0;                     // NaN: told apart by put_scale
-        const int e = v ? max((int)(sr & 0x7c00u) - 0x0800, 0x0400) : 0x3c00;
-        const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
-        const f16 fh = (as_half2(sr)[1] - f16(16)) * eh;
-        const half2v e2 = {eh, eh}, f2 = {fh, fh};
-        const int swz = v ? vswz<D>(crow) : kswz<D>(crow);
+    const uint32_t lds0 = lds_at(tiles);
+    const uint32_t kput = 2 * ((kPage * wave + crow) * D) + 16 * ((D / 32 * cc) ^ kswz<D>(kPage * wave + crow));
+    const uint32_t vput = 2 * ((kPage * wave + crow) * D) + 16 * ((D / 32 * cc) ^ vswz<D>(kPage * wave + crow));
+    auto convert = [&](const uint8_t* codes, half2v e2, half2v f2, uint32_t to) {
+        uint32_t x[D / 32];
+        if constexpr (D == 128) {
+            const u32x4 y = *reinterpret_cast<const u32x4*>(codes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            store_half8(tile + crow * D + 8 * ((4 * cc + i) ^ swz), operand(w.x[i], e2, f2, bits));
-    };
-    // A row's s and m, by one of its threads: key 32 n + 8 q + 4 h + e to [h][16 n + 4 q + e].
-    const int sat = 32 * (crow >> 2 & 1) + 16 * (crow >> 5) + 4 * (crow >> 3 & 3) + (crow & 3);
-    auto put_scale = [&](int t, uint32_t sr, bool v) {
-        if (cc != 0) return;
-        if (v) {
-            const int key = (t_lo + t) * kBN + crow;
-            if (key > k.p_hi) sr = 0;
-            if ((sr & 0x7c00u) == 0x7c00u) {
-                sr = 0;
-                atomicMin(&lds.bad, key);
-            }
-            const int e = max((int)(sr & 0x7c00u) - 0x0800, 0x0400);
-            lds.m[t & 1][sat] = static_cast<float>(as_half2(sr)[0]) *
-                                static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
+            for (int i = 0; i < 4; ++i) x[i] = y[i];
         } else {
-            lds.s[t & 1][sat] = static_cast<float>(as_half2(sr)[0]) * a.scale_log2;
+            const uint2 y = *reinterpret_cast<const uint2*>(codes);
+            x[0] = y.x;
+            x[1] = y.y;
         }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+            *reinterpret_cast<__attribute__((address_space(3))) half8*>(to ^ 16 * i) = operand(x[i], e2, f2, bits);
+    };
+    // This lane's row of a tile's V: E and (r - 16) E, kept from the numbers' read to the codes'.
+    half2v v_e, v_f;
+    // A row's s and m: key 32 n + 8 q + 4 h + e to [h][16 n + 4 q + e].
+    const int srow = kPage * wave + crow;
+    const int sat = 32 * (srow >> 2 & 1) + 16 * (srow >> 5) + 4 * (srow >> 3 & 3) + (srow & 3);
+    auto put_k = [&](int t) {
+        const uint8_t* r0 = raw0 + (RST == 2 ? (t & 1) * RAW : 0);
+        const uint8_t* num = r0 + 2 * kPage * RB + 4 * crow;
+        uint32_t ks = *reinterpret_cast<const uint32_t*>(num), vs = *reinterpret_cast<const uint32_t*>(num + 64);
+        const bool behind = key0 + t * kBN > k.p_hi;   // the last key
+        if (cc == 0) scale_s[t & 1][sat] = static_cast<float>(as_half2(ks)[0]) * a.scale_log2;
+        // of NaN and of what is behind the last key: operands of 0
+        ks = behind || (ks & 0x7c00u) == 0x7c00u ? 0u : ks;
+        const bool nan = !behind && (vs & 0x7c00u) == 0x7c00u;
+        vs = behind || nan ? 0u : vs;
+        const int e = max((int)(vs & 0x7c00u) - 0x0800, 0x0400);
+        if (cc == 0) {
+            scale_m[t & 1][sat] = static_cast<float>(as_half2(vs)[0]) *
+                                  static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
+            if (nan) atomicMin(&bad, key0 + t * kBN);
+        }
+        const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
+        v_e = half2v{eh, eh};
+        v_f = (half2v{as_half2(vs)[1], as_half2(vs)[1]} + half2v{f16(-16), f16(-16)}) * v_e;
+        const half2v k_f = half2v{as_half2(ks)[1], as_half2(ks)[1]} + half2v{f16(-16), f16(-16)};
+        convert(r0 + RB / 4 * lane, half2v{f16(1), f16(1)}, k_f, lds0 + (t & 1) * TB + kput);
+    };
+    auto put_v = [&](int t) {
+        convert(raw0 + (RST == 2 ? (t & 1) * RAW : 0) + kPage * RB + RB / 4 * lane, v_e, v_f,
+                lds0 + (2 + (t & 1)) * TB + vput);
     };
 
     // ---- operand reads: K's chunk 2 c + h of row c32 (and 32), V's of 32-dim block db
-    constexpr uint32_t TB = 2 * kBN * D;   // bytes of a stage
-    const uint32_t lds0 = lds_at(&lds);
     const uint32_t kat = lds0 + 2 * c32 * D + 16 * (h ^ kswz<D>(c32));
     uint32_t vat;
     {
@@ -219,35 +248,31 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
     float m_run = -1e30f, l_part = 0.f;
 
-    auto qk = [&](int j, floatx16 (&s)[2]) {
+    // Scores of half u of tile j: element i is key 32 u + 8 (i / 4) + 4 h + i % 4.
+    auto qk = [&](int j, int u) {
         const uint32_t Kt = kat + (j & 1) * TB;
-#pragma unroll
-        for (int n2 = 0; n2 < 2; ++n2)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[n2][e] = 0.f;
+        floatx16 s = {};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int n2 = 0; n2 < 2; ++n2)
-                s[n2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    lds_read<half8>((Kt ^ 32 * c) + 64 * n2 * D), qop[c], s[n2], 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_read<half8>((Kt ^ 32 * c) + 64 * u * D), qop[c], s, 0, 0, 0);
+        return s;
     };
-    // Weights of tile j as the operands of O^T's product; element (n, i) is key 32 n + 8 (i / 4)
-    // + 4 h + i % 4.  Returns the largest and adds up the sum before the rounding.
-    auto weights = [&](auto MASKED_, int j, const floatx16 (&s)[2], half8 (&w)[4], float& sum) {
+    // Weights as the operands of O^T's product; returns the largest and adds up the sum before
+    // the rounding.
+    auto weights = [&](auto MASKED_, int j, int u, const floatx16& s, half8 (&w)[2], float& sum) {
         constexpr bool MASKED = decltype(MASKED_)::value;
         float most = 0.f, ps[2] = {0.f, 0.f};
-        int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
-        asm volatile("" : "+v"(seen));   // compared where it is used: 32 kept masks would spill
-        const float* ks = &lds.s[j & 1][32 * h];
-        const float* vm = &lds.m[j & 1][32 * h];
+        int seen = seen0 - j * kBN - 32 * u;
+        asm volatile("" : "+v"(seen));   // compared where it is used: kept masks would spill
+        const float* ks = &scale_s[j & 1][32 * h + 16 * u];
+        const float* vm = &scale_m[j & 1][32 * h + 16 * u];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
+        for (int i = 0; i < 16; i += 4) {
             const floatx4 k4 = *reinterpret_cast<const floatx4*>(ks + i);
             const floatx4 m4 = *reinterpret_cast<const floatx4*>(vm + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = fast_exp2(fmaf(s[i / 16][i % 16 + e], k4[e], -m_run));
+                float x = fast_exp2(fmaf(s[i + e], k4[e], -m_run));
                 if (MASKED && 2 * i + e > seen) x = 0.f;
                 w[i / 8][i % 8 + e] = static_cast<f16>(x * m4[e]);
                 most = fmaxf(most, x);
@@ -258,17 +283,15 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         return most;
     };
     // Moves the reference of rows with a weight past 2^12 to 2^4 below their largest score.
-    auto refer = [&](int j, const floatx16 (&s)[2]) {
+    auto refer = [&](int j, int u, const floatx16& s) {
         float t = -INFINITY;
-        int seen = live ? pos - (t_lo + j) * kBN - 4 * h : -1;
+        int seen = seen0 - j * kBN - 32 * u;
         asm volatile("" : "+v"(seen));
 #pragma unroll
-        for (int n2 = 0; n2 < 2; ++n2)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = s[n2][i] * lds.s[j & 1][32 * h + 16 * n2 + i];
-                if (32 * n2 + 8 * (i / 4) + i % 4 <= seen) t = fmaxf(t, x);
-            }
+        for (int i = 0; i < 16; ++i) {
+            const float x = s[i] * scale_s[j & 1][32 * h + 16 * u + i];
+            if (8 * (i / 4) + i % 4 <= seen) t = fmaxf(t, x);
+        }
         t = halves_max(t);
         const float mn = fmaxf(m_run, t - kRefLog2);
         const float alpha = fast_exp2(m_run - mn);
@@ -277,10 +300,10 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         for (int db = 0; db < NDB; ++db) o[db] *= alpha;
         m_run = mn;
     };
-    auto pv = [&](int j, const half8 (&w)[4]) {
-        const uint32_t Vt = vat + (j & 1) * TB;
+    auto pv = [&](int j, int u, const half8 (&w)[2]) {
+        const uint32_t Vt = vat + (j & 1) * TB + 64 * u * D;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int db = 0; db < NDB; ++db) {
                 const uint32_t q = (Vt ^ 64 * db) + 32 * t * D;
@@ -288,69 +311,70 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
                     cat_half8(lds_tr16(q), lds_tr16(q + 16 * D)), w[t], o[db], 0, 0, 0);
             }
     };
+    auto checked = [&](int j, int u, float most, const floatx16& s, half8 (&w)[2], float& sum) {
+        if (__builtin_amdgcn_read_exec() & __ballot(most > kMostWeight)) {
+            refer(j, u, s);   // now none is past 2^4
+            weights(std::true_type{}, j, u, s, w, sum);
+        }
+        l_part += sum;
+    };
 
     // ---- the pipeline: iteration j works on tile j, converts the codes of tile j + 1 and asks
-    // for those of j + 2
-    Raw rk, rv;
-    uint32_t rs;      // K's numbers of the tile whose V is in rv
-    int pid;          // page to ask for next
-    auto ask_k = [&](int pid) { rk = load_raw(pid, false); };
-    auto ask_v = [&](int pid) {
-        rv = load_raw(pid, true);
-        rs = *reinterpret_cast<const uint32_t*>(head + (int64_t)pid * PB + kPage * D + 4 * (crow & 15));
-    };
-    // without BOTH, half a wave's lanes have K's chunk in rk and the other half V's in rv
-    auto put_k = [&](int t) {
-        if (BOTH || !is_v) convert(t, rk, false, lds.k[t & 1]);
-    };
-    auto put_v = [&](int t) {
-        if (BOTH || is_v) {
-            convert(t, rv, true, lds.v[t & 1]);
-            put_scale(t, rv.sr, true);
-            put_scale(t, rs, false);
-        }
-    };
-    if (threadIdx.x == 0) lds.bad = INT32_MAX;
-    __syncthreads();
-    {
-        const int p0 = page_of(0), p1 = page_of(1);
-        pid = page_of(2);
-        ask_k(p0);
-        ask_v(p0);
-        put_k(0);
-        put_v(0);
-        ask_k(p1);
-        ask_v(p1);
-    }
+    // for those of j + 2: S of the first half beside K's conversion, S of the second beside the
+    // first's weights, O of the first beside the second's weights, O of the second beside V's
+    // conversion
+    int pid = page_of(0);
+    if (threadIdx.x == 0) bad = INT32_MAX;
+    wait_raw<0>();
+    ask_k(0, pid);
+    ask_v(pid);
+    pid = page_of(1);
+    __syncthreads();   // bad
+    wait_raw<0>();
+    put_k(0);
+    put_v(0);
+    reads_done();
+    ask_k(1, pid);
+    ask_v(pid);
+    pid = page_of(2);
     auto iterate = [&](auto LAST_, int j) {
         constexpr bool LAST = decltype(LAST_)::value;
-        __syncthreads();
-        floatx16 s[2];
-        half8 w[4];
-        float sum;
-        qk(j, s);
-        __builtin_amdgcn_sched_barrier(0);
-        const float most = t_lo + j >= past ? weights(std::true_type{}, j, s, w, sum)
-                                            : weights(std::false_type{}, j, s, w, sum);
-        if (__builtin_amdgcn_read_exec() & __ballot(most > kMostWeight)) {
-            refer(j, s);   // now none is past 2^4
-            weights(std::true_type{}, j, s, w, sum);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        l_part += sum;
-        pv(j, w);
+        reads_done();   // and this wave's writes are in LDS
+        ring_barrier();
+        if constexpr (!LAST && RST == 2) ask_k(j + 2, pid);
+        const floatx16 s0 = qk(j, 0);
         if constexpr (!LAST) {
+            wait_raw<RST == 2 ? 2 : 1>();
             put_k(j + 1);
+            if constexpr (RST == 1) {
+                reads_done();
+                ask_k(j + 2, pid);
+            }
+        }
+        const floatx16 s1 = qk(j, 1);
+        half8 w0[2], w1[2];
+        float sum0, sum1;
+        float most = 2 * j >= past ? weights(std::true_type{}, j, 0, s0, w0, sum0)
+                                   : weights(std::false_type{}, j, 0, s0, w0, sum0);
+        checked(j, 0, most, s0, w0, sum0);
+        pv(j, 0, w0);
+        most = 2 * j + 1 >= past ? weights(std::true_type{}, j, 1, s1, w1, sum1)
+                                 : weights(std::false_type{}, j, 1, s1, w1, sum1);
+        checked(j, 1, most, s1, w1, sum1);
+        pv(j, 1, w1);
+        if constexpr (!LAST) {
+            if constexpr (RST == 1) wait_raw<2>();
             put_v(j + 1);
-            ask_k(pid);
+            reads_done();
             ask_v(pid);
             pid = page_of(j + 3);
         }
     };
     for (int j = 0; j + 1 < n; ++j) iterate(std::false_type{}, j);
+    wait_raw<0>();   // the trailing loads
     iterate(std::true_type{}, n - 1);
     if (!live) return;
-    if (pos >= lds.bad) {   // no writes since the last barrier
+    if (pos >= bad) {   // no writes since the last barrier
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -459,9 +483,6 @@ __global__ void __launch_bounds__(256) q4_prefill_join_kernel(const Q4Args a, co
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
-constexpr int kWaves = 4;
-constexpr int kPairs = 32 * kWaves;
-
 // Ranges of keys until every CU has two workgroups, each of at least 3 tiles.
 PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len) {
     PrefillPlan p{};
@@ -502,9 +523,9 @@ int q4_prefill(const Q4Args& a, int batch, void* ws, hipStream_t s) {
     p.ws_ml = p.ws_o + rh * p.nsplit * a.D;
     const dim3 grid(p.blocks * a.Hkv, batch, p.nsplit), threads(kWaves * kWave);
     if (a.D == 64)
-        hipLaunchKernelGGL((q4_prefill_kernel<64, kWaves>), grid, threads, 0, s, a, p);
+        hipLaunchKernelGGL((q4_prefill_kernel<64>), grid, threads, 0, s, a, p);
     else
-        hipLaunchKernelGGL((q4_prefill_kernel<128, kWaves>), grid, threads, 0, s, a, p);
+        hipLaunchKernelGGL((q4_prefill_kernel<128>), grid, threads, 0, s, a, p);
     const int rc = check_launch("q4_prefill");
     if (rc || p.nsplit == 1) return rc;
     // A wave per (row, head) while they all run at once, D / 8 lanes above.
