@@ -68,12 +68,12 @@ __device__ __forceinline__ Block block_of(const Q4Args& a, const PrefillPlan& p,
 
 // The 16-byte chunks of LDS rows lie at c ^ swizzle(row): the 16 rows of an operand read of K,
 // the four rows x four chunks of a transposing read of V, and the conversion's writes each on
-// distinct banks (V's two by two at D = 128).  V's is the same for rows 8 apart.
+// distinct banks.  V's is the same for rows 8 apart.
 template <int D>
 __device__ __forceinline__ int kswz(int r) { return D == 128 ? r & 15 : r >> 1 & 7; }
 template <int D>
 __device__ __forceinline__ int vswz(int r) {
-    return (D == 128 ? 4 * (r & 3) : (r & 3) << 1) | (r >> 2 & 1);
+    return D == 128 ? 5 * (r & 3) : 2 * (r & 3) + (r >> 1 & 1);
 }
 
 __device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
@@ -104,6 +104,14 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(to), "v"(voff), "s"(base) : "memory", "m0");
 }
+// The same for the first 8 lanes of a whole wave (a branch would part the block that the
+// products and the conversion share).
+__device__ __forceinline__ void dma16_8(const void* base, uint32_t voff, uint32_t to) {
+    uint64_t all;
+    asm volatile("s_mov_b64 %0, exec\n\ts_mov_b64 exec, 0xff\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
+                 : "=&s"(all) : "s"(to), "v"(voff), "s"(base) : "memory", "m0");
+}
 template <int N>
 __device__ __forceinline__ void wait_raw() {   // all but N loads have landed, and reads of LDS returned
     wait_ring<N>();
@@ -119,7 +127,7 @@ constexpr int kPairs = 32 * kWaves;   // (row, head) pairs per workgroup
 static_assert(kBN == kWaves * kPage, "a page per wave");
 
 template <int D>
-__global__ void __launch_bounds__(kWaves * kWave) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(kWaves * kWave) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3)))
 q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     constexpr int NC = D / 16, NDB = D / 32, RB = D / 2, PB = q4_page_bytes(D);
     constexpr uint32_t TB = 2 * kBN * D;   // bytes of a stage of operands
@@ -131,7 +139,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     __shared__ __attribute__((aligned(16))) uint8_t raw[kWaves][RST][RAW];
     // a tile's s log2(e) / sqrt(D) and m in the order a lane of half h takes them: [h][32 keys]
     __shared__ __attribute__((aligned(16))) float scale_s[2][kBN], scale_m[2][kBN];
-    __shared__ int bad;                    // first key whose V is NaN
+    __shared__ int bad[kWaves];            // each wave's first key whose V is NaN
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int h = lane >> 5, c32 = lane & 31;
@@ -150,9 +158,9 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     const int row = row_of(p, pair), qh = kvh * a.G + pair - row * a.G, pos = k.first + row;
     const bool live = row < a.rows && pos >= k.p_lo && pos <= k.p_hi;
     const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
-    // halves of tiles from `past` on (of the range's) hold keys that some pair of the wave does not see
+    // tiles from `past` on (of the range's) hold keys that some pair of the wave does not see
     const int lo = k.first + row_of(p, pair0), hi = k.first + row_of(p, pair0 + 31);
-    const int past = (lo < k.p_lo || hi > k.p_hi || lo < 31 ? 0 : (lo - 31) / 32 + 1) - 2 * t_lo;
+    const int past = (lo < k.p_lo || hi > k.p_hi || lo < kBN - 1 ? 0 : (lo - (kBN - 1)) / kBN + 1) - t_lo;
     const int seen0 = live ? pos - t_lo * kBN - 4 * h : -1;
     half8 qop[NC];   // in the codes' order
 #pragma unroll
@@ -178,7 +186,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         const uint8_t* pg = head + (int64_t)pid * PB;
         const uint32_t to = raw_at + (RST == 2 ? (t & 1) * RAW : 0);
         dma16(pg, 16 * lane, to);
-        if (lane < 8) dma16(pg, kPage * D + 16 * lane, to + 2 * kPage * RB);
+        dma16_8(pg, kPage * D + 16 * lane, to + 2 * kPage * RB);
     };
     auto ask_v = [&](int pid) {
         if constexpr (D == 128) dma16(head + (int64_t)pid * PB, 1024 + 16 * lane, raw_at + 1024);
@@ -204,6 +212,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     };
     // This lane's row of a tile's V: E and (r - 16) E, kept from the numbers' read to the codes'.
     half2v v_e, v_f;
+    int nan_at = INT32_MAX;   // the wave's first key whose V is NaN
     // A row's s and m: key 32 n + 8 q + 4 h + e to [h][16 n + 4 q + e].
     const int srow = kPage * wave + crow;
     const int sat = 32 * (srow >> 2 & 1) + 16 * (srow >> 5) + 4 * (srow >> 3 & 3) + (srow & 3);
@@ -212,17 +221,16 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         const uint8_t* num = r0 + 2 * kPage * RB + 4 * crow;
         uint32_t ks = *reinterpret_cast<const uint32_t*>(num), vs = *reinterpret_cast<const uint32_t*>(num + 64);
         const bool behind = key0 + t * kBN > k.p_hi;   // the last key
-        if (cc == 0) scale_s[t & 1][sat] = static_cast<float>(as_half2(ks)[0]) * a.scale_log2;
+        scale_s[t & 1][sat] = static_cast<float>(as_half2(ks)[0]) * a.scale_log2;   // by four lanes alike
         // of NaN and of what is behind the last key: operands of 0
         ks = behind || (ks & 0x7c00u) == 0x7c00u ? 0u : ks;
         const bool nan = !behind && (vs & 0x7c00u) == 0x7c00u;
         vs = behind || nan ? 0u : vs;
         const int e = max((int)(vs & 0x7c00u) - 0x0800, 0x0400);
-        if (cc == 0) {
-            scale_m[t & 1][sat] = static_cast<float>(as_half2(vs)[0]) *
-                                  static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
-            if (nan) atomicMin(&bad, key0 + t * kBN);
-        }
+        scale_m[t & 1][sat] = static_cast<float>(as_half2(vs)[0]) *
+                              static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
+        const uint64_t nans = __ballot(nan);
+        nan_at = nans && nan_at == INT32_MAX ? t_lo * kBN + t * kBN + kPage * wave + (__builtin_ctzll(nans) >> 2) : nan_at;
         const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
         v_e = half2v{eh, eh};
         v_f = (half2v{as_half2(vs)[1], as_half2(vs)[1]} + half2v{f16(-16), f16(-16)}) * v_e;
@@ -248,13 +256,39 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
     float m_run = -1e30f, l_part = 0.f;
 
-    // Scores of half u of tile j: element i is key 32 u + 8 (i / 4) + 4 h + i % 4.
-    auto qk = [&](int j, int u) {
+    // Operands are read a phase ahead of their products: left to itself the compiler reads one
+    // and waits for it, product by product.
+    struct KOps {
+        half8 x[NC];
+    };
+    struct VOps {
+        half8 x[2][NDB];
+    };
+    auto read_k = [&](int j, int u) {
         const uint32_t Kt = kat + (j & 1) * TB;
+        KOps k8;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) k8.x[c] = lds_read<half8>((Kt ^ 32 * c) + 64 * u * D);
+        return k8;
+    };
+    auto read_v = [&](int j, int u) {
+        const uint32_t Vt = vat + (j & 1) * TB + 64 * u * D;
+        VOps v8;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) {
+                const uint32_t q = (Vt ^ 64 * db) + 32 * t * D;
+                v8.x[t][db] = cat_half8(lds_tr16(q), lds_tr16(q + 16 * D));
+            }
+        return v8;
+    };
+    auto fence = []() { asm volatile("" ::: "memory"); };
+    // Scores of half u of tile j: element i is key 32 u + 8 (i / 4) + 4 h + i % 4.
+    auto qk = [&](const KOps& k8) {
         floatx16 s = {};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_read<half8>((Kt ^ 32 * c) + 64 * u * D), qop[c], s, 0, 0, 0);
+        for (int c = 0; c < NC; ++c) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8.x[c], qop[c], s, 0, 0, 0);
         return s;
     };
     // Weights as the operands of O^T's product; returns the largest and adds up the sum before
@@ -300,16 +334,12 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         for (int db = 0; db < NDB; ++db) o[db] *= alpha;
         m_run = mn;
     };
-    auto pv = [&](int j, int u, const half8 (&w)[2]) {
-        const uint32_t Vt = vat + (j & 1) * TB + 64 * u * D;
+    auto pv = [&](const VOps& v8, const half8 (&w)[2]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int db = 0; db < NDB; ++db) {
-                const uint32_t q = (Vt ^ 64 * db) + 32 * t * D;
-                o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    cat_half8(lds_tr16(q), lds_tr16(q + 16 * D)), w[t], o[db], 0, 0, 0);
-            }
+            for (int db = 0; db < NDB; ++db)
+                o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8.x[t][db], w[t], o[db], 0, 0, 0);
     };
     auto checked = [&](int j, int u, float most, const floatx16& s, half8 (&w)[2], float& sum) {
         if (__builtin_amdgcn_read_exec() & __ballot(most > kMostWeight)) {
@@ -324,12 +354,10 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     // first's weights, O of the first beside the second's weights, O of the second beside V's
     // conversion
     int pid = page_of(0);
-    if (threadIdx.x == 0) bad = INT32_MAX;
     wait_raw<0>();
     ask_k(0, pid);
     ask_v(pid);
     pid = page_of(1);
-    __syncthreads();   // bad
     wait_raw<0>();
     put_k(0);
     put_v(0);
@@ -337,12 +365,15 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     ask_k(1, pid);
     ask_v(pid);
     pid = page_of(2);
-    auto iterate = [&](auto LAST_, int j) {
+    // MASKED: some row of the wave does not see all of the tile
+    auto iterate = [&](auto LAST_, auto MASKED_, int j) {
         constexpr bool LAST = decltype(LAST_)::value;
         reads_done();   // and this wave's writes are in LDS
         ring_barrier();
         if constexpr (!LAST && RST == 2) ask_k(j + 2, pid);
-        const floatx16 s0 = qk(j, 0);
+        const KOps k0 = read_k(j, 0), k1 = read_k(j, 1);
+        fence();
+        const floatx16 s0 = qk(k0);
         if constexpr (!LAST) {
             wait_raw<RST == 2 ? 2 : 1>();
             put_k(j + 1);
@@ -351,17 +382,19 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
                 ask_k(j + 2, pid);
             }
         }
-        const floatx16 s1 = qk(j, 1);
+        const VOps v0 = read_v(j, 0);
+        fence();
+        const floatx16 s1 = qk(k1);
         half8 w0[2], w1[2];
         float sum0, sum1;
-        float most = 2 * j >= past ? weights(std::true_type{}, j, 0, s0, w0, sum0)
-                                   : weights(std::false_type{}, j, 0, s0, w0, sum0);
+        float most = weights(MASKED_, j, 0, s0, w0, sum0);
         checked(j, 0, most, s0, w0, sum0);
-        pv(j, 0, w0);
-        most = 2 * j + 1 >= past ? weights(std::true_type{}, j, 1, s1, w1, sum1)
-                                 : weights(std::false_type{}, j, 1, s1, w1, sum1);
+        const VOps v1 = read_v(j, 1);
+        fence();
+        pv(v0, w0);
+        most = weights(MASKED_, j, 1, s1, w1, sum1);
         checked(j, 1, most, s1, w1, sum1);
-        pv(j, 1, w1);
+        pv(v1, w1);
         if constexpr (!LAST) {
             if constexpr (RST == 1) wait_raw<2>();
             put_v(j + 1);
@@ -370,11 +403,17 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
             pid = page_of(j + 3);
         }
     };
-    for (int j = 0; j + 1 < n; ++j) iterate(std::false_type{}, j);
+    int j = 0;
+    for (const int whole = min(past, n - 1); j < whole; ++j) iterate(std::false_type{}, std::false_type{}, j);
+    for (; j + 1 < n; ++j) iterate(std::false_type{}, std::true_type{}, j);
     wait_raw<0>();   // the trailing loads
-    iterate(std::true_type{}, n - 1);
+    bad[wave] = nan_at;
+    iterate(std::true_type{}, std::true_type{}, j);
     if (!live) return;
-    if (pos >= bad) {   // no writes since the last barrier
+    int first_bad = bad[0];   // written before the last barrier
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) first_bad = min(first_bad, bad[w]);
+    if (pos >= first_bad) {
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
