@@ -391,10 +391,12 @@ int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int32_t* ages,
  * already, or never is).  q_out [batch][rows][Hq][D] may be q itself if q_stride is
  * Hq D; q and q_out both NULL: K and V only.
  * Rows at negative slots or at or past seq_lens[b] (device int32, NULL: no limit) are
- * padding: neither read nor written, q_out included.  K and V of a slot past the block
+ * padding: they reach nothing, and their q_out stays as it was.  K and V of a slot past the block
  * table, or whose page id lies outside [0, num_pages), are dropped (write tables hold -1
- * for shared pages); its q is rotated all the same.  batch rows (Hq + 2 Hkv) is at most
- * 2^31 - 1, head_dim even and at most 256. */
+ * for shared pages); its q is rotated all the same.  head_dim is even and at most 256;
+ * batch rows (Hq + 2 Hkv) is at most 2^25 where head_dim is neither 64 nor 128 or a tensor
+ * is off 16-byte alignment (rows then go one by one, several times slower).
+ * Asynchronous, allocates nothing, may be captured. */
 int kvhp_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
                      int64_t k_stride, int64_t v_stride, const int32_t* positions,
                      const int32_t* slots, const int32_t* seq_lens, float rope_theta, void* q_out,

@@ -4,10 +4,17 @@
 // The rotation's angle is counted in turns in 64 bits, p theta^(-2i/D) / 2 pi, and its sine
 // and cosine are rounded to fp32 once, so that far positions lose nothing: in fp32 the angle
 // itself is off by up to 2^-11 at position 2^13 and 2^-10 at 2^14, more than fp16 rounds.
-// One wave per (token, head), a lane per pair of dims.
+//
+// head_dim 64 and 128, 16-byte aligned tensors: a workgroup takes 1 to 16 tokens and some of
+// their heads, computes the tokens' rotations once, into LDS, and moves rows by 16-byte chunks,
+// a lane both halves' chunks of 8 pairs, three rows' loads in flight.  In 4 bits the 4 or 8
+// lanes of a row find its range among themselves and write a word of codes per chunk.  Bound by
+// HBM for prompts, by latency for a step's tokens.
+// Other shapes: one wave per (token, head), a lane per pair of dims.
 #include "q4.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace kvhp {
 namespace {
@@ -145,6 +152,133 @@ __global__ void __launch_bounds__(kWave) append_row_kernel(const AppendArgs a) {
     if (lane == 0) *reinterpret_cast<uint32_t*>(pg + q4_params_at(D, is_v, o)) = z.bits;
 }
 
+// The same by 16-byte chunks, D = 64 and 128.  Grid (groups of TB tokens, pieces of HP heads).
+template <int D, bool Q4>
+__global__ void __launch_bounds__(256) append_vec_kernel(const AppendArgs a, int TB, int HP, uint32_t inv_hp) {
+    constexpr int half = D / 2, CPH = half / 8, RPI = 256 / CPH, U = 3, kMostTokens = 16;
+    __shared__ float2 cs[kMostTokens * half];
+    __shared__ int64_t pos_of[kMostTokens];
+    __shared__ int slot_of[kMostTokens], pid_of[kMostTokens];   // slot -1: padding; page -1: dropped
+    const int tid = threadIdx.x, H = a.Hq + 2 * a.Hkv;
+    const int64_t token0 = (int64_t)blockIdx.x * TB;
+    const int nt = static_cast<int>(min((int64_t)TB, (int64_t)a.batch * a.rows - token0));
+    const int h0 = blockIdx.y * HP, nh = min(HP, H - h0);
+    const int nrows = nt * HP, c = tid % CPH;
+    half8 x[U], y[U];
+    auto head_of = [&](int rr, int& tt) {
+        tt = inv_hp ? static_cast<int>(__umulhi(static_cast<uint32_t>(rr), inv_hp)) : rr;
+        return h0 + rr - tt * HP;
+    };
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int rr = base + RPI * u + tid / CPH;
+            int tt;
+            const int h = head_of(rr, tt);
+            if (rr >= nrows || h >= h0 + nh) continue;
+            const int64_t token = token0 + tt;
+            const f16* src = h < a.Hq ? a.q + token * a.sq + (int64_t)h * D
+                             : h < a.Hq + a.Hkv ? a.k + token * a.sk + (int64_t)(h - a.Hq) * D
+                                                : a.v + token * a.sv + (int64_t)(h - a.Hq - a.Hkv) * D;
+            x[u] = load_half8(src + 8 * c);
+            y[u] = load_half8(src + half + 8 * c);
+        }
+    };
+    load(0);
+    if (tid < nt) {
+        const int64_t token = token0 + tid;
+        const int b = static_cast<int>(token / a.rows), row = static_cast<int>(token - (int64_t)b * a.rows);
+        const int64_t pos = (a.positions ? a.positions[b] : 0) + (int64_t)row;
+        const int64_t slot = a.slots ? a.slots[b] + (int64_t)row : pos;
+        const bool live = slot >= 0 && !(a.seq_lens && slot >= a.seq_lens[b]);
+        int pid = -1;
+        if (live && slot < (int64_t)a.max_pages * kPage) {
+            pid = a.bt[(int64_t)b * a.max_pages + (slot >> 4)];
+            if (pid >= a.num_pages) pid = -1;
+        }
+        pos_of[tid] = pos;
+        slot_of[tid] = live ? static_cast<int>(slot & 15) : -1;
+        pid_of[tid] = pid;
+    }
+    __syncthreads();
+    if (a.rotate) {
+        for (int i = tid; i < nt * half; i += 256) cs[i] = rotation(pos_of[i / half], i % half, D, a.log2_theta);
+        __syncthreads();
+    }
+    for (int base = 0; base < nrows; base += U * RPI) {
+        if (base > 0) load(base);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int rr = base + RPI * u + tid / CPH;
+            int tt;
+            const int h = head_of(rr, tt);
+            // the lanes of a row all go on or none
+            if (rr >= nrows || h >= h0 + nh || slot_of[tt] < 0) continue;
+            const int64_t token = token0 + tt;
+            const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+            half8 lo8 = x[u], hi8 = y[u];
+            if (a.rotate && !is_v) {
+                const float2* r = cs + tt * half + 8 * c;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f16 f, g;
+                    rotate(static_cast<float>(x[u][e]), static_cast<float>(y[u][e]), r[e], f, g);
+                    lo8[e] = f;
+                    hi8[e] = g;
+                }
+            }
+            if (is_q) {
+                f16* dst = a.q_out + (token * a.Hq + h) * D + 8 * c;
+                store_half8(dst, lo8);
+                store_half8(dst + half, hi8);
+                continue;
+            }
+            const int kvh = is_v ? h - a.Hq - a.Hkv : h - a.Hq, pid = pid_of[tt], o = slot_of[tt];
+            if (pid < 0) continue;
+            const int64_t page = (int64_t)kvh * a.num_pages + pid;
+            if constexpr (!Q4) {
+                f16* dst = (is_v ? a.pool_v : a.pool_k) + (page * kPage + o) * D + 8 * c;
+                store_half8(dst, lo8);
+                store_half8(dst + half, hi8);
+            } else {
+                float lo = INFINITY, hi = -INFINITY;
+                uint32_t bad = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = static_cast<float>(lo8[e]), g = static_cast<float>(hi8[e]);
+                    lo = fminf(lo, fminf(f, g));
+                    hi = fmaxf(hi, fmaxf(f, g));
+                    bad |= fabsf(f) < INFINITY && fabsf(g) < INFINITY ? 0u : 1u;
+                }
+                auto across = [&](auto ctrl) {
+                    constexpr int CTRL = decltype(ctrl)::value;
+                    lo = fminf(lo, dpp_f32<CTRL>(lo));
+                    hi = fmaxf(hi, dpp_f32<CTRL>(hi));
+                    bad |= __float_as_uint(dpp_f32<CTRL>(__uint_as_float(bad)));
+                };
+                across(std::integral_constant<int, 0xB1>{});
+                across(std::integral_constant<int, 0x4E>{});
+                if constexpr (CPH == 8) across(std::integral_constant<int, 0x141>{});
+                Q4Quant z = q4_quant(bad ? 0.f : lo, bad ? 0.f : hi);
+                if (bad) z.bits = kQ4NanRow;
+                uint32_t n0 = 0, n1 = 0;
+                if (!bad && !z.flat) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        n0 |= q4_code(z, static_cast<float>(lo8[e])) << 4 * e;
+                        n1 |= q4_code(z, static_cast<float>(hi8[e])) << 4 * e;
+                    }
+                }
+                uint8_t* pg = a.pool + page * q4_page_bytes(D);
+                uint8_t* codes = pg + q4_codes_at(D, is_v, o) + 4 * c;
+                *reinterpret_cast<uint32_t*>(codes) = n0;
+                *reinterpret_cast<uint32_t*>(codes + D / 4) = n1;
+                if (c == 0) *reinterpret_cast<uint32_t*>(pg + q4_params_at(D, is_v, o)) = z.bits;
+            }
+        }
+    }
+}
+
 int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq, int hkv, int d,
            float theta, hipStream_t s) {
     KVHP_REQUIRE(a.k && a.v && a.bt && (q4 ? a.pool != nullptr : a.pool_k && a.pool_v) &&
@@ -176,9 +310,36 @@ int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq
                  KVHP_ERR_INVALID, "%s: a token's rows overlap the next one's", what);
     a.rotate = theta > 0.f;
     a.log2_theta = a.rotate ? std::log2(static_cast<double>(theta)) : 0.0;
-    const int64_t waves = (int64_t)batch * rows * (a.Hq + 2 * hkv);
-    KVHP_REQUIRE((int64_t)batch * rows <= 1 << 25 && waves <= 1 << 25, KVHP_ERR_UNSUPPORTED,
-                 "%s: %d x %d rows of %d heads", what, batch, rows, a.Hq + 2 * hkv);
+    const int64_t tokens = (int64_t)batch * rows;
+    const int H = a.Hq + 2 * hkv;
+    auto whole = [](const void* x, int64_t stride) { return !x || (aligned16(x) && stride % 8 == 0); };
+    if ((d == 64 || d == 128) && tokens <= INT32_MAX && H <= 1 << 16 && whole(a.q, a.sq) &&
+        whole(a.k, a.sk) && whole(a.v, a.sv) && aligned16(a.q_out) && aligned16(a.pool_k) &&
+        aligned16(a.pool_v)) {
+        // Two workgroups a CU where there are tokens for them, of up to 16 tokens (a page); where
+        // there are not, the heads of a token are parted too.
+        int TB = 1;
+        while (TB < 16 && tokens >= 2 * TB * 512) TB *= 2;
+        const int64_t groups = (tokens + TB - 1) / TB;
+        const int per = 256 / (d / 16);   // rows of a workgroup at once
+        const int64_t most = ((int64_t)H * TB + per - 1) / per;
+        const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(most, 512 / groups));
+        const int HP = static_cast<int>((H + pieces - 1) / pieces);
+        const uint32_t inv = HP == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + HP - 1) / HP);
+        const dim3 grid(static_cast<unsigned>(groups), (H + HP - 1) / HP);
+        if (d == 64 && q4)
+            hipLaunchKernelGGL((append_vec_kernel<64, true>), grid, dim3(256), 0, s, a, TB, HP, inv);
+        else if (d == 64)
+            hipLaunchKernelGGL((append_vec_kernel<64, false>), grid, dim3(256), 0, s, a, TB, HP, inv);
+        else if (q4)
+            hipLaunchKernelGGL((append_vec_kernel<128, true>), grid, dim3(256), 0, s, a, TB, HP, inv);
+        else
+            hipLaunchKernelGGL((append_vec_kernel<128, false>), grid, dim3(256), 0, s, a, TB, HP, inv);
+        return check_launch(what);
+    }
+    const int64_t waves = tokens * H;
+    KVHP_REQUIRE(tokens <= 1 << 25 && waves <= 1 << 25, KVHP_ERR_UNSUPPORTED,
+                 "%s: %d x %d rows of %d heads", what, batch, rows, H);
     const dim3 grid(static_cast<unsigned>(waves));
     if (q4)
         hipLaunchKernelGGL(append_row_kernel<true>, grid, dim3(kWave), 0, s, a);
