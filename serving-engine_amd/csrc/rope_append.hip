@@ -7,7 +7,7 @@
 //
 // head_dim 64 and 128, 16-byte aligned tensors: a workgroup takes 1 to 16 tokens and some of
 // their heads, computes the tokens' rotations once, into LDS, and moves rows by 16-byte chunks,
-// a lane both halves' chunks of 8 pairs, three rows' loads in flight.  In 4 bits the 4 or 8
+// a lane both halves' chunks of 8 pairs, two rows' loads in flight.  In 4 bits the 4 or 8
 // lanes of a row find its range among themselves and write a word of codes per chunk.  Bound by
 // HBM for prompts, by latency for a step's tokens.
 // Other shapes: one wave per (token, head), a lane per pair of dims.
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kWave) append_row_kernel(const AppendArgs a) {
 // The same by 16-byte chunks, D = 64 and 128.  Grid (groups of TB tokens, pieces of HP heads).
 template <int D, bool Q4>
 __global__ void __launch_bounds__(256) append_vec_kernel(const AppendArgs a, int TB, int HP, uint32_t inv_hp) {
-    constexpr int half = D / 2, CPH = half / 8, RPI = 256 / CPH, U = 3, kMostTokens = 16;
+    constexpr int half = D / 2, CPH = half / 8, RPI = 256 / CPH, U = 2, kMostTokens = 16;
     __shared__ float2 cs[kMostTokens * half];
     __shared__ int64_t pos_of[kMostTokens];
     __shared__ int slot_of[kMostTokens], pid_of[kMostTokens];   // slot -1: padding; page -1: dropped
@@ -316,12 +316,14 @@ int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq
     if ((d == 64 || d == 128) && tokens <= INT32_MAX && H <= 1 << 16 && whole(a.q, a.sq) &&
         whole(a.k, a.sk) && whole(a.v, a.sv) && aligned16(a.q_out) && aligned16(a.pool_k) &&
         aligned16(a.pool_v)) {
-        // Two workgroups a CU where there are tokens for them, of up to 16 tokens (a page); where
-        // there are not, the heads of a token are parted too.
-        int TB = 1;
-        while (TB < 16 && tokens >= 2 * TB * 512) TB *= 2;
-        const int64_t groups = (tokens + TB - 1) / TB;
+        // Four workgroups a CU where there are tokens for them, of up to 16 tokens (a page); fewer
+        // where a workgroup's threads would not have a row each; where tokens are few, the heads of
+        // one are parted too.  (8192 tokens of 32/8 heads of 128: two a CU 52.4 us, four 44.2,
+        // eight 44.5; 3108 of 14/2 heads of 64: 4 tokens 5.4, 2 6.3, 1 7.9.)
         const int per = 256 / (d / 16);   // rows of a workgroup at once
+        int TB = 1;
+        while (TB < 16 && (tokens >= 2 * TB * 1024 || (H * TB < per && tokens >= 2 * TB * 256))) TB *= 2;
+        const int64_t groups = (tokens + TB - 1) / TB;
         const int64_t most = ((int64_t)H * TB + per - 1) / per;
         const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(most, 512 / groups));
         const int HP = static_cast<int>((H + pieces - 1) / pieces);

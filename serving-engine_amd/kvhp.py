@@ -542,10 +542,25 @@ def _token_rows(t, what):
 
 
 def _append_rows(q, k, v, q_out, what):
-    B, R, sk = _token_rows(k, what)
-    sv = _token_rows(v, what)[2]
-    sq = 0 if q is None else _token_rows(q, what)[2]
-    if any(t is not None and tuple(t.shape[:2]) != (B, R) for t in (q, v, q_out)):
+    """(batch, rows, q_stride, k_stride, v_stride) of an append's tensors."""
+    shape = k.shape
+    B, R, H, D = shape
+    same = v.shape == shape
+    kb, sk, kh, kd = k.stride()
+    vb, sv, vh, vd = v.stride()
+    # as slices of contiguous tensors are; others by _token_rows, which knows what it can take
+    if not (kd == vd == 1 and kh == vh == D and kb == R * sk and vb == R * sv):
+        sk, sv = _token_rows(k, what)[2], _token_rows(v, what)[2]
+    sq = 0
+    if q is not None:
+        qb, sq, qh, qd = q.stride()
+        if not (qd == 1 and qh == D and qb == R * sq):
+            sq = _token_rows(q, what)[2]
+        qs = q.shape
+        same = same and qs[0] == B and qs[1] == R and qs[3] == D
+        if q_out is not None:
+            same = same and q_out.shape == qs
+    if not same:
         raise KVHPError(KVHP_ERR_INVALID, f"{what}: q, k, v and q_out of different rows")
     if q_out is not None and not q_out.is_contiguous():
         raise KVHPError(KVHP_ERR_INVALID, f"{what}: q_out must be contiguous")
