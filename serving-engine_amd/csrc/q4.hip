@@ -69,38 +69,52 @@ __global__ void __launch_bounds__(kWave) q4_rows_kernel(const Q4Args a) {
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Rows read back: one thread per 8 dims of a position, K and V.
+// Rows read back: a thread takes 8 dims of K and V of two positions, the loads of both in
+// flight together (8192 positions of 8 heads of 128: 9.2 us, 4.6 TB/s; one position 11.4).
+// Grid (positions; KV head; sequence).  DT: head_dim, 0 for any.
+template <int DT>
 __global__ void __launch_bounds__(256)
 q4_gather_kernel(const uint8_t* pool, const int32_t* bt, int max_pages, int num_pages,
-                 const int32_t* start, const int32_t* seq_lens, f16* out_k, f16* out_v,
-                 int64_t items, int Hkv, int D, int max_len) {
-    const int cpr = D / 8;
-    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < items;
-         i += (int64_t)gridDim.x * 256) {
-        const int c = static_cast<int>(i % cpr);
-        const int64_t row = i / cpr;                 // (b Hkv + h) max_len + t
-        const int t = static_cast<int>(row % max_len);
-        const int64_t bh = row / max_len;
-        const int b = static_cast<int>(bh / Hkv), h = static_cast<int>(bh % Hkv);
-        const int64_t pos = (start ? start[b] : 0) + (int64_t)t;
-        const int n = static_cast<int>(min((int64_t)max(seq_lens[b], 0), (int64_t)max_pages * kPage));
-        const bool in = pos >= 0 && pos < n;
-        const uint8_t* pg = nullptr;
-        if (in) pg = q4_page(pool, num_pages, D, h, bt[(int64_t)b * max_pages + (pos >> 4)]);
+                 const int32_t* start, const int32_t* seq_lens, f16* out_k, f16* out_v, int Hkv,
+                 int any_d, int max_len) {
+    const int D = DT ? DT : any_d;
+    const uint32_t cpr = D / 8;
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int n = static_cast<int>(min((int64_t)max(seq_lens[b], 0), (int64_t)max_pages * kPage));
+    const int64_t first = start ? start[b] : 0;
+    constexpr int U = 2;
+    uint32_t x[U][2], sr[U][2];
+    int t[U], c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint64_t i = (uint64_t)blockIdx.x * (256 * U) + 256 * u + threadIdx.x;
+        t[u] = static_cast<int>(min(i / cpr, (uint64_t)INT32_MAX));
+        c[u] = static_cast<int>(i % cpr);
+        const int64_t pos = first + t[u];
+        x[u][0] = x[u][1] = sr[u][0] = sr[u][1] = 0;   // zeros stand for zeros
+        if (t[u] >= max_len || pos < 0 || pos >= n) continue;
+        const uint8_t* pg = q4_page(pool, num_pages, D, h, bt[(int64_t)b * max_pages + (pos >> 4)]);
         const int o = static_cast<int>(pos & 15);
+#pragma unroll
+        for (int is_v = 0; is_v < 2; ++is_v) {
+            sr[u][is_v] = *reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, is_v, o));
+            x[u][is_v] = *reinterpret_cast<const uint32_t*>(pg + q4_codes_at(D, is_v, o) + 4 * c[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (t[u] >= max_len) continue;
+        const int64_t at = (((int64_t)b * Hkv + h) * max_len + t[u]) * D + 8 * c[u];
 #pragma unroll
         for (int is_v = 0; is_v < 2; ++is_v) {
             f16* out = is_v ? out_v : out_k;
             if (!out) continue;
-            half8 y = {};
-            if (in) {
-                const Q4Row p = q4_row(*reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, is_v, o)));
-                const uint32_t x = *reinterpret_cast<const uint32_t*>(pg + q4_codes_at(D, is_v, o) + 4 * c);
+            const Q4Row p = q4_row(sr[u][is_v]);
+            half8 y;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    y[e] = static_cast<f16>(p.s * (static_cast<float>(x >> 4 * e & 15) + p.r));
-            }
-            store_half8(out + i * 8, y);
+            for (int e = 0; e < 8; ++e)
+                y[e] = static_cast<f16>(p.s * (static_cast<float>(x[u][is_v] >> 4 * e & 15) + p.r));
+            store_half8(out + at, y);
         }
     }
 }
@@ -175,12 +189,20 @@ extern "C" int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int
     if (rc) return rc;
     KVHP_REQUIRE(aligned16(out_k) && aligned16(out_v), KVHP_ERR_INVALID,
                  "%s: outputs not 16-byte aligned", what);
-    const int64_t items = (int64_t)batch * num_kv_heads * max_len * (head_dim / 8);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((items + 255) / 256, 1 << 20));
-    hipLaunchKernelGGL(q4_gather_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       a.pool, block_tables, max_pages, num_pages, start, seq_lens,
-                       static_cast<f16*>(out_k), static_cast<f16*>(out_v), items, num_kv_heads,
-                       head_dim, max_len);
+    const dim3 grid(static_cast<unsigned>(((int64_t)max_len * (head_dim / 8) + 511) / 512),
+                    num_kv_heads, batch);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a.pool,
+                           block_tables, max_pages, num_pages, start, seq_lens,
+                           static_cast<f16*>(out_k), static_cast<f16*>(out_v), num_kv_heads,
+                           head_dim, max_len);
+    };
+    if (head_dim == 64)
+        go(q4_gather_kernel<64>);
+    else if (head_dim == 128)
+        go(q4_gather_kernel<128>);
+    else
+        go(q4_gather_kernel<0>);
     return check_launch(what);
 }
 
