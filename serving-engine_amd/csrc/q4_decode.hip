@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kTok = 64;          // keys per tile: one page per 16 lanes
 constexpr int kMaxTiles = 16;     // per wave and split: 64 page ids, one per lane
+constexpr int kMinTiles = 4;      // per balanced split
 constexpr int kHeads = 16;        // query heads per workgroup
 constexpr float kLazyLog2 = 3.f;  // a row's reference moves when a score passes it by this
 constexpr float kMostM = 4096.f;  // s / E: weights up to 2^15 in fp16
@@ -38,6 +39,7 @@ struct DecodePlan {
     int chunk;        // keys per split, a multiple of kTok
     int nsplit;       // split slots in the workspace
     int batch;
+    int waves;        // per workgroup
     int balance;      // > 0: about this many splits per KV head over the batch
     int groups;       // workgroups per KV head and split, of up to kHeads query heads
     float* ws_o;      // [B * Hq][nsplit][D]
@@ -72,12 +74,12 @@ __device__ __forceinline__ bool share_of(const Q4Args& a, const DecodePlan& p, u
         const int l = g0 == 0 ? li : g0 + lane < p.batch ? q4_len(a, g0 + lane) : 0;
         tiles = min(tiles + (uint32_t)__builtin_amdgcn_readlane(prefix_sum(tiles_of(l)), kWave - 1), 1u << 30);
     }
-    const uint32_t target = min((tiles + p.balance - 1) / p.balance, (uint32_t)kMaxTiles);
+    const uint32_t target = min(max((tiles + p.balance - 1) / p.balance, (uint32_t)kMinTiles), (uint32_t)kMaxTiles);
     uint32_t base = 0;
     for (int g0 = 0; g0 < p.batch; g0 += kWave) {
         const bool in = g0 + lane < p.batch;
         if (g0 > 0) li = in ? q4_len(a, g0 + lane) : 0;
-        const uint32_t t = tiles_of(li), ti = share_tiles(p, t, max(target, 1u));
+        const uint32_t t = tiles_of(li), ti = share_tiles(p, t, target);
         const uint32_t ni = in ? max((t + ti - 1) / ti, 1u) : 0;
         const uint32_t inc = prefix_sum(ni), tot = __builtin_amdgcn_readlane(inc, kWave - 1);
         if (i < base + tot) {
@@ -203,7 +205,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     const int g = lane >> 4, col = lane & 15;
     const int kvh = blockIdx.x / p.groups, h0 = blockIdx.x % p.groups * kHeads;
     int b, split, L, chunk;
-    if (W == 1 && p.balance > 0) {
+    if constexpr (W == 1) {
         if (!share_of(a, p, blockIdx.y, lane, b, split, L, chunk)) return;
     } else {
         split = blockIdx.y;
@@ -566,22 +568,37 @@ __global__ void __launch_bounds__(kJoinRows * kWave) q4_join_kernel(const Q4Args
     store_half8(a.out + row * D + 8 * c, h);
 }
 
+// Where one split of eight waves holds a sequence, it saves the join's launch: 5 to 7 us against
+// 7 to 8 for splits up to 1024 keys at D = 64 and 768 at D = 128, of one to four sequences; past
+// that its waves' own tiles take longer (1024 keys at D = 128: 8.1 against 7.5).  Batches fill the
+// card with one split each up to 2048 keys (32 sequences of 8 heads, D = 128: 13.7 against 14.9;
+// of 4 heads, D = 64: 9.3 against 11.0; 64 of 8 heads are level, 4096 keys are not better).
 constexpr int kBalanced = 16;      // sequences from which the splits are the whole batch's
 constexpr int kWaveSlots = 2048;   // one wave per split, two per SIMD of 256 CUs
 constexpr int kWaves = 4;          // per workgroup in fixed splits
+constexpr int kShortWaves = 8;     // and where a sequence is one split
 
-DecodePlan plan_of(int batch, int hkv, int G, int64_t max_len) {
+DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t max_len) {
     DecodePlan p{};
     p.batch = batch;
     p.groups = (G + kHeads - 1) / kHeads;
     const int64_t heads = (int64_t)hkv * p.groups, tiles = (max_len + kTok - 1) / kTok;
+    if (tiles <= (batch >= kBalanced ? 32 : d == 64 ? 16 : 12)) {
+        p.waves = kShortWaves;
+        p.chunk = static_cast<int>(tiles * kTok);
+        p.nsplit = 1;
+        return p;
+    }
     if (batch >= kBalanced) {
+        p.waves = 1;
         p.balance = static_cast<int>(std::max<int64_t>(1, kWaveSlots / heads - batch / 2));
         // splits of a sequence: of the target, which is the least where it alone has keys
-        const int64_t target = std::min<int64_t>((tiles + p.balance - 1) / p.balance, kMaxTiles);
+        const int64_t target =
+            std::min<int64_t>(std::max<int64_t>((tiles + p.balance - 1) / p.balance, kMinTiles), kMaxTiles);
         p.nsplit = static_cast<int>((tiles + target - 1) / target);
         return p;
     }
+    p.waves = kWaves;
     const int64_t want = std::max<int64_t>(1, 512 / (heads * batch));   // workgroups per head
     const int64_t per = std::min<int64_t>(std::max<int64_t>((tiles + want - 1) / want, kWaves), kWaves * kMaxTiles);
     p.chunk = static_cast<int>(per * kTok);
@@ -599,29 +616,32 @@ int64_t units_of(const DecodePlan& p, int64_t max_len) {
 
 size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len) {
     if (!bound_sizes(batch, hq, hkv, max_len, 0, 0) || (d != 64 && d != 128)) return 0;
-    const DecodePlan p = plan_of(batch, hkv, hq / hkv, max_len);
+    const DecodePlan p = plan_of(batch, hkv, hq / hkv, d, max_len);
     return p.nsplit == 1 ? 0 : sizeof(float) * ((size_t)batch * hq * p.nsplit * (d + 2) + batch);
 }
 
 bool q4_decode_fits(const Q4Args& a, int batch) {
-    const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.max_len);
+    const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, a.max_len);
     return (a.D == 64 || a.D == 128) && aligned16(a.q) && aligned16(a.out) &&
            units_of(p, a.max_len) <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
 }
 
 // The workspace holds q4_decode_workspace bytes.
 int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s) {
-    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.max_len);
+    DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, a.max_len);
     p.ws_o = static_cast<float*>(ws);
     p.ws_ml = p.ws_o + (size_t)batch * a.Hq * p.nsplit * a.D;
     p.ws_n = reinterpret_cast<int32_t*>(p.ws_ml + (size_t)batch * a.Hq * p.nsplit * 2);
     const dim3 grid(a.Hkv * p.groups, static_cast<unsigned>(units_of(p, a.max_len)), p.balance ? 1 : batch);
     auto go = [&](auto d, auto pk) {
         constexpr int D = decltype(d)::value, PK = decltype(pk)::value;
-        if (p.balance)
-            hipLaunchKernelGGL((q4_decode_kernel<D, 1, PK>), grid, dim3(kWave), 0, s, a, p);
+        const dim3 threads(p.waves * kWave);
+        if (p.waves == 1)
+            hipLaunchKernelGGL((q4_decode_kernel<D, 1, PK>), grid, threads, 0, s, a, p);
+        else if (p.waves == kWaves)
+            hipLaunchKernelGGL((q4_decode_kernel<D, kWaves, PK>), grid, threads, 0, s, a, p);
         else
-            hipLaunchKernelGGL((q4_decode_kernel<D, kWaves, PK>), grid, dim3(kWaves * kWave), 0, s, a, p);
+            hipLaunchKernelGGL((q4_decode_kernel<D, kShortWaves, PK>), grid, threads, 0, s, a, p);
     };
     auto parts = [&](auto d) {
         if (a.G <= 4)

@@ -313,9 +313,10 @@ int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq
     const int64_t tokens = (int64_t)batch * rows;
     const int H = a.Hq + 2 * hkv;
     auto whole = [](const void* x, int64_t stride) { return !x || (aligned16(x) && stride % 8 == 0); };
-    if ((d == 64 || d == 128) && tokens <= INT32_MAX && H <= 1 << 16 && whole(a.q, a.sq) &&
+    if ((d == 64 || d == 128) && tokens <= INT32_MAX && H <= 1 << 14 && whole(a.q, a.sq) &&
         whole(a.k, a.sk) && whole(a.v, a.sv) && aligned16(a.q_out) && aligned16(a.pool_k) &&
         aligned16(a.pool_v)) {
+        // (16 H rows of a workgroup, part by part: __umulhi is exact to 2^32 of row x heads.)
         // Four workgroups a CU where there are tokens for them, of up to 16 tokens (a page); fewer
         // where a workgroup's threads would not have a row each; where tokens are few, the heads of
         // one are parted too.  (8192 tokens of 32/8 heads of 128: two a CU 52.4 us, four 44.2,
