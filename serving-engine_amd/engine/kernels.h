@@ -259,6 +259,71 @@ inline void evict_apply(half* pool_k, half* pool_v, float* weights, int32_t* age
                                 stream));
 }
 
+// ---- Appends that rotate on the way, and caches held in 4 bits (no reference
+// counterpart; kvhp_c.h has the semantics).  q [B][rows][Hq][D], k, v
+// [B][rows][Hkv][D], tokens *_stride halfs apart; positions, slots and seq_lens
+// may be nullptr; 4-bit pools [Hkv][num_pages][q4_page_bytes(D)].
+inline void rope_append(const half* q, const half* k, const half* v, int64_t q_stride,
+                        int64_t k_stride, int64_t v_stride, const int32_t* positions,
+                        const int32_t* slots, const int32_t* seq_lens, float rope_theta,
+                        half* q_out, half* pool_k, half* pool_v, const int32_t* block_tables,
+                        int max_pages, int num_pages, int batch_size, int rows, int num_q_heads,
+                        int num_kv_heads, int head_dim, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_rope_append(q, k, v, q_stride, k_stride, v_stride, positions, slots, seq_lens,
+                                rope_theta, q_out, pool_k, pool_v, block_tables, max_pages,
+                                num_pages, batch_size, rows, num_q_heads, num_kv_heads, head_dim,
+                                stream));
+}
+inline size_t q4_page_bytes(int head_dim) { return kvhp_q4_page_bytes(head_dim); }
+inline void q4_rope_append(const half* q, const half* k, const half* v, int64_t q_stride,
+                           int64_t k_stride, int64_t v_stride, const int32_t* positions,
+                           const int32_t* slots, const int32_t* seq_lens, float rope_theta,
+                           half* q_out, uint8_t* pool, const int32_t* block_tables, int max_pages,
+                           int num_pages, int batch_size, int rows, int num_q_heads,
+                           int num_kv_heads, int head_dim, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_q4_rope_append(q, k, v, q_stride, k_stride, v_stride, positions, slots,
+                                   seq_lens, rope_theta, q_out, pool, block_tables, max_pages,
+                                   num_pages, batch_size, rows, num_q_heads, num_kv_heads,
+                                   head_dim, stream));
+}
+// Positions start[b] + t (start may be nullptr: 0) as fp16 [B][Hkv][max_len][D].
+inline void q4_gather(const uint8_t* pool, const int32_t* block_tables, int max_pages,
+                      int num_pages, const int32_t* start, const int32_t* seq_lens, half* out_k,
+                      half* out_v, int batch_size, int num_kv_heads, int head_dim, int max_len,
+                      Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_q4_gather(pool, block_tables, max_pages, num_pages, start, seq_lens, out_k,
+                              out_v, batch_size, num_kv_heads, head_dim, max_len, stream));
+}
+inline size_t q4_decode_workspace_bytes(int batch_size, int num_q_heads, int num_kv_heads,
+                                        int head_dim, int max_seq_len) {
+    return kvhp_q4_decode_workspace_bytes(batch_size, num_q_heads, num_kv_heads, head_dim,
+                                          max_seq_len);
+}
+inline void q4_decode(const half* q, const uint8_t* pool, const int32_t* block_tables,
+                      int max_pages, int num_pages, const int32_t* seq_lens, half* out,
+                      int batch_size, int num_q_heads, int num_kv_heads, int head_dim,
+                      int max_seq_len, void* workspace, size_t workspace_bytes,
+                      Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_q4_decode(q, pool, block_tables, max_pages, num_pages, seq_lens, out,
+                              batch_size, num_q_heads, num_kv_heads, head_dim, max_seq_len,
+                              workspace, workspace_bytes, stream));
+}
+inline size_t q4_prefill_workspace_bytes(int batch_size, int rows, int num_q_heads,
+                                         int num_kv_heads, int head_dim, int max_seq_len) {
+    return kvhp_q4_prefill_workspace_bytes(batch_size, rows, num_q_heads, num_kv_heads, head_dim,
+                                           max_seq_len);
+}
+// Rows q [B][rows][Hq][D] at positions q_start[b] + r; lse [B][Hq][rows] may be nullptr.
+inline void q4_prefill(const half* q, const uint8_t* pool, const int32_t* block_tables,
+                       int max_pages, int num_pages, const int32_t* q_start,
+                       const int32_t* seq_lens, half* out, float* lse, int batch_size, int rows,
+                       int num_q_heads, int num_kv_heads, int head_dim, int max_seq_len,
+                       void* workspace, size_t workspace_bytes, Stream stream = nullptr) {
+    KVHP_CHECK(kvhp_q4_prefill(q, pool, block_tables, max_pages, num_pages, q_start, seq_lens, out,
+                               lse, batch_size, rows, num_q_heads, num_kv_heads, head_dim,
+                               max_seq_len, workspace, workspace_bytes, stream));
+}
+
 }  // namespace hip
 
 namespace cuda = hip;

@@ -19,12 +19,19 @@
 // as the reference runner asserts (:51), and prefill writes go through a
 // write table in which shared pages are -1, so they are never overwritten
 // ("share" mode, :33).
+//
+// PagedKVCache::Format::kQ4 holds the same pages in 4 bits (kvhp_c.h): one pool
+// per layer, [num_kv_heads][num_pages][q4_page_bytes(head_dim)], about a fourth
+// of the memory, filled by rope_append and read by q4_decode, q4_prefill and
+// hip::q4_gather.  Pages, tables and prefix sharing are the same; the members
+// for fp16 pools throw.
 #pragma once
 
 #include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "half.h"
@@ -106,11 +113,13 @@ inline void append_kv_cache(const half* src_k, const half* src_v, half* dst_k_he
 class PagedKVCache {
 public:
     static constexpr int kPage = KVHP_PAGE_SIZE;
+    enum class Format { kHalf, kQ4 };
 
     PagedKVCache() = default;
     PagedKVCache(int num_layers, int num_kv_heads, int head_dim, int num_pages, int max_batch,
-                 int max_pages_per_seq) {
-        allocate(num_layers, num_kv_heads, head_dim, num_pages, max_batch, max_pages_per_seq);
+                 int max_pages_per_seq, Format format = Format::kHalf) {
+        allocate(num_layers, num_kv_heads, head_dim, num_pages, max_batch, max_pages_per_seq,
+                 format);
     }
     ~PagedKVCache() { release_staging(); }
     PagedKVCache(const PagedKVCache&) = delete;
@@ -118,17 +127,20 @@ public:
 
     // Pages that fit in `bytes` of pool for this model shape (K and V of
     // every layer).
-    static int pages_for_bytes(size_t bytes, int num_layers, int num_kv_heads, int head_dim) {
-        const size_t per_page = (size_t)num_layers * 2 * num_kv_heads * kPage * head_dim * sizeof(half);
+    static int pages_for_bytes(size_t bytes, int num_layers, int num_kv_heads, int head_dim,
+                               Format format = Format::kHalf) {
+        const size_t per_page =
+            (size_t)num_layers * num_kv_heads * page_halfs(head_dim, format) * sizeof(half);
         const size_t n = bytes / per_page;
         return n > (size_t)INT32_MAX ? INT32_MAX : (int)n;
     }
 
     void allocate(int num_layers, int num_kv_heads, int head_dim, int num_pages, int max_batch,
-                  int max_pages_per_seq) {
+                  int max_pages_per_seq, Format format = Format::kHalf) {
         if (num_layers <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_pages <= 0 ||
             max_batch <= 0 || max_pages_per_seq <= 0)
             throw std::invalid_argument("PagedKVCache::allocate: sizes must be positive");
+        const size_t page = page_halfs(head_dim, format);
         release_staging();
         num_layers_ = num_layers;
         num_kv_heads_ = num_kv_heads;
@@ -136,8 +148,9 @@ public:
         num_pages_ = num_pages;
         max_batch_ = max_batch;
         max_pages_ = max_pages_per_seq;
-        pool_.allocate((size_t)num_layers * 2 * num_kv_heads * num_pages * kPage * head_dim);
-        pool_.zero();
+        format_ = format;
+        pool_.allocate((size_t)num_layers * num_kv_heads * num_pages * page);
+        pool_.zero();   // in 4 bits: rows of zeros
         // one device block: tables [max_batch][max_pages], seq_lens [max_batch],
         // write positions [max_batch], write tables [max_batch][max_pages]
         meta_words_ = 2 * (size_t)max_batch * max_pages_per_seq + 2 * (size_t)max_batch;
@@ -164,9 +177,23 @@ public:
 
     // --- device side ------------------------------------------------------
     // Pool of one layer's K (is_v = 0) or V: [Hkv][num_pages][16][D].
-    half* get_layer_ptr(int layer, int is_v) { return pool_.data() + layer_offset(layer, is_v); }
-    const half* get_layer_ptr(int layer, int is_v) const {
+    half* get_layer_ptr(int layer, int is_v) {
+        need(Format::kHalf);
         return pool_.data() + layer_offset(layer, is_v);
+    }
+    const half* get_layer_ptr(int layer, int is_v) const {
+        need(Format::kHalf);
+        return pool_.data() + layer_offset(layer, is_v);
+    }
+    // Pool of one layer in 4 bits: [Hkv][num_pages][q4_page_bytes(D)].
+    uint8_t* get_q4_layer_ptr(int layer) {
+        return const_cast<uint8_t*>(std::as_const(*this).get_q4_layer_ptr(layer));
+    }
+    const uint8_t* get_q4_layer_ptr(int layer) const {
+        need(Format::kQ4);
+        check_layer(layer);
+        return reinterpret_cast<const uint8_t*>(
+            pool_.data() + (size_t)layer * num_kv_heads_ * num_pages_ * page_halfs(head_dim_, format_));
     }
     const int32_t* block_tables() const { return meta_.data(); }
     const int32_t* seq_lens() const { return meta_.data() + (size_t)max_batch_ * max_pages_; }
@@ -233,6 +260,7 @@ public:
     // shorter one and no more first tokens, and its length only grows.  Returns
     // how many pages it gave up.
     int drop_hidden(int slot, int window, int sinks) {
+        need(Format::kHalf);
         check_slot(slot);
         if (window <= 0 || sinks < 0)
             throw std::invalid_argument("PagedKVCache::drop_hidden: window must be positive and "
@@ -410,6 +438,47 @@ public:
                                  num_kv_heads_, head_dim_, max_seq_len, stream);
     }
 
+    // Rotates the rows of one layer, q [batch][rows][Hq][D] (to q_out) and k
+    // [batch][rows][Hkv][D] (tokens *_stride halfs apart), to each slot's write position
+    // on, and appends K and V there, in the cache's format.  Rows at or past a slot's length
+    // are padding.
+    void rope_append(int layer, const half* q, const half* k, const half* v, int64_t q_stride,
+                     int64_t k_stride, int64_t v_stride, float rope_theta, half* q_out, int batch,
+                     int rows, int num_q_heads, Stream stream = nullptr) {
+        check_layer(layer);
+        check_batch(batch);
+        if (format_ == Format::kQ4)
+            hip::q4_rope_append(q, k, v, q_stride, k_stride, v_stride, write_positions(), nullptr,
+                                seq_lens(), rope_theta, q_out, get_q4_layer_ptr(layer),
+                                write_block_tables(), max_pages_, num_pages_, batch, rows,
+                                num_q_heads, num_kv_heads_, head_dim_, stream);
+        else
+            hip::rope_append(q, k, v, q_stride, k_stride, v_stride, write_positions(), nullptr,
+                             seq_lens(), rope_theta, q_out, get_layer_ptr(layer, 0),
+                             get_layer_ptr(layer, 1), write_block_tables(), max_pages_, num_pages_,
+                             batch, rows, num_q_heads, num_kv_heads_, head_dim_, stream);
+    }
+    // Decode attention of q [batch][Hq][D] over each slot's seq_len keys in 4 bits.
+    void q4_decode(int layer, const half* q, half* out, int batch, int num_q_heads,
+                   int max_seq_len, void* workspace, size_t workspace_bytes,
+                   Stream stream = nullptr) const {
+        check_batch(batch);
+        hip::q4_decode(q, get_q4_layer_ptr(layer), block_tables(), max_pages_, num_pages_,
+                       seq_lens(), out, batch, num_q_heads, num_kv_heads_, head_dim_, max_seq_len,
+                       workspace, workspace_bytes, stream);
+    }
+    // Attention of rows q [batch][rows][Hq][D] from each slot's write position on, over its
+    // keys in 4 bits up to each; lse [batch][Hq][rows] may be nullptr.
+    void q4_prefill(int layer, const half* q, half* out, float* lse, int batch, int rows,
+                    int num_q_heads, int max_seq_len, void* workspace, size_t workspace_bytes,
+                    Stream stream = nullptr) const {
+        check_batch(batch);
+        hip::q4_prefill(q, get_q4_layer_ptr(layer), block_tables(), max_pages_, num_pages_,
+                        write_positions(), seq_lens(), out, lse, batch, rows, num_q_heads,
+                        num_kv_heads_, head_dim_, max_seq_len, workspace, workspace_bytes, stream);
+    }
+
+    Format format() const { return format_; }
     int num_layers() const { return num_layers_; }
     int num_kv_heads() const { return num_kv_heads_; }
     int head_dim() const { return head_dim_; }
@@ -420,6 +489,20 @@ public:
     size_t pool_bytes() const { return pool_.size_bytes(); }
 
 private:
+    // K and V of a KV head's page.
+    static size_t page_halfs(int head_dim, Format format) {
+        if (format == Format::kHalf) return (size_t)2 * kPage * head_dim;
+        const size_t bytes = hip::q4_page_bytes(head_dim);
+        if (bytes == 0)
+            throw std::invalid_argument("PagedKVCache: no 4-bit pages of head_dim " +
+                                        std::to_string(head_dim));
+        return bytes / sizeof(half);
+    }
+    void need(Format format) const {
+        if (format_ != format)
+            throw std::logic_error(format == Format::kQ4 ? "PagedKVCache: the cache holds fp16"
+                                                         : "PagedKVCache: the cache is held in 4 bits");
+    }
     size_t layer_offset(int l, int is_v) const {
         return ((size_t)l * 2 + is_v) * num_kv_heads_ * (size_t)num_pages_ * kPage * head_dim_;
     }
@@ -467,6 +550,7 @@ private:
 
     int num_layers_ = 0, num_kv_heads_ = 0, head_dim_ = 0, num_pages_ = 0;
     int max_batch_ = 0, max_pages_ = 0;
+    Format format_ = Format::kHalf;
     DeviceBuffer<half> pool_;
     DeviceBuffer<int32_t> meta_;
     size_t meta_words_ = 0;
