@@ -412,6 +412,7 @@ int kvhp_rope_append(const void* q, const void* k, const void* v, int64_t q_stri
  *   r = min x / s, to the nearest multiple of 2^(floor(log2(|min x / s| + 16)) - 10), so
  *       that n + r is an exact fp16 number;
  *   n = x / s - r, to the nearest, in 0..15.
+ * Each step is rounded to fp32, the quotients of s as products with 1 / 15 and 1 / 1984.
  * A row of equal values c: s = c, r = 1, n = 0.  A row with a value that is not finite
  * stands for NaN throughout.  A page of a KV head is 16 (D + 8) bytes: K codes [16][D/2]
  * (the even dim in the low half of a byte), V codes, K's (s, r) [16], V's.  At D = 128

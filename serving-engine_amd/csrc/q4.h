@@ -6,7 +6,9 @@
 // two fp16 numbers s and r, and stands for s (n + r):
 //   s = max((max x - min x) / 15, max |x| / 1984), rounded up to fp16,
 //   r = min x / s to the nearest multiple of 2^(floor(log2(|min x / s| + 16)) - 10),
-//   n = x / s - r to the nearest, in 0..15.
+//   n = x / s - r to the nearest, in 0..15,
+// in fp32, the first two quotients as products with 1 / 15 and 1 / 1984 in fp32 (1 / 15 is
+// rounded up, so that a quotient that fp16 holds may go up by one of its steps).
 // That multiple, and |r| <= 1984, make n + r and r - 16 exact in fp16 for every n (rows about
 // 0 have multiples of 2^-6: the range is off by s/128 at most; the second bound on s costs
 // 2^-12 of a row's largest, as much as fp16 itself).  So n + r is an operand of the matrix
@@ -54,7 +56,7 @@ __device__ __forceinline__ Q4Quant q4_quant(float lo, float hi) {
     z.s = lo;
     float r = 1.f;
     if (!z.flat) {
-        const float t = fmaxf((hi - lo) / 15.f, fmaxf(fabsf(lo), fabsf(hi)) / 1984.f);
+        const float t = fmaxf((hi - lo) * (1.f / 15.f), fmaxf(fabsf(lo), fabsf(hi)) * (1.f / 1984.f));
         f16 s16 = static_cast<f16>(t);
         if (static_cast<float>(s16) < t)   // positive: the next one up
             s16 = __builtin_bit_cast(f16, static_cast<uint16_t>(__builtin_bit_cast(uint16_t, s16) + 1));

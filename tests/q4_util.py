@@ -22,8 +22,8 @@ def quantise(x):
     f = np.where(bad, np.float32(0), f)
     lo, hi = f.min(-1, keepdims=True) + np.float32(0), f.max(-1, keepdims=True)   # no -0
     flat = lo == hi
-    t = np.maximum((hi - lo) / np.float32(15),
-                   np.maximum(np.abs(lo), np.abs(hi)) / np.float32(1984))
+    t = np.maximum((hi - lo) * (np.float32(1) / np.float32(15)),
+                   np.maximum(np.abs(lo), np.abs(hi)) * (np.float32(1) / np.float32(1984)))
     s = t.astype(np.float16)
     s = np.where(s.astype(np.float32) < t, (s.view(np.uint16) + np.uint16(1)).view(np.float16), s)
     s = np.where(flat, np.float32(1), s.astype(np.float32))
