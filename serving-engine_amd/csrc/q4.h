@@ -112,6 +112,27 @@ __device__ __forceinline__ const uint8_t* q4_page(const uint8_t* pool, int num_p
     return pool + ((int64_t)kvh * num_pages + min(max(pid, 0), num_pages - 1)) * q4_page_bytes(d);
 }
 
+// Sums over lanes 0 .. this one, by row shifts and row broadcasts.
+__device__ __forceinline__ uint32_t prefix_sum(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+// The largest of all lanes' x, which are not negative.
+__device__ __forceinline__ int wave_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, kWave - 1);
+}
+
 // q4_decode.hip: one token per sequence at D = 64 and 128.
 size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len);
 bool q4_decode_fits(const Q4Args& a, int batch);

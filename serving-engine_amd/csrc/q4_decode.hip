@@ -48,16 +48,6 @@ struct DecodePlan {
 };
 
 __device__ __forceinline__ int tiles_of(int L) { return (L + kTok - 1) / kTok; }
-// Sums over lanes 0 .. this one, by row shifts and row broadcasts.
-__device__ __forceinline__ uint32_t prefix_sum(uint32_t x) {
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);
-    return x;
-}
 // Tiles of a sequence's splits where the batch has `tiles`.
 __device__ __forceinline__ uint32_t share_tiles(const DecodePlan& p, uint32_t t, uint32_t target) {
     const uint32_t n = min((t + target - 1) / target, (uint32_t)p.nsplit);

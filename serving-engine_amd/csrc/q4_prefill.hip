@@ -33,15 +33,22 @@ namespace {
 constexpr int kBN = 64;               // keys per tile
 constexpr int kMaxRowHeads = 1 << 29; // (row, query head) pairs of a sequence: a grid of 2^22
 constexpr int kCUs = 256;
+constexpr int kLeastTiles = 3;        // of a range of keys
 constexpr float kRefLog2 = 4.f;       // weights where a row's reference is set,
 constexpr float kMostWeight = 4096.f; // and where it moves
 
 struct PrefillPlan {
     uint32_t inv_g;        // ceil(2^32 / G), 0 for G = 1
     int blocks;            // of pairs, per sequence and KV head
-    int tiles_per_split, nsplit;
+    int batch;
+    int tiles;             // of the longest sequence there may be
+    int nsplit;            // ranges of keys a sequence may have
+    // > 0: ranges over the batch, shared out by its lengths, where a CU has one workgroup, and
+    // where it has as many as it holds
+    int slots, slots_full;
     float* ws_o;           // [batch * rows * Hq][nsplit][D]
     float* ws_ml;          // [batch * rows * Hq][nsplit][2], the reference in log2 units
+    int32_t* ws_range;     // tiles of a range
 };
 
 // Row of a pair: pair / G, exact for pair * G below 2^32.
@@ -64,6 +71,38 @@ __device__ __forceinline__ Block block_of(const Q4Args& a, const PrefillPlan& p,
     k.p_lo = static_cast<int>(max(first + r0, (int64_t)0));
     k.p_hi = static_cast<int>(min(first + r1, (int64_t)n - 1));
     return k;
+}
+
+// What ranges cost in tiles of a workgroup that has its CU to itself (1.4 to 1.65 us at D = 128, 1.1 to
+// 1.3 at 64): a tile of one of two (three; 2.7 us), and what they are written and joined in, the more
+// ranges the longer.  (Chunks of 128 rows in four sequences of 1062 to 8192 keys, 32/8 heads of 128:
+// 256 ranges of 47 tiles 86.6 us, 488 of 23 80.1; of 200 rows and up to 4096 keys, 32/4 of 64: 208 of
+// 64 87.9, 724 of 13 53.0.  Without a regard to lengths 94.9 and 66.9.)
+__host__ __device__ constexpr float full_tiles(int d, float tiles) { return (d == 128 ? 1.65f : 2.1f) * tiles + 4.f; }
+constexpr int kJoinTiles = 5;
+
+// Tiles of a range of keys where the batch's are shared out: the least with which there are no
+// more ranges than slots, either way, and of the two the cheaper.  Each lane tries its own.
+template <int D>
+__device__ __forceinline__ int range_tiles(const Q4Args& a, const PrefillPlan& p, int lane, int& t) {
+    t = 0;
+    if (lane < p.batch) {
+        const int n = q4_len(a, lane);
+        const int64_t first = q4_first(a, lane, n), hi = min(first + a.rows - 1, (int64_t)n - 1);
+        t = hi >= max(first, (int64_t)0) ? static_cast<int>(hi) / kBN + 1 : 0;
+    }
+    const int most = wave_max(t);
+    const int total = __builtin_amdgcn_readlane(prefix_sum(t), kWave - 1);
+    const int slots = lane < kWave / 2 ? p.slots : p.slots_full;
+    const int least = max(max((total + slots - 1) / slots, kLeastTiles), (most + p.nsplit - 1) / p.nsplit);
+    const int mine = least + (lane & (kWave / 2 - 1)) * (1 + least / 16);
+    int count = 0;
+    for (int b = 0; b < p.batch; ++b) count += (__builtin_amdgcn_readlane(t, b) + mine - 1) / mine;
+    const uint64_t fit = __ballot(count <= slots);
+    const uint32_t one = static_cast<uint32_t>(fit), full = static_cast<uint32_t>(fit >> 32);
+    const int x = one ? __builtin_amdgcn_readlane(mine, __builtin_ctz(one)) : p.tiles;
+    const int y = full ? __builtin_amdgcn_readlane(mine, kWave / 2 + __builtin_ctz(full)) : p.tiles;
+    return full_tiles(D, y) < x ? y : x;
 }
 
 // The 16-byte chunks of LDS rows lie at c ^ swizzle(row): the 16 rows of an operand read of K,
@@ -145,12 +184,22 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     const int h = lane >> 5, c32 = lane & 31;
     const int kvh = blockIdx.x % a.Hkv;
     const int blk = p.blocks - 1 - static_cast<int>(blockIdx.x / a.Hkv);   // longest first
-    const int b = blockIdx.y;
+    int b = blockIdx.y, split = blockIdx.z, range = (p.tiles + p.nsplit - 1) / p.nsplit;
+    if (p.slots) {   // the blockIdx.y-th range of the batch
+        int t;
+        range = range_tiles<D>(a, p, lane, t);
+        const uint32_t mine = (t + range - 1) / range, upto = prefix_sum(mine);
+        const uint64_t past = __ballot(upto > blockIdx.y);
+        if (past == 0) return;
+        b = __builtin_ctzll(past);
+        split = blockIdx.y - (__builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(mine, b));
+    }
+    if (p.nsplit > 1 && (blockIdx.x | blockIdx.y | blockIdx.z | threadIdx.x) == 0) *p.ws_range = range;
     const Block k = block_of(a, p, b, blk, kPairs);
     if (k.p_lo > k.p_hi) return;
-    const int t_lo = static_cast<int>(blockIdx.z) * p.tiles_per_split;
+    const int t_lo = split * range;
     const int all_tiles = k.tiles();
-    const int n = min(all_tiles - t_lo, p.tiles_per_split);
+    const int n = min(all_tiles - t_lo, range);
     if (n <= 0) return;
 
     // This lane's pair.
@@ -175,9 +224,15 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     const int32_t* bt = a.bt + (int64_t)b * a.max_pages;
     const uint8_t* head = a.pool + (int64_t)kvh * a.num_pages * PB;
     const int last_page = k.p_hi >> 4;
-    auto page_of = [&](int t) {   // ids are clamped into the pool
-        const int pi = min((t_lo + min(t, n - 1)) * kWaves + wave, last_page);
-        return __builtin_amdgcn_readfirstlane(min(max(bt[pi], 0), a.num_pages - 1));
+    // Page ids of 64 tiles, a lane each (clamped into the pool): loaded tile by tile, each would be
+    // waited for with the next reads of LDS.
+    int ids = 0;
+    auto page_of = [&](int t) {
+        if (t % kWave == 0 && t < n) {
+            const int pi = min((t_lo + min(t + lane, n - 1)) * kWaves + wave, last_page);
+            ids = min(max(bt[pi], 0), a.num_pages - 1);
+        }
+        return __builtin_amdgcn_readlane(ids, t % kWave);
     };
     const uint8_t* const raw0 = raw[wave][0];
     const uint32_t raw_at = __builtin_amdgcn_readfirstlane(lds_at(raw0));
@@ -409,49 +464,62 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     wait_raw<0>();   // the trailing loads
     bad[wave] = nan_at;
     iterate(std::true_type{}, std::true_type{}, j);
-    if (!live) return;
-    int first_bad = bad[0];   // written before the last barrier
+    ring_barrier();   // the operands' place takes the results
+    int first_bad = bad[0];   // written before the last tile's barrier
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) first_bad = min(first_bad, bad[w]);
-    if (pos >= first_bad) {
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[db][i] = NAN;
-    }
-
-    // Dims of a lane: 32 db + 8 q + (0 4 1 5 for h = 0, 2 6 3 7 for h = 1).
+    const bool cut = all_tiles > range;   // joined by q4_prefill_join_kernel
     const float l = halves_sum(l_part);
-    const int d0 = 2 * h;
-    if (all_tiles > p.tiles_per_split) {   // joined by q4_prefill_join_kernel
-        const int64_t prow = at * p.nsplit + blockIdx.z;
-        float* po = p.ws_o + prow * D + d0;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                *reinterpret_cast<float2*>(po + 32 * db + 8 * q4) = float2{o[db][4 * q4], o[db][4 * q4 + 2]};
-                *reinterpret_cast<float2*>(po + 32 * db + 8 * q4 + 4) = float2{o[db][4 * q4 + 1], o[db][4 * q4 + 3]};
-            }
-        if (h == 0) {
+    if (live && h == 0) {
+        if (cut) {
+            const int64_t prow = at * p.nsplit + split;
             p.ws_ml[prow * 2] = m_run;
             p.ws_ml[prow * 2 + 1] = l;
+        } else if (a.lse) {
+            a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m_run + __builtin_amdgcn_logf(l)) * kLn2;
         }
-        return;
     }
-    const float inv = 1.f / l;
-    f16* orow = a.out + at * D + d0;
+    // Rows of D floats in LDS, 16-byte chunk c of row r at c ^ r: a lane has dims 32 db + 8 q +
+    // 2 h + (0 4 1 5) of its pair and writes whole rows out.
+    constexpr int CPR = D / 4;
+    const float scale = pos >= first_bad ? NAN : cut ? 1.f : 1.f / l;
+    float* const mine = reinterpret_cast<float*>(tiles) + 32 * D * wave;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const half2v x = {static_cast<f16>(o[db][4 * q4] * inv), static_cast<f16>(o[db][4 * q4 + 2] * inv)};
-            const half2v y = {static_cast<f16>(o[db][4 * q4 + 1] * inv), static_cast<f16>(o[db][4 * q4 + 3] * inv)};
-            *reinterpret_cast<half2v*>(orow + 32 * db + 8 * q4) = x;
-            *reinterpret_cast<half2v*>(orow + 32 * db + 8 * q4 + 4) = y;
+        for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<float2*>(mine + D * c32 + 4 * ((8 * db + 2 * q4 + e) ^ (c32 & (CPR - 1))) + 2 * h) =
+                    float2{o[db][4 * q4 + e] * scale, o[db][4 * q4 + 2 + e] * scale};
+    auto row_at = [&](int r, int64_t& to) {   // where the wave's r-th pair goes, if anywhere
+        const int pr = pair0 + r, rw = row_of(p, pr);
+        to = ((int64_t)b * a.rows + rw) * a.Hq + kvh * a.G + pr - rw * a.G;
+        return rw < a.rows && k.first + rw >= k.p_lo && k.first + rw <= k.p_hi;
+    };
+    auto chunk = [&](int r, int c) {
+        return *reinterpret_cast<const floatx4*>(mine + D * r + 4 * (c ^ (r & (CPR - 1))));
+    };
+    int64_t to;
+    if (cut) {
+        for (int i = lane; i < 32 * CPR; i += kWave) {
+            const int r = i / CPR, c = i % CPR;
+            if (row_at(r, to)) *reinterpret_cast<floatx4*>(p.ws_o + (to * p.nsplit + split) * D + 4 * c) = chunk(r, c);
         }
-    if (a.lse && h == 0)
-        a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m_run + __builtin_amdgcn_logf(l)) * kLn2;
+        return;
+    }
+    for (int i = lane; i < 32 * (CPR / 2); i += kWave) {
+        const int r = i / (CPR / 2), c = i % (CPR / 2);
+        if (!row_at(r, to)) continue;
+        const floatx4 x = chunk(r, 2 * c), y = chunk(r, 2 * c + 1);
+        half8 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = static_cast<f16>(x[e]);
+            v[4 + e] = static_cast<f16>(y[e]);
+        }
+        store_half8(a.out + to * D + 8 * c, v);
+    }
 }
 
 // Joins the partials of the blocks that were cut into ranges of keys: R times D / 8 lanes per
@@ -468,8 +536,9 @@ __global__ void __launch_bounds__(256) q4_prefill_join_kernel(const Q4Args a, co
     const int64_t pos = (int64_t)k.first + row;
     if (pos < k.p_lo || pos > k.p_hi) return;
     const int tiles = k.tiles();
-    if (tiles <= p.tiles_per_split) return;
-    const int n = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+    const int range = *p.ws_range;
+    if (tiles <= range) return;
+    const int n = (tiles + range - 1) / range;
     const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
     const float* po = p.ws_o + at * p.nsplit * D + 8 * c;
     const float2* pml = reinterpret_cast<const float2*>(p.ws_ml) + at * p.nsplit;
@@ -522,17 +591,32 @@ __global__ void __launch_bounds__(256) q4_prefill_join_kernel(const Q4Args a, co
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
-// Ranges of keys until every CU has two workgroups, each of at least 3 tiles.
-PrefillPlan plan_of(int batch, int rows, int hkv, int G, int max_len) {
+// Blocks of few rows are cut into ranges of keys, one a CU or as many as it holds, where that
+// saves more than it costs.  Up to 64 sequences' ranges are shared out by their lengths as they are.
+PrefillPlan plan_of(int batch, int rows, int hkv, int G, int d, int max_len) {
     PrefillPlan p{};
     const int64_t pairs = (int64_t)rows * G;
-    const int64_t wgs = (pairs + kPairs - 1) / kPairs * hkv * batch;
+    const int64_t per = (pairs + kPairs - 1) / kPairs * hkv;   // workgroups of a sequence
     p.inv_g = G == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + G - 1) / G);
     p.blocks = static_cast<int>((pairs + kPairs - 1) / kPairs);
-    const int64_t tiles = ((int64_t)max_len + kBN - 1) / kBN;
-    const int64_t n = std::max<int64_t>(std::min<int64_t>(2 * kCUs / wgs, tiles / 3), 1);
-    p.tiles_per_split = static_cast<int>((tiles + n - 1) / n);
-    p.nsplit = static_cast<int>((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+    p.batch = batch;
+    p.tiles = static_cast<int>(((int64_t)max_len + kBN - 1) / kBN);
+    p.nsplit = 1;
+    const int64_t one = kCUs / per, full = (d == 64 ? 3 : 2) * kCUs / per;
+    const auto range = [&](int64_t slots) {   // of equal sequences
+        const int64_t n = slots / batch;
+        return n > 1 ? std::max<int64_t>((p.tiles + n - 1) / n, kLeastTiles) : p.tiles;
+    };
+    if (kJoinTiles + std::min<float>(range(one), full_tiles(d, range(full))) >= p.tiles) return p;
+    const int64_t most = p.tiles / kLeastTiles;
+    if (batch > kWave) {
+        p.nsplit = static_cast<int>(std::min(full / batch, most));
+    } else {
+        p.slots = static_cast<int>(std::max<int64_t>(one, batch));
+        p.slots_full = static_cast<int>(full);
+        // a sequence's at most twice its share
+        p.nsplit = static_cast<int>(std::min(batch == 1 ? full : 2 * ((full + batch - 1) / batch), most));
+    }
     return p;
 }
 
@@ -542,13 +626,13 @@ size_t q4_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int max
     if (rows <= 0 || !bound_sizes(batch, hq, hkv, max_len, 0, 0) ||
         (int64_t)rows * hq > kMaxRowHeads || (d != 64 && d != 128))
         return 0;
-    const PrefillPlan p = plan_of(batch, rows, hkv, hq / hkv, max_len);
-    return p.nsplit == 1 ? 0 : sizeof(float) * (size_t)batch * rows * hq * p.nsplit * (d + 2);
+    const PrefillPlan p = plan_of(batch, rows, hkv, hq / hkv, d, max_len);
+    return p.nsplit == 1 ? 0 : sizeof(float) * ((size_t)batch * rows * hq * p.nsplit * (d + 2) + 1);
 }
 
 bool q4_prefill_fits(const Q4Args& a, int batch) {
     if ((int64_t)a.rows * a.Hq > kMaxRowHeads) return false;   // the plan counts them in an int
-    const PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len);
+    const PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.D, a.max_len);
     return (a.D == 64 || a.D == 128) && aligned16(a.q) && aligned16(a.out) && p.nsplit <= 65535 &&
            (int64_t)p.blocks * a.Hkv <= kMaxRowHeads / kPairs &&
            (int64_t)a.rows * a.G * a.G < (int64_t)1 << 31;   // row_of, and pairs in an int
@@ -556,11 +640,13 @@ bool q4_prefill_fits(const Q4Args& a, int batch) {
 
 // The workspace holds q4_prefill_workspace bytes.
 int q4_prefill(const Q4Args& a, int batch, void* ws, hipStream_t s) {
-    PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.max_len);
+    PrefillPlan p = plan_of(batch, a.rows, a.Hkv, a.G, a.D, a.max_len);
     const size_t rh = (size_t)batch * a.rows * a.Hq;
     p.ws_o = static_cast<float*>(ws);
     p.ws_ml = p.ws_o + rh * p.nsplit * a.D;
-    const dim3 grid(p.blocks * a.Hkv, batch, p.nsplit), threads(kWaves * kWave);
+    p.ws_range = reinterpret_cast<int32_t*>(p.ws_ml + rh * p.nsplit * 2);
+    const dim3 threads(kWaves * kWave);
+    const dim3 grid = p.slots ? dim3(p.blocks * a.Hkv, p.slots_full) : dim3(p.blocks * a.Hkv, batch, p.nsplit);
     if (a.D == 64)
         hipLaunchKernelGGL((q4_prefill_kernel<64>), grid, threads, 0, s, a, p);
     else

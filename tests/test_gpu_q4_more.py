@@ -83,6 +83,29 @@ def test_one_key_above_all(d, late):
     _check_prefill(np.repeat(q[:, None], 390, 1), c, [10], every=29)
 
 
+@pytest.mark.parametrize("B,rows,hq,hkv,d", [(3, 5, 8, 1, 64), (7, 40, 8, 2, 128), (64, 3, 4, 1, 64),
+                                             (65, 3, 4, 1, 64), (5, 130, 7, 1, 128), (16, 9, 20, 1, 64)])
+def test_chunks_of_many_sequences(B, rows, hq, hkv, d):
+    """Ranges of keys shared out by ragged lengths: long sequences among short ones and
+    empty ones, one long one alone, all as long as can be."""
+    rng = np.random.default_rng(B + rows)
+    most = 2600
+    for kind in ("ragged", "one", "all"):
+        lens = rng.integers(0, 150, B)
+        lens[rng.integers(0, B, 2)] = most, 0
+        if kind == "one":
+            lens[:] = rows
+            lens[B // 2] = most
+        elif kind == "all":
+            lens[:] = most if B < 16 else 1300
+        c = Q4Cache(rng, lens, hkv, d).upload()
+        note(f"q4_prefill B={B} rows={rows} {hq}/{hkv} x {d} {kind}")
+        q = _q(rng, B, rows, hq, d)
+        _check_prefill(q, c, np.asarray(lens) - rows, kind, every=17)
+        c.cap = 9000 if kind == "one" else 1000   # a limit above and below the lengths
+        _check_prefill(q, c, np.asarray(lens) - rows, f"{kind} cap", every=17)
+
+
 def test_pools_past_32_bits():
     """Pages of more than 4 GiB per head: the bits of the same rows in a small pool."""
     rng = np.random.default_rng(9)
