@@ -1,27 +1,38 @@
 // q4_prefill.hip -- rows of prompts and chunks over a paged cache held in 4 bits (gfx950,
 // head_dim 64 and 128).
 //
-// A workgroup of W waves takes one KV head of one sequence and 32 W of its (row, query head)
+// A workgroup of four waves takes one KV head of one sequence and 128 of its (row, query head)
 // pairs, query head fastest, 32 pairs a wave, and walks the keys up to its last row in tiles of
-// 64.  Each tile's codes are turned into operands once for all its waves: a wave loads the
-// codes of its share of the tile's pages into registers, one tile ahead, and writes them to LDS
-// as fp16 while the matrix cores are at the tile before.  The operands are exact (q4.h): a code
-// with its four bits in mantissa bits 6..9 below the exponent of 16 is 16 + n, and times E
-// plus (r - 16) E it is (n + r) E; E = 1 for K, for V the power of two that leaves s / E = m
-// between 4 and 8 (less for scales below 2^-12).  K's s multiplies the scores inside the
-// exponent's multiply-add, V's m a weight before its one rounding to fp16.
+// 64.  Each tile's codes are turned into operands once for all its waves: a wave brings its page
+// of the tile into LDS as it is, one tile ahead (global_load_lds), and writes it out again as
+// fp16 while the matrix cores are at the tile before.  The operands are exact (q4.h).  K's are
+// (n + r) 2^-9 from the denormals that the codes are in a half's low bits (q4_decode.hip has the
+// same); V's are (n + r) E: four bits in mantissa bits 6..9 below the exponent of 16 are 16 + n,
+// and times E plus (r - 16) E that is it; E is the power of two that leaves s / E = m between 4
+// and 8 (less for scales below 2^-12).  K's s multiplies the scores inside the exponent's
+// multiply-add, V's m a weight before its one rounding to fp16.
 //
-// Per tile, on v_mfma_f32_32x32x16_f16 with one lane per pair: S^T = K Q^T of the next tile
-// beside the exponentials of this one; then O^T += V^T W^T beside the next codes' conversion.
-// Weights are taken against a reference that moves when one of a row passes it by 2^12 (to
-// 2^4), seen from the weights themselves, so that no maximum of the scores is needed: 2^-11 of
-// each holds down to 2^-16 of the reference, below it is an absolute 2^-27 of it.
+// Per tile, on v_mfma_f32_32x32x16_f16 with one lane per pair, in halves of 32 keys: S^T = K Q^T
+// and O^T += V^T W^T beside the exponentials and the next codes' conversion, each operand read
+// from LDS a phase before its product.
+// Weights are taken against a reference that moves when a sum of 16 of a row's passes 2^12 (to
+// 2^4 for the largest), seen from the weights themselves, so that no maximum of the scores is
+// needed: 2^-11 of each holds down to 2^-16 of the reference, below it is an absolute 2^-27 of it.
 //
 // A key that holds NaN has operands of 0.  K's scale is NaN, which a row that does not see the
 // key drops with its weight; of V's the first is kept, and the rows at or past it are NaN.
 //
-// Few rows over a long cache are cut into ranges of keys (blockIdx.z) whose partials a second
-// launch joins.
+// Few rows over a long cache are cut into ranges of keys whose partials a second launch joins.
+//
+// What bounds it: the vector unit.  8192 rows of 32/8 heads of 128 take 642 to 660 us (550 GFLOP,
+// 833 to 857 TFLOP/s, a third of the matrix cores' peak): of a tile's 2700 cycles a SIMD spends
+// some 1400 on vector instructions (32 exponentials of 16 cycles each, their multiply-adds, sums
+// and conversions: 960; the codes: 340), 1024 on products, and LDS is busy for half of them (each
+// wave reads all of a tile's operands: 32 KB).  Two waves a SIMD is what 245 registers leave; more
+// pairs a wave would halve the operand reads but not fit beside O.  Of what was tried: eight waves
+// a workgroup (fewer conversions a pair, longer waits at its barriers) and hints to the scheduler
+// were slower; pages through registers spilled (930 us); the row maxima in place of the check of
+// the sums cost 11 us, sixteens in place of denormals for K 8.
 #include "q4.h"
 
 #include <algorithm>
@@ -117,9 +128,9 @@ __device__ __forceinline__ int vswz(int r) {
 
 __device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
 struct CodeBits {
-    uint32_t mask = 0x03c003c0u, sixteen = 0x4c004c00u;
+    uint32_t mask = 0x03c003c0u, sixteen = 0x4c004c00u, low = 0x000f000fu, high = 0x00f000f0u;
     // in registers: as literals they would keep v_and_or_b32 from taking both
-    __device__ __forceinline__ CodeBits() { asm("" : "+s"(mask), "+v"(sixteen)); }
+    __device__ __forceinline__ CodeBits() { asm("" : "+s"(mask), "+v"(sixteen), "+s"(low), "+s"(high)); }
 };
 // Eight codes as (n + r) E, in the order 0 4 1 5 2 6 3 7.
 __device__ __forceinline__ half8 operand(uint32_t x, half2v e, half2v f, const CodeBits& c) {
@@ -127,6 +138,18 @@ __device__ __forceinline__ half8 operand(uint32_t x, half2v e, half2v f, const C
         return __builtin_elementwise_fma(as_half2((y & c.mask) | c.sixteen), e, f);
     };
     const half2v p0 = pair(x << 6), p1 = pair(x << 2), p2 = pair(x >> 2), p3 = pair(x >> 6);
+    return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+
+// Eight codes as (n + r) 2^-9, in the same order, given r 2^-9: four bits at the bottom of a half are
+// n 2^-24, at bits 4..7 n 2^-20.
+__device__ __forceinline__ half8 small_operand(uint32_t x, half2v f, const CodeBits& c) {
+    auto pair = [&](uint32_t y, f16 e) {
+        return __builtin_elementwise_fma(as_half2(y), half2v{e, e}, f);
+    };
+    const f16 e0 = 32768.f, e4 = 2048.f;
+    const uint32_t y = x >> 8;
+    const half2v p0 = pair(x & c.low, e0), p1 = pair(x & c.high, e4), p2 = pair(y & c.low, e0), p3 = pair(y & c.high, e4);
     return half8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
@@ -250,7 +273,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     const uint32_t lds0 = lds_at(tiles);
     const uint32_t kput = 2 * ((kPage * wave + crow) * D) + 16 * ((D / 32 * cc) ^ kswz<D>(kPage * wave + crow));
     const uint32_t vput = 2 * ((kPage * wave + crow) * D) + 16 * ((D / 32 * cc) ^ vswz<D>(kPage * wave + crow));
-    auto convert = [&](const uint8_t* codes, half2v e2, half2v f2, uint32_t to) {
+    auto convert = [&](const uint8_t* codes, auto&& operand_of, uint32_t to) {
         uint32_t x[D / 32];
         if constexpr (D == 128) {
             const u32x4 y = *reinterpret_cast<const u32x4*>(codes);
@@ -263,7 +286,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         }
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
-            *reinterpret_cast<__attribute__((address_space(3))) half8*>(to ^ 16 * i) = operand(x[i], e2, f2, bits);
+            *reinterpret_cast<__attribute__((address_space(3))) half8*>(to ^ 16 * i) = operand_of(x[i]);
     };
     // This lane's row of a tile's V: E and (r - 16) E, kept from the numbers' read to the codes'.
     half2v v_e, v_f;
@@ -276,7 +299,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         const uint8_t* num = r0 + 2 * kPage * RB + 4 * crow;
         uint32_t ks = *reinterpret_cast<const uint32_t*>(num), vs = *reinterpret_cast<const uint32_t*>(num + 64);
         const bool behind = key0 + t * kBN > k.p_hi;   // the last key
-        scale_s[t & 1][sat] = static_cast<float>(as_half2(ks)[0]) * a.scale_log2;   // by four lanes alike
+        scale_s[t & 1][sat] = static_cast<float>(as_half2(ks)[0]) * (512.f * a.scale_log2);   // by four lanes alike
         // of NaN and of what is behind the last key: operands of 0
         ks = behind || (ks & 0x7c00u) == 0x7c00u ? 0u : ks;
         const bool nan = !behind && (vs & 0x7c00u) == 0x7c00u;
@@ -289,12 +312,13 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
         v_e = half2v{eh, eh};
         v_f = (half2v{as_half2(vs)[1], as_half2(vs)[1]} + half2v{f16(-16), f16(-16)}) * v_e;
-        const half2v k_f = half2v{as_half2(ks)[1], as_half2(ks)[1]} + half2v{f16(-16), f16(-16)};
-        convert(r0 + RB / 4 * lane, half2v{f16(1), f16(1)}, k_f, lds0 + (t & 1) * TB + kput);
+        const half2v k_f = half2v{as_half2(ks)[1], as_half2(ks)[1]} * half2v{f16(0x1p-9f), f16(0x1p-9f)};
+        convert(r0 + RB / 4 * lane, [&](uint32_t x) { return small_operand(x, k_f, bits); },
+                lds0 + (t & 1) * TB + kput);
     };
     auto put_v = [&](int t) {
-        convert(raw0 + (RST == 2 ? (t & 1) * RAW : 0) + kPage * RB + RB / 4 * lane, v_e, v_f,
-                lds0 + (2 + (t & 1)) * TB + vput);
+        convert(raw0 + (RST == 2 ? (t & 1) * RAW : 0) + kPage * RB + RB / 4 * lane,
+                [&](uint32_t x) { return operand(x, v_e, v_f, bits); }, lds0 + (2 + (t & 1)) * TB + vput);
     };
 
     // ---- operand reads: K's chunk 2 c + h of row c32 (and 32), V's of 32-dim block db
@@ -346,11 +370,10 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         for (int c = 0; c < NC; ++c) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8.x[c], qop[c], s, 0, 0, 0);
         return s;
     };
-    // Weights as the operands of O^T's product; returns the largest and adds up the sum before
-    // the rounding.
-    auto weights = [&](auto MASKED_, int j, int u, const floatx16& s, half8 (&w)[2], float& sum) {
+    // Weights as the operands of O^T's product; returns their sum before the rounding.
+    auto weights = [&](auto MASKED_, int j, int u, const floatx16& s, half8 (&w)[2]) {
         constexpr bool MASKED = decltype(MASKED_)::value;
-        float most = 0.f, ps[2] = {0.f, 0.f};
+        float ps[2] = {0.f, 0.f};
         int seen = seen0 - j * kBN - 32 * u;
         asm volatile("" : "+v"(seen));   // compared where it is used: kept masks would spill
         const float* ks = &scale_s[j & 1][32 * h + 16 * u];
@@ -364,12 +387,10 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
                 float x = fast_exp2(fmaf(s[i + e], k4[e], -m_run));
                 if (MASKED && 2 * i + e > seen) x = 0.f;
                 w[i / 8][i % 8 + e] = static_cast<f16>(x * m4[e]);
-                most = fmaxf(most, x);
                 ps[e & 1] += x;
             }
         }
-        sum = ps[0] + ps[1];
-        return most;
+        return ps[0] + ps[1];
     };
     // Moves the reference of rows with a weight past 2^12 to 2^4 below their largest score.
     auto refer = [&](int j, int u, const floatx16& s) {
@@ -396,10 +417,12 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
             for (int db = 0; db < NDB; ++db)
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8.x[t][db], w[t], o[db], 0, 0, 0);
     };
-    auto checked = [&](int j, int u, float most, const floatx16& s, half8 (&w)[2], float& sum) {
-        if (__builtin_amdgcn_read_exec() & __ballot(most > kMostWeight)) {
+    // A weight past 2^12 shows in the sum (which passes it with none that large only where the
+    // reference would have moved before long).
+    auto checked = [&](int j, int u, float sum, const floatx16& s, half8 (&w)[2]) {
+        if (__builtin_amdgcn_read_exec() & __ballot(sum > kMostWeight)) {
             refer(j, u, s);   // now none is past 2^4
-            weights(std::true_type{}, j, u, s, w, sum);
+            sum = weights(std::true_type{}, j, u, s, w);
         }
         l_part += sum;
     };
@@ -441,14 +464,11 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         fence();
         const floatx16 s1 = qk(k1);
         half8 w0[2], w1[2];
-        float sum0, sum1;
-        float most = weights(MASKED_, j, 0, s0, w0, sum0);
-        checked(j, 0, most, s0, w0, sum0);
+        checked(j, 0, weights(MASKED_, j, 0, s0, w0), s0, w0);
         const VOps v1 = read_v(j, 1);
         fence();
         pv(v0, w0);
-        most = weights(MASKED_, j, 1, s1, w1, sum1);
-        checked(j, 1, most, s1, w1, sum1);
+        checked(j, 1, weights(MASKED_, j, 1, s1, w1), s1, w1);
         pv(v1, w1);
         if constexpr (!LAST) {
             if constexpr (RST == 1) wait_raw<2>();
