@@ -393,7 +393,8 @@ int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int32_t* ages,
  * Rows at negative slots or at or past seq_lens[b] (device int32, NULL: no limit) are
  * padding: they reach nothing, and their q_out stays as it was.  K and V of a slot past the block
  * table, or whose page id lies outside [0, num_pages), are dropped (write tables hold -1
- * for shared pages); its q is rotated all the same.  head_dim is even and at most 256;
+ * for shared pages); its q is rotated all the same.  Where two rows go to the same slot of a
+ * page, what it holds then is undefined.  head_dim is even and at most 256;
  * batch rows (Hq + 2 Hkv) is at most 2^25 where head_dim is neither 64 nor 128 or a tensor
  * is off 16-byte alignment (rows then go one by one, several times slower).
  * Asynchronous, allocates nothing, may be captured. */

@@ -568,6 +568,11 @@ constexpr int kWaveSlots = 2048;   // one wave per split, two per SIMD of 256 CU
 constexpr int kWaves = 4;          // per workgroup in fixed splits
 constexpr int kShortWaves = 8;     // and where a sequence is one split
 
+// Most splits that a batch may have: along a grid's second axis.
+int64_t most_splits(int64_t batch, int64_t tiles, int balance) {
+    return std::max<int64_t>(balance, (batch * tiles + kMaxTiles - 1) / kMaxTiles) + batch;
+}
+
 DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t max_len) {
     DecodePlan p{};
     p.batch = batch;
@@ -579,9 +584,10 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t max_len) {
         p.nsplit = 1;
         return p;
     }
-    if (batch >= kBalanced) {
+    const int64_t balance = std::max<int64_t>(1, kWaveSlots / heads - batch / 2);
+    if (batch >= kBalanced && most_splits(batch, tiles, balance) <= 65535) {
         p.waves = 1;
-        p.balance = static_cast<int>(std::max<int64_t>(1, kWaveSlots / heads - batch / 2));
+        p.balance = static_cast<int>(balance);
         // splits of a sequence: of the target, which is the least where it alone has keys
         const int64_t target =
             std::min<int64_t>(std::max<int64_t>((tiles + p.balance - 1) / p.balance, kMinTiles), kMaxTiles);
@@ -595,13 +601,6 @@ DecodePlan plan_of(int batch, int hkv, int G, int d, int64_t max_len) {
     p.nsplit = static_cast<int>((tiles + per - 1) / per);
     return p;
 }
-// Workgroups of the first launch along its second axis.
-int64_t units_of(const DecodePlan& p, int64_t max_len) {
-    if (p.balance == 0) return p.nsplit;
-    const int64_t worst = (p.batch * ((max_len + kTok - 1) / kTok) + kMaxTiles - 1) / kMaxTiles;
-    return std::max<int64_t>(p.balance, worst) + p.batch;
-}
-
 }  // namespace
 
 size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len) {
@@ -613,7 +612,7 @@ size_t q4_decode_workspace(int batch, int hq, int hkv, int d, int max_len) {
 bool q4_decode_fits(const Q4Args& a, int batch) {
     const DecodePlan p = plan_of(batch, a.Hkv, a.G, a.D, a.max_len);
     return (a.D == 64 || a.D == 128) && aligned16(a.q) && aligned16(a.out) &&
-           units_of(p, a.max_len) <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
+           p.nsplit <= 65535 && (int64_t)a.Hkv * p.groups <= INT32_MAX;
 }
 
 // The workspace holds q4_decode_workspace bytes.
@@ -622,7 +621,9 @@ int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s) {
     p.ws_o = static_cast<float*>(ws);
     p.ws_ml = p.ws_o + (size_t)batch * a.Hq * p.nsplit * a.D;
     p.ws_n = reinterpret_cast<int32_t*>(p.ws_ml + (size_t)batch * a.Hq * p.nsplit * 2);
-    const dim3 grid(a.Hkv * p.groups, static_cast<unsigned>(units_of(p, a.max_len)), p.balance ? 1 : batch);
+    const int64_t tiles = ((int64_t)a.max_len + kTok - 1) / kTok;
+    const int64_t splits = p.balance ? most_splits(batch, tiles, p.balance) : p.nsplit;
+    const dim3 grid(a.Hkv * p.groups, static_cast<unsigned>(splits), p.balance ? 1 : batch);
     auto go = [&](auto d, auto pk) {
         constexpr int D = decltype(d)::value, PK = decltype(pk)::value;
         const dim3 threads(p.waves * kWave);

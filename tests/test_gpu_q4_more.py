@@ -230,6 +230,40 @@ def test_addresses_off_16_bytes(d):
     assert (holds(from_gpu(out), "prefill") == 7).all()
 
 
+def test_more_sequences_than_a_grid_axis_of_splits():
+    """5000 sequences that might have 16384 keys each."""
+    rng = np.random.default_rng(50)
+    B, d = 5000, 64
+    c = Q4Cache(rng, rng.integers(0, 40, B), 1, d, cap=16384).upload()
+    note(f"q4_decode B={B}")
+    _check_decode(_q(rng, B, 2, d), c)
+
+
+@pytest.mark.parametrize("d", [40, 64, 128])
+def test_positions_before_the_text(d):
+    """Negative positions rotate the other way, if their slots are not."""
+    rng = np.random.default_rng(d)
+    hq, hkv, R = 4, 2, 9
+    x = _q(rng, 2, R, hq + 2 * hkv, d)
+    t = to_gpu(x)
+    pos, slots = np.array([-5, -(1 << 31)], np.int32), np.array([0, 3], np.int32)
+    pk, pv = (torch.zeros((hkv, 2, PAGE, d), dtype=torch.float16, device="cuda") for _ in range(2))
+    q = torch.zeros((2, R, hq, d), dtype=torch.float16, device="cuda")
+    note(f"rope_append at negative positions d={d}")
+    kvhp.rope_append(t[:, :, :hq], t[:, :, hq:hq + hkv], t[:, :, hq + hkv:], to_gpu(pos), q, pk, pv,
+                     to_gpu(np.array([[0], [1]], np.int32)), hq, hkv, d, 10000.0, slots=to_gpu(slots))
+    sync()
+    at = (pos[:, None].astype(np.int64) + np.arange(R))[..., None]
+    want, e = rotated(x[:, :, :hq], at, 10000.0)
+    assert (np.abs(from_gpu(q) - want) <= np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + e * 1.01).all()
+    want, e = rotated(x[:, :, hq:hq + hkv], at, 10000.0)
+    got = from_gpu(pk)
+    for b in range(2):
+        g = got[:, b, slots[b]:slots[b] + R].transpose(1, 0, 2)
+        assert (np.abs(g - want[b]) <= np.abs(want[b]) * 2.0 ** -11 + 2.0 ** -25 + e[b] * 1.01).all()
+        assert np.array_equal(from_gpu(pv)[:, b, slots[b]:slots[b] + R].transpose(1, 0, 2), x[b, :, hq + hkv:])
+
+
 @pytest.mark.parametrize("hq,hkv", [(16380, 2), (16381, 2), (4, 9000)])
 def test_append_of_many_heads(hq, hkv):
     """Both sides of the most heads a workgroup's rows are counted for."""
