@@ -200,7 +200,8 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
     __shared__ __attribute__((aligned(8192))) f16 tiles[4 * kBN * D];
     __shared__ __attribute__((aligned(16))) uint8_t raw[kWaves][RST][RAW];
     // a tile's s log2(e) / sqrt(D) and m in the order a lane of half h takes them: [h][32 keys]
-    __shared__ __attribute__((aligned(16))) float scale_s[2][kBN], scale_m[2][kBN];
+    __shared__ __attribute__((aligned(16))) float scale_s[2][kBN];
+    __shared__ __attribute__((aligned(16))) f16 scale_m[2][kBN];
     __shared__ int bad[kWaves];            // each wave's first key whose V is NaN
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -305,8 +306,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         const bool nan = !behind && (vs & 0x7c00u) == 0x7c00u;
         vs = behind || nan ? 0u : vs;
         const int e = max((int)(vs & 0x7c00u) - 0x0800, 0x0400);
-        scale_m[t & 1][sat] = static_cast<float>(as_half2(vs)[0]) *
-                              static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e)));
+        scale_m[t & 1][sat] = as_half2(vs)[0] * __builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e));   // exact
         const uint64_t nans = __ballot(nan);
         nan_at = nans && nan_at == INT32_MAX ? t_lo * kBN + t * kBN + kPage * wave + (__builtin_ctzll(nans) >> 2) : nan_at;
         const f16 eh = __builtin_bit_cast(f16, static_cast<uint16_t>(e));
@@ -377,16 +377,17 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         int seen = seen0 - j * kBN - 32 * u;
         asm volatile("" : "+v"(seen));   // compared where it is used: kept masks would spill
         const float* ks = &scale_s[j & 1][32 * h + 16 * u];
-        const float* vm = &scale_m[j & 1][32 * h + 16 * u];
+        const f16* vm = &scale_m[j & 1][32 * h + 16 * u];
+        // in fp16, where it is exact, and multiplied from there (v_fma_mix_f32; a product gets no such)
+        const half8 m8[2] = {*reinterpret_cast<const half8*>(vm), *reinterpret_cast<const half8*>(vm + 8)};
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const floatx4 k4 = *reinterpret_cast<const floatx4*>(ks + i);
-            const floatx4 m4 = *reinterpret_cast<const floatx4*>(vm + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float x = fast_exp2(fmaf(s[i + e], k4[e], -m_run));
                 if (MASKED && 2 * i + e > seen) x = 0.f;
-                w[i / 8][i % 8 + e] = static_cast<f16>(x * m4[e]);
+                w[i / 8][i % 8 + e] = static_cast<f16>(fmaf(x, static_cast<float>(m8[i / 8][i % 8 + e]), 0.f));
                 ps[e & 1] += x;
             }
         }
