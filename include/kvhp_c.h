@@ -443,7 +443,7 @@ int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int max_pages,
  * and hold *_workspace_bytes bytes (0: NULL is fine); calls that overlap need one each.
  * How the work is cut goes by max_seq_len: pass the longest length of the step.  The fast
  * kernels take head_dim 64 and 128 with q and out 16-byte aligned; other shapes run on a
- * kernel for any, which is tens of times slower in long caches. */
+ * kernel for any, which takes two to four times as long. */
 size_t kvhp_q4_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
                                       int max_seq_len);
 int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables, int max_pages,

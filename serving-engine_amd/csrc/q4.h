@@ -1,6 +1,6 @@
 // q4.h -- the paged KV cache held in 4 bits: page layout, quantiser, arguments, shared by
-// its append, gather and attention kernels (q4.hip, q4_append.hip, q4_decode.hip,
-// q4_prefill.hip).
+// its append, gather and attention kernels (rope_append.hip, q4.hip, q4_decode.hip,
+// q4_prefill.hip, q4_any.hip).
 //
 // A row x of D values (one token's K or V of one KV head) is held as D codes n of 0..15 and
 // two fp16 numbers s and r, and stands for s (n + r):
@@ -141,5 +141,8 @@ int q4_decode(const Q4Args& a, int batch, void* ws, hipStream_t s);
 size_t q4_prefill_workspace(int batch, int rows, int hq, int hkv, int d, int max_len);
 bool q4_prefill_fits(const Q4Args& a, int batch);
 int q4_prefill(const Q4Args& a, int batch, void* ws, hipStream_t s);
+// q4_any.hip: either at any shape.
+size_t q4_any_workspace(int batch, int rows, int hq, int hkv, int d, int max_len);
+int q4_any(const Q4Args& a, int batch, const char* what, void* ws, size_t room, hipStream_t s);
 
 }  // namespace kvhp

@@ -1,73 +1,11 @@
 // q4.hip -- attention over a paged cache held in 4 bits, and its rows read back: entry
-// points, and the attention kernel that takes any shape.
-//
-// Any head_dim that is a multiple of 8, any group: one wave per (query head, row), one pass
-// over its visible keys with an online softmax, fp32 throughout.  For rare shapes and no
-// more: one key per trip behind a six-step sum over the wave.
+// points, and the kernel that reads back.
 #include "q4.h"
 
 #include <algorithm>
 
 namespace kvhp {
 namespace {
-
-// One wave per (row, query head) of a sequence.
-__global__ void __launch_bounds__(kWave) q4_rows_kernel(const Q4Args a) {
-    const int lane = threadIdx.x;
-    const int row = blockIdx.x / a.Hq, qh = blockIdx.x % a.Hq, b = blockIdx.y;
-    const int kvh = qh / a.G, D = a.D;
-    const int64_t at = ((int64_t)b * a.rows + row) * a.Hq + qh;
-    const int n = q4_len(a, b);
-    const int64_t p = q4_first(a, b, n) + row;
-    if (p < 0 || p >= n) {
-        if (a.last_row)   // no keys
-            for (int d = lane; d < D; d += kWave) a.out[at * D + d] = f16(0);
-        return;
-    }
-    float qv[4], acc[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + kWave * i;
-        qv[i] = d < D ? static_cast<float>(a.q[at * D + d]) : 0.f;
-        acc[i] = 0.f;
-    }
-    const int32_t* bt = a.bt + (int64_t)b * a.max_pages;
-    const int sh = 4 * (lane & 1);   // dims lane + 64 i: the same half of a byte
-    float m = -1e30f, l = 0.f;
-    for (int j = 0; j <= static_cast<int>(p); ++j) {
-        const uint8_t* pg = q4_page(a.pool, a.num_pages, D, kvh, bt[j >> 4]);
-        const int o = j & 15;
-        const Q4Row kp = q4_row(*reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, 0, o)));
-        const Q4Row vp = q4_row(*reinterpret_cast<const uint32_t*>(pg + q4_params_at(D, 1, o)));
-        float dot = 0.f, v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = lane + kWave * i;
-            v[i] = 0.f;
-            if (d < D) {
-                const int kn = pg[q4_codes_at(D, 0, o) + d / 2] >> sh & 15;
-                const int vn = pg[q4_codes_at(D, 1, o) + d / 2] >> sh & 15;
-                dot = fmaf(qv[i], static_cast<float>(kn) + kp.r, dot);
-                v[i] = vp.s * (static_cast<float>(vn) + vp.r);
-            }
-        }
-        const float s = wave_sum(dot) * kp.s * a.scale_log2;
-        const float mn = fmaxf(m, s);
-        const float al = fast_exp2(m - mn), w = fast_exp2(s - mn);
-        l = l * al + w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * al);
-        m = mn;
-    }
-    const float inv = 1.f / l;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + kWave * i;
-        if (d < D) a.out[at * D + d] = static_cast<f16>(acc[i] * inv);
-    }
-    if (a.lse && lane == 0)
-        a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
-}
 
 // Rows read back: a thread takes 8 dims of K and V of two positions, the loads of both in
 // flight together (8192 positions of 8 heads of 128: 9.2 us, 4.6 TB/s; one position 11.4).
@@ -158,14 +96,6 @@ int workspace_check(const char* what, const void* ws, size_t bytes, size_t need)
     return KVHP_OK;
 }
 
-int launch_rows(const Q4Args& a, int batch, const char* what, hipStream_t s) {
-    KVHP_REQUIRE((int64_t)a.rows * a.Hq <= 1 << 25, KVHP_ERR_UNSUPPORTED,   // 2^31 threads
-                 "%s: %d rows of %d heads", what, a.rows, a.Hq);
-    hipLaunchKernelGGL(q4_rows_kernel, dim3(static_cast<unsigned>(a.rows) * a.Hq, batch),
-                       dim3(kWave), 0, s, a);
-    return check_launch(what);
-}
-
 }  // namespace
 }  // namespace kvhp
 
@@ -208,7 +138,10 @@ extern "C" int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int
 
 extern "C" size_t kvhp_q4_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
                                                  int head_dim, int max_seq_len) {
-    return q4_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len);
+    // at 64 and 128 the same rows off their alignment make do with it
+    return head_dim == 64 || head_dim == 128
+               ? q4_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len)
+               : q4_any_workspace(batch, 1, num_q_heads, num_kv_heads, head_dim, max_seq_len);
 }
 
 extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables,
@@ -229,18 +162,21 @@ extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* bl
     a.seq_lens = seq_lens;
     a.rows = 1;
     a.last_row = 1;
-    rc = workspace_check(what, workspace, workspace_bytes,
-                         q4_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len));
+    const size_t need =
+        kvhp_q4_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len);
+    rc = workspace_check(what, workspace, workspace_bytes, need);
     if (rc) return rc;
     if (q4_decode_fits(a, batch))
         return q4_decode(a, batch, workspace, static_cast<hipStream_t>(stream));
-    return launch_rows(a, batch, what, static_cast<hipStream_t>(stream));
+    return q4_any(a, batch, what, workspace, need, static_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t kvhp_q4_prefill_workspace_bytes(int batch, int rows, int num_q_heads,
                                                   int num_kv_heads, int head_dim,
                                                   int max_seq_len) {
-    return q4_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
+    return head_dim == 64 || head_dim == 128
+               ? q4_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len)
+               : q4_any_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
 }
 
 extern "C" int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* block_tables,
@@ -262,11 +198,11 @@ extern "C" int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* b
     a.q_start = q_start;
     a.seq_lens = seq_lens;
     a.rows = rows;
-    rc = workspace_check(what, workspace, workspace_bytes,
-                         q4_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim,
-                                              max_seq_len));
+    const size_t need = kvhp_q4_prefill_workspace_bytes(batch, rows, num_q_heads, num_kv_heads,
+                                                        head_dim, max_seq_len);
+    rc = workspace_check(what, workspace, workspace_bytes, need);
     if (rc) return rc;
     if (q4_prefill_fits(a, batch))
         return q4_prefill(a, batch, workspace, static_cast<hipStream_t>(stream));
-    return launch_rows(a, batch, what, static_cast<hipStream_t>(stream));
+    return q4_any(a, batch, what, workspace, need, static_cast<hipStream_t>(stream));
 }

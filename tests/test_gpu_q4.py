@@ -252,7 +252,7 @@ def test_hidden_rows_reach_nothing(d):
 def test_garbage_in_hidden_slots():
     """Any bytes behind the lengths and in other pages: the same bits."""
     rng = np.random.default_rng(3)
-    for d in (64, 128):
+    for d in (64, 128, 96):
         c = Q4Cache(rng, [75, 33, 1], 2, d).upload()
         q = _q(rng, 3, 8, d)
         qp = _q(rng, 3, 33, 8, d)

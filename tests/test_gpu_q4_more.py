@@ -106,6 +106,55 @@ def test_chunks_of_many_sequences(B, rows, hq, hkv, d):
         _check_prefill(q, c, np.asarray(lens) - rows, f"{kind} cap", every=17)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 8), (6, 2, 24), (8, 1, 56), (32, 2, 72), (6, 6, 80), (14, 2, 96),
+                                      (8, 2, 112), (20, 1, 136), (4, 1, 160), (3, 1, 192), (34, 2, 200),
+                                      (8, 2, 248), (4, 2, 256)])
+def test_any_head_dim(hq, hkv, d):
+    """Tokens, chunks and prompts over ragged lengths, with ranges of keys and without."""
+    rng = np.random.default_rng(hq + d)
+    c = Q4Cache(rng, [1500, 0, 77, 64, 1], hkv, d).upload()
+    note(f"q4_decode {hq}/{hkv} x {d}")
+    _check_decode(_q(rng, 5, hq, d), c)
+    note("chunks")
+    _check_prefill(_q(rng, 5, 11, hq, d), c, [1489, 0, 66, 60, -3], every=3)
+    note("a prompt")
+    c = Q4Cache(rng, [150, 131], hkv, d).upload()
+    _check_prefill(_q(rng, 2, 150, hq, d), c, None, every=31)
+    note("steep scores and rows of many sizes")
+    c = Q4Cache(rng, [300], hkv, d, scale=3.0, offset=20.0)
+    c.parts[3][:, ::2, ::3, 0] *= np.float16(50)
+    c.parts[3][:, 1::2, ::2, 0] *= np.float16(1e-4)
+    c.parts[3][:, :, 5, 0] *= np.float16(-1)
+    c.stand()
+    c.upload()
+    _check_decode(_q(rng, 1, hq, d), c)
+    _check_prefill(_q(rng, 1, 40, hq, d), c, [260], every=7)
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_chunks_off_16_bytes(d):
+    """More rows than one wave takes, q and out off their alignment, over ranges of keys."""
+    rng = np.random.default_rng(d)
+    c = Q4Cache(rng, [1900, 60], 2, d).upload()
+    x = _q(rng, 2, 30, 8, d)
+    q = torch.empty(x.size + 1, dtype=torch.float16, device="cuda")[1:].view(x.shape)
+    q.copy_(to_gpu(x))
+    out = torch.full((x.size + 1,), 7.0, dtype=torch.float16, device="cuda")[1:].view(x.shape)
+    note(f"q4_prefill off 16 bytes d={d}")
+    kvhp.q4_prefill(q, c.pool, c.bt_d, out, 8, 2, d, c.cap, q_start=to_gpu(np.array([1870, 40], np.int32)),
+                    seq_lens=c.lens_d,
+                    workspace=workspace(kvhp.q4_prefill_workspace_bytes(2, 30, 8, 2, d, c.cap)))
+    sync()
+    got = from_gpu(out)
+    assert (got[1, 20:] == 7).all()
+    for b, first, rows in ((0, 1870, 30), (1, 40, 20)):
+        for r in range(0, rows, 6):
+            for h in range(2):
+                n, hs = first + r + 1, slice(4 * h, 4 * h + 4)
+                o, tol, _, _, _ = attend(x[b, r, hs], c.k[b, h, :n], c.v[b, h, :n], np.ones(n, bool))
+                check(got[b, r, hs], o, tol, f"sequence {b} row {r} head {h}")
+
+
 def test_pools_past_32_bits():
     """Pages of more than 4 GiB per head: the bits of the same rows in a small pool."""
     rng = np.random.default_rng(9)
