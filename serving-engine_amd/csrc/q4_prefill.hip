@@ -24,12 +24,12 @@
 //
 // Few rows over a long cache are cut into ranges of keys whose partials a second launch joins.
 //
-// What bounds it: the vector unit.  8192 rows of 32/8 heads of 128 take 642 to 660 us (550 GFLOP,
-// 833 to 857 TFLOP/s, a third of the matrix cores' peak): of a tile's 2700 cycles a SIMD spends
-// some 1400 on vector instructions (32 exponentials of 16 cycles each, their multiply-adds, sums
-// and conversions: 960; the codes: 340), 1024 on products, and LDS is busy for half of them (each
-// wave reads all of a tile's operands: 32 KB).  Two waves a SIMD is what 245 registers leave; more
-// pairs a wave would halve the operand reads but not fit beside O.  Of what was tried: eight waves
+// What bounds it: the vector unit.  8192 rows of 32/8 heads of 128 take 637 to 660 us (550 GFLOP,
+// 833 to 863 TFLOP/s, a third of the matrix cores' peak): it is busy for 62 % of the SIMDs' cycles
+// (a tile's 32 exponentials of 16 cycles each, their multiply-adds, sums and conversions: some 960
+// of 2600; the codes: 340), the matrix cores for 43 %, LDS for 55 % (each wave reads all of a
+// tile's operands, 32 KB).  Two waves a SIMD is what 240 registers leave; more pairs a wave would
+// halve the operand reads but not fit beside O.  Of what was tried: eight waves
 // a workgroup (fewer conversions a pair, longer waits at its barriers) and hints to the scheduler
 // were slower; pages through registers spilled (930 us); the row maxima in place of the check of
 // the sums cost 11 us, sixteens in place of denormals for K 8.
