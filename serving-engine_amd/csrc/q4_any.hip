@@ -230,38 +230,58 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
     }
 }
 
-// Joins the ranges of a (row, head): a thread takes four dims.
+// Joins the ranges of a (row, head): P threads of a workgroup, D / 4 of them side by side, each four
+// dims of every (P / (D / 4))-th range, four loads in flight.  P = 256 for many ranges; else 64, where
+// a workgroup has four (row, head)s.
+template <int P>
 __global__ void __launch_bounds__(256) q4_any_join_kernel(const Q4Args a, const AnyPlan p) {
-    const int D = a.D, cpr = D / 4, b = blockIdx.y;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t rh = i / cpr;
-    const int d0 = 4 * static_cast<int>(i % cpr);
-    if (rh >= (int64_t)a.rows * a.Hq) return;
-    const int row = static_cast<int>(rh / a.Hq), qh = static_cast<int>(rh % a.Hq);
+    __shared__ __attribute__((aligned(16))) floatx4 part[256];
+    __shared__ float2 state[256];
+    const int cpr = a.D / 4, lanes = P / cpr, b = blockIdx.y;
+    const int sub = threadIdx.x / P, tid = threadIdx.x % P, r = tid / cpr, c = tid % cpr;
+    const int rh = static_cast<int>(blockIdx.x) * (256 / P) + sub;   // at most 2^29
+    const int row = rh / a.Hq, qh = rh - row * a.Hq;
     const int n = q4_len(a, b);
-    const int64_t first = q4_first(a, b, n), pos = first + row;
-    if (pos < 0 || pos >= n) return;
+    const int64_t first = q4_first(a, b, n), pos = first + row, at = (int64_t)b * a.rows * a.Hq + rh;
     // the block's tiles, as the first launch has them
     const int pair = row * a.G + qh % a.G, r1 = min((pair / kCols * kCols + kCols - 1) / a.G, a.rows - 1);
-    const int tiles = static_cast<int>(min(first + r1, (int64_t)n - 1)) / kTile + 1;
-    if (tiles <= p.range) return;
-    const int ranges = (tiles + p.range - 1) / p.range;
-    const int64_t at = (int64_t)b * a.rows * a.Hq + rh;
+    const int64_t last = min(first + r1, (int64_t)n - 1);
+    int ranges = 0;
+    if (row < a.rows && pos >= 0 && pos < n) ranges = (static_cast<int>(last) / kTile + p.range) / p.range;
+    if (ranges < 2) ranges = 0;   // no row, or written by its one range
     float m = -3.0e38f, l = 0.f;
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < ranges; ++j) {
-        const float2 ml = reinterpret_cast<const float2*>(p.ws_ml)[at * p.nsplit + j];
-        const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + (at * p.nsplit + j) * D + d0);
+    auto fold = [&](float2 ml, floatx4 x) {
         const float mn = fmaxf(m, ml.x), al = fast_exp2(m - mn), be = fast_exp2(ml.x - mn);
         o = o * al + x * be;
         l = fmaf(l, al, ml.y * be);
         m = mn;
-    }
+    };
+    constexpr int U = 4;
+    if (r < lanes)
+        for (int j0 = r; j0 < ranges; j0 += U * lanes) {
+            float2 ml[U];
+            floatx4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t j = at * p.nsplit + min(j0 + u * lanes, ranges - 1);
+                ml[u] = reinterpret_cast<const float2*>(p.ws_ml)[j];
+                x[u] = *reinterpret_cast<const floatx4*>(p.ws_o + j * a.D + 4 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + u * lanes < ranges) fold(ml[u], x[u]);
+        }
+    part[threadIdx.x] = o;
+    state[threadIdx.x] = float2{m, l};
+    __syncthreads();
+    if (r > 0 || ranges == 0) return;
+    for (int k = 1; k < min(lanes, ranges); ++k) fold(state[threadIdx.x + k * cpr], part[threadIdx.x + k * cpr]);
     const float inv = 1.f / l;
-    f16* to = a.out + at * D + d0;
+    f16* to = a.out + at * a.D + 4 * c;
 #pragma unroll
     for (int e = 0; e < 4; ++e) to[e] = static_cast<f16>(o[e] * inv);
-    if (a.lse && d0 == 0) a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+    if (a.lse && c == 0) a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 int64_t bytes(int64_t nsplit, int batch, int rows, int hq, int d) {
@@ -313,9 +333,11 @@ int q4_any(const Q4Args& a, int batch, const char* what, void* ws, size_t room, 
         go(std::integral_constant<int, 8>{});
     const int rc = check_launch(what);
     if (rc || p.nsplit == 1) return rc;
-    const int64_t threads = (int64_t)a.rows * a.Hq * (a.D / 4);
-    hipLaunchKernelGGL(q4_any_join_kernel, dim3(static_cast<unsigned>((threads + 255) / 256), batch), dim3(256), 0, s,
-                       a, p);
+    const unsigned heads = static_cast<unsigned>(a.rows) * a.Hq;
+    if (p.nsplit > 8)
+        hipLaunchKernelGGL(q4_any_join_kernel<256>, dim3(heads, batch), dim3(256), 0, s, a, p);
+    else
+        hipLaunchKernelGGL(q4_any_join_kernel<64>, dim3((heads + 3) / 4, batch), dim3(256), 0, s, a, p);
     return check_launch(what);
 }
 
