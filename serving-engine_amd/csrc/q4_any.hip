@@ -13,10 +13,10 @@
 // last are operands of 0; a key that holds NaN has those too, and a scale of NaN for the pairs
 // that see it.
 //
-// Ranges of keys until the card has 4096 waves, of two tiles at least (one sequence of 2048 keys, 32/8
-// heads of 96: 18.0 us; of four 23.1, of one 19.9); a second launch joins them.  Nothing is loaded
+// Ranges of keys until the card has 4096 waves, down to one tile (one sequence of 2048 keys, 32/8 heads
+// of 96: 10.6 us; of two tiles 14.2, of four 20.8); a second launch joins them.  Nothing is loaded
 // ahead but a tile's V: what bounds it is the waits for page ids, then for codes, which the waves of
-// a SIMD hide from each other (32 sequences of up to 8192 keys, 32/8 heads of 96, 117 MB: 85 us with
+// a SIMD hide from each other (32 sequences of up to 8192 keys, 32/8 heads of 96, 117 MB: 82 us with
 // three, 136 with the two that the compiler takes by itself, 131 with four, which spill; 2048 rows
 // of them 166, 175 and 228).  A wave per (row, query head) and a key per trip took 4300 and 6444.
 #include "q4.h"
@@ -30,7 +30,6 @@ namespace {
 constexpr int kTile = 64;       // keys
 constexpr int kCols = 16;       // pairs of a wave
 constexpr int kWaves = 4096;    // wanted
-constexpr int kLeastTiles = 2;  // of a range
 constexpr int64_t kMostRowHeads = 1 << 29;
 
 struct AnyPlan {
@@ -230,16 +229,17 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
     }
 }
 
-// Joins the ranges of a (row, head): P threads of a workgroup, D / 4 of them side by side, each four
-// dims of every (P / (D / 4))-th range, four loads in flight.  P = 256 for many ranges; else 64, where
-// a workgroup has four (row, head)s.
-template <int P>
+// Joins the ranges of a (row, head), D / 4 threads side by side, each four dims and four ranges' loads
+// in flight.  ALL: a whole workgroup takes one (row, head), the threads past the first D / 4 the next
+// ranges; else a workgroup takes 256 / (D / 4) of them (512 rows of 32/8 heads of 96, four ranges: 26.3
+// us with both launches, 29.3 where four threads of every (row, head) part the ranges).
+template <bool ALL>
 __global__ void __launch_bounds__(256) q4_any_join_kernel(const Q4Args a, const AnyPlan p) {
-    __shared__ __attribute__((aligned(16))) floatx4 part[256];
-    __shared__ float2 state[256];
-    const int cpr = a.D / 4, lanes = P / cpr, b = blockIdx.y;
-    const int sub = threadIdx.x / P, tid = threadIdx.x % P, r = tid / cpr, c = tid % cpr;
-    const int rh = static_cast<int>(blockIdx.x) * (256 / P) + sub;   // at most 2^29
+    const int cpr = a.D / 4, most = 256 / cpr, b = blockIdx.y;
+    const int group = threadIdx.x / cpr, c = threadIdx.x % cpr;
+    if (!ALL && group >= most) return;
+    const int lanes = ALL ? most : 1, r = ALL ? group : 0;
+    const int rh = ALL ? blockIdx.x : blockIdx.x * most + group;   // at most 2^29
     const int row = rh / a.Hq, qh = rh - row * a.Hq;
     const int n = q4_len(a, b);
     const int64_t first = q4_first(a, b, n), pos = first + row, at = (int64_t)b * a.rows * a.Hq + rh;
@@ -272,11 +272,16 @@ __global__ void __launch_bounds__(256) q4_any_join_kernel(const Q4Args a, const 
             for (int u = 0; u < U; ++u)
                 if (j0 + u * lanes < ranges) fold(ml[u], x[u]);
         }
-    part[threadIdx.x] = o;
-    state[threadIdx.x] = float2{m, l};
-    __syncthreads();
-    if (r > 0 || ranges == 0) return;
-    for (int k = 1; k < min(lanes, ranges); ++k) fold(state[threadIdx.x + k * cpr], part[threadIdx.x + k * cpr]);
+    if constexpr (ALL) {
+        __shared__ __attribute__((aligned(16))) floatx4 part[256];
+        __shared__ float2 state[256];
+        part[threadIdx.x] = o;
+        state[threadIdx.x] = float2{m, l};
+        __syncthreads();
+        if (r > 0) return;
+        for (int k = 1; k < min(lanes, ranges); ++k) fold(state[threadIdx.x + k * cpr], part[threadIdx.x + k * cpr]);
+    }
+    if (ranges == 0) return;
     const float inv = 1.f / l;
     f16* to = a.out + at * a.D + 4 * c;
 #pragma unroll
@@ -292,8 +297,7 @@ AnyPlan plan_of(int batch, int rows, int hq, int hkv, int d, int max_len, int64_
     AnyPlan p{};
     const int64_t pairs = (int64_t)rows * (hq / hkv), tiles = ((int64_t)max_len + kTile - 1) / kTile;
     p.blocks = static_cast<int>((pairs + kCols - 1) / kCols);
-    const int64_t most = std::max<int64_t>(tiles / kLeastTiles, 1);
-    int64_t n = std::min(std::max<int64_t>(kWaves / ((int64_t)p.blocks * hkv * batch), 1), most);
+    int64_t n = std::min(std::max<int64_t>(kWaves / ((int64_t)p.blocks * hkv * batch), 1), tiles);
     if (d == 64 || d == 128) n = std::min(n, std::max<int64_t>(room / bytes(1, batch, rows, hq, d), 1));
     p.range = static_cast<int>((tiles + n - 1) / n);
     p.nsplit = static_cast<int>((tiles + p.range - 1) / p.range);
@@ -333,11 +337,11 @@ int q4_any(const Q4Args& a, int batch, const char* what, void* ws, size_t room, 
         go(std::integral_constant<int, 8>{});
     const int rc = check_launch(what);
     if (rc || p.nsplit == 1) return rc;
-    const unsigned heads = static_cast<unsigned>(a.rows) * a.Hq;
+    const unsigned heads = static_cast<unsigned>(a.rows) * a.Hq, per = 256 / (a.D / 4);
     if (p.nsplit > 8)
-        hipLaunchKernelGGL(q4_any_join_kernel<256>, dim3(heads, batch), dim3(256), 0, s, a, p);
+        hipLaunchKernelGGL(q4_any_join_kernel<true>, dim3(heads, batch), dim3(256), 0, s, a, p);
     else
-        hipLaunchKernelGGL(q4_any_join_kernel<64>, dim3((heads + 3) / 4, batch), dim3(256), 0, s, a, p);
+        hipLaunchKernelGGL(q4_any_join_kernel<false>, dim3((heads + per - 1) / per, batch), dim3(256), 0, s, a, p);
     return check_launch(what);
 }
 
