@@ -88,6 +88,18 @@ int q4_shapes(Q4Args& a, const char* what, const void* pool, const int32_t* bt, 
     return KVHP_OK;
 }
 
+// Rows that the kernel for any head_dim, which works on 16 (row, query head) pairs a wave, takes before
+// the one that works on 128 a workgroup: up to 64 pairs of a KV head, contexts of four tiles of 64 keys
+// and more, up to 1024 of a wave's tiles in all.  (32/8 heads of 128: 4 rows of 1024 keys 12.6 us
+// against 17.4, of 4096 15.8 and 18.0, of 8 times 1024 17.8 and 18.5; past it, 8 rows of 8192 keys 25.0
+// and 22.0; below, 4 of 128 11.6 and 9.4.  32/4 heads of 64: 2, 4 and 8 rows of 4096 keys 10.9, 11.5 and
+// 13.3 against 15.0 to 15.6; 8 of 8192 17.2 and 16.4.)
+bool few_pairs(int batch, int rows, int hq, int hkv, int max_len) {
+    if (batch <= 0 || rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_len <= 0) return false;
+    const int64_t pairs = (int64_t)rows * (hq / hkv), tiles = ((int64_t)max_len + 63) / 64;
+    return pairs <= 64 && tiles >= 4 && tiles <= 1024 && (pairs + 15) / 16 * hkv * batch * tiles <= 1024;
+}
+
 int workspace_check(const char* what, const void* ws, size_t bytes, size_t need) {
     if (need == 0) return KVHP_OK;
     KVHP_REQUIRE(ws && bytes >= need, KVHP_ERR_WORKSPACE,
@@ -174,7 +186,7 @@ extern "C" int kvhp_q4_decode(const void* q, const void* pool, const int32_t* bl
 extern "C" size_t kvhp_q4_prefill_workspace_bytes(int batch, int rows, int num_q_heads,
                                                   int num_kv_heads, int head_dim,
                                                   int max_seq_len) {
-    return head_dim == 64 || head_dim == 128
+    return (head_dim == 64 || head_dim == 128) && !few_pairs(batch, rows, num_q_heads, num_kv_heads, max_seq_len)
                ? q4_prefill_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len)
                : q4_any_workspace(batch, rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
 }
@@ -202,7 +214,7 @@ extern "C" int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* b
                                                         head_dim, max_seq_len);
     rc = workspace_check(what, workspace, workspace_bytes, need);
     if (rc) return rc;
-    if (q4_prefill_fits(a, batch))
+    if (q4_prefill_fits(a, batch) && !few_pairs(batch, rows, num_q_heads, num_kv_heads, max_seq_len))
         return q4_prefill(a, batch, workspace, static_cast<hipStream_t>(stream));
     return q4_any(a, batch, what, workspace, need, static_cast<hipStream_t>(stream));
 }

@@ -1,5 +1,6 @@
 // q4_any.hip -- attention over a paged cache held in 4 bits for any head_dim (a multiple of 8 up to
-// 256) and any alignment of the rows (gfx950): what q4_decode.hip and q4_prefill.hip do not take.
+// 256) and any alignment of the rows (gfx950): what q4_decode.hip and q4_prefill.hip do not take, and
+// few rows (q4.hip).
 //
 // One wave takes one KV head of one sequence, 16 of its (row, query head) pairs and a range of
 // keys, in tiles of 64, four whole pages:
@@ -292,13 +293,13 @@ __global__ void __launch_bounds__(256) q4_any_join_kernel(const Q4Args a, const 
 int64_t bytes(int64_t nsplit, int batch, int rows, int hq, int d) {
     return nsplit * (int64_t)sizeof(float) * batch * rows * hq * (d + 2);
 }
-// room: bytes of workspace that the other kernels ask for, at 64 and 128 all that there is.
+// room: bytes of workspace (at head_dim 64 and 128 off 16 bytes what the other kernels asked for).
 AnyPlan plan_of(int batch, int rows, int hq, int hkv, int d, int max_len, int64_t room) {
     AnyPlan p{};
     const int64_t pairs = (int64_t)rows * (hq / hkv), tiles = ((int64_t)max_len + kTile - 1) / kTile;
     p.blocks = static_cast<int>((pairs + kCols - 1) / kCols);
     int64_t n = std::min(std::max<int64_t>(kWaves / ((int64_t)p.blocks * hkv * batch), 1), tiles);
-    if (d == 64 || d == 128) n = std::min(n, std::max<int64_t>(room / bytes(1, batch, rows, hq, d), 1));
+    n = std::min(n, std::max<int64_t>(room / bytes(1, batch, rows, hq, d), 1));
     p.range = static_cast<int>((tiles + n - 1) / n);
     p.nsplit = static_cast<int>((tiles + p.range - 1) / p.range);
     return p;
@@ -310,11 +311,11 @@ size_t q4_any_workspace(int batch, int rows, int hq, int hkv, int d, int max_len
     if (rows <= 0 || !bound_sizes(batch, hq, hkv, max_len, 0, 0) || (int64_t)rows * hq > kMostRowHeads || d <= 0 ||
         d > 256 || d % 8)
         return 0;
-    const AnyPlan p = plan_of(batch, rows, hq, hkv, d, max_len, 0);
+    const AnyPlan p = plan_of(batch, rows, hq, hkv, d, max_len, INT64_MAX);
     return p.nsplit == 1 ? 0 : bytes(p.nsplit, batch, rows, hq, d);
 }
 
-// The workspace holds q4_any_workspace bytes, or at head_dim 64 and 128 `room`.
+// The workspace holds `room` bytes.
 int q4_any(const Q4Args& a, int batch, const char* what, void* ws, size_t room, hipStream_t s) {
     KVHP_REQUIRE((int64_t)a.rows * a.Hq <= kMostRowHeads, KVHP_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what,
                  a.rows, a.Hq);
