@@ -13,8 +13,8 @@
 // 4.7 to 5.0; into 4 bits 41.8 (177 MB).  The same with the rotation computed per row took 134 and
 // 163: 64-bit sines and cosines, 40 times a token instead of once.  A step's tokens are bound by
 // their three dependent waits: 32 of them 4.3 us, one 2.7.
-// Other shapes: one wave per (token, head), a lane per pair of dims (2048 tokens of 32/8 heads of 96:
-// 39 us, a quarter of the tokens above).
+// Other shapes: one wave per token and up to 8 of its heads, a lane per pair of dims (2048 tokens of 32/8
+// heads of 96: 19.2 us; a head a wave, each with its own rotation, 38).
 #include "q4.h"
 
 #include <algorithm>
@@ -78,82 +78,104 @@ __device__ __forceinline__ void rotate(float a, float b, float2 cs, f16& x, f16&
     y = static_cast<f16>(v);
 }
 
-// One wave per (token, head).
+// One wave per token and `per` of its heads, whose rotation it computes once; the next head's row is on
+// its way meanwhile.
 template <bool Q4>
-__global__ void __launch_bounds__(kWave) append_row_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kWave) append_row_kernel(const AppendArgs a, int per) {
     const int lane = threadIdx.x, D = a.D, half = D / 2;
-    const int H = a.Hq + 2 * a.Hkv;
-    const int64_t token = blockIdx.x / H;
-    const int h = blockIdx.x % H;
+    const int H = a.Hq + 2 * a.Hkv, parts = (H + per - 1) / per;
+    const int64_t token = blockIdx.x / parts;
+    const int h0 = static_cast<int>(blockIdx.x % parts) * per, h1 = min(h0 + per, H);
     const int b = static_cast<int>(token / a.rows), row = static_cast<int>(token % a.rows);
     const int64_t pos = (a.positions ? a.positions[b] : 0) + (int64_t)row;
     const int64_t slot = a.slots ? a.slots[b] + (int64_t)row : pos;
     if (slot < 0 || (a.seq_lens && slot >= a.seq_lens[b])) return;
-    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
-    const int kvh = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
-    int pid = -1;
-    if (!is_q) {
-        if (slot >= (int64_t)a.max_pages * kPage) return;
+    int pid = -1;   // -1: K and V are dropped
+    if (h1 > a.Hq && slot < (int64_t)a.max_pages * kPage) {
         pid = a.bt[(int64_t)b * a.max_pages + (slot >> 4)];
-        if (pid < 0 || pid >= a.num_pages) return;
-    }
-    const f16* src = is_q ? a.q + token * a.sq + (int64_t)h * D
-                          : (is_v ? a.v + token * a.sv : a.k + token * a.sk) + (int64_t)kvh * D;
-    f16 x[2][2] = {};   // pairs lane, lane + 64: dims i, i + half
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int i = lane + kWave * u;
-        if (i >= half) continue;
-        x[u][0] = src[i];
-        x[u][1] = src[i + half];
-        if (a.rotate && !is_v)
-            rotate(static_cast<float>(x[u][0]), static_cast<float>(x[u][1]),
-                   rotation(pos, i, D, a.log2_theta), x[u][0], x[u][1]);
+        if (pid >= a.num_pages) pid = -1;
     }
     const int o = static_cast<int>(slot & 15);
-    if (is_q || !Q4) {
-        f16* dst = is_q ? a.q_out + (token * a.Hq + h) * D
-                        : (is_v ? a.pool_v : a.pool_k) +
-                              (((int64_t)kvh * a.num_pages + pid) * kPage + o) * D;
+    f16 next[2][2] = {};   // pairs lane, lane + 64: dims i, i + half
+    auto load = [&](int h) {
+        const f16* src = h < a.Hq ? a.q + token * a.sq + (int64_t)h * D
+                         : h < a.Hq + a.Hkv ? a.k + token * a.sk + (int64_t)(h - a.Hq) * D
+                                            : a.v + token * a.sv + (int64_t)(h - a.Hq - a.Hkv) * D;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int i = lane + kWave * u;
             if (i >= half) continue;
-            dst[i] = x[u][0];
-            dst[i + half] = x[u][1];
+            next[u][0] = src[i];
+            next[u][1] = src[i + half];
         }
-        return;
-    }
-    float lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-        if (lane + kWave * u < half)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f = static_cast<float>(x[u][e]);
-                lo = fminf(lo, f);
-                hi = fmaxf(hi, f);
-                bad |= !(fabsf(f) < INFINITY);
-            }
-    lo = -wave_max(-lo);
-    hi = wave_max(hi);
-    bad = __ballot(bad) != 0;
-    Q4Quant z = q4_quant(bad ? 0.f : lo, bad ? 0.f : hi);
-    if (bad) z.bits = kQ4NanRow;
-    uint8_t* pg = a.pool + ((int64_t)kvh * a.num_pages + pid) * q4_page_bytes(D);
+    };
+    load(h0);
+    float2 cs[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const int i = lane + kWave * u;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint32_t n = bad || z.flat ? 0 : q4_code(z, static_cast<float>(x[u][e]));
-            const uint32_t next = __shfl_down(n, 1);   // half is even: the pair's other dim
-            if (i < half && !(i & 1))
-                pg[q4_codes_at(D, is_v, o) + (i + e * half) / 2] = static_cast<uint8_t>(n | next << 4);
-        }
+        cs[u] = float2{1.f, 0.f};
+        if (a.rotate && h0 < a.Hq + a.Hkv && lane + kWave * u < half)
+            cs[u] = rotation(pos, lane + kWave * u, D, a.log2_theta);
     }
-    if (lane == 0) *reinterpret_cast<uint32_t*>(pg + q4_params_at(D, is_v, o)) = z.bits;
+    for (int h = h0; h < h1; ++h) {
+        const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+        const int kvh = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
+        f16 x[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            x[u][0] = next[u][0];
+            x[u][1] = next[u][1];
+        }
+        if (h + 1 < h1) load(h + 1);
+        if (!is_q && pid < 0) continue;
+        if (a.rotate && !is_v)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                rotate(static_cast<float>(x[u][0]), static_cast<float>(x[u][1]), cs[u], x[u][0], x[u][1]);
+        if (is_q || !Q4) {
+            f16* dst = is_q ? a.q_out + (token * a.Hq + h) * D
+                            : (is_v ? a.pool_v : a.pool_k) +
+                                  (((int64_t)kvh * a.num_pages + pid) * kPage + o) * D;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = lane + kWave * u;
+                if (i >= half) continue;
+                dst[i] = x[u][0];
+                dst[i + half] = x[u][1];
+            }
+            continue;
+        }
+        float lo = INFINITY, hi = -INFINITY;
+        bool bad = false;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (lane + kWave * u < half)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float f = static_cast<float>(x[u][e]);
+                    lo = fminf(lo, f);
+                    hi = fmaxf(hi, f);
+                    bad |= !(fabsf(f) < INFINITY);
+                }
+        lo = -wave_max(-lo);
+        hi = wave_max(hi);
+        bad = __ballot(bad) != 0;
+        Q4Quant z = q4_quant(bad ? 0.f : lo, bad ? 0.f : hi);
+        if (bad) z.bits = kQ4NanRow;
+        uint8_t* pg = a.pool + ((int64_t)kvh * a.num_pages + pid) * q4_page_bytes(D);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = lane + kWave * u;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t n = bad || z.flat ? 0 : q4_code(z, static_cast<float>(x[u][e]));
+                const uint32_t odd = __shfl_down(n, 1);   // half is even: the pair's other dim
+                if (i < half && !(i & 1))
+                    pg[q4_codes_at(D, is_v, o) + (i + e * half) / 2] = static_cast<uint8_t>(n | odd << 4);
+            }
+        }
+        if (lane == 0) *reinterpret_cast<uint32_t*>(pg + q4_params_at(D, is_v, o)) = z.bits;
+    }
 }
 
 // The same by 16-byte chunks, D = 64 and 128.  Grid (groups of TB tokens, pieces of HP heads).
@@ -344,14 +366,15 @@ int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq
             hipLaunchKernelGGL((append_vec_kernel<128, false>), grid, dim3(256), 0, s, a, TB, HP, inv);
         return check_launch(what);
     }
-    const int64_t waves = tokens * H;
-    KVHP_REQUIRE(tokens <= 1 << 25 && waves <= 1 << 25, KVHP_ERR_UNSUPPORTED,
+    KVHP_REQUIRE(tokens <= 1 << 25 && tokens * H <= 1 << 25, KVHP_ERR_UNSUPPORTED,
                  "%s: %d x %d rows of %d heads", what, batch, rows, H);
-    const dim3 grid(static_cast<unsigned>(waves));
+    int per = 1;   // heads of a wave, once there are some 8 waves a SIMD
+    while (per < 8 && tokens * H >= 16384 * per) per *= 2;
+    const dim3 grid(static_cast<unsigned>(tokens * ((H + per - 1) / per)));
     if (q4)
-        hipLaunchKernelGGL(append_row_kernel<true>, grid, dim3(kWave), 0, s, a);
+        hipLaunchKernelGGL(append_row_kernel<true>, grid, dim3(kWave), 0, s, a, per);
     else
-        hipLaunchKernelGGL(append_row_kernel<false>, grid, dim3(kWave), 0, s, a);
+        hipLaunchKernelGGL(append_row_kernel<false>, grid, dim3(kWave), 0, s, a, per);
     return check_launch(what);
 }
 
