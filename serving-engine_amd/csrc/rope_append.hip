@@ -183,7 +183,6 @@ template <int D, bool Q4>
 __global__ void __launch_bounds__(256) append_vec_kernel(const AppendArgs a, int TB, int HP, uint32_t inv_hp) {
     constexpr int half = D / 2, CPH = half / 8, RPI = 256 / CPH, U = 2, kMostTokens = 16;
     __shared__ float2 cs[kMostTokens * half];
-    __shared__ int64_t pos_of[kMostTokens];
     __shared__ int slot_of[kMostTokens], pid_of[kMostTokens];   // slot -1: padding; page -1: dropped
     const int tid = threadIdx.x, H = a.Hq + 2 * a.Hkv;
     const int64_t token0 = (int64_t)blockIdx.x * TB;
@@ -211,26 +210,28 @@ __global__ void __launch_bounds__(256) append_vec_kernel(const AppendArgs a, int
         }
     };
     load(0);
-    if (tid < nt) {
-        const int64_t token = token0 + tid;
-        const int b = static_cast<int>(token / a.rows), row = static_cast<int>(token - (int64_t)b * a.rows);
-        const int64_t pos = (a.positions ? a.positions[b] : 0) + (int64_t)row;
-        const int64_t slot = a.slots ? a.slots[b] + (int64_t)row : pos;
+    // where the tokens go, by the last wave; their rotations meanwhile, by the first ones at least
+    if (tid >= 256 - kMostTokens && tid - (256 - kMostTokens) < nt) {
+        const int t = tid - (256 - kMostTokens);
+        const uint32_t token = static_cast<uint32_t>(token0) + t, b = token / a.rows;   // tokens fit an int
+        const int64_t row = token - b * a.rows;
+        const int64_t slot = (a.slots ? a.slots[b] : a.positions ? a.positions[b] : 0) + row;
         const bool live = slot >= 0 && !(a.seq_lens && slot >= a.seq_lens[b]);
         int pid = -1;
         if (live && slot < (int64_t)a.max_pages * kPage) {
             pid = a.bt[(int64_t)b * a.max_pages + (slot >> 4)];
             if (pid >= a.num_pages) pid = -1;
         }
-        pos_of[tid] = pos;
-        slot_of[tid] = live ? static_cast<int>(slot & 15) : -1;
-        pid_of[tid] = pid;
+        slot_of[t] = live ? static_cast<int>(slot & 15) : -1;
+        pid_of[t] = pid;
     }
+    if (a.rotate)
+        for (int i = tid; i < nt * half; i += 256) {
+            const uint32_t token = static_cast<uint32_t>(token0) + i / half, b = token / a.rows;
+            const int64_t pos = (a.positions ? a.positions[b] : 0) + static_cast<int64_t>(token - b * a.rows);
+            cs[i] = rotation(pos, i % half, D, a.log2_theta);
+        }
     __syncthreads();
-    if (a.rotate) {
-        for (int i = tid; i < nt * half; i += 256) cs[i] = rotation(pos_of[i / half], i % half, D, a.log2_theta);
-        __syncthreads();
-    }
     for (int base = 0; base < nrows; base += U * RPI) {
         if (base > 0) load(base);
 #pragma unroll
