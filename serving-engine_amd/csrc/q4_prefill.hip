@@ -24,8 +24,8 @@
 //
 // Few rows over a long cache are cut into ranges of keys whose partials a second launch joins.
 //
-// What bounds it: the vector unit.  8192 rows of 32/8 heads of 128 take 627 to 660 us (550 GFLOP,
-// 833 to 877 TFLOP/s, a third of the matrix cores' peak): it is busy for 62 % of the SIMDs' cycles
+// What bounds it: the vector unit.  8192 rows of 32/8 heads of 128 take 619 to 660 us (550 GFLOP,
+// 833 to 889 TFLOP/s, a third of the matrix cores' peak): it is busy for 62 % of the SIMDs' cycles
 // (a tile's 32 exponentials of 16 cycles each, their multiply-adds, sums and conversions: some 960
 // of 2600; the codes: 340), the matrix cores for 43 %, LDS for 55 % (each wave reads all of a
 // tile's operands, 32 KB).  Two waves a SIMD is what 240 registers leave; more pairs a wave would
