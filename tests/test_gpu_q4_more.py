@@ -155,10 +155,11 @@ def test_chunks_off_16_bytes(d):
                 check(got[b, r, hs], o, tol, f"sequence {b} row {r} head {h}")
 
 
-def test_pools_past_32_bits():
+@pytest.mark.parametrize("d", [96, 128])
+def test_pools_past_32_bits(d):
     """Pages of more than 4 GiB per head: the bits of the same rows in a small pool."""
     rng = np.random.default_rng(9)
-    hq, hkv, d, n = 8, 2, 128, 200
+    hq, hkv, n = 8, 2, 400
     pages = (n + PAGE - 1) // PAGE
     rows = to_gpu(_q(rng, 1, n, hq + 2 * hkv, d))
     parts = [rows[:, :, :hq], rows[:, :, hq:hq + hkv], rows[:, :, hq + hkv:]]
@@ -178,12 +179,16 @@ def test_pools_past_32_bits():
         note("prefill")
         kvhp.q4_prefill(q, pool, bt, out, hq, hkv, d, n,
                         workspace=workspace(kvhp.q4_prefill_workspace_bytes(1, n, hq, hkv, d, n)))
+        few = torch.empty((1, 5, hq, d), dtype=torch.float16, device="cuda")
+        note("prefill of few rows")
+        kvhp.q4_prefill(q[:, -5:].contiguous(), pool, bt, few, hq, hkv, d, n, q_start=lens - 5,
+                        workspace=workspace(kvhp.q4_prefill_workspace_bytes(1, 5, hq, hkv, d, n)))
         one = torch.empty((1, hq, d), dtype=torch.float16, device="cuda")
         note("decode")
         kvhp.q4_decode(q[:, -1].contiguous(), pool, bt, lens, one, hq, hkv, d, n,
                        workspace=workspace(kvhp.q4_decode_workspace_bytes(1, hq, hkv, d, n)))
         sync()
-        got.append([t.clone() for t in (q, *back, out, one)])
+        got.append([t.clone() for t in (q, *back, out, few, one)])
         del pool
     assert all(torch.equal(a, b) for a, b in zip(*got))
     assert torch.isfinite(got[0][3]).all()
