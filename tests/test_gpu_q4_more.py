@@ -337,3 +337,48 @@ def test_append_of_many_heads(hq, hkv):
     _, _, vn, vp = unpack(from_gpu(pool), d)
     n, p = quantise(x[0, :, hq + hkv:].transpose(1, 0, 2))
     assert np.array_equal(vn[:, 0, :R], n) and np.array_equal(vp[:, 0, :R], p)
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_replays_follow_the_lengths(d):
+    """Lengths and starts are read where the kernels run: a captured step and a captured chunk
+    over lengths that change between replays, against eager calls, bit for bit."""
+    rng = np.random.default_rng(d)
+    B, rows, hq, hkv = 18, 40, 8, 2
+    most = 2600
+    c = Q4Cache(rng, [most] * B, hkv, d).upload()
+    q, x = to_gpu(_q(rng, B, hq, d)), to_gpu(_q(rng, 4, rows, hq, d))
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+    start = torch.zeros(4, dtype=torch.int32, device="cuda")
+    bt4 = c.bt_d[:4].contiguous()
+
+    def buffers():
+        return (torch.zeros_like(q), torch.zeros_like(x), torch.zeros((4, hq, rows), device="cuda"),
+                workspace(kvhp.q4_decode_workspace_bytes(B, hq, hkv, d, most)),
+                workspace(kvhp.q4_prefill_workspace_bytes(4, rows, hq, hkv, d, most)))
+
+    def run(one, out, lse, dws, pws):
+        kvhp.q4_decode(q, c.pool, c.bt_d, lens, one, hq, hkv, d, most, workspace=dws)
+        kvhp.q4_prefill(x, c.pool, bt4, out, hq, hkv, d, most, q_start=start, seq_lens=lens[:4], lse=lse,
+                        workspace=pws)
+
+    got = buffers()
+    graph = torch.cuda.CUDAGraph()
+    note(f"q4 capture d={d}")
+    with torch.cuda.graph(graph):
+        run(*got)
+    for i, new in enumerate(([most] * B, [40] * B, list(rng.integers(0, most + 1, B)), [most] + [0] * (B - 1))):
+        note(f"q4 replay {i} d={d}")
+        lens.copy_(to_gpu(np.asarray(new, np.int32)))
+        start.copy_(lens[:4] - rows)
+        for t in got[:3]:
+            t.fill_(3)
+        graph.replay()
+        sync()
+        want = buffers()
+        for t in want[:3]:
+            t.fill_(3)
+        run(*want)
+        sync()
+        assert all(torch.equal(a, b) for a, b in zip(got[:3], want[:3]))
+        assert torch.isfinite(got[0]).all() and (i > 0 or not (got[1] == 3).all())
