@@ -9,8 +9,9 @@
 // (n + r) 2^-9 from the denormals that the codes are in a half's low bits (q4_decode.hip has the
 // same); V's are (n + r) E: four bits in mantissa bits 6..9 below the exponent of 16 are 16 + n,
 // and times E plus (r - 16) E that is it; E is the power of two that leaves s / E = m between 4
-// and 8 (less for scales below 2^-12).  K's s multiplies the scores inside the exponent's
-// multiply-add, V's m a weight before its one rounding to fp16.
+// and 8 (less for scales below 2^-12, up to 16 for those from 2^15 on, which rows of equal values
+// have: a higher E would take their (r - 16) E past fp16).  K's s multiplies the scores inside
+// the exponent's multiply-add, V's m a weight before its one rounding to fp16.
 //
 // Per tile, on v_mfma_f32_32x32x16_f16 with one lane per pair, in halves of 32 keys: S^T = K Q^T
 // and O^T += V^T W^T beside the exponentials and the next codes' conversion, each operand read
@@ -46,7 +47,7 @@ constexpr int kMaxRowHeads = 1 << 29; // (row, query head) pairs of a sequence: 
 constexpr int kCUs = 256;
 constexpr int kLeastTiles = 3;        // of a range of keys
 constexpr float kRefLog2 = 4.f;       // weights where a row's reference is set,
-constexpr float kMostWeight = 4096.f; // and where it moves
+constexpr float kMostWeight = 4096.f; // and where it moves: times m, below 16, no more than 65504
 
 struct PrefillPlan {
     uint32_t inv_g;        // ceil(2^32 / G), 0 for G = 1
@@ -305,7 +306,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
         ks = behind || (ks & 0x7c00u) == 0x7c00u ? 0u : ks;
         const bool nan = !behind && (vs & 0x7c00u) == 0x7c00u;
         vs = behind || nan ? 0u : vs;
-        const int e = max((int)(vs & 0x7c00u) - 0x0800, 0x0400);
+        const int e = min(max((int)(vs & 0x7c00u) - 0x0800, 0x0400), 0x6c00);   // 2^-14 .. 2^12
         scale_m[t & 1][sat] = as_half2(vs)[0] * __builtin_bit_cast(f16, static_cast<uint16_t>(0x7800 - e));   // exact
         const uint64_t nans = __ballot(nan);
         nan_at = nans && nan_at == INT32_MAX ? t_lo * kBN + t * kBN + kPage * wave + (__builtin_ctzll(nans) >> 2) : nan_at;
