@@ -427,7 +427,8 @@ int kvhp_q4_rope_append(const void* q, const void* k, const void* v, int64_t q_s
                         void* q_out, void* pool, const int32_t* block_tables, int max_pages,
                         int num_pages, int batch, int rows, int num_q_heads, int num_kv_heads,
                         int head_dim, void* stream);
-/* Rows read back, each value rounded to fp16: out_k, out_v [batch][Hkv][max_len][D] (either
+/* Rows read back, each value rounded to fp16 (+-65504 what lies past it: s and r are rounded, so
+ * a row may stand for up to 65700): out_k, out_v [batch][Hkv][max_len][D] (either
  * may be NULL; 16-byte aligned) <- positions start[b] + t (device int32, NULL: 0), t <
  * max_len; zeros at negative positions and from seq_lens[b] (device int32) on.  Page ids
  * are clamped into the pool. */
@@ -439,6 +440,7 @@ int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int max_pages,
  * Lengths above max_seq_len (or the block table's reach) count as that, page ids are
  * clamped, and whatever slots past the lengths hold reaches no output.  Scores, softmax
  * states and sums are fp32; a weight is rounded to fp16 once, with its row's share of s.
+ * Outputs past fp16's range, which the rows' rounding alone can bring about, are +-65504.
  * Asynchronous, allocates nothing, may be captured.  The workspace must be 16-byte aligned
  * and hold *_workspace_bytes bytes (0: NULL is fine); calls that overlap need one each.
  * How the work is cut goes by max_seq_len: pass the longest length of the step.  The fast

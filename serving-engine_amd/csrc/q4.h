@@ -16,6 +16,9 @@
 // rounded a second time.  (Scale and minimum, the usual pair, need either a rounded operand
 // or a term of their own per key and head.)  A row of equal values c: s = c, r = 1, n = 0.  A
 // row with a value that is not finite: s = r = NaN, n = 0, all NaN as its product would be.
+// s and r are rounded, so that a row with values past 65400 or so may stand for up to 65700 (s is
+// up by 2^-10 of its 15 steps, at most 128, and s r by s 2^-7): what is written in fp16, values
+// read back and weighted means, then is +-65504 (q4_finite), never infinite.
 //
 // A page of a KV head is 16 (D + 8) bytes in a row, whole 128-byte lines at any D that is a
 // multiple of 8: K codes [16][D/2] (the even dim in the low half of a byte), V codes, K's
@@ -81,6 +84,13 @@ __device__ __forceinline__ uint32_t q4_code(const Q4Quant& z, float x) {
     return static_cast<uint32_t>(fminf(fmaxf(rintf(q), 0.f), 15.f));
 }
 constexpr uint32_t kQ4NanRow = 0x7e007e00u;
+// Values rounded to fp16, where infinite its largest (NaN stays: the minimum and maximum that keep
+// it, packed, an instruction a value).
+template <typename T>
+__device__ __forceinline__ T q4_finite(T h) {
+    const T most = static_cast<f16>(65504.f);
+    return __builtin_elementwise_maximum(__builtin_elementwise_minimum(h, most), -most);
+}
 
 // What the attention over a 4-bit cache reads and writes.  Rows: q, out [batch][rows][Hq][D],
 // row r of sequence b at position first(b) + r.

@@ -52,7 +52,7 @@ q4_gather_kernel(const uint8_t* pool, const int32_t* bt, int max_pages, int num_
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 y[e] = static_cast<f16>(p.s * (static_cast<float>(x[u][is_v] >> 4 * e & 15) + p.r));
-            store_half8(out + at, y);
+            store_half8(out + at, q4_finite(y));
         }
     }
 }

@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
         half4 h;
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = static_cast<f16>(o[db][e] * inv);
+        h = q4_finite(h);
         f16* to = a.out + at * D + d0;
         if (p.aligned) {
             *reinterpret_cast<half4*>(to) = h;
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(256) q4_any_join_kernel(const Q4Args a, const 
     const float inv = 1.f / l;
     f16* to = a.out + at * a.D + 4 * c;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = static_cast<f16>(o[e] * inv);
+    for (int e = 0; e < 4; ++e) to[e] = q4_finite(static_cast<f16>(o[e] * inv));
     if (a.lse && c == 0) a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 

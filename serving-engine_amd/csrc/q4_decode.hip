@@ -492,7 +492,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             half4 h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[e] = static_cast<f16>(r[i][e] * inv);
-            *reinterpret_cast<half4*>(a.out + (row0 + col) * D + 16 * db + 4 * g) = h;
+            *reinterpret_cast<half4*>(a.out + (row0 + col) * D + 16 * db + 4 * g) = q4_finite(h);
         } else {
             *reinterpret_cast<floatx4*>(p.ws_o + prow * D + 16 * db + 4 * g) = r[i];
         }
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kJoinRows * kWave) q4_join_kernel(const Q4Args
         h[e] = static_cast<f16>(x0[e] * inv);
         h[4 + e] = static_cast<f16>(x1[e] * inv);
     }
-    store_half8(a.out + row * D + 8 * c, h);
+    store_half8(a.out + row * D + 8 * c, q4_finite(h));
 }
 
 // Where one split of eight waves holds a sequence, it saves the join's launch: 5 to 7 us against

@@ -540,7 +540,7 @@ q4_prefill_kernel(const Q4Args a, const PrefillPlan p) {
             v[e] = static_cast<f16>(x[e]);
             v[4 + e] = static_cast<f16>(y[e]);
         }
-        store_half8(a.out + to * D + 8 * c, v);
+        store_half8(a.out + to * D + 8 * c, q4_finite(v));
     }
 }
 
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(256) q4_prefill_join_kernel(const Q4Args a, co
         hv[e] = static_cast<f16>(o0[e] * inv);
         hv[4 + e] = static_cast<f16>(o1[e] * inv);
     }
-    store_half8(a.out + at * D + 8 * c, hv);
+    store_half8(a.out + at * D + 8 * c, q4_finite(hv));
     if (a.lse && c == 0)
         a.lse[((int64_t)b * a.Hq + qh) * a.rows + row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
