@@ -152,8 +152,9 @@ public:
         pool_.allocate((size_t)num_layers * num_kv_heads * num_pages * page);
         pool_.zero();   // in 4 bits: rows of zeros
         // one device block: tables [max_batch][max_pages], seq_lens [max_batch],
-        // write positions [max_batch], write tables [max_batch][max_pages]
-        meta_words_ = 2 * (size_t)max_batch * max_pages_per_seq + 2 * (size_t)max_batch;
+        // write positions [max_batch], write tables [max_batch][max_pages], text
+        // positions [max_batch]
+        meta_words_ = 2 * (size_t)max_batch * max_pages_per_seq + 3 * (size_t)max_batch;
         meta_.allocate(meta_words_);
         void* p = nullptr;
         HIP_CHECK(hipHostMalloc(&p, meta_words_ * sizeof(int32_t), hipHostMallocDefault));
@@ -164,6 +165,7 @@ public:
         pos_.assign(max_batch, -1);
         pages_used_.assign(max_batch, 0);
         cached_.assign(max_batch, 0);
+        cut_.assign(max_batch, 0);
         active_.assign(max_batch, false);
         free_pages_.resize(num_pages);
         for (int i = 0; i < num_pages; ++i) free_pages_[i] = num_pages - 1 - i;  // pop 0 first
@@ -201,6 +203,9 @@ public:
     // Block tables for writes: as block_tables(), with pages that more than
     // one sequence holds set to -1 (writes there are dropped).
     const int32_t* write_block_tables() const { return write_positions() + max_batch_; }
+    // Where in the text the tokens at write_positions() stand: behind those, in
+    // sequences that were cut, by as many as were given up.
+    const int32_t* text_positions() const { return write_block_tables() + (size_t)max_batch_ * max_pages_; }
     hip::KVView k_view(int layer) const { return view(layer, 0); }
     hip::KVView v_view(int layer) const { return view(layer, 1); }
 
@@ -211,6 +216,7 @@ public:
                 active_[s] = true;
                 lens_[s] = 0;
                 pos_[s] = -1;
+                cut_[s] = 0;
                 return s;
             }
         }
@@ -252,6 +258,7 @@ public:
                                    "pages that were given up");
         reserve(slot, len);
         lens_[slot] = len;
+        if (len == 0) cut_[slot] = 0;   // a text of its own
     }
     // Gives up the pages of which no row at the sequence's last position or later
     // sees a key, attending its last `window` keys and the text's first `sinks`
@@ -289,7 +296,9 @@ public:
     // Cuts a sequence to its first `len` tokens and gives up the pages behind
     // them, after an eviction moved the kept tokens into the first slots (so none
     // of its pages may be shared; by now that is too late to find out, see
-    // require_private).
+    // require_private).  The text goes on where it was: rope_append rotates what
+    // follows to text_positions().  (Taking the last tokens of a text back is
+    // set_seq_len's.)
     void shrink(int slot, int len) {
         require_private(slot);
         if (len < 0 || len > lens_[slot])
@@ -297,6 +306,7 @@ public:
         const int keep = (len + kPage - 1) / kPage;
         for (int i = keep; i < pages_used_[slot]; ++i) give_up(slot, i);
         pages_used_[slot] = std::min(pages_used_[slot], keep);
+        cut_[slot] += lens_[slot] - len;
         lens_[slot] = len;
         cached_[slot] = 0;   // what the first slots hold is no shared prefix now
         pos_[slot] = -1;
@@ -304,7 +314,8 @@ public:
     // Prefix sharing: `dst` (an active slot holding no pages) takes the
     // full pages covering the first num_tokens positions of `src` (a partial
     // last page is never shared, so later writes stay private) and starts
-    // with that many cached tokens.  Returns the shared token count.
+    // with that many cached tokens.  Behind the pages of a sequence that was cut its
+    // text goes on as that one's would there.  Returns the shared token count.
     int share_prefix(int dst, int src, int num_tokens) {
         check_slot(dst);
         check_slot(src);
@@ -326,6 +337,7 @@ public:
         pages_used_[dst] = n;
         lens_[dst] = n * kPage;
         cached_[dst] = n * kPage;
+        cut_[dst] = n > 0 ? cut_[src] : 0;
         return n * kPage;
     }
     // Leading positions of `slot` whose K/V came from share_prefix (0 after
@@ -334,6 +346,8 @@ public:
     // Sequences holding physical page `page` (0: free).
     int page_refs(int page) const { return refs_.at(page); }
     int seq_len(int slot) const { return lens_.at(slot); }
+    // Tokens of the text so far, those given up among them.
+    int64_t text_len(int slot) const { return (int64_t)lens_.at(slot) + cut_.at(slot); }
     int pages_used(int slot) const { return pages_used_.at(slot); }
     int free_page_count() const { return (int)free_pages_.size(); }
     const int32_t* host_block_table(int slot) const { return tables_.data() + (size_t)slot * max_pages_; }
@@ -402,6 +416,7 @@ public:
         int32_t* wt = staging_ + tables_.size() + 2 * (size_t)max_batch_;
         for (size_t i = 0; i < tables_.size(); ++i)
             wt[i] = tables_[i] >= 0 && refs_[tables_[i]] > 1 ? -1 : tables_[i];
+        for (int s = 0; s < max_batch_; ++s) wt[tables_.size() + s] = pos_[s] < 0 ? -1 : pos_[s] + cut_[s];
         HIP_CHECK(hipMemcpyAsync(meta_.data(), staging_, meta_words_ * sizeof(int32_t),
                                  hipMemcpyHostToDevice, stream));
         HIP_CHECK(hipEventRecord(staged_, stream));
@@ -439,22 +454,22 @@ public:
     }
 
     // Rotates the rows of one layer, q [batch][rows][Hq][D] (to q_out) and k
-    // [batch][rows][Hkv][D] (tokens *_stride halfs apart), to each slot's write position
-    // on, and appends K and V there, in the cache's format.  Rows at or past a slot's length
-    // are padding.
+    // [batch][rows][Hkv][D] (tokens *_stride halfs apart), to each slot's text position
+    // on, and appends K and V at its write position on, in the cache's format.  Rows at or
+    // past a slot's length are padding.
     void rope_append(int layer, const half* q, const half* k, const half* v, int64_t q_stride,
                      int64_t k_stride, int64_t v_stride, float rope_theta, half* q_out, int batch,
                      int rows, int num_q_heads, Stream stream = nullptr) {
         check_layer(layer);
         check_batch(batch);
         if (format_ == Format::kQ4)
-            hip::q4_rope_append(q, k, v, q_stride, k_stride, v_stride, write_positions(), nullptr,
-                                seq_lens(), rope_theta, q_out, get_q4_layer_ptr(layer),
+            hip::q4_rope_append(q, k, v, q_stride, k_stride, v_stride, text_positions(),
+                                write_positions(), seq_lens(), rope_theta, q_out, get_q4_layer_ptr(layer),
                                 write_block_tables(), max_pages_, num_pages_, batch, rows,
                                 num_q_heads, num_kv_heads_, head_dim_, stream);
         else
-            hip::rope_append(q, k, v, q_stride, k_stride, v_stride, write_positions(), nullptr,
-                             seq_lens(), rope_theta, q_out, get_layer_ptr(layer, 0),
+            hip::rope_append(q, k, v, q_stride, k_stride, v_stride, text_positions(),
+                             write_positions(), seq_lens(), rope_theta, q_out, get_layer_ptr(layer, 0),
                              get_layer_ptr(layer, 1), write_block_tables(), max_pages_, num_pages_,
                              batch, rows, num_q_heads, num_kv_heads_, head_dim_, stream);
     }
@@ -559,6 +574,7 @@ private:
     std::vector<int32_t> tables_, lens_, pos_;
     std::vector<int> pages_used_;
     std::vector<int> cached_;
+    std::vector<int32_t> cut_;   // tokens of the text that cuts gave up
     std::vector<bool> active_;
     std::vector<int32_t> free_pages_;
     std::vector<int> refs_;
