@@ -541,11 +541,12 @@ def _token_rows(t, what):
     return B, R, step
 
 
-def _append_rows(q, k, v, q_out, what):
-    """(batch, rows, q_stride, k_stride, v_stride) of an append's tensors."""
+def _append_rows(q, k, v, q_out, what, heads=None):
+    """(batch, rows, q_stride, k_stride, v_stride) of an append's tensors, of `heads` =
+    (num_q_heads, num_kv_heads, head_dim)."""
     shape = k.shape
     B, R, H, D = shape
-    same = v.shape == shape
+    same = v.shape == shape and (heads is None or H == heads[1] and D == heads[2])
     kb, sk, kh, kd = k.stride()
     vb, sv, vh, vd = v.stride()
     # as slices of contiguous tensors are; others by _token_rows, which knows what it can take
@@ -557,14 +558,34 @@ def _append_rows(q, k, v, q_out, what):
         if not (qd == 1 and qh == D and qb == R * sq):
             sq = _token_rows(q, what)[2]
         qs = q.shape
-        same = same and qs[0] == B and qs[1] == R and qs[3] == D
+        same = (same and qs[0] == B and qs[1] == R and qs[3] == D
+                and (heads is None or qs[2] == heads[0]))
         if q_out is not None:
             same = same and q_out.shape == qs
     if not same:
-        raise KVHPError(KVHP_ERR_INVALID, f"{what}: q, k, v and q_out of different rows")
+        raise KVHPError(KVHP_ERR_INVALID, f"{what}: q, k, v and q_out of different rows"
+                                          + (f", or of others than {heads} heads and dims" if heads else ""))
     if q_out is not None and not q_out.is_contiguous():
         raise KVHPError(KVHP_ERR_INVALID, f"{what}: q_out must be contiguous")
     return B, R, sq, sk, sv
+
+
+def _refuse_sizes(what, whole, sequences, n):
+    """The library takes addresses and goes by the numbers it is called with.  Raises for the
+    first of `whole`, name: (tensor or None, values), that is not contiguous or holds another
+    number of values (block tables: fewer), or of `sequences` that has no value for each of
+    n.  Called where a call's own check of all of them failed."""
+    for name, (t, values) in whole.items():
+        if t is None:
+            continue
+        got = t.numel()
+        if got < values or (got > values and name != "block_tables") or not t.is_contiguous():
+            raise KVHPError(KVHP_ERR_INVALID, f"{what}: {name}: {values} contiguous values wanted, got "
+                                              f"{tuple(t.shape)} with strides {t.stride()}")
+    for name, t in sequences.items():
+        if t is not None and (t.numel() < n or not t.is_contiguous()):
+            raise KVHPError(KVHP_ERR_INVALID, f"{what}: {name}: a value for each of {n} sequences wanted, got "
+                                              f"{tuple(t.shape)} with strides {t.stride()}")
 
 
 def rope_append(q, k, v, positions, q_out, pool_k, pool_v, block_tables, num_q_heads,
@@ -572,12 +593,21 @@ def rope_append(q, k, v, positions, q_out, pool_k, pool_v, block_tables, num_q_h
     """Rotates rows q [B][rows][Hq][D] (to q_out) and k [B][rows][Hkv][D] to text
     positions positions[b] + r and writes K and V to slots slots[b] + r of the pools
     [Hkv][P][16][D].  q, k, v may be parts of one fused projection; theta 0: no rotation."""
-    B, R, sq, sk, sv = _append_rows(q, k, v, q_out, "rope_append")
+    B, R, sq, sk, sv = _append_rows(q, k, v, q_out, "rope_append", (num_q_heads, num_kv_heads, head_dim))
+    max_pages, pages = block_tables.shape[1], pool_k.shape[1]
+    pooled = num_kv_heads * pages * PAGE_SIZE * head_dim
+    if not (pool_k.numel() == pooled == pool_v.numel() and block_tables.numel() >= B * max_pages
+            and (positions is None or positions.numel() >= B and positions.is_contiguous())
+            and (slots is None or slots.numel() >= B and slots.is_contiguous())
+            and (seq_lens is None or seq_lens.numel() >= B and seq_lens.is_contiguous())
+            and pool_k.is_contiguous() and pool_v.is_contiguous() and block_tables.is_contiguous()):
+        _refuse_sizes("rope_append", {"pool_k": (pool_k, pooled), "pool_v": (pool_v, pooled),
+                                      "block_tables": (block_tables, B * max_pages)},
+                      {"positions": positions, "slots": slots, "seq_lens": seq_lens}, B)
     _check(load().kvhp_rope_append(
-        _ptr(q), _ptr(k), _ptr(v), sq, sk, sv, _ptr(positions), _ptr(slots), _ptr(seq_lens),
-        theta, _ptr(q_out), _ptr(pool_k), _ptr(pool_v), _ptr(block_tables),
-        block_tables.shape[1], pool_k.shape[1], B, R, num_q_heads, num_kv_heads, head_dim,
-        _stream(stream)))
+        _ptr(q), k.data_ptr(), v.data_ptr(), sq, sk, sv, _ptr(positions), _ptr(slots), _ptr(seq_lens),
+        theta, _ptr(q_out), pool_k.data_ptr(), pool_v.data_ptr(), block_tables.data_ptr(),
+        max_pages, pages, B, R, num_q_heads, num_kv_heads, head_dim, _stream(stream)))
 
 
 def q4_page_bytes(head_dim) -> int:
@@ -588,10 +618,19 @@ def q4_page_bytes(head_dim) -> int:
 def q4_rope_append(q, k, v, positions, q_out, pool, block_tables, num_q_heads, num_kv_heads,
                    head_dim, theta, slots=None, seq_lens=None, stream=None):
     """rope_append into a 4-bit pool, uint8 [Hkv][P][q4_page_bytes(D)]."""
-    B, R, sq, sk, sv = _append_rows(q, k, v, q_out, "q4_rope_append")
+    B, R, sq, sk, sv = _append_rows(q, k, v, q_out, "q4_rope_append", (num_q_heads, num_kv_heads, head_dim))
+    max_pages, pages = block_tables.shape[1], pool.shape[1]
+    pooled = num_kv_heads * pages * PAGE_SIZE * (head_dim + 8)
+    if not (pool.numel() == pooled and block_tables.numel() >= B * max_pages
+            and (positions is None or positions.numel() >= B and positions.is_contiguous())
+            and (slots is None or slots.numel() >= B and slots.is_contiguous())
+            and (seq_lens is None or seq_lens.numel() >= B and seq_lens.is_contiguous())
+            and pool.is_contiguous() and block_tables.is_contiguous()):
+        _refuse_sizes("q4_rope_append", {"pool": (pool, pooled), "block_tables": (block_tables, B * max_pages)},
+                      {"positions": positions, "slots": slots, "seq_lens": seq_lens}, B)
     _check(load().kvhp_q4_rope_append(
-        _ptr(q), _ptr(k), _ptr(v), sq, sk, sv, _ptr(positions), _ptr(slots), _ptr(seq_lens),
-        theta, _ptr(q_out), _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1],
+        _ptr(q), k.data_ptr(), v.data_ptr(), sq, sk, sv, _ptr(positions), _ptr(slots), _ptr(seq_lens),
+        theta, _ptr(q_out), pool.data_ptr(), block_tables.data_ptr(), max_pages, pages,
         B, R, num_q_heads, num_kv_heads, head_dim, _stream(stream)))
 
 
@@ -599,9 +638,20 @@ def q4_gather(pool, block_tables, seq_lens, out_k, out_v, start=None, stream=Non
     """Positions start[b] + t of a 4-bit pool as fp16 [B][Hkv][max_len][D] (either output
     may be None), zeros from seq_lens[b] on."""
     B, hkv, n, d = (out_k if out_k is not None else out_v).shape
+    max_pages, pages = block_tables.shape[1], pool.shape[1]
+    values, pooled = B * hkv * n * d, hkv * pages * PAGE_SIZE * (d + 8)
+    if not (pool.numel() == pooled and block_tables.numel() >= B * max_pages
+            and (out_k is None or out_k.is_contiguous())
+            and (out_v is None or out_v.numel() == values and out_v.is_contiguous())
+            and seq_lens.numel() >= B and seq_lens.is_contiguous()
+            and (start is None or start.numel() >= B and start.is_contiguous())
+            and pool.is_contiguous() and block_tables.is_contiguous()):
+        _refuse_sizes("q4_gather", {"out_k": (out_k, values), "out_v": (out_v, values), "pool": (pool, pooled),
+                                    "block_tables": (block_tables, B * max_pages)},
+                      {"seq_lens": seq_lens, "start": start}, B)
     _check(load().kvhp_q4_gather(
-        _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1], _ptr(start),
-        _ptr(seq_lens), _ptr(out_k), _ptr(out_v), B, hkv, d, n, _stream(stream)))
+        pool.data_ptr(), block_tables.data_ptr(), max_pages, pages, _ptr(start),
+        seq_lens.data_ptr(), _ptr(out_k), _ptr(out_v), B, hkv, d, n, _stream(stream)))
 
 
 def q4_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_seq_len) -> int:
@@ -613,9 +663,17 @@ def q4_decode(q, pool, block_tables, seq_lens, out, num_q_heads, num_kv_heads, h
               max_seq_len, workspace=None, stream=None):
     """decode_attention over a 4-bit pool; workspace: a tensor of
     q4_decode_workspace_bytes bytes."""
+    B, max_pages, pages = seq_lens.shape[0], block_tables.shape[1], pool.shape[1]
+    values, pooled = B * num_q_heads * head_dim, num_kv_heads * pages * PAGE_SIZE * (head_dim + 8)
+    if not (q.numel() == values == out.numel() and pool.numel() == pooled
+            and block_tables.numel() >= B * max_pages
+            and q.is_contiguous() and out.is_contiguous() and seq_lens.is_contiguous()
+            and pool.is_contiguous() and block_tables.is_contiguous()):
+        _refuse_sizes("q4_decode", {"q": (q, values), "out": (out, values), "pool": (pool, pooled),
+                                    "block_tables": (block_tables, B * max_pages)}, {"seq_lens": seq_lens}, B)
     _check(load().kvhp_q4_decode(
-        _ptr(q), _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1],
-        _ptr(seq_lens), _ptr(out), seq_lens.shape[0], num_q_heads, num_kv_heads, head_dim,
+        q.data_ptr(), pool.data_ptr(), block_tables.data_ptr(), max_pages, pages,
+        seq_lens.data_ptr(), out.data_ptr(), B, num_q_heads, num_kv_heads, head_dim,
         max_seq_len, _ptr(workspace), _bytes(workspace), _stream(stream)))
 
 
@@ -630,9 +688,23 @@ def q4_prefill(q, pool, block_tables, out, num_q_heads, num_kv_heads, head_dim, 
     """Rows q [B][rows][Hq][D] at positions q_start[b] + r, each over the keys of the 4-bit
     pool up to itself; out as q, lse fp32 [B][Hq][rows] (optional); padding rows are left
     as they were."""
+    B, R, _, _ = q.shape
+    max_pages, pages = block_tables.shape[1], pool.shape[1]
+    values, pooled = B * R * num_q_heads * head_dim, num_kv_heads * pages * PAGE_SIZE * (head_dim + 8)
+    if not (q.numel() == values == out.numel() and pool.numel() == pooled
+            and block_tables.numel() >= B * max_pages
+            and (lse is None or lse.numel() == B * R * num_q_heads and lse.is_contiguous())
+            and (q_start is None or q_start.numel() >= B and q_start.is_contiguous())
+            and (seq_lens is None or seq_lens.numel() >= B and seq_lens.is_contiguous())
+            and q.is_contiguous() and out.is_contiguous() and pool.is_contiguous()
+            and block_tables.is_contiguous()):
+        _refuse_sizes("q4_prefill", {"q": (q, values), "out": (out, values), "pool": (pool, pooled),
+                                     "lse": (lse, B * R * num_q_heads),
+                                     "block_tables": (block_tables, B * max_pages)},
+                      {"q_start": q_start, "seq_lens": seq_lens}, B)
     _check(load().kvhp_q4_prefill(
-        _ptr(q), _ptr(pool), _ptr(block_tables), block_tables.shape[1], pool.shape[1],
-        _ptr(q_start), _ptr(seq_lens), _ptr(out), _ptr(lse), q.shape[0], q.shape[1], num_q_heads,
+        q.data_ptr(), pool.data_ptr(), block_tables.data_ptr(), max_pages, pages,
+        _ptr(q_start), _ptr(seq_lens), out.data_ptr(), _ptr(lse), B, R, num_q_heads,
         num_kv_heads, head_dim, max_seq_len, _ptr(workspace), _bytes(workspace),
         _stream(stream)))
 
