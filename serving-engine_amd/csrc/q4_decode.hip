@@ -14,9 +14,10 @@
 // for V, without rounding (q4.h): a shift, four ands and four multiply-adds for eight codes.
 // K's scale s multiplies the fp32 score.  V's is split into a power of two E of 2^-14 to 2^-9,
 // which goes with the codes, and s / E, of 4 to 4096, which multiplies the weight before its
-// one rounding to fp16.  (Scales past 8, rows with values past 60 or so, lower a wave's weights
-// by a common power of two.)  A weight's 2^-11 holds down to 2^-16 of the largest; below it is
-// an absolute 2^-25 of at most a quarter of that.
+// one rounding to fp16.  A weight's 2^-11 holds down to 2^-16 of the largest; below it is an
+// absolute 2^-25 of at most a quarter of that.  (Keys of scales past 8, rows with values past 60
+// or so, would take it past fp16: their weights are 2^-13 of it, in products of their own that are
+// multiplied back, so that the other keys' keep their bits.  Theirs hold 2^-11 down to 2^-13.)
 //
 // What bounds it: 32 sequences of up to 8192 keys, 32/8 heads of 128 (152 MB): 34.2 us, 4.5 TB/s, of
 // which reading the pages alone takes 31 (a probe that reads pages of 2176 bytes in a random order
@@ -40,7 +41,8 @@ constexpr int kMaxTiles = 16;     // per wave and split: 64 page ids, one per la
 constexpr int kMinTiles = 4;      // per balanced split
 constexpr int kHeads = 16;        // query heads per workgroup
 constexpr float kLazyLog2 = 3.f;  // a row's reference moves when a score passes it by this
-constexpr float kMostM = 4096.f;  // s / E: weights up to 2^15 in fp16
+constexpr float kMostM = 4096.f;  // s / E: weights up to 2^15 in fp16,
+constexpr float kLarge = 8192.f;  // and this part of larger ones, which are up to 2^25
 
 struct DecodePlan {
     int chunk;        // keys per split, a multiple of kTok
@@ -185,12 +187,14 @@ struct __attribute__((aligned(16))) Prepared {
     float2 sm[kTok];        // K's s and V's m
     uint16_t e[kTok];       // V's E 2^24 or E 2^20 ...
     f16 f[kTok];            // ... and E r
+    float large[kTok];      // m / kLarge where it is past kMostM (and 0 in sm)
 };
 
 // W waves per workgroup take the tiles of one split round robin and meet in LDS.
-// PK: parts that a tile's scores are dealt out to, 16 / PK query heads or fewer.
+// PK: parts that a tile's scores are dealt out to, 16 / PK query heads or fewer.  Four waves a SIMD
+// where their registers allow it without spills.
 template <int D, int W, int PK>
-__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 4)))
+__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(D == 128 || PK < 4 ? 3 : 4)))
 q4_decode_kernel(const Q4Args a, const DecodePlan p) {
     using St = Stage<D>;
     constexpr int NS = D / 32, ND = D / 16, PB = q4_page_bytes(D), RB = St::RB;
@@ -267,7 +271,7 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         issue(j, vo, st0 + St::VOFF, [](int i) { return i * St::PAGE; });
     };
 
-    float m_run = -1e30f, l_part = 0.f, down = 1.f;
+    float m_run = -1e30f, l_part = 0.f;
     floatx4 o[ND];   // lane (g, col): dims 16 db + 4 g + e of head col
 #pragma unroll
     for (int db = 0; db < ND; ++db) o[db] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -289,19 +293,19 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         const int T0 = t_begin + kTok * (wv + W * j);
         wait_ring<St::LOADS>();   // K and the numbers have landed, V may be on its way
         asm volatile("" ::: "memory");
+        bool large;   // some key's scale is past 8
         {   // this lane's key, for all
             const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 4 * col);
             uint32_t vp = *reinterpret_cast<const uint32_t*>(st + St::PAR + g * 128 + 64 + 4 * col);
             if (LAST && T0 + lane >= t_end) vp = 0;   // nothing of a row behind the last key
             Scale z = scale_of(vp, col);
-            const float size = fabsf(z.m);
-            if (__ballot(size * down > kMostM)) {
-                const float most = wave_max_fast(size < INFINITY ? size : 0.f) * (1.f / kMostM);
-                const float to = __uint_as_float(0x7f000000u - ((__float_as_uint(most) + 0x007fffffu) & 0x7f800000u));
-                scale_o(to / down);
-                down = to;
+            large = __ballot(fabsf(z.m) > kMostM) != 0;
+            if (large) {
+                const bool mine = fabsf(z.m) > kMostM;
+                prep.large[at] = mine ? z.m * (1 / kLarge) : 0.f;
+                z.m = mine ? 0.f : z.m;
             }
-            prep.sm[at] = float2{q4_row(kp).s, z.m * down};
+            prep.sm[at] = float2{q4_row(kp).s, z.m};
             prep.e[at] = z.e;
             prep.f[at] = z.f;
         }
@@ -385,34 +389,65 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
             l_part += y + z;
             w[t / 2] = __builtin_bit_cast(uint32_t, half2v{static_cast<f16>(y * m[t]), static_cast<f16>(z * m[t + 1])});
         }
-        u32x4 pt[2];   // the weights of page g's keys, of head col
+        // the weights of page g's keys, of head col
+        auto deal = [&](const uint32_t (&w)[X / 2], u32x4 (&pt)[2]) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (PK == 1) pt[u][i] = w[4 * u + i];
-                if constexpr (PK == 2) pt[u][i] = u == 0 ? w[i] : row_move<kShl + 8, 0xf>(w[i], w[i]);
-                if constexpr (PK == 4) {
-                    const uint32_t v = w[i % 2];
-                    pt[u][i] = u == 0 ? (i < 2 ? v : row_move<kShl + 4, 0xf>(v, v))
-                                      : (i < 2 ? row_move<kShl + 8, 0xf>(v, v) : row_move<kShl + 12, 0xf>(v, v));
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (PK == 1) pt[u][i] = w[4 * u + i];
+                    if constexpr (PK == 2) pt[u][i] = u == 0 ? w[i] : row_move<kShl + 8, 0xf>(w[i], w[i]);
+                    if constexpr (PK == 4) {
+                        const uint32_t v = w[i % 2];
+                        pt[u][i] = u == 0 ? (i < 2 ? v : row_move<kShl + 4, 0xf>(v, v))
+                                          : (i < 2 ? row_move<kShl + 8, 0xf>(v, v) : row_move<kShl + 12, 0xf>(v, v));
+                    }
                 }
-            }
-        u32x4 e[2], f[2];
+        };
+        const uint8_t* vr = st + St::VOFF + g * St::PAGE + col * RB;
+        auto codes = [&](int db) { return lds_read_tr4(vr + 16 * (db / 2 ^ St::vswz(col)) + 8 * (db & 1)); };
+        u32x4 pt[2], e[2], f[2];
+        auto scales = [&]() {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            e[u] = *reinterpret_cast<const u32x4*>(&prep.e[16 * g + 8 * u]);
-            f[u] = *reinterpret_cast<const u32x4*>(&prep.f[16 * g + 8 * u]);
+            for (int u = 0; u < 2; ++u) {
+                e[u] = *reinterpret_cast<const u32x4*>(&prep.e[16 * g + 8 * u]);
+                f[u] = *reinterpret_cast<const u32x4*>(&prep.f[16 * g + 8 * u]);
+            }
+        };
+        if (large) {   // seldom: what those keys add, before the others
+            uint32_t wl[X / 2];
+#pragma unroll
+            for (int t = 0; t < X; t += 2) {
+                const float2 z = *reinterpret_cast<const float2*>(&prep.large[16 * g + X * part + t]);
+                wl[t / 2] = __builtin_bit_cast(uint32_t, half2v{static_cast<f16>(fast_exp2(fmaf(x[t], sc, nm)) * z.x),
+                                                                static_cast<f16>(fast_exp2(fmaf(x[t + 1], sc, nm)) * z.y)});
+            }
+            deal(wl, pt);
+            scales();
+            wait_ring<0>();
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int db = 0; db < ND; ++db) {
+                const v2i y = codes(db);
+                floatx4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(y[u], e[u], f[u]),
+                                                               __builtin_bit_cast(half8, pt[u]), c, 0, 0, 0);
+                o[db] += c * kLarge;
+                __builtin_amdgcn_sched_barrier(0);   // registers count here, not waits
+            }
         }
+        deal(w, pt);
+        scales();
         if constexpr (LAST)
             wait_ring<0>();
         else
             wait_ring<St::LOADS + 1>();
         asm volatile("" ::: "memory");
-        const uint8_t* vr = st + St::VOFF + g * St::PAGE + col * RB;
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
-            const v2i y = lds_read_tr4(vr + 16 * (db / 2 ^ St::vswz(col)) + 8 * (db & 1));
+            const v2i y = codes(db);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
                 o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand(y[u], e[u], f[u]),
@@ -434,7 +469,6 @@ q4_decode_kernel(const Q4Args a, const DecodePlan p) {
         step(std::true_type{}, n_w - 1);
         asm volatile("" ::: "memory");
     }
-    if (down != 1.f) scale_o(1.f / down);
     if constexpr (PK == 4) l_part += row_move<kRor + 4, 0xf>(l_part, l_part);
     if constexpr (PK >= 2) l_part += row_move<kRor + 8, 0xf>(l_part, l_part);
 
