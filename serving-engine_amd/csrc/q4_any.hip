@@ -10,7 +10,9 @@
 //                     keys for one dim, gathered by bytes from the pages' codes in LDS
 // Both operands are (n + r) 2^-9, exact (q4.h), from the denormal that a code is in a half's low
 // bits.  s multiplies the fp32 scores, and the weight before its one rounding to fp16, by a power
-// of two per tile that brings the tile's largest s to 2^14.  dims past head_dim and keys past the
+// of two per tile that brings the tile's largest s up to 8 to 2^14; keys of larger ones, rows with
+// values past 60 or so, have no weight then, and their tile is gone through once more for them
+// alone, so that the others' weights keep their bits.  dims past head_dim and keys past the
 // last are operands of 0; a key that holds NaN has those too, and a scale of NaN for the pairs
 // that see it.
 //
@@ -31,6 +33,7 @@ namespace {
 constexpr int kTile = 64;       // keys
 constexpr int kCols = 16;       // pairs of a wave
 constexpr int kWaves = 4096;    // wanted
+constexpr float kMostScale = 8.f;   // of keys whose weights share a power of two
 constexpr int64_t kMostRowHeads = 1 << 29;
 
 struct AnyPlan {
@@ -97,7 +100,8 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
     const half2v lo15 = {f16(32768), f16(32768)}, hi15 = {f16(2048), f16(2048)};
     const float sc = 512.f * a.scale_log2;
 
-    for (int t = t0; t < t1; ++t) {
+    bool again = false;   // the tile's keys of large scales
+    for (int t = t0; t < t1; t += again ? 0 : 1) {
         const uint8_t* pg[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -114,7 +118,16 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
                 const int ch = lane + kWave * u;
                 v[i][u] = ch < RB ? *reinterpret_cast<const u32x4*>(pg[i] + kPage * RB + 16 * ch) : u32x4{};
             }
-        float s[4][4], vscale[4][4], mx = -INFINITY, big = 0.f;
+        float s[4][4], mx = -INFINITY, big = 0.f;
+        // V's scales; as they lie in the page where floats would spill (4 rows of 1024 keys of 32/8 heads
+        // of 128: 12.4 us, as floats 12.8; 32 sequences of up to 8192 of 96: 82.4, as they lie 85.5)
+        std::conditional_t<NC == 4, uint32_t, float> vnum[4][4];
+        auto vscale = [&](int i, int e) {
+            if constexpr (NC == 4)
+                return static_cast<float>(as_half2(vnum[i][e])[0]);
+            else
+                return vnum[i][e];
+        };
         f16 voff[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -142,15 +155,20 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
                 s[i][e] = live && j <= pos ? acc[e] * (static_cast<float>(as_half2(ks[e])[0]) * sc) : -INFINITY;
                 mx = fmaxf(mx, s[i][e]);
                 voff[i][e] = offset_of(vp[e], j <= p_hi);
-                vscale[i][e] = static_cast<float>(as_half2(vp[e])[0]);
+                if constexpr (NC == 4)
+                    vnum[i][e] = vp[e];
+                else
+                    vnum[i][e] = static_cast<float>(as_half2(vp[e])[0]);
                 // a NaN is none of the largest, an infinity is only behind the last key
-                big = fmaxf(big, j <= p_hi ? fabsf(vscale[i][e]) : 0.f);
+                big = fmaxf(big, j <= p_hi ? fabsf(vscale(i, e)) : 0.f);
             }
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         big = fmaxf(big, __shfl_xor(big, 16));
         big = fmaxf(big, __shfl_xor(big, 32));
+        const bool large = __ballot(big > kMostScale) != 0;
+        if (large) big = again ? 65504.f : kMostScale;   // for all that the pass may have
         const float mn = fmaxf(m, mx), alpha = fast_exp2(m - mn);
         m = mn;
         // 2^14 over big's power of two, and its inverse; big is 0 or at least 2^-24
@@ -164,10 +182,17 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = fast_exp2(s[i][e] - mn);
-                l += x;
+                l = fmaf(x, again ? 0.f : 1.f, l);
                 // of keys not seen nothing, whatever their scale
-                w[i / 2][4 * (i & 1) + e] = s[i][e] == -INFINITY ? f16(0) : static_cast<f16>(x * (vscale[i][e] * up));
+                w[i / 2][4 * (i & 1) + e] = s[i][e] == -INFINITY ? f16(0) : static_cast<f16>(x * (vscale(i, e) * up));
             }
+        if (large) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if ((fabsf(vscale(i, e)) > kMostScale) != again) w[i / 2][4 * (i & 1) + e] = f16(0);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -197,6 +222,7 @@ __global__ void __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(NC <
             o[db] = o[db] * alpha + acc * down;
         }
         __syncthreads();
+        again = large && !again;
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);

@@ -58,11 +58,11 @@ def _q(rng, d, *lead):
 
 
 @pytest.mark.parametrize("kind", list(LARGE))
-@pytest.mark.parametrize("G,d", [(1, 64), (5, 64), (9, 64), (4, 128), (8, 128), (9, 128)])
+@pytest.mark.parametrize("G,d", [(1, 64), (5, 64), (9, 64), (4, 128), (8, 128), (9, 128), (1, 96), (2, 256)])
 def test_decode_beside_large_rows(G, d, kind):
     """So many sequences and heads that a wave takes 16 tiles, the first key's among them."""
     rng = np.random.default_rng(G + d)
-    hkv, B = 64, 24
+    hkv, B = 64, 24 if d in (64, 128) else 64
     c = _cache(rng, 1000, hkv, d, kind, B)
     q = _q(rng, d, B, G * hkv)
     for c.cap in (4096, 1000):   # splits by the batch; one of eight waves
