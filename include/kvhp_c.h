@@ -394,9 +394,10 @@ int kvhp_evict_apply(void* pool_k, void* pool_v, float* weights, int32_t* ages,
  * padding: they reach nothing, and their q_out stays as it was.  K and V of a slot past the block
  * table, or whose page id lies outside [0, num_pages), are dropped (write tables hold -1
  * for shared pages); its q is rotated all the same.  Where two rows go to the same slot of a
- * page, what it holds then is undefined.  head_dim is even and at most 256;
- * batch rows (Hq + 2 Hkv) is at most 2^25 where head_dim is neither 64 nor 128 or a tensor
- * is off 16-byte alignment (rows then go one by one, several times slower).
+ * page, what it holds then is undefined.  head_dim is even and at most 256.  batch rows is at most
+ * 2^27; where head_dim is neither 64 nor 128, a tensor or a stride is off 16 bytes or Hq + 2 Hkv
+ * is past 2^14, batch rows (Hq + 2 Hkv) is at most 2^25 (a wave then takes a token's rows, up to
+ * eight, one after the other: two to three times as long).
  * Asynchronous, allocates nothing, may be captured. */
 int kvhp_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
                      int64_t k_stride, int64_t v_stride, const int32_t* positions,

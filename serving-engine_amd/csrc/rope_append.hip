@@ -23,6 +23,8 @@
 namespace kvhp {
 namespace {
 
+constexpr int kMostVecTokens = 1 << 27;   // 16 tokens a workgroup, 2^31 threads along a grid's axis
+
 struct AppendArgs {
     const f16 *q, *k, *v;
     int64_t sq, sk, sv;       // between tokens
@@ -340,7 +342,7 @@ int append(AppendArgs& a, const char* what, bool q4, int batch, int rows, int hq
     const int64_t tokens = (int64_t)batch * rows;
     const int H = a.Hq + 2 * hkv;
     auto whole = [](const void* x, int64_t stride) { return !x || (aligned16(x) && stride % 8 == 0); };
-    if ((d == 64 || d == 128) && tokens <= INT32_MAX && H <= 1 << 14 && whole(a.q, a.sq) &&
+    if ((d == 64 || d == 128) && tokens <= kMostVecTokens && H <= 1 << 14 && whole(a.q, a.sq) &&
         whole(a.k, a.sk) && whole(a.v, a.sv) && aligned16(a.q_out) && aligned16(a.pool_k) &&
         aligned16(a.pool_v)) {
         // (16 H rows of a workgroup, part by part: __umulhi is exact to 2^32 of row x heads.)
