@@ -443,10 +443,13 @@ int kvhp_q4_gather(const void* pool, const int32_t* block_tables, int max_pages,
  * states and sums are fp32; a weight is rounded to fp16 once, with its row's share of s.
  * Outputs past fp16's range, which the rows' rounding alone can bring about, are +-65504.
  * Asynchronous, allocates nothing, may be captured.  The workspace must be 16-byte aligned
- * and hold *_workspace_bytes bytes (0: NULL is fine); calls that overlap need one each.
+ * and hold *_workspace_bytes bytes (0: NULL is fine); calls that overlap need one each.  Ask for
+ * the sizes that a call is made with: less work is cut into more pieces, so fewer rows or
+ * sequences, or a shorter max_seq_len, may need more than the most there will be of them.
  * How the work is cut goes by max_seq_len: pass the longest length of the step.  The fast
- * kernels take head_dim 64 and 128 with q and out 16-byte aligned; other shapes run on a
- * kernel for any, which takes two to four times as long. */
+ * kernels take head_dim 64 and 128 with q and out 16-byte aligned; other shapes, and few rows
+ * of q4_prefill (up to 64 (row, query head) pairs of a KV head, where it is the faster), run on
+ * a kernel for any, which takes two to four times as long otherwise. */
 size_t kvhp_q4_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
                                       int max_seq_len);
 int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables, int max_pages,
@@ -459,7 +462,8 @@ int kvhp_q4_decode(const void* q, const void* pool, const int32_t* block_tables,
  * negative positions or at or past seq_lens[b] (device int32, NULL: max_seq_len) are
  * padding: their out and lse stay as they were.  lse (may be NULL): fp32
  * [batch][Hq][rows], the natural logarithm of the sum over a row's keys of
- * exp(q.k / sqrt(D)).  Otherwise as kvhp_q4_decode. */
+ * exp(q.k / sqrt(D)).  Otherwise as kvhp_q4_decode; a chunk may need more workspace than a whole
+ * prompt (32/8 heads of 128, 8192 keys: none for 8192 rows, 34 MB for 128). */
 size_t kvhp_q4_prefill_workspace_bytes(int batch, int rows, int num_q_heads, int num_kv_heads,
                                        int head_dim, int max_seq_len);
 int kvhp_q4_prefill(const void* q, const void* pool, const int32_t* block_tables, int max_pages,
