@@ -10,7 +10,7 @@
 // a lane both halves' chunks of 8 pairs, two rows' loads in flight.  In 4 bits the 4 or 8
 // lanes of a row find its range among themselves and write a word of codes per chunk.
 // 8192 tokens of 32/8 heads of 128: 43.3 us, 201 MB at 4.65 TB/s, where a copy of 1 GiB reaches
-// 4.7 to 5.0; into 4 bits 41.3 (177 MB).  The same with the rotation computed per row took 134 and
+// 5.04; into 4 bits 41.3 (177 MB).  The same with the rotation computed per row took 134 and
 // 163: 64-bit sines and cosines, 40 times a token instead of once.  A step's tokens are bound by
 // their dependent waits: 32 of them 4.0 us, one 2.2.
 // Other shapes: one wave per token and up to 8 of its heads, a lane per pair of dims (2048 tokens of 32/8
