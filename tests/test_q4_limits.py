@@ -19,4 +19,4 @@ def test_less_work_may_need_more_workspace():
     rows, step = kvhp.q4_prefill_workspace_bytes, kvhp.q4_decode_workspace_bytes
     assert rows(1, 8192, 32, 8, 128, 8192) == 0 < rows(1, 128, 32, 8, 128, 8192) < 34.1e6
     assert rows(1, 1, 32, 8, 128, 8192) < rows(1, 20, 32, 8, 128, 8192)
-    assert step(5, 32, 8, 128, 3136) < step(5, 32, 8, 128, 3072)
+    assert step(5, 32, 8, 128, 3904) < step(5, 32, 8, 128, 3840)
